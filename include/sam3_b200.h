@@ -244,6 +244,116 @@ int sam3b200_conv_2d(sam3b200_backend *be, const void *w_f16, const float *x, in
 int sam3b200_get_rows(sam3b200_backend *be, int type, const void *src, int64_t ncols, int64_t nrows,
                       const int32_t *idx, int64_t n, float *dst);
 
+/* ---- Sequence cache: rotary positions, 8-bit paged keys and values, attention ----
+ * What a causal transformer over tokens of text, images or video needs next to
+ * the ops above (FLASH_ATTN_EXT, GET_ROWS): queries and keys are turned by
+ * their positions, keys and values are quantised into a cache, and the
+ * attention reads the cache.  The reference keeps no such cache (its memory
+ * bank holds f32 maps, sam3.cpp:11175-11306); its axial rotation
+ * (sam3.cpp:3690-3712, 3848-3870) is the two-axis case of sam3b200_rope.
+ *
+ * Element types of rows: F32, F16, BF16 (enum ggml_type values).  Row tensors
+ * are [rows][heads][head_dim] with consecutive elements of a head; *_nb are
+ * the element strides {row, head}, NULL for packed rows (any strides >= 0 for
+ * inputs, so one row may serve many; outputs may not hold an element twice).
+ * 16-byte aligned rows are read and written 16 bytes at a time, others element
+ * by element, with the same results.  Every call is asynchronous on the
+ * backend stream, allocates nothing and may be captured into a CUDA graph. */
+#define SAM3B200_TYPE_BF16 30 /* enum ggml_type GGML_TYPE_BF16 */
+
+/* Rotary positions of one to four axes, as ggml_rope_ext / ggml_rope_multi
+ * turn them.  Pair i of a head, i < pairs = sum of sections, is turned by
+ * pos_scale * pos[axis(i)] * w(i):
+ *   neighbours 0: elements i and i + pairs; 1: elements 2i and 2i + 1;
+ *   deal 0: the first sections[0] pairs belong to axis 0, the next to axis 1,
+ *     ...; 1: pairs are dealt to the axes in turn, skipping those that have
+ *     their number (an axis of many pairs ends up alone behind the others);
+ *   restart 0: w(i) = base^(-i / pairs); 1: base^(-j / sections[axis]) for the
+ *     j-th pair of its axis.
+ * Elements from 2 * pairs on are copied.  head_dim 2 to 256. */
+typedef struct sam3b200_rope_hparams {
+    int32_t head_dim, n_axes, sections[4];
+    int32_t neighbours, deal, restart;
+    double base, pos_scale;
+} sam3b200_rope_hparams;
+typedef struct sam3b200_rope sam3b200_rope;
+/* NULL on error.  The handle is a host table; free it before the backend. */
+sam3b200_rope *sam3b200_rope_create(sam3b200_backend *be, const sam3b200_rope_hparams *hp);
+void sam3b200_rope_free(sam3b200_rope *r);
+/* y = x turned (inverse 1: turned back, which is also the gradient).  pos:
+ * device int32, the position of row r on axis k at pos[k * pos_stride + r].
+ * y may be x (same type and strides); it may not overlap x otherwise. */
+int sam3b200_rope_run(sam3b200_rope *r, int x_type, const void *x, const int64_t x_nb[2], const int32_t *pos,
+                      int64_t pos_stride, int64_t n_rows, int64_t n_heads, int inverse, int y_type, void *y,
+                      const int64_t y_nb[2]);
+
+/* The cache: int8 codes and one f32 scale per page and kv head, value = code *
+ * scale.  All memory is the caller's (sam3b200_buffer_alloc, codes 16-byte
+ * aligned); nothing has to be initialised.  A page holds page_tokens (16, 32,
+ * 64 or 128) consecutive tokens of one sequence; head_dim 64 or 128. */
+typedef struct sam3b200_kv_cache {
+    void *k_codes, *v_codes; /* device int8 [n_pages][n_kv_heads][page_tokens][head_dim] */
+    float *k_scale, *v_scale; /* device [n_pages][n_kv_heads] */
+    int32_t n_pages, n_kv_heads, page_tokens, head_dim;
+} sam3b200_kv_cache;
+
+/* A ragged batch over the cache.  Sequence s has kv_len[s] cached tokens,
+ * token t in page table[s * table_width + t / page_tokens], and the rows
+ * row_start[s] .. row_start[s + 1] - 1 of the row tensors.  The arrays are
+ * device memory, read by the kernels (a captured graph sees their new
+ * contents); the sizes are the host's bounds on them.  Contents that
+ * contradict the sizes, or a page outside [0, n_pages), make the next
+ * sam3b200_backend_synchronize fail; nothing is then accessed out of range,
+ * and the results of the sequences concerned are undefined.  Rows in front of
+ * row_start[0] and behind row_start[n_seqs] are not touched. */
+typedef struct sam3b200_kv_batch {
+    const int32_t *table;     /* device [n_seqs][table_width] */
+    int64_t table_width;
+    const int32_t *row_start; /* device [n_seqs + 1], not falling */
+    const int32_t *kv_len;    /* device [n_seqs] */
+    int32_t n_seqs, n_rows;   /* n_rows: rows of the row tensors, >= row_start[n_seqs] */
+    int32_t max_rows;         /* most rows of one sequence */
+    int64_t max_len;          /* largest kv_len, at most 2^30; decides how the work is split */
+} sam3b200_kv_batch;
+
+/* Quantise rows of k and v into the cache: the rows of a sequence become its
+ * last tokens, kv_len - rows .. kv_len - 1 (kv_len counts them already).  In
+ * each page that they touch the scale becomes max(s, amax * (1.0f / 127.0f)), amax over
+ * the page's new finite values and s the page's scale if it holds earlier
+ * tokens, else 0; below 2^-100 amax counts as 0.  Codes are the exact quotient
+ * rounded to nearest even; the page's earlier codes are rounded to a grown
+ * scale.  NaN is stored as 0, infinities as the ends of the range.  Codes of
+ * positions >= kv_len are left as they are.  Writing the same rows again
+ * changes nothing; a shorter kv_len than before (tokens taken back) is fine.
+ * Two sequences of one batch may not write to the same page. */
+int sam3b200_kv_write(sam3b200_backend *be, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch, int type,
+                      const void *k, const int64_t k_nb[2], const void *v, const int64_t v_nb[2]);
+
+/* The reverse: the last rows of each sequence, kv_len - rows .. kv_len - 1, as
+ * code * scale rounded to `type`. */
+int sam3b200_kv_read(sam3b200_backend *be, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch, int type,
+                     void *k, const int64_t k_nb[2], void *v, const int64_t v_nb[2]);
+
+/* The attention's workspace (about 34 MB of device memory).  Calls with one
+ * handle must not overlap on the GPU: those of one backend do not, unless a
+ * captured graph is launched on another stream; give such a graph a handle of
+ * its own.  Free it before the backend; NULL on error. */
+typedef struct sam3b200_kv_attention sam3b200_kv_attention;
+sam3b200_kv_attention *sam3b200_kv_attention_create(sam3b200_backend *be);
+void sam3b200_kv_attention_free(sam3b200_kv_attention *h);
+/* y = softmax(scale * q k^T + mask) v over the cached tokens, query head h
+ * reading kv head h / (n_heads / n_kv_heads).  causal 1: the rows of a
+ * sequence are its last tokens, row i sees tokens 0 .. kv_len - rows + i, of
+ * these the last `window` if window > 0; causal 0: every row sees all kv_len
+ * tokens, which need not include the rows (window 0).  A row that sees no
+ * token yields zeros.  q: F16 or BF16; y: q's type or F32.  Products are
+ * exact in the codes, sums and softmax statistics f32, softmax weights
+ * rounded to f16: within 2^-10 of the largest cached magnitude, plus the
+ * rounding to y's type.  scale >= 0. */
+int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch,
+                              int type, const void *q, const int64_t q_nb[2], int64_t n_heads, float scale, int causal,
+                              int64_t window, int y_type, void *y, const int64_t y_nb[2]);
+
 /* ---- Graph level: the backend's supports_op and graph_compute -------------
  * ggml_backend_graph_compute (sam3.cpp:1023-1028) hands a backend the nodes
  * of one graph in execution order; ggml's scheduler first asks the backend's

@@ -18,6 +18,7 @@ HEADER = os.path.join(os.path.dirname(PKG_DIR), "include", "sam3_b200.h")
 
 STATUS_ALLOC_FAILED, STATUS_FAILED, STATUS_SUCCESS, STATUS_ABORTED = -2, -1, 0, 1
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q4_1, TYPE_Q8_0 = 0, 1, 2, 3, 8
+TYPE_BF16 = 30
 MMQ_AUTO, MMQ_TC, MMQ_SIMT = 0, 1, 2
 ARITH_EXACT, ARITH_DQ16 = 0, 1
 TYPE_I32 = 26
@@ -294,6 +295,14 @@ def lib() -> ctypes.CDLL:
         "sam3b200_conv_transpose_2d": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp]),
         "sam3b200_conv_2d": (i32, [vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, i32, i32, i32, i32, i32, vp]),
         "sam3b200_get_rows": (i32, [vp, i32, vp, i64, i64, vp, i64, vp]),
+        "sam3b200_rope_create": (vp, [vp, vp]),
+        "sam3b200_rope_free": (None, [vp]),
+        "sam3b200_rope_run": (i32, [vp, i32, vp, vp, vp, i64, i64, i64, i32, i32, vp, vp]),
+        "sam3b200_kv_write": (i32, [vp, vp, vp, i32, vp, vp, vp, vp]),
+        "sam3b200_kv_read": (i32, [vp, vp, vp, i32, vp, vp, vp, vp]),
+        "sam3b200_kv_attention_create": (vp, [vp]),
+        "sam3b200_kv_attention_free": (None, [vp]),
+        "sam3b200_kv_attention_run": (i32, [vp, vp, vp, i32, vp, vp, i64, ctypes.c_float, i32, i64, i32, vp, vp]),
         "sam3b200_supports_op": (i32, [ctypes.POINTER(GraphTensor)]),
         "sam3b200_select_memory_frames": (i32, [i32, i32, vp, i32]),
         "sam3b200_extract_obj_ptr": (i32, [i32, i32, vp, ctypes.c_float, vp, vp, vp, vp]),
@@ -1171,6 +1180,83 @@ class GeometryEncoder:
             self.h = None
 
 
+class KVCache(ctypes.Structure):
+    """sam3b200_kv_cache (include/sam3_b200.h): the caller's device memory of a paged 8-bit key/value cache.
+    KVCache(k_codes, v_codes, k_scale, v_scale, n_pages, n_kv_heads, page_tokens, head_dim); the first four are
+    device addresses."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("n_pages", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+                ("page_tokens", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class KVBatch(ctypes.Structure):
+    """sam3b200_kv_batch (include/sam3_b200.h): a ragged batch over a KVCache.  KVBatch(table, table_width,
+    row_start, kv_len, n_seqs, n_rows, max_rows, max_len); table, row_start and kv_len are device addresses."""
+    _fields_ = [("table", ctypes.c_void_p), ("table_width", ctypes.c_int64), ("row_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("n_seqs", ctypes.c_int32), ("n_rows", ctypes.c_int32),
+                ("max_rows", ctypes.c_int32), ("max_len", ctypes.c_int64)]
+
+
+def _strides(nb):
+    return None if nb is None else (ctypes.c_int64 * 2)(*[int(x) for x in nb])
+
+
+class RopeHparams(ctypes.Structure):
+    """sam3b200_rope_hparams (include/sam3_b200.h)."""
+    _fields_ = [("head_dim", ctypes.c_int32), ("n_axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4),
+                ("neighbours", ctypes.c_int32), ("deal", ctypes.c_int32), ("restart", ctypes.c_int32),
+                ("base", ctypes.c_double), ("pos_scale", ctypes.c_double)]
+
+
+class Rope:
+    """Rotary positions of one to four axes (sam3b200_rope).  sections: the pairs of each axis."""
+
+    def __init__(self, be: "Backend", head_dim: int, sections, neighbours: bool = False, deal: bool = False,
+                 restart: bool = False, base: float = 10000.0, pos_scale: float = 1.0):
+        sections = [int(x) for x in sections]
+        if not 1 <= len(sections) <= 4:
+            raise B200Error(f"rope: {len(sections)} axes (1 to 4)")
+        hp = RopeHparams(head_dim, len(sections), (ctypes.c_int32 * 4)(*sections), int(neighbours), int(deal), int(restart),
+                         base, pos_scale)
+        self.be = be
+        self.h = lib().sam3b200_rope_create(be.h, ctypes.byref(hp))
+        if not self.h:
+            raise B200Error(f"rope_create failed: {last_error()}")
+
+    def apply(self, x: int, x_type: int, pos: int, n_rows: int, n_heads: int, y: int, y_type: int, inverse: bool = False,
+              x_nb=None, y_nb=None, pos_stride: int | None = None) -> None:
+        """y = x turned by its positions; x, pos, y are device addresses, *_nb element strides (row, head)."""
+        _check(lib().sam3b200_rope_run(self.h, x_type, x, _strides(x_nb), pos, n_rows if pos_stride is None else pos_stride,
+                                       n_rows, n_heads, 1 if inverse else 0, y_type, y, _strides(y_nb)), "rope")
+
+    def free(self) -> None:
+        if self.h:
+            lib().sam3b200_rope_free(self.h)
+            self.h = None
+
+
+class KVAttention:
+    """Attention over a KVCache (sam3b200_kv_attention: the workspace of its calls)."""
+
+    def __init__(self, be: "Backend"):
+        self.be = be
+        self.h = lib().sam3b200_kv_attention_create(be.h)
+        if not self.h:
+            raise B200Error(f"kv_attention_create failed: {last_error()}")
+
+    def run(self, cache: KVCache, batch: KVBatch, q_type: int, q: int, n_heads: int, y: int, scale: float,
+            causal: bool = True, window: int = 0, y_type: int | None = None, q_nb=None, y_nb=None) -> None:
+        """y = softmax(scale q k^T + mask) v; q and y are device addresses of [rows][n_heads][head_dim]."""
+        _check(lib().sam3b200_kv_attention_run(self.h, ctypes.addressof(cache), ctypes.addressof(batch), q_type, q,
+                                               _strides(q_nb), n_heads, scale, 1 if causal else 0, window,
+                                               q_type if y_type is None else y_type, y, _strides(y_nb)), "kv_attention")
+
+    def free(self) -> None:
+        if self.h:
+            lib().sam3b200_kv_attention_free(self.h)
+            self.h = None
+
+
 class WeightFile:
     """A sam3.cpp weight file opened by the native reader (sam3b200_file_*); opening reads the header,
     hyper-parameters and tensor directory only."""
@@ -1340,6 +1426,23 @@ class Backend:
                  dst: DeviceBuffer) -> None:
         """GGML_OP_GET_ROWS: dst[i] = dequantised row idx[i] of src (F32, F16, Q4_0, Q4_1, Q8_0)."""
         _check(lib().sam3b200_get_rows(self.h, qtype, src.ptr, ncols, nrows, idx.ptr, n, dst.ptr), "get_rows")
+
+    def rope(self, head_dim: int, sections, **kw) -> Rope:
+        """Rotary positions: see Rope."""
+        return Rope(self, head_dim, sections, **kw)
+
+    def kv_write(self, cache: KVCache, batch: KVBatch, ttype: int, k: int, v: int, k_nb=None, v_nb=None) -> None:
+        """sam3b200_kv_write: rows of k and v (device addresses) quantised into the cache."""
+        _check(lib().sam3b200_kv_write(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
+                                       v, _strides(v_nb)), "kv_write")
+
+    def kv_read(self, cache: KVCache, batch: KVBatch, ttype: int, k: int, v: int, k_nb=None, v_nb=None) -> None:
+        """sam3b200_kv_read: the last rows of each sequence back from the cache."""
+        _check(lib().sam3b200_kv_read(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
+                                      v, _strides(v_nb)), "kv_read")
+
+    def kv_attention(self) -> KVAttention:
+        return KVAttention(self)
 
     def graph_compute(self, nodes) -> None:
         """sam3b200_graph_compute: run GraphTensor nodes in order and wait for them (ggml graph_compute)."""

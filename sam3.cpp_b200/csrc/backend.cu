@@ -4,6 +4,7 @@
 #include "../../include/sam3_b200.h"
 #include "backend_impl.h"
 #include "gemm_f16.cuh"
+#include "kv_cache.cuh"
 #include "mmq.cuh"
 #include "vit_ops.cuh"
 
@@ -165,6 +166,9 @@ int sam3b200_backend_synchronize(sam3b200_backend *h) {
     if (e != 0) {
         if (e == (1 << 20))  // ops.cu: a get_rows index outside the source rows
             set_error("get_rows: row index out of range (error word 0x%x)", e);
+        else if (e & (kErrKvPage | kErrKvBatch))
+            set_error("kv cache:%s%s (error word 0x%x)", e & kErrKvPage ? " page index out of range" : "",
+                      e & kErrKvBatch ? " row_start or kv_len contradicts the batch's sizes" : "", e);
         else
             set_error("kernel pipeline wait timed out (error word 0x%x)", e);
         cudaMemset(be->err, 0, sizeof(int));

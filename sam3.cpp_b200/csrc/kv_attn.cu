@@ -1,0 +1,505 @@
+// kv_attn.cu -- attention over the paged 8-bit cache: the entry points, and
+// the kernel for few query rows a kv head.
+//
+//   y = softmax(scale q K^T + mask) V,   K = ks ck, V = vs cv a page
+//
+// Products with the codes are exact in f16 (|code| <= 127), so the scales
+// stay outside the matrix products.  With t = s ks scale log2(e) + log2(vs)
+// for a raw score s, and m the running maximum of t,
+//   p = 2^(t - m),   O = sum p cv,   l = sum p / vs,   y = O / l:
+// a page's value scale moves into the exponent, p stays in [0, 1] for f16
+// whatever the scales are, and no other step sees them.
+//
+// kv_attn_few: one block of 4 warps per (16 query rows of a kv head, part of
+// the key range).  The rows are the query heads of the group, times the
+// sequence's new tokens.  Each warp takes every fourth block of 16 tokens
+// (never across a page), copies it by cp.async into its own ring of shared
+// memory, and multiplies by mma.m16n8k16 f16 with f32 sums: bound by memory
+// (1 byte per code, 4 D flops per code and 16 rows), the legacy matrix
+// instruction is wide enough, and its register layout lets a lane read 16
+// codes of a token at once and hand the softmax weights on without a shuffle.
+// Dimensions are permuted in both products so that every lane's codes lie
+// together.  The warps' partial results are joined through shared memory, the
+// parts' through the workspace by the last block to finish.
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "kv_attn.cuh"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kWarps = 4, kStages = 4;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// d += a b: a 16 x 16 (rows), b 16 x 8, f16 in, f32 sums.
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Bytes i and j of w (codes + 128) as f16: 0x64uu is 1024 + u, exactly.
+template <int SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+    const uint32_t h = __byte_perm(w, 0x64646464u, SEL);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&h), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Four consecutive query elements (d a multiple of 4).
+__device__ __forceinline__ void load_q4(const KvAttnArgs &a, int64_t at, float (&x)[4]) {
+    const uint16_t *p = static_cast<const uint16_t *>(a.q) + at;
+    uint16_t e[4];
+    if (a.qs.aligned16) {
+        *reinterpret_cast<uint2 *>(e) = *reinterpret_cast<const uint2 *>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        x[i] = a.q_bf16 ? __uint_as_float(static_cast<uint32_t>(e[i]) << 16) : __half2float(__ushort_as_half(e[i]));
+}
+
+template <int D>
+struct Few {
+    static constexpr int kBlockBytes = 16 * D;                       // codes of 16 tokens
+    static constexpr int kStageBytes = 2 * kBlockBytes + 16;         // keys, values, their two scales
+    static constexpr int kRing = kWarps * kStages * kStageBytes;
+    static constexpr int kLane = D / 4;                              // output dimensions of a lane
+    static constexpr int kRowFloats = D + 16;                        // a merged row, padded against bank conflicts
+    static constexpr int kMerge = kWarps * kFewRows * kRowFloats * 4;
+    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+    // 16-byte chunk c of token t within a staged block.  The permutation keeps both reads free of bank
+    // conflicts: keys (8 lanes: 2 neighbouring tokens, 4 chunks) and values (8 lanes: 4 token pairs, 2 chunks).
+    static __device__ __forceinline__ int chunk(int t, int c) {
+        if (D == 128) return t * 8 + (c ^ (t & 6) ^ ((t & 1) << 2));
+        return (t >> 1) * 8 + ((((t & 1) << 2) | c) ^ (t & 6));
+    }
+    static __device__ __forceinline__ int padded(int d) { return d + d / kLane * 4; }
+};
+
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __grid_constant__ KvAttnArgs a) {
+    using F = Few<D>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float s_m[kWarps][kFewRows], s_l[kWarps][kFewRows];
+    __shared__ int s_last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int kv = blockIdx.y, G = a.group;
+    const unsigned unit = blockIdx.x / a.splits;
+    const int split = blockIdx.x % a.splits;
+    if (blockIdx.x + blockIdx.y == 0) kv_check(a.b, a.c.page_log2, false, a.err);
+    int64_t local;
+    const int s = kv_find(a.b, unit, G, 4, 1, local);
+    if (s < 0) return;
+    const KvSeq q = kv_seq(a.b, s, a.c.page_log2);
+    const int64_t R = static_cast<int64_t>(q.n) * G, row0 = local * kFewRows;
+    if (row0 >= R) return;
+    const int i_lo = static_cast<int>(row0 / G), i_hi = static_cast<int>((min(row0 + kFewRows, R) - 1) / G);
+
+    // the tile's keys, and this block's part of them
+    const int k_end = kv_last(a, q, i_hi) + 1, k_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
+    const int range = max(k_end - k_begin, 0);
+    const int chunk = max(a.chunk, ((range + a.splits - 1) / a.splits + 63) & ~63);
+    const int n_split = max((range + chunk - 1) / chunk, 1);
+    if (split >= n_split) return;
+    const int t_begin = k_begin + split * chunk, t_end = min(t_begin + chunk, k_end);
+    const int n_blocks = t_end > t_begin ? (t_end - t_begin + 15) / 16 : 0;
+    const int mine = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;  // blocks warp, warp + 4, ...
+
+    // queries: rows g and g + 8, for each 16-wide step the 4 dimensions that go with this lane's codes
+    uint32_t qf[D / 16][4];
+    float row_c[2];
+    int last[2], first[2];
+    {
+        float x[2][D / 16][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t r = row0 + g + 8 * h;
+            const int i = static_cast<int>(r / G);
+            const int64_t at = (q.r0 + static_cast<int64_t>(i)) * a.qs.token + (kv * G + r % G) * a.qs.head;
+            last[h] = kv_last(a, q, i);
+            first[h] = kv_first(a, last[h]);
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                if (r < R) load_q4(a, at + (k >> 2) * 64 + c * 16 + (k & 3) * 4, x[h][k]);
+                else x[h][k][0] = x[h][k][1] = x[h][k][2] = x[h][k][3] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[h][k][j]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // bf16 rows are brought to [1, 2) by a power of two, which f16 then holds to 2^-25 of the largest
+            const int e = a.q_bf16 ? min((__float_as_int(top) >> 23) & 0xff, 253) : 0;
+            const float down = e ? __int_as_float((254 - e) << 23) : 1.f;
+            row_c[h] = a.scale_log2 * (e ? __int_as_float(e << 23) : 1.f);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[h][k][j] *= down;
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            qf[k][0] = pack_f16(x[0][k][0], x[0][k][1]);
+            qf[k][1] = pack_f16(x[1][k][0], x[1][k][1]);
+            qf[k][2] = pack_f16(x[0][k][2], x[0][k][3]);
+            qf[k][3] = pack_f16(x[1][k][2], x[1][k][3]);
+        }
+    }
+    // tokens that some row of the tile does not see
+    const int seen_by_all = kv_last(a, q, i_lo), window_end = kv_first(a, kv_last(a, q, i_hi));
+
+    uint8_t *ring = smem + warp * kStages * F::kStageBytes;
+    int page_now = 0, page_next = 0;  // lane j: the page of block 32 b + j of this warp, for batches b and b + 1
+    auto load_page = [&](int j) -> int {
+        if (j >= mine) return 0;
+        const int p = kv_page(a.c, a.b, s, (t_begin + (j * kWarps + warp) * 16) >> a.c.page_log2, a.err);
+        return max(p, 0);
+    };
+    page_next = load_page(lane);
+    auto issue = [&](int j) {  // block j of this warp into its slot
+        if (j < mine) {
+            if ((j & 31) == 0) {
+                page_now = page_next;
+                page_next = load_page(j + 32 + lane);
+            }
+            const int page = __shfl_sync(0xffffffffu, page_now, j & 31);
+            const int tok = t_begin + (j * kWarps + warp) * 16;
+            const int64_t at = kv_slab(a.c, page, kv) + static_cast<int64_t>(tok & ((1 << a.c.page_log2) - 1)) * D;
+            const uint32_t dst = smem_u32(ring + (j % kStages) * F::kStageBytes);
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int k = 0; k < F::kBlockBytes / 512; ++k) {
+                    const int e = k * 32 + lane;  // 16-byte chunk of the block
+                    cp16(dst + w * F::kBlockBytes + F::chunk(e / (D / 16), e % (D / 16)) * 16, a.c.codes[w] + at + e * 16);
+                }
+            if (lane < 2) cp4(dst + 2 * F::kBlockBytes + lane * 4, a.c.scale[lane] + static_cast<int64_t>(page) * a.c.heads + kv);
+        }
+        cp_commit();
+    };
+    for (int j = 0; j < kStages - 1; ++j) issue(j);
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    for (int j = 0; j < mine; ++j) {
+        cp_wait<kStages - 2>();
+        __syncwarp();
+        issue(j + kStages - 1);
+        const uint8_t *st = ring + (j % kStages) * F::kStageBytes;
+        const uint4 *kc = reinterpret_cast<const uint4 *>(st), *vc = reinterpret_cast<const uint4 *>(st + F::kBlockBytes);
+        const float ks = *reinterpret_cast<const float *>(st + 2 * F::kBlockBytes);
+        const float vs = *reinterpret_cast<const float *>(st + 2 * F::kBlockBytes + 4);
+
+        // scores of tokens 2c, 2c + 1 (n = 0) and 8 + 2c, 9 + 2c (n = 1) for rows g, g + 8
+        float t[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) {
+                const uint4 w4 = kc[F::chunk(8 * n + g, 4 * h + c)];
+                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t u = w[k] ^ 0x80808080u;
+                    mma16816(t[n], qf[4 * h + k], codes2<0x4140>(u), codes2<0x4342>(u));
+                }
+            }
+        const float lv = vs > 0.f ? __log2f(vs) : kZeroScaleLog2, inv_vs = ex2_approx(-lv);
+        const float cs[2] = {row_c[0] * ks, row_c[1] * ks};
+        const int tok = t_begin + (j * kWarps + warp) * 16;
+        const bool edge = tok + 15 > seen_by_all || tok < window_end;
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int h = k >> 1, key = tok + 8 * n + 2 * c + (k & 1);
+                t[n][k] = fmaf(t[n][k], cs[h], lv);
+                if (edge && (key > last[h] || key < first[h])) t[n][k] = -INFINITY;
+                top[h] = fmaxf(top[h], t[n][k]);
+            }
+        if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                const float to = fmaxf(m[h], top[h]);
+                const float alpha = m[h] == to ? 1.f : ex2_approx(m[h] - to);
+                m[h] = to;
+                l[h] *= alpha;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) o[i][2 * h] *= alpha, o[i][2 * h + 1] *= alpha;
+            }
+        }
+        uint32_t p[4];
+        const float less[2] = {m[0] == -INFINITY ? 0.f : m[0] - kPUp, m[1] == -INFINITY ? 0.f : m[1] - kPUp};
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                t[n][k] = ex2_approx(t[n][k] - less[k >> 1]);
+                l[k >> 1] = fmaf(t[n][k], inv_vs, l[k >> 1]);
+            }
+            p[2 * n] = pack_f16(t[n][0], t[n][1]);
+            p[2 * n + 1] = pack_f16(t[n][2], t[n][3]);
+        }
+
+        // values: lane g holds dimensions D / 8 * g ... of tokens 2c, 2c + 1, 8 + 2c, 9 + 2c
+        uint32_t w[4][D / 32];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int tv = 2 * c + (r & 1) + 8 * (r >> 1);
+            if constexpr (D == 128) {
+                const uint4 x = vc[F::chunk(tv, g)];
+                w[r][0] = x.x, w[r][1] = x.y, w[r][2] = x.z, w[r][3] = x.w;
+            } else {
+                const uint2 x = reinterpret_cast<const uint2 *>(vc + F::chunk(tv, g >> 1))[g & 1];
+                w[r][0] = x.x, w[r][1] = x.y;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+            uint32_t lo[2], hi[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {  // bytes of two tokens side by side
+                lo[r] = __byte_perm(w[2 * r][k], w[2 * r + 1][k], 0x5140) ^ 0x80808080u;
+                hi[r] = __byte_perm(w[2 * r][k], w[2 * r + 1][k], 0x7362) ^ 0x80808080u;
+            }
+            mma16816(o[4 * k], p, codes2<0x4140>(lo[0]), codes2<0x4140>(lo[1]));
+            mma16816(o[4 * k + 1], p, codes2<0x4342>(lo[0]), codes2<0x4342>(lo[1]));
+            mma16816(o[4 * k + 2], p, codes2<0x4140>(hi[0]), codes2<0x4140>(hi[1]));
+            mma16816(o[4 * k + 3], p, codes2<0x4342>(hi[0]), codes2<0x4342>(hi[1]));
+        }
+    }
+    cp_wait<0>();
+    __syncthreads();  // every warp is done with its ring
+
+    // join the warps
+    float *rows = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (c == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
+        float *to = rows + (warp * kFewRows + g + 8 * h) * F::kRowFloats;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < D / 8; i += 4)
+                *reinterpret_cast<float4 *>(to + F::padded((2 * c + e) * (D / 8) + i)) =
+                    make_float4(o[i][2 * h + e], o[i + 1][2 * h + e], o[i + 2][2 * h + e], o[i + 3][2 * h + e]);
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * (D / 8);  // 8 threads a row
+    float M = -INFINITY, L = 0.f, sum[D / 8];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) sum[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][row]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const float f = s_m[w][row] == M ? 1.f : ex2_approx(s_m[w][row] - M);
+        L = fmaf(s_l[w][row], f, L);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+            sum[i] = fmaf(rows[(w * kFewRows + row) * F::kRowFloats + F::padded(d0 + i)], f, sum[i]);
+    }
+    const int64_t r = row0 + row;
+    const bool live = r < R;
+    if (n_split > 1) {
+        const int64_t group = static_cast<int64_t>(unit) * a.c.heads + kv;
+        float *base = a.part + group * a.splits * kFewRows * (D + 2);
+        float *ml = base + static_cast<int64_t>(a.splits) * kFewRows * D;
+        if (live) {
+            float *to = base + (static_cast<int64_t>(split) * kFewRows + row) * D + d0;
+#pragma unroll
+            for (int i = 0; i < D / 8; i += 4)
+                *reinterpret_cast<float4 *>(to + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+            if ((threadIdx.x & 7) == 0) *reinterpret_cast<float2 *>(ml + (split * kFewRows + row) * 2) = make_float2(M, L);
+        }
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) s_last = atomicInc(a.done + group, n_split - 1) == static_cast<unsigned>(n_split - 1);
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+        if (!live) return;
+        // join the parts, in their order
+        M = -INFINITY, L = 0.f;
+        for (int k = 0; k < n_split; ++k) M = fmaxf(M, __ldcg(ml + (k * kFewRows + row) * 2));
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) sum[i] = 0.f;
+        for (int k = 0; k < n_split; ++k) {
+            const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + (k * kFewRows + row) * 2));
+            const float f = x.x == M ? 1.f : ex2_approx(x.x - M);
+            L = fmaf(x.y, f, L);
+            const float *from = base + (static_cast<int64_t>(k) * kFewRows + row) * D + d0;
+#pragma unroll
+            for (int i = 0; i < D / 8; i += 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + i));
+                sum[i] = fmaf(v.x, f, sum[i]);
+                sum[i + 1] = fmaf(v.y, f, sum[i + 1]);
+                sum[i + 2] = fmaf(v.z, f, sum[i + 2]);
+                sum[i + 3] = fmaf(v.w, f, sum[i + 3]);
+            }
+        }
+    }
+    if (!live) return;
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees no key yields zeros
+    const int64_t at = (q.r0 + r / G) * a.ys.token + (kv * G + r % G) * a.ys.head + d0;
+#pragma unroll
+    for (int i = 0; i < D / 8; i += 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = sum[i + k] * inv;
+        kv_store8(a, at + i, v);
+    }
+}
+
+template <int D>
+cudaError_t launch_few(const KvAttnArgs &a, int64_t units, cudaStream_t st) {
+    using F = Few<D>;
+    // set at every call: the attribute belongs to the current device
+    const cudaError_t e = cudaFuncSetAttribute(kv_attn_few_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+    if (e != cudaSuccess) return e;
+    const dim3 grid(static_cast<unsigned>(units * a.splits), a.c.heads);
+    kv_attn_few_kernel<D><<<grid, kWarps * 32, F::kSmem, st>>>(a);
+    return cudaGetLastError();
+}
+
+struct KvAttention {
+    Backend *be = nullptr;
+    float *part = nullptr;
+    unsigned *done = nullptr;
+};
+
+}  // namespace
+
+cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st) {
+    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 4) + a.b.n_seqs;
+    // three blocks an SM: one wave of equal parts where there are few, four waves' worth where the lengths
+    // of many sequences have to even out
+    const int64_t wave = 3 * num_sms, groups = units * a.c.heads;
+    const int64_t span = a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len;
+    int64_t splits = 2 * groups < wave ? (wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
+    splits = std::min(splits, (span + 255) / 256);
+    splits = std::min(splits, static_cast<int64_t>(kMaxParts) / groups);
+    splits = std::max(splits, static_cast<int64_t>(1));
+    if (units * splits > 0x7fffffff) return cudaErrorInvalidValue;
+    a.splits = static_cast<int>(splits);
+    a.chunk = static_cast<int>((span + splits - 1) / splits + 63) & ~63;
+    return a.c.D == 64 ? launch_few<64>(a, units, st) : launch_few<128>(a, units, st);
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" sam3b200_kv_attention *sam3b200_kv_attention_create(sam3b200_backend *h) {
+    auto *be = reinterpret_cast<Backend *>(h);
+    if (!be) {
+        set_error("kv_attention_create: null backend");
+        return nullptr;
+    }
+    auto *k = new (std::nothrow) KvAttention();
+    if (!k) {
+        set_error("kv_attention_create: out of host memory");
+        return nullptr;
+    }
+    k->be = be;
+    DeviceScope dev(be->device);
+    if (!cuda_ok(cudaMalloc(&k->part, kPartFloats * sizeof(float)), "cudaMalloc(attention workspace)") ||
+        !cuda_ok(cudaMalloc(&k->done, kMaxParts * sizeof(unsigned)), "cudaMalloc(attention counters)") ||
+        !cuda_ok(cudaMemsetAsync(k->done, 0, kMaxParts * sizeof(unsigned), be->stream), "memset(attention counters)") ||
+        !cuda_ok(cudaStreamSynchronize(be->stream), "kv_attention_create sync")) {
+        cudaFree(k->part);
+        cudaFree(k->done);
+        delete k;
+        return nullptr;
+    }
+    return reinterpret_cast<sam3b200_kv_attention *>(k);
+}
+
+extern "C" void sam3b200_kv_attention_free(sam3b200_kv_attention *h) {
+    auto *k = reinterpret_cast<KvAttention *>(h);
+    if (!k) return;
+    DeviceScope dev(k->be->device);
+    cudaStreamSynchronize(k->be->stream);
+    cudaFree(k->part);
+    cudaFree(k->done);
+    delete k;
+}
+
+extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b200_kv_cache *cache,
+                                         const sam3b200_kv_batch *batch, int type, const void *q, const int64_t *q_nb,
+                                         int64_t n_heads, float scale, int causal, int64_t window, int y_type, void *y,
+                                         const int64_t *y_nb) {
+    auto *k = reinterpret_cast<KvAttention *>(h);
+    KvAttnArgs a;
+    if (!kv_views("kv_attention", cache, batch, a.c, a.b)) return SAM3B200_STATUS_FAILED;
+    if (!q || !y) {
+        set_error("kv_attention: null argument");
+        return SAM3B200_STATUS_FAILED;
+    }
+    const int yb = type_bytes(y_type);
+    if ((type != SAM3B200_TYPE_F16 && type != SAM3B200_TYPE_BF16) || (y_type != type && y_type != SAM3B200_TYPE_F32) ||
+        reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(y) % yb) {
+        set_error("kv_attention: unsupported types %d -> %d (q F16=1 or BF16=30, y q's type or F32=0) or unaligned data", type,
+                  y_type);
+        return SAM3B200_STATUS_FAILED;
+    }
+    if (n_heads < 1 || n_heads > 65535 || n_heads % a.c.heads != 0) {
+        set_error("kv_attention: %lld query heads over %d kv heads (a positive multiple is needed)", (long long)n_heads, a.c.heads);
+        return SAM3B200_STATUS_FAILED;
+    }
+    if (!(scale >= 0.f) || !std::isfinite(scale) || window < 0 || (window && !causal)) {
+        set_error("kv_attention: bad scale %g or window %lld (a window needs the causal mask)", scale, (long long)window);
+        return SAM3B200_STATUS_FAILED;
+    }
+    a.q = q, a.y = y;
+    a.qs = row_tensor(q, type, q_nb, n_heads, a.c.D);
+    a.ys = row_tensor(y, y_type, y_nb, n_heads, a.c.D);
+    if (!rows_ok("kv_attention", "q", a.qs, a.b.n_rows, n_heads, a.c.D, false) ||
+        !rows_ok("kv_attention", "y", a.ys, a.b.n_rows, n_heads, a.c.D, true))
+        return SAM3B200_STATUS_FAILED;
+    if (!k) {
+        set_error("kv_attention: null handle");
+        return SAM3B200_STATUS_FAILED;
+    }
+    if (a.b.n_seqs == 0 || a.b.n_rows == 0) return SAM3B200_STATUS_SUCCESS;
+    a.q_bf16 = type == SAM3B200_TYPE_BF16;
+    a.y_type = y_type;
+    a.heads = static_cast<int>(n_heads), a.group = static_cast<int>(n_heads / a.c.heads);
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.causal = causal != 0, a.window = static_cast<int>(std::min<int64_t>(window, 0x7fffffff));
+    a.part = k->part, a.done = k->done, a.err = k->be->err;
+    DeviceScope dev(k->be->device);
+    const cudaError_t e = kv_attn_few(a, k->be->num_sms, k->be->stream);
+    k->be->count();
+    return cuda_ok(e, "kv_attention launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
+}

@@ -1,0 +1,60 @@
+// kv_attn.cuh -- attention over the paged 8-bit cache: what its kernels share.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace b200 {
+
+struct KvAttnArgs {
+    KvView c;
+    KvRows b;
+    const void *q;
+    void *y;
+    RowTensor qs, ys;
+    int q_bf16;           // else f16
+    int y_type;           // SAM3B200_TYPE_*
+    int heads, group;     // query heads, query heads of a kv head
+    float scale_log2;     // scale * log2(e)
+    int causal, window;   // window 0: none
+    int splits;           // most parts of a key range
+    int chunk;            // tokens of a part (a multiple of 64)
+    float *part;          // partial results: see kPartFloats
+    unsigned *done;       // parts finished, one counter a unit and kv head; 0 between calls
+    int *err;
+};
+
+// 2^x scores: P = 2^(t - m + kPUp) with m within kLazy of the running
+// maximum, so f16 P reaches 2^(kPUp + kLazy) < 65504 at most, and what falls
+// below f16's smallest number is 2^-32 of the largest.
+constexpr float kPUp = 7.f, kLazy = 8.f;
+
+// Scale of a value page that holds only zeros, as the softmax weights see it.
+constexpr float kZeroScaleLog2 = -107.f;
+
+// The device workspace of a handle.
+constexpr int kMaxParts = 4096;
+constexpr int kFewRows = 16;
+constexpr size_t kPartFloats = static_cast<size_t>(kMaxParts) * kFewRows * (128 + 2);
+
+// Last key that row i of a sequence sees, and the first.
+__device__ __forceinline__ int kv_last(const KvAttnArgs &a, const KvSeq &q, int i) {
+    return a.causal ? q.len - q.n + i : q.len - 1;
+}
+__device__ __forceinline__ int kv_first(const KvAttnArgs &a, int last) {
+    return a.window ? max(last - a.window + 1, 0) : 0;
+}
+
+// Stores 8 results of one row.
+__device__ __forceinline__ void kv_store8(const KvAttnArgs &a, int64_t at, const float (&v)[8]) {
+    auto put = [&](auto *y) {
+        if (a.ys.aligned16) store8<true>(y + at, v);
+        else store8<false>(y + at, v);
+    };
+    if (a.y_type == SAM3B200_TYPE_F32) put(static_cast<float *>(a.y));
+    else if (a.y_type == SAM3B200_TYPE_F16) put(static_cast<__half *>(a.y));
+    else put(static_cast<__nv_bfloat16 *>(a.y));
+}
+
+cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st);
+
+}  // namespace b200

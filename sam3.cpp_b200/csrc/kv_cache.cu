@@ -1,0 +1,309 @@
+// kv_cache.cu -- writing rows of keys and values into the paged 8-bit cache
+// and reading them back.
+//
+// A page holds the codes of 16 to 128 consecutive tokens of one sequence for
+// each kv head, with one f32 scale s per (page, head): value = code s.
+// Writing rows into a page takes
+//   s = max(s_old, fl32(amax c))         c = fl32(1 / 127), amax over the finite new values,
+//                                        s_old = 0 where the page held no token
+//   code = round(x / s)                  of the exact quotient, ties to even
+// and rounds the page's older codes again, round(code s_old / s), if s grew.
+// Both roundings are decided exactly, so the codes do not depend on how the
+// rows of a prompt are cut into calls' blocks or on the order of anything.
+//
+// One block per (page, head, keys or values): the page's new rows are read
+// once into registers, their largest magnitude is reduced over the block and
+// the codes are written from the registers.  Bound by memory: 2 (f16) bytes
+// in and 1 out per value.
+#include "kv_cache.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr float kF32Max = 3.402823466e38f;
+
+// round(x / s), ties to even, for |x| <= 127.5 s, s a normal f32.  The magic
+// sum rounds x * inv (inv ~ 1 / s) to an integer q that is at most one off;
+// r = x - q s is exact wherever |r| is near s / 2 (x and q s are multiples of
+// the smaller of their units, and r needs no more bits than s), so comparing
+// it with s / 2 tells on which side of the border x lies.
+__device__ __forceinline__ int round_quotient(float x, float s, float inv) {
+    const float m = __fmaf_rn(x, inv, 12582912.f), q = __fsub_rn(m, 12582912.f);
+    const float r = __fmaf_rn(-q, s, x), h = 0.5f * s;
+    int c = __float_as_int(m) - 0x4B400000;
+    if (fabsf(r) >= h) {
+        const bool tie = fabsf(r) == h;
+        if (!tie || (c & 1)) c += r > 0.f ? 1 : -1;
+    }
+    return c;
+}
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+    return (a & 0xff) | ((b & 0xff) << 8) | ((c & 0xff) << 16) | (static_cast<uint32_t>(d) << 24);
+}
+
+struct WriteArgs {
+    KvView c;
+    KvRows b;
+    const void *x[2];
+    RowTensor xs[2];
+    int *err;
+};
+
+// Grid (units of one page, kv heads, keys / values); PER groups of 8 values a thread.
+template <typename T, bool VEC, int THREADS, int PER>
+__global__ void __launch_bounds__(THREADS) kv_write_kernel(WriteArgs a) {
+    __shared__ float wmax[THREADS / 32];
+    const int P = 1 << a.c.page_log2, D = a.c.D, head = blockIdx.y, w = blockIdx.z;
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) kv_check(a.b, a.c.page_log2, true, a.err);
+    int64_t local;
+    const int s = kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, local);
+    if (s < 0) return;
+    const KvSeq q = kv_seq(a.b, s, a.c.page_log2);
+    const int begin = q.len - q.n;  // first new position
+    if (q.n == 0 || begin < 0) return;
+    const int64_t i = (begin >> a.c.page_log2) + local;
+    const int64_t p0 = i << a.c.page_log2;
+    if (p0 >= q.len) return;
+    const int page = kv_page(a.c, a.b, s, i, a.err);
+    if (page < 0) return;
+    const int lo = static_cast<int>(max(begin - p0, static_cast<int64_t>(0)));          // first new token of the page
+    const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(P)));          // past its last one
+    int8_t *codes = a.c.codes[w] + kv_slab(a.c, page, head);
+    float *scale = a.c.scale[w] + static_cast<int64_t>(page) * a.c.heads + head;
+    const T *x = static_cast<const T *>(a.x[w]) + head * a.xs[w].head;
+    const int64_t row0 = q.r0 + p0 - begin;  // row of the page's token 0
+
+    float v[PER][8];
+    float amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int e = (k * THREADS + threadIdx.x) * 8, t = e / D, d = e % D;
+        if (t < lo || t >= hi) continue;
+        load8<VEC>(x + (row0 + t) * a.xs[w].token + d, v[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float m = fabsf(v[k][j]);
+            if (!(m == m)) v[k][j] = 0.f;  // NaN is stored as 0
+            amax = fmaxf(amax, m <= kF32Max ? m : 0.f);
+        }
+    }
+    const float held = lo > 0 ? *scale : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = amax;
+    __syncthreads();  // also: every thread has read the old scale
+#pragma unroll
+    for (int j = 0; j < THREADS / 32; ++j) amax = fmaxf(amax, wmax[j]);
+    const float to = fmaxf(held, amax < kKvSmallest ? 0.f : __fmul_rn(amax, 1.f / 127.f));
+    const float inv = to > 0.f ? __frcp_rn(to) : 0.f, top = fminf(__fmul_rn(127.f, to), kF32Max);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int e = (k * THREADS + threadIdx.x) * 8, t = e / D;
+        if (t >= hi) continue;
+        uint32_t out[2];
+        if (t >= lo) {
+            int c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)  // infinities go to the ends
+                c[j] = to > 0.f ? round_quotient(fminf(fmaxf(v[k][j], -top), top), to, inv) : 0;
+            out[0] = pack4(c[0], c[1], c[2], c[3]);
+            out[1] = pack4(c[4], c[5], c[6], c[7]);
+        } else {
+            if (to == held) continue;
+            const uint2 old = *reinterpret_cast<const uint2 *>(codes + e);
+            int c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {  // code * held is exact in 64 bits, and no quotient rounds onto a tie
+                const int8_t o = static_cast<int8_t>((j < 4 ? old.x : old.y) >> (8 * (j & 3)));
+                c[j] = __double2int_rn(static_cast<double>(o) * held / to);
+            }
+            out[0] = pack4(c[0], c[1], c[2], c[3]);
+            out[1] = pack4(c[4], c[5], c[6], c[7]);
+        }
+        *reinterpret_cast<uint2 *>(codes + e) = make_uint2(out[0], out[1]);
+    }
+    if (threadIdx.x == 0) *scale = to;
+}
+
+struct ReadArgs {
+    KvView c;
+    KvRows b;
+    void *y[2];
+    RowTensor ys[2];
+    int *err;
+};
+
+// Grid (units of one page, kv heads, keys / values).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(128) kv_read_kernel(ReadArgs a) {
+    const int P = 1 << a.c.page_log2, D = a.c.D, head = blockIdx.y, w = blockIdx.z;
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) kv_check(a.b, a.c.page_log2, true, a.err);
+    int64_t local;
+    const int s = kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, local);
+    if (s < 0) return;
+    const KvSeq q = kv_seq(a.b, s, a.c.page_log2);
+    const int begin = q.len - q.n;
+    if (q.n == 0 || begin < 0) return;
+    const int64_t i = (begin >> a.c.page_log2) + local;
+    const int64_t p0 = i << a.c.page_log2;
+    if (p0 >= q.len) return;
+    const int page = kv_page(a.c, a.b, s, i, a.err);
+    const int lo = static_cast<int>(max(begin - p0, static_cast<int64_t>(0)));
+    const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(P)));
+    const int8_t *codes = a.c.codes[w] + kv_slab(a.c, max(page, 0), head);
+    const float scale = page < 0 ? 0.f : a.c.scale[w][static_cast<int64_t>(page) * a.c.heads + head];
+    T *y = static_cast<T *>(a.y[w]) + head * a.ys[w].head;
+    const int64_t row0 = q.r0 + p0 - begin;
+    for (int e = lo * D + threadIdx.x * 8; e < hi * D; e += 128 * 8) {
+        const uint2 raw = *reinterpret_cast<const uint2 *>(codes + e);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = page < 0 ? 0.f : __fmul_rn(static_cast<float>(static_cast<int8_t>((j < 4 ? raw.x : raw.y) >> (8 * (j & 3)))), scale);
+        store8<VEC>(y + (row0 + e / D) * a.ys[w].token + e % D, v);
+    }
+}
+
+template <typename T, bool VEC>
+void launch_write(const WriteArgs &a, dim3 grid, cudaStream_t st) {
+    switch ((a.c.D << a.c.page_log2) / 1024) {
+        case 1: kv_write_kernel<T, VEC, 128, 1><<<grid, 128, 0, st>>>(a); break;
+        case 2: kv_write_kernel<T, VEC, 128, 2><<<grid, 128, 0, st>>>(a); break;
+        case 4: kv_write_kernel<T, VEC, 128, 4><<<grid, 128, 0, st>>>(a); break;
+        case 8: kv_write_kernel<T, VEC, 256, 4><<<grid, 256, 0, st>>>(a); break;
+        default: kv_write_kernel<T, VEC, 512, 4><<<grid, 512, 0, st>>>(a); break;
+    }
+}
+
+}  // namespace
+
+bool rows_ok(const char *op, const char *what, const RowTensor &t, int64_t rows, int64_t heads, int64_t D, bool written) {
+    const int64_t most = int64_t(1) << 40;
+    bool ok = t.token >= 0 && t.head >= 0 && t.token < most && t.head < most;
+    if (ok && written)  // no element twice: one of the two strides steps over all that the other reaches
+        ok = (t.token >= (heads - 1) * t.head + D || rows == 1) && (t.head >= D || heads == 1);
+    if (ok || rows <= 0) return true;
+    if (written && t.token >= D && t.head >= (rows - 1) * t.token + D) return true;
+    set_error("%s: bad strides of %s: token %lld, head %lld elements", op, what, (long long)t.token, (long long)t.head);
+    return false;
+}
+
+bool kv_views(const char *op, const sam3b200_kv_cache *c, const sam3b200_kv_batch *b, KvView &cv, KvRows &bv) {
+    if (!c || !b || !c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale || !b->table || !b->row_start || !b->kv_len) {
+        set_error("%s: null argument", op);
+        return false;
+    }
+    if (c->n_pages < 1 || c->n_kv_heads < 1 || c->n_kv_heads > 65535 ||
+        (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128) ||
+        (c->head_dim != 64 && c->head_dim != 128)) {
+        set_error("%s: unsupported cache: %d pages of %d tokens, %d kv heads of %d (pages of 16, 32, 64 or 128 tokens, "
+                  "head dims 64 and 128)",
+                  op, c->n_pages, c->page_tokens, c->n_kv_heads, c->head_dim);
+        return false;
+    }
+    for (const void *p : {static_cast<const void *>(c->k_codes), static_cast<const void *>(c->v_codes)})
+        if (reinterpret_cast<uintptr_t>(p) % 16) {
+            set_error("%s: cache codes must be 16-byte aligned", op);
+            return false;
+        }
+    for (const void *p : {static_cast<const void *>(c->k_scale), static_cast<const void *>(c->v_scale),
+                          static_cast<const void *>(b->table), static_cast<const void *>(b->row_start),
+                          static_cast<const void *>(b->kv_len)})
+        if (reinterpret_cast<uintptr_t>(p) % 4) {
+            set_error("%s: scales, table, row_start and kv_len must be 4-byte aligned", op);
+            return false;
+        }
+    if (b->n_seqs < 0 || b->n_rows < 0 || b->max_rows < 0 || b->table_width < 1 || b->max_len < 0 ||
+        b->n_seqs > (1 << 20) || b->n_rows > (1 << 27) || b->max_len > (1 << 30) || b->table_width > (1 << 30)) {
+        set_error("%s: bad batch: %d sequences, %d rows (at most %d a sequence), table width %lld, max_len %lld", op,
+                  b->n_seqs, b->n_rows, b->max_rows, (long long)b->table_width, (long long)b->max_len);
+        return false;
+    }
+    int lg = 4;
+    while ((1 << lg) < c->page_tokens) ++lg;
+    cv = KvView{{static_cast<int8_t *>(c->k_codes), static_cast<int8_t *>(c->v_codes)},
+                {c->k_scale, c->v_scale}, c->n_pages, c->n_kv_heads, lg, c->head_dim};
+    bv = KvRows{b->table, b->row_start, b->kv_len, b->table_width, b->n_seqs, b->n_rows, b->max_rows, b->max_len};
+    return true;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int sam3b200_kv_write(sam3b200_backend *h, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch,
+                                 int type, const void *k, const int64_t *k_nb, const void *v, const int64_t *v_nb) {
+    auto *be = reinterpret_cast<Backend *>(h);
+    WriteArgs a;
+    if (!kv_views("kv_write", cache, batch, a.c, a.b)) return SAM3B200_STATUS_FAILED;
+    const int bytes = type_bytes(type);
+    if (!k || !v || !bytes || reinterpret_cast<uintptr_t>(k) % bytes || reinterpret_cast<uintptr_t>(v) % bytes) {
+        if (!k || !v) set_error("kv_write: null argument");
+        else set_error("kv_write: unsupported type %d (F32=0, F16=1, BF16=30) or unaligned rows", type);
+        return SAM3B200_STATUS_FAILED;
+    }
+    a.x[0] = k, a.x[1] = v;
+    a.xs[0] = row_tensor(k, type, k_nb, a.c.heads, a.c.D);
+    a.xs[1] = row_tensor(v, type, v_nb, a.c.heads, a.c.D);
+    if (!rows_ok("kv_write", "k", a.xs[0], a.b.n_rows, a.c.heads, a.c.D, false) ||
+        !rows_ok("kv_write", "v", a.xs[1], a.b.n_rows, a.c.heads, a.c.D, false))
+        return SAM3B200_STATUS_FAILED;
+    if (!be) {
+        set_error("kv_write: null backend");
+        return SAM3B200_STATUS_FAILED;
+    }
+    if (a.b.n_seqs == 0 || a.b.n_rows == 0) return SAM3B200_STATUS_SUCCESS;
+    a.err = be->err;
+    DeviceScope dev(be->device);
+    const dim3 grid((a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs, a.c.heads, 2);
+    const bool vec = a.xs[0].aligned16 && a.xs[1].aligned16;
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        if (vec) launch_write<T, true>(a, grid, be->stream);
+        else launch_write<T, false>(a, grid, be->stream);
+    };
+    if (type == SAM3B200_TYPE_F32) go(float());
+    else if (type == SAM3B200_TYPE_F16) go(__half());
+    else go(__nv_bfloat16());
+    be->count();
+    return cuda_ok(cudaGetLastError(), "kv_write launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
+}
+
+extern "C" int sam3b200_kv_read(sam3b200_backend *h, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch,
+                                int type, void *k, const int64_t *k_nb, void *v, const int64_t *v_nb) {
+    auto *be = reinterpret_cast<Backend *>(h);
+    ReadArgs a;
+    if (!kv_views("kv_read", cache, batch, a.c, a.b)) return SAM3B200_STATUS_FAILED;
+    const int bytes = type_bytes(type);
+    if (!k || !v || !bytes || reinterpret_cast<uintptr_t>(k) % bytes || reinterpret_cast<uintptr_t>(v) % bytes) {
+        if (!k || !v) set_error("kv_read: null argument");
+        else set_error("kv_read: unsupported type %d (F32=0, F16=1, BF16=30) or unaligned rows", type);
+        return SAM3B200_STATUS_FAILED;
+    }
+    a.y[0] = k, a.y[1] = v;
+    a.ys[0] = row_tensor(k, type, k_nb, a.c.heads, a.c.D);
+    a.ys[1] = row_tensor(v, type, v_nb, a.c.heads, a.c.D);
+    if (!rows_ok("kv_read", "k", a.ys[0], a.b.n_rows, a.c.heads, a.c.D, true) ||
+        !rows_ok("kv_read", "v", a.ys[1], a.b.n_rows, a.c.heads, a.c.D, true))
+        return SAM3B200_STATUS_FAILED;
+    if (!be) {
+        set_error("kv_read: null backend");
+        return SAM3B200_STATUS_FAILED;
+    }
+    if (a.b.n_seqs == 0 || a.b.n_rows == 0) return SAM3B200_STATUS_SUCCESS;
+    a.err = be->err;
+    DeviceScope dev(be->device);
+    const dim3 grid((a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs, a.c.heads, 2);
+    const bool vec = a.ys[0].aligned16 && a.ys[1].aligned16;
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        if (vec) kv_read_kernel<T, true><<<grid, 128, 0, be->stream>>>(a);
+        else kv_read_kernel<T, false><<<grid, 128, 0, be->stream>>>(a);
+    };
+    if (type == SAM3B200_TYPE_F32) go(float());
+    else if (type == SAM3B200_TYPE_F16) go(__half());
+    else go(__nv_bfloat16());
+    be->count();
+    return cuda_ok(cudaGetLastError(), "kv_read launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
+}

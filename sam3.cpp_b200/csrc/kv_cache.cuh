@@ -1,0 +1,183 @@
+// kv_cache.cuh -- the paged 8-bit key/value cache as its kernels see it: the
+// device views of sam3b200_kv_cache and sam3b200_kv_batch, how a kernel finds
+// its sequence, and the host checks shared by the entry points.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/sam3_b200.h"
+#include "backend_impl.h"
+
+namespace b200 {
+
+// Bits of the backend's error word (read by sam3b200_backend_synchronize).
+constexpr int kErrKvPage = 1 << 21;   // a block table names a page outside [0, n_pages)
+constexpr int kErrKvBatch = 1 << 22;  // row_start / kv_len contradict the batch's sizes
+
+// Pages whose largest magnitude is below this store zeros under scale 0, so
+// that reciprocals of scales stay finite.
+constexpr float kKvSmallest = 7.888609052210118e-31f;  // 2^-100
+
+struct KvView {
+    int8_t *codes[2];  // keys, values: [n_pages][heads][1 << page_log2][D]
+    float *scale[2];   // [n_pages][heads]
+    int n_pages, heads, page_log2, D;
+};
+
+struct KvRows {
+    const int32_t *table, *row_start, *kv_len;
+    int64_t table_width;
+    int n_seqs, n_rows, max_rows;
+    int64_t max_len;
+};
+
+// One sequence of the batch, with its numbers cut to what the buffers hold:
+// rows [r0, r0 + n) of the row tensors, len cached tokens.
+struct KvSeq {
+    int s, r0, n;
+    int len;
+};
+
+__device__ __forceinline__ KvSeq kv_seq(const KvRows &b, int s, int page_log2) {
+    KvSeq q;
+    q.s = s;
+    q.r0 = min(max(b.row_start[s], 0), b.n_rows);
+    q.n = min(max(b.row_start[s + 1], q.r0), b.n_rows) - q.r0;
+    const int64_t cap = min(b.table_width << page_log2, b.max_len);
+    q.len = static_cast<int>(min(static_cast<int64_t>(max(b.kv_len[s], 0)), cap));
+    return q;
+}
+
+// Checks every sequence against the sizes that the host gave and records
+// kErrKvBatch; one block of a launch runs it.
+__device__ __forceinline__ void kv_check(const KvRows &b, int page_log2, bool rows_are_cached, int *err) {
+    for (int s = threadIdx.x; s < b.n_seqs; s += blockDim.x) {
+        const int64_t r0 = b.row_start[s], r1 = b.row_start[s + 1], len = b.kv_len[s];
+        if (r0 < 0 || r1 < r0 || r1 > b.n_rows || r1 - r0 > b.max_rows || len < 0 || len > b.max_len ||
+            len > (b.table_width << page_log2) || (rows_are_cached && r1 - r0 > len))
+            atomicOr(err, kErrKvBatch);
+    }
+}
+
+// Work is cut into units of `unit` consecutive items of a sequence that has
+// items [row_start[s] m, row_start[s + 1] m).  Sequence s starts at unit
+// first(s) = floor(row_start[s] m / unit) + spare s, which leaves it at least
+// floor(n m / unit) + spare units; the launch has first(n_seqs) of them.  The
+// block's threads count the sequences that start at or before unit u.
+// Every thread of the block calls this.  Returns the sequence, or -1;
+// `local` is the unit's number within it.
+__device__ __forceinline__ int kv_find(const KvRows &b, int64_t u, int m, int unit_log2, int spare, int64_t &local) {
+    int before = 0;
+    for (int base = 0; base < b.n_seqs; base += blockDim.x) {
+        const int s = base + threadIdx.x;
+        int in = 0;
+        if (s < b.n_seqs)
+            in = ((static_cast<int64_t>(max(b.row_start[s], 0)) * m) >> unit_log2) + static_cast<int64_t>(spare) * s <= u;
+        before += __syncthreads_count(in);
+    }
+    if (before == 0) return -1;
+    const int s = before - 1;
+    local = u - (((static_cast<int64_t>(max(b.row_start[s], 0)) * m) >> unit_log2) + static_cast<int64_t>(spare) * s);
+    return local < 0 ? -1 : s;  // only starts that fall (kErrKvBatch) give a negative number
+}
+
+// The page of tokens [i << page_log2, ...) of sequence s; a bad entry is
+// recorded and reads as -1.
+__device__ __forceinline__ int kv_page(const KvView &c, const KvRows &b, int s, int64_t i, int *err) {
+    const int p = b.table[s * b.table_width + i];
+    if (p >= 0 && p < c.n_pages) return p;
+    atomicOr(err, kErrKvPage);
+    return -1;
+}
+
+__device__ __forceinline__ int64_t kv_slab(const KvView &c, int page, int head) {
+    return ((static_cast<int64_t>(page) * c.heads + head) << c.page_log2) * c.D;
+}
+
+// ---- element types ------------------------------------------------------------
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Eight consecutive elements; VEC: p is 16-byte aligned.
+template <bool VEC, typename T>
+__device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
+    if constexpr (VEC) {
+        uint4 raw[sizeof(T) / 2];
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = reinterpret_cast<const uint4 *>(p)[i];
+        const T *e = reinterpret_cast<const T *>(raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+    }
+}
+
+template <bool VEC, typename T>
+__device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
+    if constexpr (VEC) {
+        uint4 raw[sizeof(T) / 2];
+        T *e = reinterpret_cast<T *>(raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4 *>(p)[i] = raw[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = from_f32<T>(x[i]);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------
+
+// Makes `device` current for the scope and restores the caller's device.
+struct DeviceScope {
+    int prev = -1;
+    explicit DeviceScope(int device) {
+        if (cudaGetDevice(&prev) != cudaSuccess || prev == device) prev = -1;
+        else cudaSetDevice(device);
+    }
+    ~DeviceScope() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope &operator=(const DeviceScope &) = delete;
+};
+
+inline int type_bytes(int type) {
+    return type == SAM3B200_TYPE_F32 ? 4 : type == SAM3B200_TYPE_F16 || type == SAM3B200_TYPE_BF16 ? 2 : 0;
+}
+
+// Rows of [rows][heads][D] elements given by the element strides nb (token,
+// head; NULL: packed).  aligned16: every 8-element group starts on 16 bytes.
+struct RowTensor {
+    int64_t token, head;
+    bool aligned16;
+};
+inline RowTensor row_tensor(const void *p, int type, const int64_t *nb, int64_t heads, int64_t D) {
+    RowTensor t{nb ? nb[0] : heads * D, nb ? nb[1] : D, false};
+    const int64_t b = type_bytes(type);
+    t.aligned16 = reinterpret_cast<uintptr_t>(p) % 16 == 0 && t.token * b % 16 == 0 && t.head * b % 16 == 0;
+    return t;
+}
+
+// Host check of a row tensor's strides (`written`: no element may lie twice in it).
+bool rows_ok(const char *op, const char *what, const RowTensor &t, int64_t rows, int64_t heads, int64_t D, bool written);
+// Host checks of a cache and a batch; on failure the message names `op`.
+bool kv_views(const char *op, const sam3b200_kv_cache *c, const sam3b200_kv_batch *b, KvView &cv, KvRows &bv);
+
+}  // namespace b200
