@@ -499,7 +499,8 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
     a.causal = causal != 0, a.window = static_cast<int>(std::min<int64_t>(window, 0x7fffffff));
     a.part = k->part, a.done = k->done, a.err = k->be->err;
     DeviceScope dev(k->be->device);
-    const cudaError_t e = kv_attn_few(a, k->be->num_sms, k->be->stream);
+    const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= kFewRows;
+    const cudaError_t e = few ? kv_attn_few(a, k->be->num_sms, k->be->stream) : kv_attn_tc(a, k->be->stream);
     k->be->count();
     return cuda_ok(e, "kv_attention launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
 }

@@ -55,6 +55,7 @@ __device__ __forceinline__ void kv_store8(const KvAttnArgs &a, int64_t at, const
     else put(static_cast<__nv_bfloat16 *>(a.y));
 }
 
-cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st);
+cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st);  // kv_attn.cu: 16 rows a block
+cudaError_t kv_attn_tc(const KvAttnArgs &a, cudaStream_t st);          // kv_attn_tc.cu: 256 rows a block
 
 }  // namespace b200
