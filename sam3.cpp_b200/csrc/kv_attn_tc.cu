@@ -5,11 +5,12 @@
 // A block owns 256 query rows of one kv head (the group's query heads times
 // tokens) as two tiles of 128 and streams the keys in tiles of 128 tokens.
 //   warps 0-7:  softmax, one thread a row; warps 0-3 tile 0, 4-7 tile 1;
-//   warps 8-11: read the codes (16 bytes a lane straight from the pages, the
-//               next tile's in registers meanwhile) and write them as f16,
-//               exactly, into 128-byte-swizzled shared memory, and each 16
-//               tokens' scales beside them;
-//   warp 12:    issues the MMAs (13-15 only give their registers away): S_t(j) = Q_t K_j^T, and once softmax t has
+//   warps 8-11: read the keys' codes (16 bytes a lane straight from the
+//               pages, the next tile's in registers meanwhile) and write them
+//               as f16, exactly, into 128-byte-swizzled shared memory, and
+//               each 16 tokens' scales beside them;
+//   warps 12-15: the same for the values;
+//   warp 16:    issues the MMAs (17-19 only give their registers away): S_t(j) = Q_t K_j^T, and once softmax t has
 //               written its weights over S_t(j), O_t += P_t(j) V_j and
 //               S_t(j + 1).  One tile's products run under the other's
 //               softmax.
@@ -29,10 +30,10 @@ namespace {
 
 enum { TERR_Q = 1 << 8, TERR_K = 1 << 9, TERR_V = 1 << 10, TERR_FREE = 1 << 11, TERR_S = 1 << 12, TERR_P = 1 << 13 };
 
-// Registers a thread after the split: a block starts with 128 for each of its
-// four warpgroups, and the shares may not add up to more.
-constexpr int kRegsStart = 128, kRegsSoftmax = 176, kRegsCodes = 104, kRegsMma = 56;
-static_assert(2 * kRegsSoftmax + kRegsCodes + kRegsMma <= 4 * kRegsStart, "register shares");
+// Registers a thread after the split: a block starts with 96 for each of its
+// five warpgroups, and the shares may not add up to more.
+constexpr int kRegsStart = 96, kRegsSoftmax = 144, kRegsCodes = 72, kRegsMma = 48;
+static_assert(2 * kRegsSoftmax + 2 * kRegsCodes + kRegsMma <= 5 * kRegsStart, "register shares");
 
 template <int REGS>
 __device__ __forceinline__ void take_regs() {
@@ -46,13 +47,13 @@ __device__ __forceinline__ void give_regs() {
 template <int D>
 struct Tc {
     static constexpr int kRows = 256, kKeys = 128;
-    static constexpr int kThreads = 16 * 32;
+    static constexpr int kThreads = 20 * 32;
     static constexpr int kHalf = kKeys * 128;             // 64 dimensions of 128 rows
     static constexpr int kTile = kHalf * (D / 64);        // f16 tile of 128 rows
     static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile, kScales = 6 * kTile;
-    static constexpr int kScaleSlots = 4;                 // a slot is written again three key tiles later
+    static constexpr int kScaleSlots = 4;                 // see sc_full
     static constexpr int kBars = kScales + kScaleSlots * 8 * 16;
-    static constexpr int kSmem = kBars + 128 + 1024;      // + alignment
+    static constexpr int kSmem = kBars + 256 + 1024;      // + alignment
 };
 
 __device__ __forceinline__ uint32_t f16_codes(uint32_t w, uint32_t sel) {
@@ -84,6 +85,15 @@ __device__ __forceinline__ uint64_t sw128_nmajor_desc(uint32_t smem_addr, uint32
            (static_cast<uint64_t>(next_n >> 4) << 16);
 }
 
+// Waits for a tcgen05.ld of 16 columns; the registers pass through, so that no use of them moves in front.
+__device__ __forceinline__ void wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
 // The softmax constants of 16 tokens: ks scale log2(e), log2(vs), 1 / vs.
 struct Scales {
     float k, lv, inv_v, pad;
@@ -95,18 +105,21 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + C::kBars);
-    uint64_t *k_full = q_full + 1;       // [2] keys of tile j in slot j % 2, and their scales
+    uint64_t *k_full = q_full + 1;       // [2] keys of tile j in slot j % 2
     uint64_t *v_full = k_full + 2;       // [2]
     uint64_t *pair_free = v_full + 2;    // [2] pair p = keys p and values p - 1: read by all their MMAs
     uint64_t *s_full = pair_free + 2;    // [2 tiles] phase j: S_t(j) and O_t up to j - 1 are in tensor memory
     uint64_t *p_full = s_full + 2;       // [2 tiles] phase j: P_t(j) is
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(p_full + 2);
+    // Scales of tile j, in slot j % 4: written again at tile j + 4, which waits for P_t(j + 1), so a slow softmax
+    // warp never sees its phase pass by (keys may run two tiles ahead of it: it must not wait on k_full).
+    uint64_t *sc_full = p_full + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sc_full + C::kScaleSlots);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kv = blockIdx.y, G = a.group;
-    if (blockIdx.x + blockIdx.y == 0) kv_check(a.b, a.c.page_log2, false, a.err);
+    const int kv = blockIdx.x % a.c.heads, G = a.group;
+    if (blockIdx.x == 0) kv_check(a.b, a.c.page_log2, false, a.err);
     int64_t local;
-    const int s = kv_find(a.b, gridDim.x - 1 - blockIdx.x, G, 8, 1, local);  // late rows, with the most keys, first
+    const int s = kv_find(a.b, (gridDim.x - 1 - blockIdx.x) / a.c.heads, G, 8, 1, local);  // late rows, with the most keys, first
     if (s < 0) return;
     const KvSeq q = kv_seq(a.b, s, a.c.page_log2);
     const int64_t R = static_cast<int64_t>(q.n) * G, row0 = local * C::kRows;
@@ -125,9 +138,10 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
         }
+        for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(&sc_full[i], 1);
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 16) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -136,81 +150,66 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp >= 8 && warp < 12) {
+    if (warp >= 8 && warp < 16) {
         // ---- codes -> f16 ----
         give_regs<kRegsCodes>();
-        const int w = warp - 8;
+        const int which = (warp - 8) >> 2, w = warp & 3;  // keys or values
         constexpr int kChunks = D / 16, kPer = C::kKeys * kChunks / 128;  // 16-code chunks a token, a thread
         constexpr int kTokens = 128 / kChunks;                            // tokens a step of all 128 threads
         const int token0 = (w * 32 + lane) / kChunks, chunk = lane % kChunks;
-        uint4 kx[kPer], vx[kPer];
-        // lane g < 8: the page of tokens 16 g ... of a tile, -1 behind the end
+        const int8_t *codes = a.c.codes[which] + static_cast<int64_t>(token0 & 15) * D + chunk * 16;
+        const bool scaling = which == 0 && w == 0 && lane < 8;  // lane g: the scales of tokens 16 g ...
+        uint4 x[kPer];
+        float ks = 0.f, vs = 0.f;
+        // lane g & 7: the page of tokens 16 g ... of tile j, -1 behind the end
         auto page_of = [&](int j) -> int {
             const int tok = k_begin + j * C::kKeys + (lane & 7) * 16;
             if (j >= ntiles || tok >= k_end) return -1;
             return max(kv_page(a.c, a.b, s, tok >> a.c.page_log2, a.err), 0);
         };
-        auto fetch = [&](int which, int j, int pages, uint4 (&x)[kPer]) {
+        auto fetch = [&](int j, int page) {
+            const int in_page = (k_begin + j * C::kKeys + (lane & 7) * 16) & ((1 << a.c.page_log2) - 1);
+            const int64_t at = page < 0 ? -1 : kv_slab(a.c, page, kv) + static_cast<int64_t>(in_page) * D;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                const int t = i * kTokens + token0;
-                const int page = __shfl_sync(0xffffffffu, pages, t >> 4);
-                const int in_page = (k_begin + j * C::kKeys + t) & ((1 << a.c.page_log2) - 1);
+                const int64_t from = __shfl_sync(0xffffffffu, at, (i * kTokens + token0) >> 4);
                 x[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (page >= 0)
-                    x[i] = __ldg(reinterpret_cast<const uint4 *>(a.c.codes[which] + kv_slab(a.c, page, kv) +
-                                                                 static_cast<int64_t>(in_page) * D + chunk * 16));
+                if (from >= 0) x[i] = __ldg(reinterpret_cast<const uint4 *>(codes + from));
+            }
+            if (scaling) {
+                const int64_t h = static_cast<int64_t>(max(page, 0)) * a.c.heads + kv;
+                ks = page < 0 ? 0.f : a.c.scale[0][h];
+                vs = page < 0 ? 0.f : a.c.scale[1][h];
             }
         };
-        auto put = [&](uint8_t *tile, const uint4 (&x)[kPer]) {
+        // Pair p of the pipeline is keys p and values p - 1: keys j reuse the slot of pair j - 2, values j that
+        // of pair j - 1 (values 1 wait without need, so that no phase is left out).  Pages are looked up two tiles ahead, codes and scales one.
+        uint64_t *full = which == 0 ? k_full : v_full;
+        uint8_t *slots = smem + (which == 0 ? C::kK : C::kV);
+        int page_next = page_of(1);
+        fetch(0, page_of(0));
+        for (int j = 0; j < ntiles; ++j) {
+            const int page_then = page_of(j + 2), pair = j - 2 + which;
+            if (pair >= 0 && !__all_sync(0xffffffffu, mbar_wait(&pair_free[pair & 1], (pair >> 1) & 1, a.err, TERR_FREE))) break;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) put_codes(tile, C::kHalf, i * kTokens + token0, chunk, x[i]);
-        };
-        auto scales = [&](int j, int pages) {  // lanes 0-7 of the first warp
-            if (w != 0 || lane >= 8) return;
-            Scales v{0.f, kZeroScaleLog2, 0.f, 0.f};
-            if (pages >= 0) {
-                const int64_t at = static_cast<int64_t>(pages) * a.c.heads + kv;
-                const float vs = a.c.scale[1][at];
-                v.k = a.c.scale[0][at] * a.scale_log2;
-                v.lv = vs > 0.f ? __log2f(vs) : kZeroScaleLog2;
+            for (int i = 0; i < kPer; ++i)
+                put_codes(slots + (j & 1) * C::kTile, C::kHalf, i * kTokens + token0, chunk, x[i]);
+            if (scaling) {
+                Scales v{ks * a.scale_log2, vs > 0.f ? __log2f(vs) : kZeroScaleLog2, 0.f, 0.f};
                 v.inv_v = ex2_approx(-v.lv);
+                reinterpret_cast<Scales *>(smem + C::kScales)[(j % C::kScaleSlots) * 8 + lane] = v;
             }
-            reinterpret_cast<Scales *>(smem + C::kScales)[(j % C::kScaleSlots) * 8 + lane] = v;
-        };
-        auto publish = [&](uint64_t *bar) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-        };
-        if (ntiles > 0) {
-            int pages = page_of(0), pages_next = page_of(1);
-            fetch(0, 0, pages, kx);
-            fetch(1, 0, pages, vx);
-            put(smem + C::kK, kx);
-            scales(0, pages);
-            publish(&k_full[0]);
-            fetch(0, 1, pages_next, kx);
-            for (int j = 0; j < ntiles; ++j) {  // keys j + 1, then values j; both slots were those of pair j - 1
-                if (j >= 1 && !__all_sync(0xffffffffu, mbar_wait(&pair_free[(j - 1) & 1], ((j - 1) >> 1) & 1, a.err, TERR_FREE)))
-                    break;
-                const int pages_then = page_of(j + 2);
-                if (j + 1 < ntiles) {
-                    put(smem + C::kK + ((j + 1) & 1) * C::kTile, kx);
-                    scales(j + 1, pages_next);
-                    publish(&k_full[(j + 1) & 1]);
-                    fetch(0, j + 2, pages_then, kx);
-                }
-                put(smem + C::kV + (j & 1) * C::kTile, vx);
-                publish(&v_full[j & 1]);
-                fetch(1, j + 1, pages_next, vx);
-                pages_next = pages_then;
-            }
+            if (lane == 0) mbar_arrive(&full[j & 1]);
+            if (lane == 0 && which == 0 && w == 0) mbar_arrive(&sc_full[j % C::kScaleSlots]);
+            fetch(j + 1, page_next);
+            page_next = page_then;
         }
-    } else if (warp >= 12) {
+    } else if (warp >= 16) {
         // ---- MMA issuer ----
         give_regs<kRegsMma>();
-        if (warp == 12) {
+        if (warp == 16) {
             constexpr uint32_t idesc_s = idesc_f16_f32(128, C::kKeys);
             constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // B is N-major
             auto mma_s = [&](int t, int j) {
@@ -326,55 +325,64 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
             bool ok = true;
             for (int j = 0; j < ntiles; ++j) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, a.err, TERR_S) &&
-                                                 mbar_wait(&k_full[j & 1], (j >> 1) & 1, a.err, TERR_K));
+                                                 mbar_wait(&sc_full[j % C::kScaleSlots], (j / C::kScaleSlots) & 1, a.err, TERR_K));
                 if (!ok) break;
                 tc_fence_after();
                 const Scales *sc = reinterpret_cast<const Scales *>(smem + C::kScales) + (j % C::kScaleSlots) * 8;
                 const int tok = k_begin + j * C::kKeys;
-                const bool edge = tok + C::kKeys - 1 > all_end || tok < all_begin;
-                // columns that the row sees: lo .. hi of this tile
-                const int hi = last - tok, lo = first - tok;
-                float top = -INFINITY;
-                auto max32 = [&](const uint32_t (&x)[32], int c) {
+                if (tok + C::kKeys - 1 > all_end || tok < all_begin) {
+                    // hidden scores become -inf in place; the row sees columns lo .. hi
+                    const int hi = last - tok, lo = first - tok;
+#pragma unroll 1
+                    for (int c = 0; c < C::kKeys; c += 32) {
+                        uint32_t x[32];
+                        tmem_ld_32x32b_x32(s_col + c, x);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const Scales v = sc[2 * c + g];
-                        const float k = v.k * row_c;
-                        if (!edge) {
-                            float mx = __uint_as_float(x[16 * g]);
-#pragma unroll
-                            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(x[16 * g + e]));
-                            top = fmaxf(top, fmaf(mx, k, v.lv));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const int col = 32 * c + 16 * g + e;
-                                const float y = fmaf(__uint_as_float(x[16 * g + e]), k, v.lv);
-                                if (col <= hi && col >= lo) top = fmaxf(top, y);
-                            }
-                        }
+                        for (int e = 0; e < 32; ++e)
+                            if (c + e > hi || c + e < lo) x[e] = 0xff800000u;
+                        tmem_st_32x32b_x32(s_col + c, x);
                     }
-                };
-                uint32_t x0[32], x1[32];
-                tmem_ld_32x32b_x32(s_col + 64, x0);
-                tmem_ld_32x32b_x32(s_col + 96, x1);
-                tmem_wait_ld();
-                max32(x0, 2);
-                max32(x1, 3);
-                tmem_ld_32x32b_x32(s_col, x0);
-                tmem_ld_32x32b_x32(s_col + 32, x1);
-                tmem_wait_ld();
-                max32(x0, 0);
-                max32(x1, 1);
-                float alpha = 1.f;
-                if (top > m + kLazy) {
-                    alpha = ex2_approx(m - top);
-                    m = top;
-                    l *= alpha;
+                    tmem_wait_st();
                 }
-                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {  // S_t(j) being there, P_t(j - 1) V is in O_t
+                // P for the maximum known so far; where a row passes it by more than kLazy (always in its first
+                // tile, rarely later) the maximum is raised and P formed again
+                uint32_t pk[C::kKeys / 2];
+                float sum = 0.f;
+                for (int pass = 0;; ++pass) {
+                    const float less = m == -INFINITY ? 0.f : m - kPUp;
+                    float top = -INFINITY;
+                    sum = 0.f;
+                    uint32_t x[2][16];
+                    tmem_ld_32x32b_x16(s_col, x[0]);
 #pragma unroll
-                    for (int c = 0; c < D; c += 32) {
+                    for (int g = 0; g < 8; ++g) {
+                        wait_ld16(x[g & 1]);
+                        if (g < 7) tmem_ld_32x32b_x16(s_col + 16 * (g + 1), x[(g + 1) & 1]);
+                        const Scales v = sc[g];
+                        // a factor of 0 (keys or scale 0) would make NaN of -inf; a tiny one leaves 0 of the others
+                        const float k = fmaxf(v.k * row_c, 1e-37f), b = v.lv - less;
+                        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            float y0 = b, y1 = b;
+                            ffma2(y0, y1, __uint_as_float(x[g & 1][e]), __uint_as_float(x[g & 1][e + 1]), k, k);
+                            top = fmaxf(top, fmaxf(y0, y1));
+                            y0 = ex2_approx(y0);
+                            y1 = ex2_approx(y1);
+                            fadd2(s0, s1, s0, s1, y0, y1);
+                            const __half2 h = __floats2half2_rn(y0, y1);
+                            pk[8 * g + e / 2] = *reinterpret_cast<const uint32_t *>(&h);
+                        }
+                        sum = fmaf(s0 + s1, v.inv_v, sum);
+                    }
+                    if (pass == 1 || !__any_sync(0xffffffffu, top > (m == -INFINITY ? -INFINITY : kPUp + kLazy))) break;
+                    const float to = fmaxf(m, top + less), alpha = m == to ? 1.f : ex2_approx(m - to);
+                    m = to;
+                    l *= alpha;
+                    if (j == 0) continue;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {  // S_t(j) being there, P_t(j - 1) V_(j - 1) is in O_t
                         uint32_t o[32];
                         tmem_ld_32x32b_x32(o_col + c, o);
                         tmem_wait_ld();
@@ -383,40 +391,14 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                         tmem_st_32x32b_x32(o_col + c, o);
                     }
                 }
-                const float less = m == -INFINITY ? 0.f : m - kPUp;
-                auto exp32 = [&](const uint32_t (&x)[32], int c) {
-                    uint32_t pk[16];
+                l += sum;
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const Scales v = sc[2 * c + g];
-                        const float k = v.k * row_c, b = v.lv - less;
-                        float s0 = 0.f, s1 = 0.f;
+                for (int c = 0; c < C::kKeys / 2; c += 16) {
+                    uint32_t part[16];
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            float y0 = b, y1 = b;
-                            ffma2(y0, y1, __uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]), k, k);
-                            if (edge) {
-                                const int col = 32 * c + 16 * g + e;
-                                if (col > hi || col < lo) y0 = -INFINITY;
-                                if (col + 1 > hi || col + 1 < lo) y1 = -INFINITY;
-                            }
-                            y0 = ex2_approx(y0);
-                            y1 = ex2_approx(y1);
-                            fadd2(s0, s1, s0, s1, y0, y1);
-                            const __half2 h = __floats2half2_rn(y0, y1);
-                            pk[8 * g + e / 2] = *reinterpret_cast<const uint32_t *>(&h);
-                        }
-                        l = fmaf(s0 + s1, v.inv_v, l);
-                    }
-                    tmem_st_32x32b_x16(s_col + 16 * c, pk);
-                };
-                exp32(x0, 0);
-                exp32(x1, 1);
-                tmem_ld_32x32b_x32(s_col + 64, x0);
-                tmem_ld_32x32b_x32(s_col + 96, x1);
-                tmem_wait_ld();
-                exp32(x0, 2);
-                exp32(x1, 3);
+                    for (int e = 0; e < 16; ++e) part[e] = pk[c + e];
+                    tmem_st_32x32b_x16(s_col + c, part);
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -448,7 +430,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12) tmem_dealloc(tmem, 512);
+    if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 template <int D>
@@ -460,7 +442,7 @@ cudaError_t launch_tc(const KvAttnArgs &a, int64_t units, cudaStream_t st) {
     e = cudaFuncGetAttributes(&f, kv_attn_tc_kernel<D>);
     if (e != cudaSuccess) return e;
     if (f.numRegs < kRegsStart) return cudaErrorInvalidConfiguration;
-    kv_attn_tc_kernel<D><<<dim3(static_cast<unsigned>(units), a.c.heads), C::kThreads, C::kSmem, st>>>(a);
+    kv_attn_tc_kernel<D><<<static_cast<unsigned>(units * a.c.heads), C::kThreads, C::kSmem, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -468,7 +450,7 @@ cudaError_t launch_tc(const KvAttnArgs &a, int64_t units, cudaStream_t st) {
 
 cudaError_t kv_attn_tc(const KvAttnArgs &a, cudaStream_t st) {
     const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 8) + a.b.n_seqs;
-    if (units > 0x7fffffff) return cudaErrorInvalidValue;
+    if (units * a.c.heads > 0x7fffffff) return cudaErrorInvalidValue;
     return a.c.D == 64 ? launch_tc<64>(a, units, st) : launch_tc<128>(a, units, st);
 }
 
