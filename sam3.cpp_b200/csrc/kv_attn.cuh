@@ -29,7 +29,7 @@ struct KvAttnArgs {
 constexpr float kPUp = 7.f, kLazy = 8.f;
 
 // Scale of a value page that holds only zeros, as the softmax weights see it.
-constexpr float kZeroScaleLog2 = -107.f;
+constexpr float kZeroScaleLog2 = -80.f;
 
 // The device workspace of a handle.
 constexpr int kMaxParts = 4096;
