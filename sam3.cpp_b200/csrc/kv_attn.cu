@@ -10,17 +10,19 @@
 // a page's value scale moves into the exponent, p stays in [0, 1] for f16
 // whatever the scales are, and no other step sees them.
 //
-// kv_attn_few: one block of 4 warps per (16 query rows of a kv head, part of
-// the key range).  The rows are the query heads of the group, times the
-// sequence's new tokens.  Each warp takes every fourth block of 16 tokens
+// kv_attn_few: one block of 4 warps per (8 or 16 query rows of a kv head,
+// part of the key range).  The rows are the query heads of the group, times
+// the sequence's new tokens.  Each warp takes every fourth block of 16 tokens
 // (never across a page), copies it by cp.async into its own ring of shared
 // memory, and multiplies by mma.m16n8k16 f16 with f32 sums: bound by memory
-// (1 byte per code, 4 D flops per code and 16 rows), the legacy matrix
-// instruction is wide enough, and its register layout lets a lane read 16
-// codes of a token at once and hand the softmax weights on without a shuffle.
-// Dimensions are permuted in both products so that every lane's codes lie
-// together.  The warps' partial results are joined through shared memory, the
-// parts' through the workspace by the last block to finish.
+// (1 byte per code), the legacy matrix instruction is wide enough.  The codes
+// are its 16-row operand and the queries its 8 columns: S^T = K Q^T, then
+// O^T = V^T P^T, so one token a sequence and up to 8 query heads a kv head
+// fill an instruction.  Dimensions are permuted in both products so that a
+// lane reads 16 codes of a token at once, and P^T goes from the first
+// product's layout to the second's by movmatrix.  The warps' partial results
+// are joined through shared memory, the parts' through the workspace by the
+// last block to finish.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -31,7 +33,7 @@
 namespace b200 {
 namespace {
 
-constexpr int kWarps = 4, kStages = 4;
+constexpr int kWarps = 4;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -46,10 +48,17 @@ __device__ __forceinline__ void cp_wait() {
 }
 
 // d += a b: a 16 x 16 (rows), b 16 x 8, f16 in, f32 sums.
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An 8 x 8 matrix of f16, a row's pair of columns a lane, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 // Bytes i and j of w (codes + 128) as f16: 0x64uu is 1024 + u, exactly.
@@ -80,29 +89,34 @@ __device__ __forceinline__ void load_q4(const KvAttnArgs &a, int64_t at, float (
         x[i] = a.q_bf16 ? __uint_as_float(static_cast<uint32_t>(e[i]) << 16) : __half2float(__ushort_as_half(e[i]));
 }
 
-template <int D>
+// NT tiles of 8 query rows.
+template <int D, int NT>
 struct Few {
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kStages = NT == 1 ? 3 : 4, kBlocks = NT == 1 ? 4 : 3;  // stages of a warp, blocks an SM
     static constexpr int kBlockBytes = 16 * D;                       // codes of 16 tokens
     static constexpr int kStageBytes = 2 * kBlockBytes + 16;         // keys, values, their two scales
     static constexpr int kRing = kWarps * kStages * kStageBytes;
-    static constexpr int kLane = D / 4;                              // output dimensions of a lane
-    static constexpr int kRowFloats = D + 16;                        // a merged row, padded against bank conflicts
-    static constexpr int kMerge = kWarps * kFewRows * kRowFloats * 4;
-    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
-    // 16-byte chunk c of token t within a staged block.  The permutation keeps both reads free of bank
-    // conflicts: keys (8 lanes: 2 neighbouring tokens, 4 chunks) and values (8 lanes: 4 token pairs, 2 chunks).
-    static __device__ __forceinline__ int chunk(int t, int c) {
-        if (D == 128) return t * 8 + (c ^ (t & 6) ^ ((t & 1) << 2));
-        return (t >> 1) * 8 + ((((t & 1) << 2) | c) ^ (t & 6));
+    static constexpr int kLane = D / 8;                              // output dimensions of a lane
+    static constexpr int kRowFloats = D + 36;                        // a joined row, padded against bank conflicts
+    static constexpr int kJoin = kWarps * kRows * kRowFloats * 4;
+    static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+    static constexpr int kEach = D * kRows / 128 > 8 ? D * kRows / 128 : 8;  // dimensions of a thread that joins
+    // Byte of 16-byte chunk c of token t within a staged block.  The permutation keeps the reads free of bank
+    // conflicts: keys (8 lanes: 2 neighbouring tokens, 4 chunks), values (8 lanes: 4 token pairs, 2 chunks).  Where
+    // a lane's tokens or chunks differ by a constant the byte differs by a sum or by ^ 64, which the loops below use.
+    static __device__ __forceinline__ uint32_t at(int t, int c) {
+        if (D == 128) return t * 128 + (c ^ (t & 6) ^ ((t & 1) << 2)) * 16;
+        return (t >> 1) * 128 + ((((t & 1) << 2) | c) ^ (t & 6)) * 16;
     }
     static __device__ __forceinline__ int padded(int d) { return d + d / kLane * 4; }
 };
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __grid_constant__ KvAttnArgs a) {
-    using F = Few<D>;
+template <int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_few_kernel(const __grid_constant__ KvAttnArgs a) {
+    using F = Few<D, NT>;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float s_m[kWarps][kFewRows], s_l[kWarps][kFewRows];
+    __shared__ float s_m[kWarps][F::kRows], s_l[kWarps][F::kRows];
     __shared__ int s_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int kv = blockIdx.y, G = a.group;
@@ -110,12 +124,11 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __gri
     const int split = blockIdx.x % a.splits;
     if (blockIdx.x + blockIdx.y == 0) kv_check(a.b, a.c.page_log2, false, a.err);
     int64_t local;
-    const int s = kv_find(a.b, unit, G, 4, 1, local);
-    if (s < 0) return;
-    const KvSeq q = kv_seq(a.b, s, a.c.page_log2);
-    const int64_t R = static_cast<int64_t>(q.n) * G, row0 = local * kFewRows;
+    KvSeq q;
+    if (!kv_find(a.b, unit, G, NT == 1 ? 3 : 4, 1, a.c.page_log2, q, local)) return;
+    const int64_t R = static_cast<int64_t>(q.n) * G, row0 = local * F::kRows;
     if (row0 >= R) return;
-    const int i_lo = static_cast<int>(row0 / G), i_hi = static_cast<int>((min(row0 + kFewRows, R) - 1) / G);
+    const int i_lo = static_cast<int>(row0 / G), i_hi = static_cast<int>((min(row0 + F::kRows, R) - 1) / G);
 
     // the tile's keys, and this block's part of them
     const int k_end = kv_last(a, q, i_hi) + 1, k_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
@@ -127,58 +140,18 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __gri
     const int n_blocks = t_end > t_begin ? (t_end - t_begin + 15) / 16 : 0;
     const int mine = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;  // blocks warp, warp + 4, ...
 
-    // queries: rows g and g + 8, for each 16-wide step the 4 dimensions that go with this lane's codes
-    uint32_t qf[D / 16][4];
-    float row_c[2];
-    int last[2], first[2];
-    {
-        float x[2][D / 16][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t r = row0 + g + 8 * h;
-            const int i = static_cast<int>(r / G);
-            const int64_t at = (q.r0 + static_cast<int64_t>(i)) * a.qs.token + (kv * G + r % G) * a.qs.head;
-            last[h] = kv_last(a, q, i);
-            first[h] = kv_first(a, last[h]);
-            float top = 0.f;
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                if (r < R) load_q4(a, at + (k >> 2) * 64 + c * 16 + (k & 3) * 4, x[h][k]);
-                else x[h][k][0] = x[h][k][1] = x[h][k][2] = x[h][k][3] = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[h][k][j]));
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // bf16 rows are brought to [1, 2) by a power of two, which f16 then holds to 2^-25 of the largest
-            const int e = a.q_bf16 ? min((__float_as_int(top) >> 23) & 0xff, 253) : 0;
-            const float down = e ? __int_as_float((254 - e) << 23) : 1.f;
-            row_c[h] = a.scale_log2 * (e ? __int_as_float(e << 23) : 1.f);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[h][k][j] *= down;
-        }
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-            qf[k][0] = pack_f16(x[0][k][0], x[0][k][1]);
-            qf[k][1] = pack_f16(x[1][k][0], x[1][k][1]);
-            qf[k][2] = pack_f16(x[0][k][2], x[0][k][3]);
-            qf[k][3] = pack_f16(x[1][k][2], x[1][k][3]);
-        }
-    }
-    // tokens that some row of the tile does not see
-    const int seen_by_all = kv_last(a, q, i_lo), window_end = kv_first(a, kv_last(a, q, i_hi));
-
-    uint8_t *ring = smem + warp * kStages * F::kStageBytes;
+    uint8_t *ring = smem + warp * F::kStages * F::kStageBytes;
+    // this lane's bytes within a stage: the copy of chunk lane (of 32 a step), keys of token g, values of token 2 c
+    const uint32_t put0 = F::at(lane / (D / 16), lane % (D / 16)), key0 = F::at(g, c);
+    const uint32_t val0 = D == 128 ? F::at(2 * c, g) : F::at(2 * c, g >> 1) + (g & 1) * 8;
     int page_now = 0, page_next = 0;  // lane j: the page of block 32 b + j of this warp, for batches b and b + 1
     auto load_page = [&](int j) -> int {
         if (j >= mine) return 0;
-        const int p = kv_page(a.c, a.b, s, (t_begin + (j * kWarps + warp) * 16) >> a.c.page_log2, a.err);
+        const int p = kv_page(a.c, a.b, q.s, (t_begin + (j * kWarps + warp) * 16) >> a.c.page_log2, a.err);
         return max(p, 0);
     };
     page_next = load_page(lane);
-    auto issue = [&](int j) {  // block j of this warp into its slot
+    auto issue = [&](int j, int slot) {  // block j of this warp into a slot
         if (j < mine) {
             if ((j & 31) == 0) {
                 page_now = page_next;
@@ -186,99 +159,154 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __gri
             }
             const int page = __shfl_sync(0xffffffffu, page_now, j & 31);
             const int tok = t_begin + (j * kWarps + warp) * 16;
-            const int64_t at = kv_slab(a.c, page, kv) + static_cast<int64_t>(tok & ((1 << a.c.page_log2) - 1)) * D;
-            const uint32_t dst = smem_u32(ring + (j % kStages) * F::kStageBytes);
+            const int64_t at = kv_slab(a.c, page, kv) + static_cast<int64_t>(tok & ((1 << a.c.page_log2) - 1)) * D + lane * 16;
+            const uint32_t dst = smem_u32(ring + slot * F::kStageBytes);
 #pragma unroll
             for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int k = 0; k < F::kBlockBytes / 512; ++k) {
-                    const int e = k * 32 + lane;  // 16-byte chunk of the block
-                    cp16(dst + w * F::kBlockBytes + F::chunk(e / (D / 16), e % (D / 16)) * 16, a.c.codes[w] + at + e * 16);
+                    // a step of 4 (D = 128) or 8 tokens
+                    const uint32_t to = (D == 128 && (k & 1) ? put0 ^ 64 : put0) + k * 512;
+                    cp16(dst + w * F::kBlockBytes + to, a.c.codes[w] + at + k * 512);
                 }
             if (lane < 2) cp4(dst + 2 * F::kBlockBytes + lane * 4, a.c.scale[lane] + static_cast<int64_t>(page) * a.c.heads + kv);
         }
         cp_commit();
     };
-    for (int j = 0; j < kStages - 1; ++j) issue(j);
-
-    float o[D / 8][4];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int j = 0; j < F::kStages - 1; ++j) issue(j, j);
 
+    // queries: row 8 n + g, for each 16-wide step the 4 dimensions that go with this lane's codes
+    uint32_t qf[NT][D / 16][2];
+    float row_c[NT][2];  // for rows 8 n + 2 c, + 1: scale log2(e), and what the power of two below took
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int64_t r = row0 + 8 * n + g;
+        const int64_t at = (q.r0 + r / G) * a.qs.token + (kv * static_cast<int64_t>(G) + r % G) * a.qs.head;
+        float x[D / 16][4], top = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
+            if (r < R) load_q4(a, at + (k >> 2) * 64 + c * 16 + (k & 3) * 4, x[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[k][j]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // bf16 rows are brought to [1, 2) by a power of two, which f16 then holds to 2^-25 of the largest
+        const int e = a.q_bf16 ? min((__float_as_int(top) >> 23) & 0xff, 253) : 0;
+        const float down = e ? __int_as_float((254 - e) << 23) : 1.f, up = a.scale_log2 * (e ? __int_as_float(e << 23) : 1.f);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            qf[n][k][0] = pack_f16(x[k][0] * down, x[k][1] * down);
+            qf[n][k][1] = pack_f16(x[k][2] * down, x[k][3] * down);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) row_c[n][j] = __shfl_sync(0xffffffffu, up, (2 * c + j) * 4);
+    }
+    // tokens that some row of the tile does not see
+    const int seen_by_all = kv_last(a, q, i_lo), window_end = kv_first(a, kv_last(a, q, i_hi));
+
+    float o[NT][D / 16][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+
+    int slot = 0, slot_in = F::kStages - 1;
     for (int j = 0; j < mine; ++j) {
-        cp_wait<kStages - 2>();
-        __syncwarp();
-        issue(j + kStages - 1);
-        const uint8_t *st = ring + (j % kStages) * F::kStageBytes;
-        const uint4 *kc = reinterpret_cast<const uint4 *>(st), *vc = reinterpret_cast<const uint4 *>(st + F::kBlockBytes);
-        const float ks = *reinterpret_cast<const float *>(st + 2 * F::kBlockBytes);
-        const float vs = *reinterpret_cast<const float *>(st + 2 * F::kBlockBytes + 4);
+        cp_wait<F::kStages - 2>();
+        __syncwarp();  // block j is there for all lanes, and block j - 1 is read by all
+        issue(j + F::kStages - 1, slot_in);
+        const uint8_t *st = ring + slot * F::kStageBytes;
+        slot_in = slot;
+        slot = slot + 1 == F::kStages ? 0 : slot + 1;
 
-        // scores of tokens 2c, 2c + 1 (n = 0) and 8 + 2c, 9 + 2c (n = 1) for rows g, g + 8
-        float t[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        // scores of tokens g (t[n][0], [1]) and g + 8 ([2], [3]) for rows 8 n + 2 c, + 1
+        float t[NT][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NT; ++n) t[n][0] = t[n][1] = t[n][2] = t[n][3] = 0.f;
 #pragma unroll
-            for (int h = 0; h < D / 64; ++h) {
-                const uint4 w4 = kc[F::chunk(8 * n + g, 4 * h + c)];
-                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t u = w[k] ^ 0x80808080u;
-                    mma16816(t[n], qf[4 * h + k], codes2<0x4140>(u), codes2<0x4342>(u));
-                }
-            }
-        const float lv = vs > 0.f ? __log2f(vs) : kZeroScaleLog2, inv_vs = ex2_approx(-lv);
-        const float cs[2] = {row_c[0] * ks, row_c[1] * ks};
-        const int tok = t_begin + (j * kWarps + warp) * 16;
-        const bool edge = tok + 15 > seen_by_all || tok < window_end;
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int h = 0; h < D / 64; ++h) {
+            const uint4 lo = *reinterpret_cast<const uint4 *>(st + (h ? key0 ^ 64 : key0));
+            const uint4 hi = *reinterpret_cast<const uint4 *>(st + (h ? key0 ^ 64 : key0) + 8 * D);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int h = k >> 1, key = tok + 8 * n + 2 * c + (k & 1);
-                t[n][k] = fmaf(t[n][k], cs[h], lv);
-                if (edge && (key > last[h] || key < first[h])) t[n][k] = -INFINITY;
-                top[h] = fmaxf(top[h], t[n][k]);
-            }
-        if (__any_sync(0xffffffffu, top[0] > m[0] + kLazy || top[1] > m[1] + kLazy)) {
+                const uint32_t u = (k == 0 ? lo.x : k == 1 ? lo.y : k == 2 ? lo.z : lo.w) ^ 0x80808080u;
+                const uint32_t v = (k == 0 ? hi.x : k == 1 ? hi.y : k == 2 ? hi.z : hi.w) ^ 0x80808080u;
+                const uint32_t a0 = codes2<0x4140>(u), a1 = codes2<0x4140>(v), a2 = codes2<0x4342>(u), a3 = codes2<0x4342>(v);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-                const float to = fmaxf(m[h], top[h]);
-                const float alpha = m[h] == to ? 1.f : ex2_approx(m[h] - to);
-                m[h] = to;
-                l[h] *= alpha;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) o[i][2 * h] *= alpha, o[i][2 * h + 1] *= alpha;
+                for (int n = 0; n < NT; ++n) mma16816(t[n], a0, a1, a2, a3, qf[n][4 * h + k][0], qf[n][4 * h + k][1]);
             }
         }
-        uint32_t p[4];
-        const float less[2] = {m[0] == -INFINITY ? 0.f : m[0] - kPUp, m[1] == -INFINITY ? 0.f : m[1] - kPUp};
+        const float2 ksvs = *reinterpret_cast<const float2 *>(st + 2 * F::kBlockBytes);
+        const float lv = ksvs.y > 0.f ? __log2f(ksvs.y) : kZeroScaleLog2, inv_vs = ex2_approx(-lv);
+        const int tok = t_begin + (j * kWarps + warp) * 16;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                t[n][k] = ex2_approx(t[n][k] - less[k >> 1]);
-                l[k >> 1] = fmaf(t[n][k], inv_vs, l[k >> 1]);
+            for (int k = 0; k < 4; ++k) t[n][k] = fmaf(t[n][k], row_c[n][k & 1] * ksvs.x, lv);
+        if (tok + 15 > seen_by_all || tok < window_end) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int i = static_cast<int>((row0 + 8 * n + 2 * c + k) / G), last = kv_last(a, q, i), first = kv_first(a, last);
+                    if (tok + g > last || tok + g < first) t[n][k] = -INFINITY;
+                    if (tok + g + 8 > last || tok + g + 8 < first) t[n][k + 2] = -INFINITY;
+                }
+        }
+        bool rise = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) rise |= fmaxf(t[n][k], t[n][k + 2]) > m[n][k] + kLazy;
+        if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float top = fmaxf(t[n][k], t[n][k + 2]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const float to = fmaxf(m[n][k], top);
+                    const float alpha = m[n][k] == to ? 1.f : ex2_approx(m[n][k] - to);
+                    m[n][k] = to;
+                    l[n][k] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) o[n][i][k] *= alpha, o[n][i][k + 2] *= alpha;
+                }
+        }
+        uint32_t p[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float less = m[n][k] == -INFINITY ? 0.f : m[n][k] - kPUp;
+                t[n][k] = ex2_approx(t[n][k] - less);
+                t[n][k + 2] = ex2_approx(t[n][k + 2] - less);
+                l[n][k] = fmaf(t[n][k] + t[n][k + 2], inv_vs, l[n][k]);
             }
-            p[2 * n] = pack_f16(t[n][0], t[n][1]);
-            p[2 * n + 1] = pack_f16(t[n][2], t[n][3]);
+            p[n][0] = transposed(pack_f16(t[n][0], t[n][1]));
+            p[n][1] = transposed(pack_f16(t[n][2], t[n][3]));
         }
 
         // values: lane g holds dimensions D / 8 * g ... of tokens 2c, 2c + 1, 8 + 2c, 9 + 2c
         uint32_t w[4][D / 32];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int tv = 2 * c + (r & 1) + 8 * (r >> 1);
+            // the odd token: its own row (D = 128), or the other half of the pair's
+            const uint8_t *from = st + F::kBlockBytes + (r & 1 ? (val0 ^ 64) + (D == 128 ? 128 : 0) : val0) + (r >> 1) * 8 * D;
             if constexpr (D == 128) {
-                const uint4 x = vc[F::chunk(tv, g)];
+                const uint4 x = *reinterpret_cast<const uint4 *>(from);
                 w[r][0] = x.x, w[r][1] = x.y, w[r][2] = x.z, w[r][3] = x.w;
             } else {
-                const uint2 x = reinterpret_cast<const uint2 *>(vc + F::chunk(tv, g >> 1))[g & 1];
+                const uint2 x = *reinterpret_cast<const uint2 *>(from);
                 w[r][0] = x.x, w[r][1] = x.y;
             }
         }
@@ -290,10 +318,14 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __gri
                 lo[r] = __byte_perm(w[2 * r][k], w[2 * r + 1][k], 0x5140) ^ 0x80808080u;
                 hi[r] = __byte_perm(w[2 * r][k], w[2 * r + 1][k], 0x7362) ^ 0x80808080u;
             }
-            mma16816(o[4 * k], p, codes2<0x4140>(lo[0]), codes2<0x4140>(lo[1]));
-            mma16816(o[4 * k + 1], p, codes2<0x4342>(lo[0]), codes2<0x4342>(lo[1]));
-            mma16816(o[4 * k + 2], p, codes2<0x4140>(hi[0]), codes2<0x4140>(hi[1]));
-            mma16816(o[4 * k + 3], p, codes2<0x4342>(hi[0]), codes2<0x4342>(hi[1]));
+            // dimensions D / 8 * g + 4 k, + 1 are rows g, g + 8 of one product, + 2, + 3 of the next
+            const uint32_t x0 = codes2<0x4140>(lo[0]), x1 = codes2<0x4342>(lo[0]), x2 = codes2<0x4140>(lo[1]), x3 = codes2<0x4342>(lo[1]);
+            const uint32_t y0 = codes2<0x4140>(hi[0]), y1 = codes2<0x4342>(hi[0]), y2 = codes2<0x4140>(hi[1]), y3 = codes2<0x4342>(hi[1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma16816(o[n][2 * k], x0, x1, x2, x3, p[n][0], p[n][1]);
+                mma16816(o[n][2 * k + 1], y0, y1, y2, y3, p[n][0], p[n][1]);
+            }
         }
     }
     cp_wait<0>();
@@ -302,45 +334,48 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __gri
     // join the warps
     float *rows = reinterpret_cast<float *>(smem);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        if (c == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
-        float *to = rows + (warp * kFewRows + g + 8 * h) * F::kRowFloats;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int k = 0; k < 2; ++k) {
+            const int row = 8 * n + 2 * c + k;
 #pragma unroll
-            for (int i = 0; i < D / 8; i += 4)
-                *reinterpret_cast<float4 *>(to + F::padded((2 * c + e) * (D / 8) + i)) =
-                    make_float4(o[i][2 * h + e], o[i + 1][2 * h + e], o[i + 2][2 * h + e], o[i + 3][2 * h + e]);
-    }
+            for (int x = 4; x < 32; x <<= 1) l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], x);
+            if (g == 0) s_m[warp][row] = m[n][k], s_l[warp][row] = l[n][k];
+            float *to = rows + (warp * F::kRows + row) * F::kRowFloats + F::padded(g * F::kLane);
+#pragma unroll
+            for (int i = 0; i < D / 16; i += 2)
+                *reinterpret_cast<float4 *>(to + 2 * i) = make_float4(o[n][i][k], o[n][i][k + 2], o[n][i + 1][k], o[n][i + 1][k + 2]);
+        }
     __syncthreads();
-    const int row = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * (D / 8);  // 8 threads a row
-    float M = -INFINITY, L = 0.f, sum[D / 8];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) sum[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][row]);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const float f = s_m[w][row] == M ? 1.f : ex2_approx(s_m[w][row] - M);
-        L = fmaf(s_l[w][row], f, L);
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-            sum[i] = fmaf(rows[(w * kFewRows + row) * F::kRowFloats + F::padded(d0 + i)], f, sum[i]);
-    }
+    constexpr int kEach = F::kEach, kPer = D / kEach;  // threads a row
+    const int row = threadIdx.x / kPer, d0 = threadIdx.x % kPer * kEach;
     const int64_t r = row0 + row;
-    const bool live = r < R;
+    const bool live = row < F::kRows && r < R;
+    float M = -INFINITY, L = 0.f, sum[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
+    if (live) {
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][row]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = s_m[w][row] == M ? 1.f : ex2_approx(s_m[w][row] - M);
+            L = fmaf(s_l[w][row], f, L);
+            const float *from = rows + (w * F::kRows + row) * F::kRowFloats;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) sum[i] = fmaf(from[F::padded(d0 + i)], f, sum[i]);
+        }
+    }
     if (n_split > 1) {
         const int64_t group = static_cast<int64_t>(unit) * a.c.heads + kv;
-        float *base = a.part + group * a.splits * kFewRows * (D + 2);
-        float *ml = base + static_cast<int64_t>(a.splits) * kFewRows * D;
+        float *base = a.part + group * a.splits * F::kRows * (D + 2);
+        float *ml = base + static_cast<int64_t>(a.splits) * F::kRows * D;
         if (live) {
-            float *to = base + (static_cast<int64_t>(split) * kFewRows + row) * D + d0;
+            float *to = base + (static_cast<int64_t>(split) * F::kRows + row) * D + d0;
 #pragma unroll
-            for (int i = 0; i < D / 8; i += 4)
+            for (int i = 0; i < kEach; i += 4)
                 *reinterpret_cast<float4 *>(to + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
-            if ((threadIdx.x & 7) == 0) *reinterpret_cast<float2 *>(ml + (split * kFewRows + row) * 2) = make_float2(M, L);
+            if (d0 == 0) *reinterpret_cast<float2 *>(ml + (split * F::kRows + row) * 2) = make_float2(M, L);
         }
         __threadfence();
         __syncthreads();
@@ -351,16 +386,17 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __gri
         if (!live) return;
         // join the parts, in their order
         M = -INFINITY, L = 0.f;
-        for (int k = 0; k < n_split; ++k) M = fmaxf(M, __ldcg(ml + (k * kFewRows + row) * 2));
+        for (int k = 0; k < n_split; ++k) M = fmaxf(M, __ldcg(ml + (k * F::kRows + row) * 2));
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) sum[i] = 0.f;
+        for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
+#pragma unroll 4
         for (int k = 0; k < n_split; ++k) {
-            const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + (k * kFewRows + row) * 2));
+            const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + (k * F::kRows + row) * 2));
             const float f = x.x == M ? 1.f : ex2_approx(x.x - M);
             L = fmaf(x.y, f, L);
-            const float *from = base + (static_cast<int64_t>(k) * kFewRows + row) * D + d0;
+            const float *from = base + (static_cast<int64_t>(k) * F::kRows + row) * D + d0;
 #pragma unroll
-            for (int i = 0; i < D / 8; i += 4) {
+            for (int i = 0; i < kEach; i += 4) {
                 const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + i));
                 sum[i] = fmaf(v.x, f, sum[i]);
                 sum[i + 1] = fmaf(v.y, f, sum[i + 1]);
@@ -371,9 +407,9 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __gri
     }
     if (!live) return;
     const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees no key yields zeros
-    const int64_t at = (q.r0 + r / G) * a.ys.token + (kv * G + r % G) * a.ys.head + d0;
+    const int64_t at = (q.r0 + r / G) * a.ys.token + (kv * static_cast<int64_t>(G) + r % G) * a.ys.head + d0;
 #pragma unroll
-    for (int i = 0; i < D / 8; i += 8) {
+    for (int i = 0; i < kEach; i += 8) {
         float v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = sum[i + k] * inv;
@@ -381,14 +417,26 @@ __global__ void __launch_bounds__(kWarps * 32, 3) kv_attn_few_kernel(const __gri
     }
 }
 
-template <int D>
-cudaError_t launch_few(const KvAttnArgs &a, int64_t units, cudaStream_t st) {
-    using F = Few<D>;
+template <int D, int NT>
+cudaError_t launch_few(KvAttnArgs &a, int num_sms, cudaStream_t st) {
+    using F = Few<D, NT>;
+    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> (NT == 1 ? 3 : 4)) + a.b.n_seqs;
+    // one wave of equal parts where there are few, four waves' worth where the lengths of many sequences have to
+    // even out
+    const int64_t wave = F::kBlocks * num_sms, groups = units * a.c.heads;
+    const int64_t span = a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len;
+    int64_t splits = 2 * groups < wave ? (wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
+    splits = std::min(splits, (span + 255) / 256);
+    splits = std::min(splits, static_cast<int64_t>(kMaxParts) / groups);
+    splits = std::max(splits, static_cast<int64_t>(1));
+    if (units * splits > 0x7fffffff) return cudaErrorInvalidValue;
+    a.splits = static_cast<int>(splits);
+    a.chunk = static_cast<int>(((span + splits - 1) / splits + 63) & ~int64_t(63));
     // set at every call: the attribute belongs to the current device
-    const cudaError_t e = cudaFuncSetAttribute(kv_attn_few_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kv_attn_few_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
     if (e != cudaSuccess) return e;
     const dim3 grid(static_cast<unsigned>(units * a.splits), a.c.heads);
-    kv_attn_few_kernel<D><<<grid, kWarps * 32, F::kSmem, st>>>(a);
+    kv_attn_few_kernel<D, NT><<<grid, kWarps * 32, F::kSmem, st>>>(a);
     return cudaGetLastError();
 }
 
@@ -401,19 +449,9 @@ struct KvAttention {
 }  // namespace
 
 cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st) {
-    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 4) + a.b.n_seqs;
-    // three blocks an SM: one wave of equal parts where there are few, four waves' worth where the lengths
-    // of many sequences have to even out
-    const int64_t wave = 3 * num_sms, groups = units * a.c.heads;
-    const int64_t span = a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len;
-    int64_t splits = 2 * groups < wave ? (wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
-    splits = std::min(splits, (span + 255) / 256);
-    splits = std::min(splits, static_cast<int64_t>(kMaxParts) / groups);
-    splits = std::max(splits, static_cast<int64_t>(1));
-    if (units * splits > 0x7fffffff) return cudaErrorInvalidValue;
-    a.splits = static_cast<int>(splits);
-    a.chunk = static_cast<int>((span + splits - 1) / splits + 63) & ~63;
-    return a.c.D == 64 ? launch_few<64>(a, units, st) : launch_few<128>(a, units, st);
+    const bool one = static_cast<int64_t>(a.b.max_rows) * a.group <= 8;
+    if (a.c.D == 64) return one ? launch_few<64, 1>(a, num_sms, st) : launch_few<64, 2>(a, num_sms, st);
+    return one ? launch_few<128, 1>(a, num_sms, st) : launch_few<128, 2>(a, num_sms, st);
 }
 
 }  // namespace b200

@@ -146,9 +146,9 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     const int kv = blockIdx.x % a.c.heads, G = a.group;
     if (blockIdx.x == 0) kv_check(a.b, a.c.page_log2, false, a.err);
     int64_t local;
-    const int s = kv_find(a.b, (gridDim.x - 1 - blockIdx.x) / a.c.heads, G, 8, 1, local);  // late rows, with the most keys, first
-    if (s < 0) return;
-    const KvSeq q = kv_seq(a.b, s, a.c.page_log2);
+    KvSeq q;  // late rows, with the most keys, come first
+    if (!kv_find(a.b, (gridDim.x - 1 - blockIdx.x) / a.c.heads, G, 8, 1, a.c.page_log2, q, local)) return;
+    const int s = q.s;
     const int64_t R = static_cast<int64_t>(q.n) * G, row0 = local * C::kRows;
     if (row0 >= R) return;
     const int i_lo = static_cast<int>(row0 / G), i_hi = static_cast<int>((min(row0 + C::kRows, R) - 1) / G);

@@ -57,15 +57,14 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(WriteArgs a) {
     const int P = 1 << a.c.page_log2, D = a.c.D, head = blockIdx.y, w = blockIdx.z;
     if (blockIdx.x + blockIdx.y + blockIdx.z == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
-    const int s = kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, local);
-    if (s < 0) return;
-    const KvSeq q = kv_seq(a.b, s, a.c.page_log2);
+    KvSeq q;
+    if (!kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, a.c.page_log2, q, local)) return;
     const int begin = q.len - q.n;  // first new position
     if (q.n == 0 || begin < 0) return;
     const int64_t i = (begin >> a.c.page_log2) + local;
     const int64_t p0 = i << a.c.page_log2;
     if (p0 >= q.len) return;
-    const int page = kv_page(a.c, a.b, s, i, a.err);
+    const int page = kv_page(a.c, a.b, q.s, i, a.err);
     if (page < 0) return;
     const int lo = static_cast<int>(max(begin - p0, static_cast<int64_t>(0)));          // first new token of the page
     const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(P)));          // past its last one
@@ -140,15 +139,14 @@ __global__ void __launch_bounds__(128) kv_read_kernel(ReadArgs a) {
     const int P = 1 << a.c.page_log2, D = a.c.D, head = blockIdx.y, w = blockIdx.z;
     if (blockIdx.x + blockIdx.y + blockIdx.z == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
-    const int s = kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, local);
-    if (s < 0) return;
-    const KvSeq q = kv_seq(a.b, s, a.c.page_log2);
+    KvSeq q;
+    if (!kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, a.c.page_log2, q, local)) return;
     const int begin = q.len - q.n;
     if (q.n == 0 || begin < 0) return;
     const int64_t i = (begin >> a.c.page_log2) + local;
     const int64_t p0 = i << a.c.page_log2;
     if (p0 >= q.len) return;
-    const int page = kv_page(a.c, a.b, s, i, a.err);
+    const int page = kv_page(a.c, a.b, q.s, i, a.err);
     const int lo = static_cast<int>(max(begin - p0, static_cast<int64_t>(0)));
     const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(P)));
     const int8_t *codes = a.c.codes[w] + kv_slab(a.c, max(page, 0), head);

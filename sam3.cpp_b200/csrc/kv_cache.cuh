@@ -41,16 +41,6 @@ struct KvSeq {
     int len;
 };
 
-__device__ __forceinline__ KvSeq kv_seq(const KvRows &b, int s, int page_log2) {
-    KvSeq q;
-    q.s = s;
-    q.r0 = min(max(b.row_start[s], 0), b.n_rows);
-    q.n = min(max(b.row_start[s + 1], q.r0), b.n_rows) - q.r0;
-    const int64_t cap = min(b.table_width << page_log2, b.max_len);
-    q.len = static_cast<int>(min(static_cast<int64_t>(max(b.kv_len[s], 0)), cap));
-    return q;
-}
-
 // Checks every sequence against the sizes that the host gave and records
 // kErrKvBatch; one block of a launch runs it.
 __device__ __forceinline__ void kv_check(const KvRows &b, int page_log2, bool rows_are_cached, int *err) {
@@ -62,26 +52,43 @@ __device__ __forceinline__ void kv_check(const KvRows &b, int page_log2, bool ro
     }
 }
 
-// Work is cut into units of `unit` consecutive items of a sequence that has
-// items [row_start[s] m, row_start[s + 1] m).  Sequence s starts at unit
-// first(s) = floor(row_start[s] m / unit) + spare s, which leaves it at least
-// floor(n m / unit) + spare units; the launch has first(n_seqs) of them.  The
-// block's threads count the sequences that start at or before unit u.
-// Every thread of the block calls this.  Returns the sequence, or -1;
-// `local` is the unit's number within it.
-__device__ __forceinline__ int kv_find(const KvRows &b, int64_t u, int m, int unit_log2, int spare, int64_t &local) {
-    int before = 0;
+// Work is cut into units of 1 << unit_log2 consecutive items of a sequence
+// that has items [row_start[s] m, row_start[s + 1] m).  Sequence s starts at
+// unit first(s) = floor(row_start[s] m >> unit_log2) + spare s, which leaves
+// it at least floor(n m >> unit_log2) + spare units; the launch has
+// first(n_seqs) of them.  The block's threads count the sequences that start
+// at or before unit u, each with its numbers already loaded, so that the one
+// that is found costs no second trip to memory.  Every thread of the block
+// calls this.  False if there is none; `local` is the unit's number within
+// the sequence.
+__device__ __forceinline__ bool kv_find(const KvRows &b, int64_t u, int m, int unit_log2, int spare, int page_log2, KvSeq &q,
+                                        int64_t &local) {
+    __shared__ int found[4];
+    int before = 0, mine = -1, r0 = 0, r1 = 0, len = 0;
     for (int base = 0; base < b.n_seqs; base += blockDim.x) {
         const int s = base + threadIdx.x;
         int in = 0;
-        if (s < b.n_seqs)
-            in = ((static_cast<int64_t>(max(b.row_start[s], 0)) * m) >> unit_log2) + static_cast<int64_t>(spare) * s <= u;
+        if (s < b.n_seqs) {
+            const int start = b.row_start[s], end = b.row_start[s + 1], n = b.kv_len[s];
+            in = ((static_cast<int64_t>(max(start, 0)) * m) >> unit_log2) + static_cast<int64_t>(spare) * s <= u;
+            if (in) mine = s, r0 = start, r1 = end, len = n;
+        }
         before += __syncthreads_count(in);
     }
-    if (before == 0) return -1;
-    const int s = before - 1;
-    local = u - (((static_cast<int64_t>(max(b.row_start[s], 0)) * m) >> unit_log2) + static_cast<int64_t>(spare) * s);
-    return local < 0 ? -1 : s;  // only starts that fall (kErrKvBatch) give a negative number
+    if (before == 0) return false;
+    // starts that fall (kErrKvBatch) may leave the last counted number with no thread: nothing is found then
+    if (threadIdx.x == 0) found[3] = -1;
+    __syncthreads();
+    if (mine == before - 1) found[0] = r0, found[1] = r1, found[2] = len, found[3] = mine;
+    __syncthreads();
+    if (found[3] < 0) return false;
+    const int64_t cap = min(b.table_width << page_log2, b.max_len);
+    q.s = found[3];
+    q.r0 = min(max(found[0], 0), b.n_rows);
+    q.n = min(max(found[1], q.r0), b.n_rows) - q.r0;
+    q.len = static_cast<int>(min(static_cast<int64_t>(max(found[2], 0)), cap));
+    local = u - (((static_cast<int64_t>(max(found[0], 0)) * m) >> unit_log2) + static_cast<int64_t>(spare) * q.s);
+    return local >= 0;
 }
 
 // The page of tokens [i << page_log2, ...) of sequence s; a bad entry is
