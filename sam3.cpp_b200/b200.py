@@ -1222,12 +1222,13 @@ class Rope:
         self.h = lib().sam3b200_rope_create(be.h, ctypes.byref(hp))
         if not self.h:
             raise B200Error(f"rope_create failed: {last_error()}")
+        self._run = lib().sam3b200_rope_run  # looked up once: a step of single tokens is a few microseconds
 
     def apply(self, x: int, x_type: int, pos: int, n_rows: int, n_heads: int, y: int, y_type: int, inverse: bool = False,
               x_nb=None, y_nb=None, pos_stride: int | None = None) -> None:
         """y = x turned by its positions; x, pos, y are device addresses, *_nb element strides (row, head)."""
-        _check(lib().sam3b200_rope_run(self.h, x_type, x, _strides(x_nb), pos, n_rows if pos_stride is None else pos_stride,
-                                       n_rows, n_heads, 1 if inverse else 0, y_type, y, _strides(y_nb)), "rope")
+        _check(self._run(self.h, x_type, x, _strides(x_nb), pos, n_rows if pos_stride is None else pos_stride,
+                         n_rows, n_heads, 1 if inverse else 0, y_type, y, _strides(y_nb)), "rope")
 
     def free(self) -> None:
         if self.h:
@@ -1243,13 +1244,13 @@ class KVAttention:
         self.h = lib().sam3b200_kv_attention_create(be.h)
         if not self.h:
             raise B200Error(f"kv_attention_create failed: {last_error()}")
+        self._run = lib().sam3b200_kv_attention_run
 
     def run(self, cache: KVCache, batch: KVBatch, q_type: int, q: int, n_heads: int, y: int, scale: float,
             causal: bool = True, window: int = 0, y_type: int | None = None, q_nb=None, y_nb=None) -> None:
         """y = softmax(scale q k^T + mask) v; q and y are device addresses of [rows][n_heads][head_dim]."""
-        _check(lib().sam3b200_kv_attention_run(self.h, ctypes.addressof(cache), ctypes.addressof(batch), q_type, q,
-                                               _strides(q_nb), n_heads, scale, 1 if causal else 0, window,
-                                               q_type if y_type is None else y_type, y, _strides(y_nb)), "kv_attention")
+        _check(self._run(self.h, ctypes.addressof(cache), ctypes.addressof(batch), q_type, q, _strides(q_nb), n_heads, scale,
+                         1 if causal else 0, window, q_type if y_type is None else y_type, y, _strides(y_nb)), "kv_attention")
 
     def free(self) -> None:
         if self.h:

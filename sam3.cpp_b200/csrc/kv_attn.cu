@@ -34,6 +34,7 @@ namespace b200 {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kMaxSplits = 256;  // most parts of a key range
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -74,19 +75,16 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Four consecutive query elements (d a multiple of 4).
-__device__ __forceinline__ void load_q4(const KvAttnArgs &a, int64_t at, float (&x)[4]) {
+// Four consecutive query elements (d a multiple of 4), as they come, and the j-th of them.
+__device__ __forceinline__ uint2 load_q4(const KvAttnArgs &a, int64_t at) {
     const uint16_t *p = static_cast<const uint16_t *>(a.q) + at;
-    uint16_t e[4];
-    if (a.qs.aligned16) {
-        *reinterpret_cast<uint2 *>(e) = *reinterpret_cast<const uint2 *>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        x[i] = a.q_bf16 ? __uint_as_float(static_cast<uint32_t>(e[i]) << 16) : __half2float(__ushort_as_half(e[i]));
+    if (a.qs.aligned16) return *reinterpret_cast<const uint2 *>(p);
+    return make_uint2(p[0] | static_cast<uint32_t>(p[1]) << 16, p[2] | static_cast<uint32_t>(p[3]) << 16);
+}
+__device__ __forceinline__ float q_value(const KvAttnArgs &a, const uint2 &x, int j) {
+    const uint32_t w = j < 2 ? x.x : x.y;
+    if (a.q_bf16) return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(j & 1 ? w >> 16 : w)));
 }
 
 // NT tiles of 8 query rows.
@@ -101,6 +99,7 @@ struct Few {
     static constexpr int kRowFloats = D + 36;                        // a joined row, padded against bank conflicts
     static constexpr int kJoin = kWarps * kRows * kRowFloats * 4;
     static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+    static_assert(kSmem >= kWarps * kRows * (D + 2) * 4, "shares of the parts");
     static constexpr int kEach = D * kRows / 128 > 8 ? D * kRows / 128 : 8;  // dimensions of a thread that joins
     // Byte of 16-byte chunk c of token t within a staged block.  The permutation keeps the reads free of bank
     // conflicts: keys (8 lanes: 2 neighbouring tokens, 4 chunks), values (8 lanes: 4 token pairs, 2 chunks).  Where
@@ -126,9 +125,9 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
     int64_t local;
     KvSeq q;
     if (!kv_find(a.b, unit, G, NT == 1 ? 3 : 4, 1, a.c.page_log2, q, local)) return;
-    const int64_t R = static_cast<int64_t>(q.n) * G, row0 = local * F::kRows;
-    if (row0 >= R) return;
-    const int i_lo = static_cast<int>(row0 / G), i_hi = static_cast<int>((min(row0 + F::kRows, R) - 1) / G);
+    const int R = q.n * G;  // the host keeps n_rows * G below 2^31
+    if (local * F::kRows >= R) return;
+    const int row0 = static_cast<int>(local) * F::kRows, i_lo = row0 / G, i_hi = (min(row0 + F::kRows, R) - 1) / G;
 
     // the tile's keys, and this block's part of them
     const int k_end = kv_last(a, q, i_hi) + 1, k_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
@@ -139,6 +138,20 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
     const int t_begin = k_begin + split * chunk, t_end = min(t_begin + chunk, k_end);
     const int n_blocks = t_end > t_begin ? (t_end - t_begin + 15) / 16 : 0;
     const int mine = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;  // blocks warp, warp + 4, ...
+
+    // the queries are on their way while the first pages are looked up
+    const int rest0 = row0 - i_lo * G;  // row 0 of the tile: token i_lo, head rest0 of the group
+    uint2 qraw[NT][D / 16];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int x = rest0 + 8 * n + g, i = i_lo + x / G;
+        const int64_t at = (q.r0 + static_cast<int64_t>(i)) * a.qs.token + (static_cast<int64_t>(kv) * G + x % G) * a.qs.head;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+            qraw[n][k] = make_uint2(0u, 0u);
+            if (row0 + 8 * n + g < R) qraw[n][k] = load_q4(a, at + (k >> 2) * 64 + c * 16 + (k & 3) * 4);
+        }
+    }
 
     uint8_t *ring = smem + warp * F::kStages * F::kStageBytes;
     // this lane's bytes within a stage: the copy of chunk lane (of 32 a step), keys of token g, values of token 2 c
@@ -181,28 +194,21 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
     float row_c[NT][2];  // for rows 8 n + 2 c, + 1: scale log2(e), and what the power of two below took
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int64_t r = row0 + 8 * n + g;
-        const int64_t at = (q.r0 + r / G) * a.qs.token + (kv * static_cast<int64_t>(G) + r % G) * a.qs.head;
-        float x[D / 16][4], top = 0.f;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-            x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
-            if (r < R) load_q4(a, at + (k >> 2) * 64 + c * 16 + (k & 3) * 4, x[k]);
-        }
+        float top = 0.f;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[k][j]));
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(q_value(a, qraw[n][k], j)));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // bf16 rows are brought to [1, 2) by a power of two, which f16 then holds to 2^-25 of the largest
         const int e = a.q_bf16 ? min((__float_as_int(top) >> 23) & 0xff, 253) : 0;
         const float down = e ? __int_as_float((254 - e) << 23) : 1.f, up = a.scale_log2 * (e ? __int_as_float(e << 23) : 1.f);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-            qf[n][k][0] = pack_f16(x[k][0] * down, x[k][1] * down);
-            qf[n][k][1] = pack_f16(x[k][2] * down, x[k][3] * down);
-        }
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                qf[n][k][j] = pack_f16(q_value(a, qraw[n][k], 2 * j) * down, q_value(a, qraw[n][k], 2 * j + 1) * down);
 #pragma unroll
         for (int j = 0; j < 2; ++j) row_c[n][j] = __shfl_sync(0xffffffffu, up, (2 * c + j) * 4);
     }
@@ -228,9 +234,11 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
         slot = slot + 1 == F::kStages ? 0 : slot + 1;
 
         // scores of tokens g (t[n][0], [1]) and g + 8 ([2], [3]) for rows 8 n + 2 c, + 1
-        float t[NT][4];
+        float t[NT][4], t2[NT][4];  // in two chains
 #pragma unroll
-        for (int n = 0; n < NT; ++n) t[n][0] = t[n][1] = t[n][2] = t[n][3] = 0.f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[n][k] = t2[n][k] = 0.f;
 #pragma unroll
         for (int h = 0; h < D / 64; ++h) {
             const uint4 lo = *reinterpret_cast<const uint4 *>(st + (h ? key0 ^ 64 : key0));
@@ -241,7 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
                 const uint32_t v = (k == 0 ? hi.x : k == 1 ? hi.y : k == 2 ? hi.z : hi.w) ^ 0x80808080u;
                 const uint32_t a0 = codes2<0x4140>(u), a1 = codes2<0x4140>(v), a2 = codes2<0x4342>(u), a3 = codes2<0x4342>(v);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma16816(t[n], a0, a1, a2, a3, qf[n][4 * h + k][0], qf[n][4 * h + k][1]);
+                for (int n = 0; n < NT; ++n) mma16816(k & 1 ? t2[n] : t[n], a0, a1, a2, a3, qf[n][4 * h + k][0], qf[n][4 * h + k][1]);
             }
         }
         const float2 ksvs = *reinterpret_cast<const float2 *>(st + 2 * F::kBlockBytes);
@@ -250,13 +258,13 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) t[n][k] = fmaf(t[n][k], row_c[n][k & 1] * ksvs.x, lv);
+            for (int k = 0; k < 4; ++k) t[n][k] = fmaf(t[n][k] + t2[n][k], row_c[n][k & 1] * ksvs.x, lv);
         if (tok + 15 > seen_by_all || tok < window_end) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const int i = static_cast<int>((row0 + 8 * n + 2 * c + k) / G), last = kv_last(a, q, i), first = kv_first(a, last);
+                    const int last = kv_last(a, q, i_lo + (rest0 + 8 * n + 2 * c + k) / G), first = kv_first(a, last);
                     if (tok + g > last || tok + g < first) t[n][k] = -INFINITY;
                     if (tok + g + 8 > last || tok + g + 8 < first) t[n][k + 2] = -INFINITY;
                 }
@@ -349,7 +357,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
     __syncthreads();
     constexpr int kEach = F::kEach, kPer = D / kEach;  // threads a row
     const int row = threadIdx.x / kPer, d0 = threadIdx.x % kPer * kEach;
-    const int64_t r = row0 + row;
+    const int r = row0 + row;
     const bool live = row < F::kRows && r < R;
     float M = -INFINITY, L = 0.f, sum[kEach];
 #pragma unroll
@@ -377,37 +385,72 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
                 *reinterpret_cast<float4 *>(to + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
             if (d0 == 0) *reinterpret_cast<float2 *>(ml + (split * F::kRows + row) * 2) = make_float2(M, L);
         }
-        __threadfence();
         __syncthreads();
-        if (threadIdx.x == 0) s_last = atomicInc(a.done + group, n_split - 1) == static_cast<unsigned>(n_split - 1);
+        if (threadIdx.x == 0) {
+            __threadfence();
+            s_last = atomicInc(a.done + group, n_split - 1) == static_cast<unsigned>(n_split - 1);
+            __threadfence();
+        }
         __syncthreads();
         if (!s_last) return;
-        __threadfence();
+        // Join the parts, in a fixed order: a warp takes a row, or with fewer than 4 rows a share of one's parts, its
+        // lanes along the dimensions; then the shares are joined.
+        const int n_rows = min(R - row0, F::kRows);
+        const int shares = n_rows >= 4 ? 1 : n_rows == 1 ? 4 : 2;
+        float *share = reinterpret_cast<float *>(smem), *share_ml = share + kWarps * F::kRows * D;
+        constexpr int kLanes = D / 4, kStep = 32 / kLanes;  // lanes a row, parts a warp and step
+        for (int id = warp; id < n_rows * shares; id += kWarps) {
+            const int i = id / shares;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float top = -INFINITY, total = 0.f;
+            const float *from = base + static_cast<int64_t>(i) * D + lane % kLanes * 4;
+            auto add = [&](float m1, float l1, const float4 &x) {
+                const float to = fmaxf(top, m1);
+                const float f = top == to ? 1.f : ex2_approx(top - to), f1 = m1 == to ? 1.f : ex2_approx(m1 - to);
+                top = to;
+                total = total * f + l1 * f1;
+                v.x = v.x * f + x.x * f1, v.y = v.y * f + x.y * f1, v.z = v.z * f + x.z * f1, v.w = v.w * f + x.w * f1;
+            };
+            for (int k0 = (id % shares) * kStep + lane / kLanes; k0 < n_split; k0 += 8 * shares * kStep) {
+                float2 y[8];
+                float4 x[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int k = k0 + u * shares * kStep;
+                    y[u] = make_float2(-INFINITY, 0.f);
+                    if (k >= n_split) continue;
+                    y[u] = __ldcg(reinterpret_cast<const float2 *>(ml + (k * F::kRows + i) * 2));
+                    x[u] = __ldcg(reinterpret_cast<const float4 *>(from + static_cast<int64_t>(k) * F::kRows * D));
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (k0 + u * shares * kStep < n_split) add(y[u].x, y[u].y, x[u]);
+            }
+            if constexpr (kStep == 2) {
+                const float4 x = make_float4(__shfl_xor_sync(0xffffffffu, v.x, 16), __shfl_xor_sync(0xffffffffu, v.y, 16),
+                                             __shfl_xor_sync(0xffffffffu, v.z, 16), __shfl_xor_sync(0xffffffffu, v.w, 16));
+                const float m1 = __shfl_xor_sync(0xffffffffu, top, 16), l1 = __shfl_xor_sync(0xffffffffu, total, 16);
+                add(m1, l1, x);
+            }
+            if (lane < kLanes) *reinterpret_cast<float4 *>(share + id * D + lane * 4) = v;
+            if (lane == 0) share_ml[2 * id] = top, share_ml[2 * id + 1] = total;
+        }
+        __syncthreads();
         if (!live) return;
-        // join the parts, in their order
         M = -INFINITY, L = 0.f;
-        for (int k = 0; k < n_split; ++k) M = fmaxf(M, __ldcg(ml + (k * F::kRows + row) * 2));
+        for (int w = row * shares; w < (row + 1) * shares; ++w) M = fmaxf(M, share_ml[2 * w]);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < n_split; ++k) {
-            const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + (k * F::kRows + row) * 2));
-            const float f = x.x == M ? 1.f : ex2_approx(x.x - M);
-            L = fmaf(x.y, f, L);
-            const float *from = base + (static_cast<int64_t>(k) * F::kRows + row) * D + d0;
+        for (int w = row * shares; w < (row + 1) * shares; ++w) {
+            const float f = share_ml[2 * w] == M ? 1.f : ex2_approx(share_ml[2 * w] - M);
+            L = fmaf(share_ml[2 * w + 1], f, L);
 #pragma unroll
-            for (int i = 0; i < kEach; i += 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + i));
-                sum[i] = fmaf(v.x, f, sum[i]);
-                sum[i + 1] = fmaf(v.y, f, sum[i + 1]);
-                sum[i + 2] = fmaf(v.z, f, sum[i + 2]);
-                sum[i + 3] = fmaf(v.w, f, sum[i + 3]);
-            }
+            for (int i = 0; i < kEach; ++i) sum[i] = fmaf(share[w * D + d0 + i], f, sum[i]);
         }
     }
     if (!live) return;
     const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees no key yields zeros
-    const int64_t at = (q.r0 + r / G) * a.ys.token + (kv * static_cast<int64_t>(G) + r % G) * a.ys.head + d0;
+    const int64_t at = (q.r0 + static_cast<int64_t>(r / G)) * a.ys.token + (kv * static_cast<int64_t>(G) + r % G) * a.ys.head + d0;
 #pragma unroll
     for (int i = 0; i < kEach; i += 8) {
         float v[8];
@@ -421,20 +464,23 @@ template <int D, int NT>
 cudaError_t launch_few(KvAttnArgs &a, int num_sms, cudaStream_t st) {
     using F = Few<D, NT>;
     const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> (NT == 1 ? 3 : 4)) + a.b.n_seqs;
-    // one wave of equal parts where there are few, four waves' worth where the lengths of many sequences have to
-    // even out
-    const int64_t wave = F::kBlocks * num_sms, groups = units * a.c.heads;
+    // parts for two waves where there are few sequences and heads, for four where the lengths of many have to even out
+    const int64_t wave = F::kBlocks * static_cast<int64_t>(num_sms), groups = units * a.c.heads;
     const int64_t span = a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len;
-    int64_t splits = 2 * groups < wave ? (wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
-    splits = std::min(splits, (span + 255) / 256);
-    splits = std::min(splits, static_cast<int64_t>(kMaxParts) / groups);
+    int64_t splits = 2 * groups < wave ? (2 * wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
+    // a block's least part: 64 tokens, one turn of its warps, while the blocks fit in one wave, else 256
+    const int64_t least = groups * ((span + 63) / 64) <= wave ? 64 : 256;
+    splits = std::min(splits, (span + least - 1) / least);
+    splits = std::min(splits, std::min(static_cast<int64_t>(kMaxParts) / groups, static_cast<int64_t>(kMaxSplits)));
     splits = std::max(splits, static_cast<int64_t>(1));
     if (units * splits > 0x7fffffff) return cudaErrorInvalidValue;
     a.splits = static_cast<int>(splits);
     a.chunk = static_cast<int>(((span + splits - 1) / splits + 63) & ~int64_t(63));
-    // set at every call: the attribute belongs to the current device
-    const cudaError_t e = cudaFuncSetAttribute(kv_attn_few_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
-    if (e != cudaSuccess) return e;
+    if (!(*a.ready & (1 << (2 * NT + (D == 64))))) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_attn_few_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+        if (e != cudaSuccess) return e;
+        *a.ready |= 1 << (2 * NT + (D == 64));
+    }
     const dim3 grid(static_cast<unsigned>(units * a.splits), a.c.heads);
     kv_attn_few_kernel<D, NT><<<grid, kWarps * 32, F::kSmem, st>>>(a);
     return cudaGetLastError();
@@ -442,6 +488,7 @@ cudaError_t launch_few(KvAttnArgs &a, int num_sms, cudaStream_t st) {
 
 struct KvAttention {
     Backend *be = nullptr;
+    unsigned ready = 0;  // kernels whose attributes are set on this handle's device
     float *part = nullptr;
     unsigned *done = nullptr;
 };
@@ -511,6 +558,10 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
                   y_type);
         return SAM3B200_STATUS_FAILED;
     }
+    if (n_heads >= 1 && a.b.n_rows * (n_heads / a.c.heads) > 0x7fffff00) {
+        set_error("kv_attention: %d rows of %lld query heads over %d kv heads are too many", a.b.n_rows, (long long)n_heads, a.c.heads);
+        return SAM3B200_STATUS_FAILED;
+    }
     if (n_heads < 1 || n_heads > 65535 || n_heads % a.c.heads != 0) {
         set_error("kv_attention: %lld query heads over %d kv heads (a positive multiple is needed)", (long long)n_heads, a.c.heads);
         return SAM3B200_STATUS_FAILED;
@@ -535,9 +586,9 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
     a.heads = static_cast<int>(n_heads), a.group = static_cast<int>(n_heads / a.c.heads);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.causal = causal != 0, a.window = static_cast<int>(std::min<int64_t>(window, 0x7fffffff));
-    a.part = k->part, a.done = k->done, a.err = k->be->err;
+    a.part = k->part, a.done = k->done, a.ready = &k->ready, a.err = k->be->err;
     DeviceScope dev(k->be->device);
-    const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= kFewRows;
+    const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= 64;
     const cudaError_t e = few ? kv_attn_few(a, k->be->num_sms, k->be->stream) : kv_attn_tc(a, k->be->stream);
     k->be->count();
     return cuda_ok(e, "kv_attention launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;

@@ -21,6 +21,7 @@ struct KvAttnArgs {
     float *part;          // partial results: see kPartFloats
     unsigned *done;       // parts finished, one counter a unit and kv head; 0 between calls
     int *err;
+    unsigned *ready;      // host: kernels whose attributes are set on the device
 };
 
 // 2^x scores: P = 2^(t - m + kPUp) with m within kLazy of the running
@@ -32,7 +33,7 @@ constexpr float kPUp = 7.f, kLazy = 8.f;
 constexpr float kZeroScaleLog2 = -80.f;
 
 // The device workspace of a handle.
-constexpr int kMaxParts = 4096;
+constexpr int kMaxParts = 8192;
 constexpr int kFewRows = 16;
 constexpr size_t kPartFloats = static_cast<size_t>(kMaxParts) * kFewRows * (128 + 2);
 

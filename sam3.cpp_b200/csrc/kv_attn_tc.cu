@@ -149,9 +149,9 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     KvSeq q;  // late rows, with the most keys, come first
     if (!kv_find(a.b, (gridDim.x - 1 - blockIdx.x) / a.c.heads, G, 8, 1, a.c.page_log2, q, local)) return;
     const int s = q.s;
-    const int64_t R = static_cast<int64_t>(q.n) * G, row0 = local * C::kRows;
-    if (row0 >= R) return;
-    const int i_lo = static_cast<int>(row0 / G), i_hi = static_cast<int>((min(row0 + C::kRows, R) - 1) / G);
+    const int R = q.n * G;  // the host keeps n_rows * G below 2^31
+    if (local * C::kRows >= R) return;
+    const int row0 = static_cast<int>(local) * C::kRows, i_lo = row0 / G, i_hi = (min(row0 + C::kRows, R) - 1) / G;
     const int k_end = kv_last(a, q, i_hi) + 1, k_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
     const int ntiles = k_end > k_begin ? (k_end - k_begin + C::kKeys - 1) / C::kKeys : 0;
     const int nq = R - row0 > 128 ? 2 : 1;
@@ -350,10 +350,10 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
         // ---- softmax: thread = row ----
         take_regs<kRegsSoftmax>();
         const int t = warp >> 2;
-        const int64_t r = row0 + threadIdx.x;  // t * 128 + row of the tile
+        const int r = row0 + static_cast<int>(threadIdx.x);  // t * 128 + row of the tile
         const bool live = r < R;
         if (t < nq) {
-            const int i = static_cast<int>(r / G);
+            const int i = r / G;
             const int64_t head = kv * static_cast<int64_t>(G) + r % G;
             const int last = live ? kv_last(a, q, i) : -1, first = live ? kv_first(a, last) : 0;
             float row_c = 1.f;
@@ -413,9 +413,9 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
             const uint32_t s_col = tmem + base + t * 128, o_col = tmem + base + 256 + t * D;
             float m = -INFINITY, l = 0.f;
             // tokens that some row of this warp does not see
-            const int64_t w_lo = row0 + (threadIdx.x & ~31), w_hi = min(w_lo + 31, R - 1);
-            const int all_end = w_lo < R ? kv_last(a, q, static_cast<int>(w_lo / G)) : 0x7fffffff;
-            const int all_begin = w_lo < R ? kv_first(a, kv_last(a, q, static_cast<int>(w_hi / G))) : 0;
+            const int w_lo = row0 + static_cast<int>(threadIdx.x & ~31u), w_hi = min(w_lo + 31, R - 1);
+            const int all_end = w_lo < R ? kv_last(a, q, w_lo / G) : 0x7fffffff;
+            const int all_begin = w_lo < R ? kv_first(a, kv_last(a, q, w_hi / G)) : 0;
             bool ok = true;
             for (int j = 0; j < ntiles; ++j) {
                 ok = warp_wait(&s_full[t], j & 1, a.err, TERR_S) &&
@@ -555,12 +555,15 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
 template <int D>
 cudaError_t launch_tc(const KvAttnArgs &a, int64_t units, cudaStream_t st) {
     using C = Tc<D>;
-    cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-    if (e != cudaSuccess) return e;
-    cudaFuncAttributes f;  // the register shares draw on what the block starts with
-    e = cudaFuncGetAttributes(&f, kv_attn_tc_kernel<D>);
-    if (e != cudaSuccess) return e;
-    if (f.numRegs < kRegsStart) return cudaErrorInvalidConfiguration;
+    if (!(*a.ready & (1u << (16 + (D == 64))))) {
+        cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        if (e != cudaSuccess) return e;
+        cudaFuncAttributes f;  // the register shares draw on what the block starts with
+        e = cudaFuncGetAttributes(&f, kv_attn_tc_kernel<D>);
+        if (e != cudaSuccess) return e;
+        if (f.numRegs < kRegsStart) return cudaErrorInvalidConfiguration;
+        *a.ready |= 1u << (16 + (D == 64));
+    }
     kv_attn_tc_kernel<D><<<static_cast<unsigned>(units * a.c.heads), C::kThreads, C::kSmem, st>>>(a);
     return cudaGetLastError();
 }

@@ -11,10 +11,15 @@
 // Both roundings are decided exactly, so the codes do not depend on how the
 // rows of a prompt are cut into calls' blocks or on the order of anything.
 //
-// One block per (page, head, keys or values): the page's new rows are read
-// once into registers, their largest magnitude is reduced over the block and
-// the codes are written from the registers.  Bound by memory: 2 (f16) bytes
-// in and 1 out per value.
+// A block owns one page of a sequence for several of its slabs (a slab: one
+// head's keys, or its values), so that finding the page is paid once; W of
+// its 8 warps share a slab.  The new rows of a slab are read once into
+// registers, their largest magnitude is reduced over the W warps, and the
+// codes are written from the registers; W follows from the rows that a call
+// can put into one page, 1 for steps of single tokens.  Bound by memory: 2
+// (f16) bytes in and 1 out per value.
+#include <algorithm>
+
 #include "kv_cache.cuh"
 
 namespace b200 {
@@ -42,6 +47,9 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
     return (a & 0xff) | ((b & 0xff) << 8) | ((c & 0xff) << 16) | (static_cast<uint32_t>(d) << 24);
 }
 
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kPer = 8;  // groups of 8 values that a thread holds
+
 struct WriteArgs {
     KvView c;
     KvRows b;
@@ -50,12 +58,32 @@ struct WriteArgs {
     int *err;
 };
 
-// Grid (units of one page, kv heads, keys / values); PER groups of 8 values a thread.
-template <typename T, bool VEC, int THREADS, int PER>
-__global__ void __launch_bounds__(THREADS) kv_write_kernel(WriteArgs a) {
-    __shared__ float wmax[THREADS / 32];
-    const int P = 1 << a.c.page_log2, D = a.c.D, head = blockIdx.y, w = blockIdx.z;
-    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) kv_check(a.b, a.c.page_log2, true, a.err);
+// 8 values as they come.
+template <typename T>
+struct alignas(16) Raw8 {
+    T v[8];
+};
+
+template <bool VEC, typename T>
+__device__ __forceinline__ Raw8<T> raw8(const T *p) {
+    Raw8<T> r;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+            reinterpret_cast<uint4 *>(&r)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = p[i];
+    }
+    return r;
+}
+
+// Grid (units of one page, groups of kWarps / W slabs); slab = head + heads * (0 keys, 1 values).
+template <typename T, bool VEC, int W>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteArgs a) {
+    __shared__ float wmax[kWarps];
+    const int D = a.c.D;
+    if (blockIdx.x + blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
     KvSeq q;
     if (!kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, a.c.page_log2, q, local)) return;
@@ -66,63 +94,70 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(WriteArgs a) {
     if (p0 >= q.len) return;
     const int page = kv_page(a.c, a.b, q.s, i, a.err);
     if (page < 0) return;
-    const int lo = static_cast<int>(max(begin - p0, static_cast<int64_t>(0)));          // first new token of the page
-    const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(P)));          // past its last one
+    const int lo = static_cast<int>(max(begin - p0, static_cast<int64_t>(0)));  // first new token of the page
+    const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(1) << a.c.page_log2));
+    const int warp = threadIdx.x >> 5, slab = blockIdx.y * (kWarps / W) + warp / W;
+    const bool there = slab < 2 * a.c.heads;
+    const int w = slab >= a.c.heads, head = there ? slab - w * a.c.heads : 0;
     int8_t *codes = a.c.codes[w] + kv_slab(a.c, page, head);
     float *scale = a.c.scale[w] + static_cast<int64_t>(page) * a.c.heads + head;
-    const T *x = static_cast<const T *>(a.x[w]) + head * a.xs[w].head;
-    const int64_t row0 = q.r0 + p0 - begin;  // row of the page's token 0
+    const T *x = static_cast<const T *>(a.x[w]) + head * a.xs[w].head + (q.r0 + p0 - begin) * a.xs[w].token;
 
-    float v[PER][8];
+    const int first = lo * D, end = there ? hi * D : 0, thread = (warp % W) * 32 + (threadIdx.x & 31);
+    Raw8<T> raw[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int e = first + (k * W * 32 + thread) * 8;
+        if (e < end) raw[k] = raw8<VEC>(x + static_cast<int64_t>(e / D) * a.xs[w].token + e % D);
+    }
+    const float held = there && lo > 0 ? *scale : 0.f;
     float amax = 0.f;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int e = (k * THREADS + threadIdx.x) * 8, t = e / D, d = e % D;
-        if (t < lo || t >= hi) continue;
-        load8<VEC>(x + (row0 + t) * a.xs[w].token + d, v[k]);
+    for (int k = 0; k < kPer; ++k) {
+        if (first + (k * W * 32 + thread) * 8 >= end) continue;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float m = fabsf(v[k][j]);
-            if (!(m == m)) v[k][j] = 0.f;  // NaN is stored as 0
+            const float m = fabsf(to_f32(raw[k].v[j]));
             amax = fmaxf(amax, m <= kF32Max ? m : 0.f);
         }
     }
-    const float held = lo > 0 ? *scale : 0.f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = amax;
-    __syncthreads();  // also: every thread has read the old scale
+    if (W > 1) {
+        if ((threadIdx.x & 31) == 0) wmax[warp] = amax;
+        __syncthreads();  // also: every thread of the slab has read the old scale
 #pragma unroll
-    for (int j = 0; j < THREADS / 32; ++j) amax = fmaxf(amax, wmax[j]);
+        for (int j = 0; j < W; ++j) amax = fmaxf(amax, wmax[warp / W * W + j]);
+    } else {
+        __syncwarp();
+    }
     const float to = fmaxf(held, amax < kKvSmallest ? 0.f : __fmul_rn(amax, 1.f / 127.f));
     const float inv = to > 0.f ? __frcp_rn(to) : 0.f, top = fminf(__fmul_rn(127.f, to), kF32Max);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int e = (k * THREADS + threadIdx.x) * 8, t = e / D;
-        if (t >= hi) continue;
-        uint32_t out[2];
-        if (t >= lo) {
-            int c[8];
+    for (int k = 0; k < kPer; ++k) {
+        const int e = first + (k * W * 32 + thread) * 8;
+        if (e >= end) continue;
+        int c[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)  // infinities go to the ends
-                c[j] = to > 0.f ? round_quotient(fminf(fmaxf(v[k][j], -top), top), to, inv) : 0;
-            out[0] = pack4(c[0], c[1], c[2], c[3]);
-            out[1] = pack4(c[4], c[5], c[6], c[7]);
-        } else {
-            if (to == held) continue;
-            const uint2 old = *reinterpret_cast<const uint2 *>(codes + e);
-            int c[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {  // code * held is exact in 64 bits, and no quotient rounds onto a tie
-                const int8_t o = static_cast<int8_t>((j < 4 ? old.x : old.y) >> (8 * (j & 3)));
-                c[j] = __double2int_rn(static_cast<double>(o) * held / to);
-            }
-            out[0] = pack4(c[0], c[1], c[2], c[3]);
-            out[1] = pack4(c[4], c[5], c[6], c[7]);
+        for (int j = 0; j < 8; ++j) {  // NaN is stored as 0, infinities go to the ends
+            float v = to_f32(raw[k].v[j]);
+            v = v == v ? fminf(fmaxf(v, -top), top) : 0.f;
+            c[j] = to > 0.f ? round_quotient(v, to, inv) : 0;
         }
-        *reinterpret_cast<uint2 *>(codes + e) = make_uint2(out[0], out[1]);
+        *reinterpret_cast<uint2 *>(codes + e) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
     }
-    if (threadIdx.x == 0) *scale = to;
+    if (there && thread == 0) *scale = to;
+    if (to == held) return;
+    for (int e = thread * 8; e < (there ? first : 0); e += W * 32 * 8) {  // older tokens, under the grown scale
+        const uint2 old = *reinterpret_cast<const uint2 *>(codes + e);
+        int c[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // code * held is exact in 64 bits, and no quotient rounds onto a tie
+            const int8_t o = static_cast<int8_t>((j < 4 ? old.x : old.y) >> (8 * (j & 3)));
+            c[j] = __double2int_rn(static_cast<double>(o) * held / to);
+        }
+        *reinterpret_cast<uint2 *>(codes + e) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+    }
 }
 
 struct ReadArgs {
@@ -130,14 +165,15 @@ struct ReadArgs {
     KvRows b;
     void *y[2];
     RowTensor ys[2];
+    int slabs;  // of a block
     int *err;
 };
 
-// Grid (units of one page, kv heads, keys / values).
+// Grid (units of one page, groups of a.slabs slabs); 16 codes a thread and step.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(128) kv_read_kernel(ReadArgs a) {
-    const int P = 1 << a.c.page_log2, D = a.c.D, head = blockIdx.y, w = blockIdx.z;
-    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) kv_check(a.b, a.c.page_log2, true, a.err);
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadArgs a) {
+    const int D = a.c.D;
+    if (blockIdx.x + blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
     KvSeq q;
     if (!kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, a.c.page_log2, q, local)) return;
@@ -146,32 +182,45 @@ __global__ void __launch_bounds__(128) kv_read_kernel(ReadArgs a) {
     const int64_t i = (begin >> a.c.page_log2) + local;
     const int64_t p0 = i << a.c.page_log2;
     if (p0 >= q.len) return;
-    const int page = kv_page(a.c, a.b, q.s, i, a.err);
+    const int page = kv_page(a.c, a.b, q.s, i, a.err);  // bad: zeros
     const int lo = static_cast<int>(max(begin - p0, static_cast<int64_t>(0)));
-    const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(P)));
-    const int8_t *codes = a.c.codes[w] + kv_slab(a.c, max(page, 0), head);
-    const float scale = page < 0 ? 0.f : a.c.scale[w][static_cast<int64_t>(page) * a.c.heads + head];
-    T *y = static_cast<T *>(a.y[w]) + head * a.ys[w].head;
+    const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(1) << a.c.page_log2));
     const int64_t row0 = q.r0 + p0 - begin;
-    for (int e = lo * D + threadIdx.x * 8; e < hi * D; e += 128 * 8) {
-        const uint2 raw = *reinterpret_cast<const uint2 *>(codes + e);
-        float v[8];
+    const int chunks = D / 16, each = (hi - lo) * chunks;  // 16-code chunks of a slab
+    const int slab0 = blockIdx.y * a.slabs, slabs = min(a.slabs, 2 * a.c.heads - slab0);
+#pragma unroll 4
+    for (int id = threadIdx.x; id < slabs * each; id += kThreads) {
+        const int slab = slab0 + id / each, at = id % each, t = lo + at / chunks, d = at % chunks * 16;
+        const int w = slab >= a.c.heads, head = slab - w * a.c.heads;
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+        float scale = 0.f;
+        if (page >= 0) {
+            raw = __ldg(reinterpret_cast<const uint4 *>(a.c.codes[w] + kv_slab(a.c, page, head) + t * D + d));
+            scale = __ldg(a.c.scale[w] + static_cast<int64_t>(page) * a.c.heads + head);
+        }
+        T *y = static_cast<T *>(a.y[w]) + head * a.ys[w].head + (row0 + t) * a.ys[w].token + d;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = page < 0 ? 0.f : __fmul_rn(static_cast<float>(static_cast<int8_t>((j < 4 ? raw.x : raw.y) >> (8 * (j & 3)))), scale);
-        store8<VEC>(y + (row0 + e / D) * a.ys[w].token + e % D, v);
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t u[2] = {h ? raw.z : raw.x, h ? raw.w : raw.y};
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[j] = page < 0 ? 0.f : __fmul_rn(static_cast<float>(static_cast<int8_t>(u[j >> 2] >> (8 * (j & 3)))), scale);
+            store8<VEC>(y + 8 * h, v);
+        }
     }
 }
 
 template <typename T, bool VEC>
-void launch_write(const WriteArgs &a, dim3 grid, cudaStream_t st) {
-    switch ((a.c.D << a.c.page_log2) / 1024) {
-        case 1: kv_write_kernel<T, VEC, 128, 1><<<grid, 128, 0, st>>>(a); break;
-        case 2: kv_write_kernel<T, VEC, 128, 2><<<grid, 128, 0, st>>>(a); break;
-        case 4: kv_write_kernel<T, VEC, 128, 4><<<grid, 128, 0, st>>>(a); break;
-        case 8: kv_write_kernel<T, VEC, 256, 4><<<grid, 256, 0, st>>>(a); break;
-        default: kv_write_kernel<T, VEC, 512, 4><<<grid, 512, 0, st>>>(a); break;
-    }
+void launch_write(const WriteArgs &a, cudaStream_t st) {
+    // values that a call can put into one slab of a page, 2048 a warp
+    const int most = std::min(1 << a.c.page_log2, a.b.max_rows) * a.c.D;
+    const int units = (a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs;
+    auto grid = [&](int w) { return dim3(units, (2 * a.c.heads + kWarps / w - 1) / (kWarps / w)); };
+    if (most <= 2048) kv_write_kernel<T, VEC, 1><<<grid(1), kThreads, 0, st>>>(a);
+    else if (most <= 4096) kv_write_kernel<T, VEC, 2><<<grid(2), kThreads, 0, st>>>(a);
+    else if (most <= 8192) kv_write_kernel<T, VEC, 4><<<grid(4), kThreads, 0, st>>>(a);
+    else kv_write_kernel<T, VEC, 8><<<grid(8), kThreads, 0, st>>>(a);
 }
 
 }  // namespace
@@ -254,12 +303,11 @@ extern "C" int sam3b200_kv_write(sam3b200_backend *h, const sam3b200_kv_cache *c
     if (a.b.n_seqs == 0 || a.b.n_rows == 0) return SAM3B200_STATUS_SUCCESS;
     a.err = be->err;
     DeviceScope dev(be->device);
-    const dim3 grid((a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs, a.c.heads, 2);
     const bool vec = a.xs[0].aligned16 && a.xs[1].aligned16;
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (vec) launch_write<T, true>(a, grid, be->stream);
-        else launch_write<T, false>(a, grid, be->stream);
+        if (vec) launch_write<T, true>(a, be->stream);
+        else launch_write<T, false>(a, be->stream);
     };
     if (type == SAM3B200_TYPE_F32) go(float());
     else if (type == SAM3B200_TYPE_F16) go(__half());
@@ -292,12 +340,15 @@ extern "C" int sam3b200_kv_read(sam3b200_backend *h, const sam3b200_kv_cache *ca
     if (a.b.n_seqs == 0 || a.b.n_rows == 0) return SAM3B200_STATUS_SUCCESS;
     a.err = be->err;
     DeviceScope dev(be->device);
-    const dim3 grid((a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs, a.c.heads, 2);
+    // about 16 K codes a block, fewer where a page gives a call few rows
+    const int most = std::min(1 << a.c.page_log2, a.b.max_rows) * a.c.D;
+    a.slabs = std::min(std::max(16384 / std::max(most, 1), 1), 2 * a.c.heads);
+    const dim3 grid((a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs, (2 * a.c.heads + a.slabs - 1) / a.slabs);
     const bool vec = a.ys[0].aligned16 && a.ys[1].aligned16;
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (vec) kv_read_kernel<T, true><<<grid, 128, 0, be->stream>>>(a);
-        else kv_read_kernel<T, false><<<grid, 128, 0, be->stream>>>(a);
+        if (vec) kv_read_kernel<T, true><<<grid, kThreads, 0, be->stream>>>(a);
+        else kv_read_kernel<T, false><<<grid, kThreads, 0, be->stream>>>(a);
     };
     if (type == SAM3B200_TYPE_F32) go(float());
     else if (type == SAM3B200_TYPE_F16) go(__half());
