@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
     const int kv = blockIdx.y, G = a.group;
     const unsigned unit = blockIdx.x / a.splits;
     const int split = blockIdx.x % a.splits;
-    if (blockIdx.x + blockIdx.y == 0) kv_check(a.b, a.c.page_log2, false, a.err);
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, false, a.err);
     int64_t local;
     KvSeq q;
     if (!kv_find(a.b, unit, G, NT == 1 ? 3 : 4, 1, a.c.page_log2, q, local)) return;

@@ -27,28 +27,36 @@ namespace {
 
 constexpr float kF32Max = 3.402823466e38f;
 
-// round(x / s), ties to even, for |x| <= 127.5 s, s a normal f32.  The magic
-// sum rounds x * inv (inv ~ 1 / s) to an integer q that is at most one off;
-// r = x - q s is exact wherever |r| is near s / 2 (x and q s are multiples of
-// the smaller of their units, and r needs no more bits than s), so comparing
-// it with s / 2 tells on which side of the border x lies.
-__device__ __forceinline__ int round_quotient(float x, float s, float inv) {
-    const float m = __fmaf_rn(x, inv, 12582912.f), q = __fsub_rn(m, 12582912.f);
-    const float r = __fmaf_rn(-q, s, x), h = 0.5f * s;
-    int c = __float_as_int(m) - 0x4B400000;
-    if (fabsf(r) >= h) {
-        const bool tie = fabsf(r) == h;
-        if (!tie || (c & 1)) c += r > 0.f ? 1 : -1;
+// round(x / s), ties to even, for finite |x| <= 127.5 s, s a normal f32, as
+// the low bytes of c.  The magic sum rounds x * inv (inv ~ 1 / s) to an
+// integer q that is at most one off; r = x - q s is exact wherever |r| is near
+// s / 2 (x and q s are multiples of the smaller of their units, and r needs no
+// more bits than s), so comparing it with s / 2 tells on which side of the
+// border x lies.  The largest |r| of 8 values decides whether any is looked
+// at again.
+__device__ __forceinline__ void round_quotients(const float (&x)[8], float s, float inv, int (&c)[8]) {
+    float far = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float m = __fmaf_rn(x[j], inv, 12582912.f);
+        c[j] = __float_as_int(m);
+        far = fmaxf(far, fabsf(__fmaf_rn(-__fsub_rn(m, 12582912.f), s, x[j])));
     }
-    return c;
+    const float h = 0.5f * s;
+    if (far < h) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float r = __fmaf_rn(-__fsub_rn(__int_as_float(c[j]), 12582912.f), s, x[j]);
+        if (fabsf(r) > h || (fabsf(r) == h && (c[j] & 1))) c[j] += r > 0.f ? 1 : -1;
+    }
 }
 
+// The low bytes of four numbers.
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-    return (a & 0xff) | ((b & 0xff) << 8) | ((c & 0xff) << 16) | (static_cast<uint32_t>(d) << 24);
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kPer = 8;  // groups of 8 values that a thread holds
 
 struct WriteArgs {
     KvView c;
@@ -79,11 +87,12 @@ __device__ __forceinline__ Raw8<T> raw8(const T *p) {
 }
 
 // Grid (units of one page, groups of kWarps / W slabs); slab = head + heads * (0 keys, 1 values).
-template <typename T, bool VEC, int W>
+// PER: groups of 8 values that a thread holds.
+template <typename T, bool VEC, int W, int PER = 4>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteArgs a) {
     __shared__ float wmax[kWarps];
     const int D = a.c.D;
-    if (blockIdx.x + blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
     KvSeq q;
     if (!kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, a.c.page_log2, q, local)) return;
@@ -104,21 +113,32 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
     const T *x = static_cast<const T *>(a.x[w]) + head * a.xs[w].head + (q.r0 + p0 - begin) * a.xs[w].token;
 
     const int first = lo * D, end = there ? hi * D : 0, thread = (warp % W) * 32 + (threadIdx.x & 31);
-    Raw8<T> raw[kPer];
+    Raw8<T> raw[PER];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
+    for (int k = 0; k < PER; ++k) {
         const int e = first + (k * W * 32 + thread) * 8;
         if (e < end) raw[k] = raw8<VEC>(x + static_cast<int64_t>(e / D) * a.xs[w].token + e % D);
     }
     const float held = there && lo > 0 ? *scale : 0.f;
-    float amax = 0.f;
+    // largest magnitude, by its bits: infinities and NaN are above all numbers and show
+    uint32_t bits = 0;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
+    for (int k = 0; k < PER; ++k) {
         if (first + (k * W * 32 + thread) * 8 >= end) continue;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float m = fabsf(to_f32(raw[k].v[j]));
-            amax = fmaxf(amax, m <= kF32Max ? m : 0.f);
+        for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_uint(fabsf(to_f32(raw[k].v[j]))));
+    }
+    const bool finite = bits < 0x7f800000u;
+    float amax = finite ? __uint_as_float(bits) : 0.f;
+    if (!finite) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            if (first + (k * W * 32 + thread) * 8 >= end) continue;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float m = fabsf(to_f32(raw[k].v[j]));
+                amax = fmaxf(amax, m <= kF32Max ? m : 0.f);
+            }
         }
     }
 #pragma unroll
@@ -134,16 +154,18 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
     const float to = fmaxf(held, amax < kKvSmallest ? 0.f : __fmul_rn(amax, 1.f / 127.f));
     const float inv = to > 0.f ? __frcp_rn(to) : 0.f, top = fminf(__fmul_rn(127.f, to), kF32Max);
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
+    for (int k = 0; k < PER; ++k) {
         const int e = first + (k * W * 32 + thread) * 8;
         if (e >= end) continue;
+        float v[8];
         int c[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {  // NaN is stored as 0, infinities go to the ends
-            float v = to_f32(raw[k].v[j]);
-            v = v == v ? fminf(fmaxf(v, -top), top) : 0.f;
-            c[j] = to > 0.f ? round_quotient(v, to, inv) : 0;
+        for (int j = 0; j < 8; ++j) {
+            v[j] = to_f32(raw[k].v[j]);
+            if (!finite) v[j] = v[j] == v[j] ? fminf(fmaxf(v[j], -top), top) : 0.f;  // NaN is stored as 0, infinities as the ends
+            c[j] = 0;
         }
+        if (to > 0.f) round_quotients(v, to, inv, c);
         *reinterpret_cast<uint2 *>(codes + e) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
     }
     if (there && thread == 0) *scale = to;
@@ -173,7 +195,7 @@ struct ReadArgs {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadArgs a) {
     const int D = a.c.D;
-    if (blockIdx.x + blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
     KvSeq q;
     if (!kv_find(a.b, blockIdx.x, 1, a.c.page_log2, 2, a.c.page_log2, q, local)) return;
@@ -213,14 +235,15 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
 
 template <typename T, bool VEC>
 void launch_write(const WriteArgs &a, cudaStream_t st) {
-    // values that a call can put into one slab of a page, 2048 a warp
+    // values that a call can put into one slab of a page, 1024 a warp
     const int most = std::min(1 << a.c.page_log2, a.b.max_rows) * a.c.D;
     const int units = (a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs;
     auto grid = [&](int w) { return dim3(units, (2 * a.c.heads + kWarps / w - 1) / (kWarps / w)); };
-    if (most <= 2048) kv_write_kernel<T, VEC, 1><<<grid(1), kThreads, 0, st>>>(a);
-    else if (most <= 4096) kv_write_kernel<T, VEC, 2><<<grid(2), kThreads, 0, st>>>(a);
-    else if (most <= 8192) kv_write_kernel<T, VEC, 4><<<grid(4), kThreads, 0, st>>>(a);
-    else kv_write_kernel<T, VEC, 8><<<grid(8), kThreads, 0, st>>>(a);
+    if (most <= 1024) kv_write_kernel<T, VEC, 1><<<grid(1), kThreads, 0, st>>>(a);
+    else if (most <= 2048) kv_write_kernel<T, VEC, 2><<<grid(2), kThreads, 0, st>>>(a);
+    else if (most <= 4096) kv_write_kernel<T, VEC, 4><<<grid(4), kThreads, 0, st>>>(a);
+    else if (most <= 8192) kv_write_kernel<T, VEC, 8><<<grid(8), kThreads, 0, st>>>(a);
+    else kv_write_kernel<T, VEC, 8, 8><<<grid(8), kThreads, 0, st>>>(a);
 }
 
 }  // namespace

@@ -42,7 +42,8 @@ struct KvSeq {
 };
 
 // Checks every sequence against the sizes that the host gave and records
-// kErrKvBatch; one block of a launch runs it.
+// kErrKvBatch; one block of a launch runs it, the one of the last unit, which
+// mostly has nothing else to do.
 __device__ __forceinline__ void kv_check(const KvRows &b, int page_log2, bool rows_are_cached, int *err) {
     for (int s = threadIdx.x; s < b.n_seqs; s += blockDim.x) {
         const int64_t r0 = b.row_start[s], r1 = b.row_start[s + 1], len = b.kv_len[s];

@@ -10,9 +10,12 @@
 // positions would lose the angle in 32 bits) and the remaining half turns go
 // to sincospif, good to 2^-23 or so.
 //
-// Bound by memory (one read, one write): a thread owns 8 pairs of a row, has
-// their cosines and sines in registers and walks over heads with 16-byte
-// loads, so an angle is computed once for many heads.
+// Bound by memory (one read, one write).  A block owns a few rows (128
+// pairs of cosines and sines, one or so for each of its threads, through
+// shared memory); a thread has 8 pairs of a row in registers and walks over
+// every eighth head with 16-byte loads.  An angle costs 50 to 100
+// instructions, so it is computed once for a row and not by each thread.
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -58,30 +61,42 @@ __device__ __forceinline__ void positions(const RopeArgs &a, int row, int (&p)[4
     for (int k = 0; k < 4; ++k) p[k] = k < a.t.n_axes ? a.pos[k * a.pos_stride + row] : 0;
 }
 
-// 8 pairs, or 16 elements behind the turned ones, a thread.
+constexpr int kHeadLanes = 8;  // threads that share a row's 8 pairs, over heads
+
+// Blocks of `rows` rows; a thread: 8 pairs, or 16 elements behind the turned ones, of every eighth head.
 template <typename TX, typename TY, bool NEIGHBOURS>
-__global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeArgs a) {
-    const int n = a.t.pairs, each = a.t.head_dim / 16;  // threads a row
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
-    const int64_t row64 = id / each;
-    if (row64 >= a.n_rows) return;
-    const int row = static_cast<int>(row64), part = static_cast<int>(id % each);
+__global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeArgs a, int rows) {
+    __shared__ float2 turn[128];
+    const int n = a.t.pairs, each = a.t.head_dim / 16;  // parts of a row
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows;
+    for (int id = threadIdx.x; id < rows * n; id += blockDim.x) {
+        const int64_t row = row0 + id / n;
+        if (row >= a.n_rows) break;
+        int p[4];
+        positions(a, static_cast<int>(row), p);
+        angle(a, id % n, p, turn[id].x, turn[id].y);
+    }
+    __syncthreads();
+    const int part = threadIdx.x % each, lane = threadIdx.x / each % kHeadLanes, row_in = threadIdx.x / (each * kHeadLanes);
+    const int64_t row = row0 + row_in;
+    if (row >= a.n_rows) return;
     const bool turned = part < n / 8;
     int d0, d1;  // first elements of the two groups of 8
     if (NEIGHBOURS || !turned) d0 = part * 16, d1 = d0 + 8;
     else d0 = part * 8, d1 = n + part * 8;
     float c[8], s[8];
     if (turned) {
-        int p[4];
-        positions(a, row, p);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) angle(a, part * 8 + j, p, c[j], s[j]);
+        for (int j = 0; j < 8; ++j) {
+            const float2 v = turn[row_in * n + part * 8 + j];
+            c[j] = v.x, s[j] = v.y;
+        }
     }
     const int h0 = blockIdx.y * a.heads_each, h1 = min(h0 + a.heads_each, a.n_heads);
     const TX *x = static_cast<const TX *>(a.x) + row * a.xs.token;
     TY *y = static_cast<TY *>(a.y) + row * a.ys.token;
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
+#pragma unroll 2
+    for (int h = h0 + lane; h < h1; h += kHeadLanes) {
         float u[8], v[8];
         load8<true>(x + h * a.xs.head + d0, u);
         load8<true>(x + h * a.xs.head + d1, v);
@@ -136,14 +151,23 @@ __global__ void __launch_bounds__(128) rope_any_kernel(const __grid_constant__ R
 
 template <typename TX, typename TY>
 void launch_rope(RopeArgs &a, bool wide, cudaStream_t st, int num_sms) {
+    if (wide) {
+        const int each = a.t.head_dim / 16, rows = std::max(16 / each, 1);  // 128 pairs at most
+        const int64_t blocks = (static_cast<int64_t>(a.n_rows) + rows - 1) / rows;
+        // heads are split over blocks only where the rows give fewer than 8 blocks an SM
+        const int64_t split = (num_sms * int64_t(8) + blocks - 1) / blocks;
+        a.heads_each = static_cast<int>((a.n_heads + split - 1) / split + kHeadLanes - 1) / kHeadLanes * kHeadLanes;
+        const dim3 grid(static_cast<unsigned>(blocks), (a.n_heads + a.heads_each - 1) / a.heads_each);
+        if (a.t.neighbours) rope_kernel<TX, TY, true><<<grid, rows * each * kHeadLanes, 0, st>>>(a, rows);
+        else rope_kernel<TX, TY, false><<<grid, rows * each * kHeadLanes, 0, st>>>(a, rows);
+        return;
+    }
     // a thread walks over all heads where the rows alone fill the GPU (2048 threads an SM), else over fewer
-    const int64_t threads = static_cast<int64_t>(a.n_rows) * (wide ? a.t.head_dim / 16 : a.t.head_dim - a.t.pairs);
+    const int64_t threads = static_cast<int64_t>(a.n_rows) * (a.t.head_dim - a.t.pairs);
     const int64_t split = (num_sms * int64_t(2048) + threads - 1) / threads;
     a.heads_each = static_cast<int>(split >= a.n_heads ? 1 : (a.n_heads + split - 1) / split);
     const dim3 grid(static_cast<unsigned>((threads + 127) / 128), (a.n_heads + a.heads_each - 1) / a.heads_each);
-    if (!wide) rope_any_kernel<TX, TY><<<grid, 128, 0, st>>>(a);
-    else if (a.t.neighbours) rope_kernel<TX, TY, true><<<grid, 128, 0, st>>>(a);
-    else rope_kernel<TX, TY, false><<<grid, 128, 0, st>>>(a);
+    rope_any_kernel<TX, TY><<<grid, 128, 0, st>>>(a);
 }
 
 }  // namespace
