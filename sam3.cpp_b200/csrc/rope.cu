@@ -63,60 +63,76 @@ __device__ __forceinline__ void positions(const RopeArgs &a, int row, int (&p)[4
 
 constexpr int kHeadLanes = 8;  // threads that share a row's 8 pairs, over heads
 
-// Blocks of `rows` rows; a thread: 8 pairs, or 16 elements behind the turned ones, of every eighth head.
+// 8 elements as they come, read past the L1 and soon to be evicted from the L2: nothing is read twice.
+template <typename T>
+struct Stream8 {
+    uint4 raw[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+    }
+    __device__ __forceinline__ float operator[](int i) const { return to_f32(reinterpret_cast<const T *>(raw)[i]); }
+};
+
+// Blocks of `rows` rows; a thread: 8 pairs, or 16 elements behind the turned ones, of every eighth head, one at a time:
+// more blocks an SM serve better than more loads a thread (21037 rows of 40 heads of 128, bf16: 80 us, two heads at a
+// time 91, the next head's loads ahead 91).
 template <typename TX, typename TY, bool NEIGHBOURS>
 __global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeArgs a, int rows) {
     __shared__ float2 turn[128];
     const int n = a.t.pairs, each = a.t.head_dim / 16;  // parts of a row
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows;
-    for (int id = threadIdx.x; id < rows * n; id += blockDim.x) {
-        const int64_t row = row0 + id / n;
-        if (row >= a.n_rows) break;
-        int p[4];
-        positions(a, static_cast<int>(row), p);
-        angle(a, id % n, p, turn[id].x, turn[id].y);
-    }
-    __syncthreads();
     const int part = threadIdx.x % each, lane = threadIdx.x / each % kHeadLanes, row_in = threadIdx.x / (each * kHeadLanes);
     const int64_t row = row0 + row_in;
-    if (row >= a.n_rows) return;
     const bool turned = part < n / 8;
     int d0, d1;  // first elements of the two groups of 8
     if (NEIGHBOURS || !turned) d0 = part * 16, d1 = d0 + 8;
     else d0 = part * 8, d1 = n + part * 8;
-    float c[8], s[8];
-    if (turned) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 v = turn[row_in * n + part * 8 + j];
-            c[j] = v.x, s[j] = v.y;
-        }
-    }
-    const int h0 = blockIdx.y * a.heads_each, h1 = min(h0 + a.heads_each, a.n_heads);
+    int h = blockIdx.y * a.heads_each + lane;
+    const int h1 = row < a.n_rows ? min(static_cast<int>(blockIdx.y + 1) * a.heads_each, a.n_heads) : 0;
     const TX *x = static_cast<const TX *>(a.x) + row * a.xs.token;
     TY *y = static_cast<TY *>(a.y) + row * a.ys.token;
-#pragma unroll 2
-    for (int h = h0 + lane; h < h1; h += kHeadLanes) {
-        float u[8], v[8];
-        load8<true>(x + h * a.xs.head + d0, u);
-        load8<true>(x + h * a.xs.head + d1, v);
+    for (int id = threadIdx.x; id < rows * n; id += blockDim.x) {
+        const int64_t r = row0 + id / n;
+        if (r >= a.n_rows) break;
+        int p[4];
+        positions(a, static_cast<int>(r), p);
+        angle(a, id % n, p, turn[id].x, turn[id].y);
+    }
+    __syncthreads();
+    float c[8], s[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float2 z = turned ? turn[row_in * n + part * 8 + j] : make_float2(1.f, 0.f);
+        c[j] = z.x, s[j] = z.y;
+    }
+#pragma unroll 1
+    while (h < h1) {
+        const int at = h;
+        Stream8<TX> u, v;
+        u.load(x + h * a.xs.head + d0);
+        v.load(x + h * a.xs.head + d1);
+        float f[8], g[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = u[j], g[j] = v[j];
+        h += kHeadLanes;
         if (turned) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (NEIGHBOURS) {  // pair j is (u, v)[2j], (u, v)[2j + 1]
-                    float &e = j < 4 ? u[2 * j] : v[2 * j - 8], &o = j < 4 ? u[2 * j + 1] : v[2 * j - 7];
+                if (NEIGHBOURS) {  // pair j is (f, g)[2j], (f, g)[2j + 1]
+                    float &e = j < 4 ? f[2 * j] : g[2 * j - 8], &o = j < 4 ? f[2 * j + 1] : g[2 * j - 7];
                     const float x0 = e, x1 = o;
                     e = x0 * c[j] - x1 * s[j];
                     o = x1 * c[j] + x0 * s[j];
                 } else {
-                    const float x0 = u[j], x1 = v[j];
-                    u[j] = x0 * c[j] - x1 * s[j];
-                    v[j] = x1 * c[j] + x0 * s[j];
+                    const float x0 = f[j], x1 = g[j];
+                    f[j] = x0 * c[j] - x1 * s[j];
+                    g[j] = x1 * c[j] + x0 * s[j];
                 }
             }
         }
-        store8<true>(y + h * a.ys.head + d0, u);
-        store8<true>(y + h * a.ys.head + d1, v);
+        store8<true>(y + at * a.ys.head + d0, f);
+        store8<true>(y + at * a.ys.head + d1, g);
     }
 }
 
