@@ -334,7 +334,7 @@ int sam3b200_kv_write(sam3b200_backend *be, const sam3b200_kv_cache *cache, cons
 int sam3b200_kv_read(sam3b200_backend *be, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch, int type,
                      void *k, const int64_t k_nb[2], void *v, const int64_t v_nb[2]);
 
-/* The attention's workspace (about 34 MB of device memory).  Calls with one
+/* The attention's workspace (about 136 MB of device memory).  Calls with one
  * handle must not overlap on the GPU: those of one backend do not, unless a
  * captured graph is launched on another stream; give such a graph a handle of
  * its own.  Free it before the backend; NULL on error. */

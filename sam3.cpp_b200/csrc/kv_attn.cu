@@ -466,7 +466,8 @@ cudaError_t launch_few(KvAttnArgs &a, int num_sms, cudaStream_t st) {
     const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> (NT == 1 ? 3 : 4)) + a.b.n_seqs;
     // parts for two waves where there are few sequences and heads, for four where the lengths of many have to even out
     const int64_t wave = F::kBlocks * static_cast<int64_t>(num_sms), groups = units * a.c.heads;
-    const int64_t span = a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len;
+    const int64_t span =
+        std::max(a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len, int64_t(1));
     int64_t splits = 2 * groups < wave ? (2 * wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
     // a block's least part: 64 tokens, one turn of its warps, while the blocks fit in one wave, else 256
     const int64_t least = groups * ((span + 63) / 64) <= wave ? 64 : 256;
@@ -589,7 +590,7 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
     a.part = k->part, a.done = k->done, a.ready = &k->ready, a.err = k->be->err;
     DeviceScope dev(k->be->device);
     const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= 64;
-    const cudaError_t e = few ? kv_attn_few(a, k->be->num_sms, k->be->stream) : kv_attn_tc(a, k->be->stream);
+    const cudaError_t e = few ? kv_attn_few(a, k->be->num_sms, k->be->stream) : kv_attn_tc(a, k->be->num_sms, k->be->stream);
     k->be->count();
     return cuda_ok(e, "kv_attention launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
 }

@@ -17,7 +17,7 @@ struct KvAttnArgs {
     float scale_log2;     // scale * log2(e)
     int causal, window;   // window 0: none
     int splits;           // most parts of a key range
-    int chunk;            // tokens of a part (a multiple of 64)
+    int chunk;            // tokens of a part (a multiple of 64, for 256 rows of 128)
     float *part;          // partial results: see kPartFloats
     unsigned *done;       // parts finished, one counter a unit and kv head; 0 between calls
     int *err;
@@ -32,10 +32,11 @@ constexpr float kPUp = 7.f, kLazy = 8.f;
 // Scale of a value page that holds only zeros, as the softmax weights see it.
 constexpr float kZeroScaleLog2 = -80.f;
 
-// The device workspace of a handle.
+// The device workspace of a handle: parts of key ranges, each [rows][D + 2] (sums, maximum, weight), of 8 or 16 rows
+// (kv_attn_few) or 256 (kv_attn_tc: 1024 parts of head dim 128); one counter a row tile.
 constexpr int kMaxParts = 8192;
-constexpr int kFewRows = 16;
-constexpr size_t kPartFloats = static_cast<size_t>(kMaxParts) * kFewRows * (128 + 2);
+constexpr int64_t kPartFloats = int64_t(1024) * 256 * (128 + 2);
+static_assert(kPartFloats >= int64_t(kMaxParts) * 16 * (128 + 2), "parts of 16 rows");
 
 // Last key that row i of a sequence sees, and the first.
 __device__ __forceinline__ int kv_last(const KvAttnArgs &a, const KvSeq &q, int i) {
@@ -57,6 +58,6 @@ __device__ __forceinline__ void kv_store8(const KvAttnArgs &a, int64_t at, const
 }
 
 cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st);  // kv_attn.cu: 16 rows a block
-cudaError_t kv_attn_tc(const KvAttnArgs &a, cudaStream_t st);          // kv_attn_tc.cu: 256 rows a block
+cudaError_t kv_attn_tc(KvAttnArgs a, int num_sms, cudaStream_t st);   // kv_attn_tc.cu: 256 rows a block
 
 }  // namespace b200

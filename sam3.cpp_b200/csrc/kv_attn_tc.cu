@@ -9,10 +9,13 @@
 //               next tile's in registers meanwhile) and write them as f16,
 //               exactly, into 128-byte-swizzled shared memory, and each 16
 //               tokens' scales beside them;
-//   warp 12:    issues the MMAs (13-15 only give their registers away): S_t(j) = Q_t K_j^T, and once softmax t has
-//               written its weights over S_t(j), O_t += P_t(j) V_j and
-//               S_t(j + 1).  One tile's products run under the other's
-//               softmax.
+//   warps 12, 13: issue the MMAs of tile 0 and 1 (14, 15 only give their
+//               registers away; one warp for both was the bottleneck), in
+//               steps of 64 tokens: S_t(i) = Q_t K_i^T into one of two
+//               buffers, and once softmax t has written its weights over
+//               S_t(i), O_t += P_t(i) V_i and S_t(i + 2).  A softmax warp thus
+//               finds its next scores ready; the products of one step run
+//               under the softmax of the next, and the tiles under each other.
 // Keys and values have one layout, [token][64 dimensions] rows of 128 bytes:
 // keys are the K-major B operand of the first product, values the N-major B
 // operand of the second, so neither is transposed.
@@ -20,7 +23,10 @@
 // kv_attn.cu), so the scales of 16 tokens enter as one multiply-add in front
 // of the exponential.  O stays in tensor memory; it is rescaled only where a
 // row's maximum rose by more than kLazy.
-// Tensor memory (512 columns): S_t, and P_t over it, at 128 t; O_t at 256 + D t.
+// Tensor memory (512 columns): S_t(i), and P_t(i) over it, at 128 t + 64 (i % 2);
+// O_t at 256 + D t.
+#include <algorithm>
+
 #include "kv_attn.cuh"
 #include "ptx.cuh"
 
@@ -31,7 +37,7 @@ enum { TERR_Q = 1 << 8, TERR_K = 1 << 9, TERR_V = 1 << 10, TERR_FREE = 1 << 11, 
 
 // Registers a thread after the split: a block starts with 128 for each of its
 // four warpgroups, and the shares may not add up to more.
-constexpr int kRegsStart = 128, kRegsSoftmax = 176, kRegsCodes = 104, kRegsMma = 56;
+constexpr int kRegsStart = 128, kRegsSoftmax = 168, kRegsCodes = 120, kRegsMma = 56;
 static_assert(2 * kRegsSoftmax + kRegsCodes + kRegsMma <= 4 * kRegsStart, "register shares");
 
 constexpr int kPolyPairs = 2;  // of 8 pairs of weights, those whose exponential runs on the FMA pipe
@@ -74,6 +80,7 @@ __device__ __forceinline__ void put_codes(uint8_t *tile, uint32_t at, const uint
 }
 
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, int *err, int code) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
 }
 
@@ -134,34 +141,48 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + C::kBars);
     uint64_t *k_full = q_full + 1;       // [2] keys of tile j in slot j % 2
     uint64_t *v_full = k_full + 2;       // [2]
-    uint64_t *pair_free = v_full + 2;    // [2] pair p = keys p and values p - 1: read by all their MMAs
-    uint64_t *s_full = pair_free + 2;    // [2 tiles] phase j: S_t(j) and O_t up to j - 1 are in tensor memory
-    uint64_t *p_full = s_full + 2;       // [2 tiles] phase j: O_t is rescaled and P_t(j) is there
-    // Scales of tile j, in slot j % 4: written again at tile j + 4, which waits for P_t(j + 1), so a slow softmax
-    // warp never sees its phase pass by (keys may run two tiles ahead of it: it must not wait on k_full).
-    uint64_t *sc_full = p_full + 2;
+    uint64_t *k_free = v_full + 2;       // [2] tile j is read by all its MMAs
+    uint64_t *v_free = k_free + 2;       // [2]
+    uint64_t *s_full = v_free + 2;       // [tile][i % 2] S_t(i) is in tensor memory, and so is O_t with P_t(i - 2) V
+    uint64_t *p_full = s_full + 4;       // [tile][i % 2] P_t(i) is there (and O_t rescaled)
+    // Scales of key tile j, in slot j % 4: written again for tile j + 4, which waits for P_t(2 j + 3), so a slow
+    // softmax warp never sees its phase pass by (the keys run ahead of it: it must not wait on k_full).
+    uint64_t *sc_full = p_full + 4;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sc_full + C::kScaleSlots);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kv = blockIdx.x % a.c.heads, G = a.group;
+    const int split = blockIdx.x % a.splits, kv = blockIdx.x / a.splits % a.c.heads, G = a.group;
+    const unsigned unit = (gridDim.x - 1 - blockIdx.x) / a.splits / a.c.heads;  // late rows, with the most keys, come first
     if (blockIdx.x == 0) kv_check(a.b, a.c.page_log2, false, a.err);
     int64_t local;
-    KvSeq q;  // late rows, with the most keys, come first
-    if (!kv_find(a.b, (gridDim.x - 1 - blockIdx.x) / a.c.heads, G, 8, 1, a.c.page_log2, q, local)) return;
+    KvSeq q;
+    if (!kv_find(a.b, unit, G, 8, 1, a.c.page_log2, q, local)) return;
     const int s = q.s;
     const int R = q.n * G;  // the host keeps n_rows * G below 2^31
     if (local * C::kRows >= R) return;
     const int row0 = static_cast<int>(local) * C::kRows, i_lo = row0 / G, i_hi = (min(row0 + C::kRows, R) - 1) / G;
-    const int k_end = kv_last(a, q, i_hi) + 1, k_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
-    const int ntiles = k_end > k_begin ? (k_end - k_begin + C::kKeys - 1) / C::kKeys : 0;
+    // the rows' keys, and this block's part of them
+    const int all_keys_end = kv_last(a, q, i_hi) + 1, all_keys_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
+    const int range = max(all_keys_end - all_keys_begin, 0);
+    const int part = max(a.chunk, ((range + a.splits - 1) / a.splits + 127) & ~127);
+    const int n_split = max((range + part - 1) / part, 1);
+    if (split >= n_split) return;
+    const int k_begin = all_keys_begin + split * part, k_end = min(k_begin + part, all_keys_end);
+    const int ntiles = k_end > k_begin ? (k_end - k_begin + C::kKeys - 1) / C::kKeys : 0;  // of 128 tokens, as they are staged
+    const int nsteps = k_end > k_begin ? (k_end - k_begin + 63) / 64 : 0;                  // of 64 tokens, as they are used
     const int nq = R - row0 > 128 ? 2 : 1;
+    const int64_t group = static_cast<int64_t>(unit) * a.c.heads + kv;
+    auto part_of = [&](int k) { return a.part + (group * a.splits + k) * (C::kRows * (D + 2)); };
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 4 * nq);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&k_full[i], 4);
             mbar_init(&v_full[i], 4);
-            mbar_init(&pair_free[i], 1);
+            mbar_init(&k_free[i], nq);
+            mbar_init(&v_free[i], nq);
+        }
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
         }
@@ -257,93 +278,83 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        // Pair p of the pipeline is keys p and values p - 1; keys j + 1 and values j reuse the slots of pair j - 1.
-        // Codes and scales are loaded a tile ahead.
-        Pages pg = checked(0, lookup(0)), pg_next = checked(1, lookup(1)), raw = lookup(2);
-        fetch(0, 0, pg, kx);
-        fetch_scales(pg);
-        fetch(1, 0, pg, vx);
-        if (ntiles > 0) {
-            put(smem + C::kK, kx);
-            put_scales(0);
-            publish(&k_full[0]);
-            if (lane == 0) mbar_arrive(&sc_full[0]);
-            fetch(0, 1, pg_next, kx);
-            fetch_scales(pg_next);
-        }
+        // Codes and scales are loaded a tile ahead, table entries two.
+        Pages pg_next = checked(0, lookup(0)), raw = lookup(1);
+        fetch(0, 0, pg_next, kx);
+        fetch_scales(pg_next);
+        fetch(1, 0, pg_next, vx);
         for (int j = 0; j < ntiles; ++j) {
-            const Pages pg_then = checked(j + 2, raw);
-            raw = lookup(j + 3);
-            if (j >= 1 && !warp_wait(&pair_free[(j - 1) & 1], ((j - 1) >> 1) & 1, a.err, TERR_FREE))
-                break;
+            pg_next = checked(j + 1, raw);
+            raw = lookup(j + 2);
+            if (j >= 2 && !warp_wait(&k_free[j & 1], ((j >> 1) - 1) & 1, a.err, TERR_FREE)) break;
+            put(smem + C::kK + (j & 1) * C::kTile, kx);
+            put_scales(j);
+            publish(&k_full[j & 1]);
+            if (lane == 0) mbar_arrive(&sc_full[j % C::kScaleSlots]);
+            fetch(0, j + 1, pg_next, kx);
+            fetch_scales(pg_next);
+            if (j >= 2 && !warp_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, a.err, TERR_FREE)) break;
             put(smem + C::kV + (j & 1) * C::kTile, vx);
             publish(&v_full[j & 1]);
             fetch(1, j + 1, pg_next, vx);
-            if (j + 1 < ntiles) {
-                put(smem + C::kK + ((j + 1) & 1) * C::kTile, kx);
-                put_scales(j + 1);
-                publish(&k_full[(j + 1) & 1]);
-                if (lane == 0) mbar_arrive(&sc_full[(j + 1) % C::kScaleSlots]);
-                fetch(0, j + 2, pg_then, kx);
-                fetch_scales(pg_then);
-            }
-            pg_next = pg_then;
         }
     } else if (warp >= 12) {
         // ---- MMA issuer ----
         give_regs<kRegsMma>();
-        if (warp == 12) {
-            constexpr uint32_t idesc_s = idesc_f16_f32(128, C::kKeys);
+        if (warp - 12 < nq) {
+            const int t = warp - 12;
+            constexpr uint32_t idesc_s = idesc_f16_f32(128, 64);
             constexpr uint32_t idesc_pv = idesc_f16_f32(128, D) | (1u << 16);  // B is N-major
             // Descriptors advance by constants (addresses in 16 bytes), so that an MMA costs its issuer little.
             const uint64_t q_desc = sw128_kmajor_desc(smem_u32(smem + C::kQ)), k_desc = sw128_kmajor_desc(smem_u32(smem + C::kK)),
                            v_desc = sw128_nmajor_desc(smem_u32(smem + C::kV), C::kHalf);
-            auto mma_s = [&](int t, int j) {
-                const uint64_t qd = q_desc + t * (C::kTile >> 4), kd = k_desc + (j & 1) * (C::kTile >> 4);
+            auto mma_s = [&](int i) {
+                const uint64_t qd = q_desc + t * (C::kTile >> 4), kd = k_desc + ((i >> 1) & 1) * (C::kTile >> 4) + (i & 1) * (64 * 128 >> 4);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t off = ((k >> 2) * C::kHalf + (k & 3) * 32) >> 4;
-                    mma_f16(tmem + t * 128, qd + off, kd + off, idesc_s, k > 0);
+                    mma_f16(tmem + t * 128 + (i & 1) * 64, qd + off, kd + off, idesc_s, k > 0);
                 }
             };
-            auto mma_pv = [&](int t, int j) {
-                const uint64_t vd = v_desc + (j & 1) * (C::kTile >> 4);
+            auto mma_pv = [&](int i) {
+                const uint64_t vd = v_desc + ((i >> 1) & 1) * (C::kTile >> 4) + (i & 1) * (64 * 128 >> 4);
 #pragma unroll
-                for (int k = 0; k < C::kKeys / 16; ++k)
-                    mma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + k * 8, vd + (k * 2048 >> 4), idesc_pv, j > 0 || k > 0);
+                for (int k = 0; k < 4; ++k)
+                    mma_f16_ts(tmem + 256 + t * D, tmem + t * 128 + (i & 1) * 64 + k * 8, vd + (k * 2048 >> 4), idesc_pv, i > 0 || k > 0);
             };
             auto wait = [&](uint64_t *bar, int phase, int code) {
                 return warp_wait(bar, phase & 1, a.err, code);
             };
-            bool ok = ntiles > 0 && wait(q_full, 0, TERR_Q) && wait(&k_full[0], 0, TERR_K);
+            bool ok = nsteps > 0 && wait(q_full, 0, TERR_Q) && wait(&k_full[0], 0, TERR_K);
             if (ok) {
                 tc_fence_after();
                 if (elect_one()) {
-                    for (int t = 0; t < nq; ++t) {
-                        mma_s(t, 0);
-                        mma_commit(&s_full[t]);
+                    for (int i = 0; i < 2 && i < nsteps; ++i) {
+                        mma_s(i);
+                        mma_commit(&s_full[2 * t + i]);
                     }
-                    mma_commit(&pair_free[0]);
+                    mma_commit(&k_free[0]);
                 }
                 __syncwarp();
             }
-            for (int j = 0; j < ntiles && ok; ++j) {
-                const bool more = j + 1 < ntiles;
-                ok = wait(&v_full[j & 1], j >> 1, TERR_V);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (t >= nq || !ok) break;
-                    ok = (!more || t > 0 || wait(&k_full[(j + 1) & 1], (j + 1) >> 1, TERR_K)) && wait(&p_full[t], j, TERR_P);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        mma_pv(t, j);
-                        if (more) mma_s(t, j + 1);
-                        mma_commit(&s_full[t]);
-                        if (more && t == nq - 1) mma_commit(&pair_free[(j + 1) & 1]);
+            // Step i: O += P(i) V, then S(i + 2) over P(i); S(i + 1) is being worked on meanwhile.
+            for (int i = 0; i < nsteps && ok; ++i) {
+                const bool more = i + 2 < nsteps, even = (i & 1) == 0;
+                ok = (!even || wait(&v_full[(i >> 1) & 1], i >> 2, TERR_V)) &&
+                     (!even || !more || wait(&k_full[((i + 2) >> 1) & 1], (i + 2) >> 2, TERR_K)) &&
+                     wait(&p_full[2 * t + (i & 1)], i >> 1, TERR_P);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    mma_pv(i);
+                    if (more) mma_s(i + 2);
+                    mma_commit(&s_full[2 * t + (i & 1)]);
+                    if (!even) {  // this tile has read values i / 2 and keys i / 2 + 1
+                        mma_commit(&v_free[(i >> 1) & 1]);
+                        mma_commit(&k_free[((i + 2) >> 1) & 1]);
                     }
-                    __syncwarp();
                 }
+                __syncwarp();
             }
         }
     } else {
@@ -417,52 +428,41 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
             const int all_end = w_lo < R ? kv_last(a, q, w_lo / G) : 0x7fffffff;
             const int all_begin = w_lo < R ? kv_first(a, kv_last(a, q, w_hi / G)) : 0;
             bool ok = true;
-            for (int j = 0; j < ntiles; ++j) {
-                ok = warp_wait(&s_full[t], j & 1, a.err, TERR_S) &&
-                     warp_wait(&sc_full[j % C::kScaleSlots], (j / C::kScaleSlots) & 1, a.err, TERR_K);
+            for (int i = 0; i < nsteps; ++i) {
+                const int j = i >> 1, buf = i & 1;
+                const uint32_t s_at = s_col + buf * 64;
+                ok = warp_wait(&s_full[2 * t + buf], j & 1, a.err, TERR_S) &&
+                     (buf != 0 || warp_wait(&sc_full[j % C::kScaleSlots], (j / C::kScaleSlots) & 1, a.err, TERR_K));
                 if (!ok) break;
                 tc_fence_after();
+                uint32_t x[2][32];
+                tmem_ld_32x32b_x32(s_at, x[0]);
+                tmem_ld_32x32b_x32(s_at + 32, x[1]);
                 // a factor of 0 (keys or scale 0) would make NaN of -inf; a tiny one leaves 0 of the other scores
-                float fk[8], lv[8], inv_v[8];
+                float fk[4], lv[4], inv_v[4];
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    const Scales v = reinterpret_cast<const Scales *>(smem + C::kScales)[(j % C::kScaleSlots) * 8 + g];
+                for (int g = 0; g < 4; ++g) {
+                    const Scales v = reinterpret_cast<const Scales *>(smem + C::kScales)[(j % C::kScaleSlots) * 8 + buf * 4 + g];
                     fk[g] = fmaxf(v.k * row_c, 1e-37f), lv[g] = v.lv, inv_v[g] = v.inv_v;
                 }
-                const int tok = k_begin + j * C::kKeys;
-                if (tok + C::kKeys - 1 > all_end || tok < all_begin) {
-                    // hidden scores become -inf in place; the row sees columns lo .. hi
+                tmem_wait_ld();
+                pass32(x[0]);
+                pass32(x[1]);
+                const int tok = k_begin + i * 64;
+                if (tok + 63 > all_end || tok < all_begin) {  // the row sees columns lo .. hi
                     const int hi = last - tok, lo = first - tok;
-#pragma unroll 1
-                    for (int c = 0; c < C::kKeys; c += 32) {
-                        uint32_t x[32];
-                        tmem_ld_32x32b_x32(s_col + c, x);
-                        tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (c + e > hi || c + e < lo) x[e] = 0xff800000u;
-                        tmem_st_32x32b_x32(s_col + c, x);
-                    }
-                    tmem_wait_st();
+                    for (int e = 0; e < 64; ++e)
+                        if (e > hi || e < lo) x[e >> 5][e & 31] = 0xff800000u;
                 }
-                // columns 64 ... 127, then 0 ... 63, which stay in registers: P goes over columns that were read last
                 float top = -INFINITY;
-                uint32_t x[2][32];
 #pragma unroll
-                for (int half = 1; half >= 0; --half) {
-                    tmem_ld_32x32b_x32(s_col + 64 * half, x[0]);
-                    tmem_ld_32x32b_x32(s_col + 64 * half + 32, x[1]);
-                    tmem_wait_ld();
-                    pass32(x[0]);
-                    pass32(x[1]);
+                for (int g = 0; g < 4; ++g) {
+                    const uint32_t *y = &x[g >> 1][16 * (g & 1)];
+                    float mx = __uint_as_float(y[0]);
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const uint32_t *y = &x[g >> 1][16 * (g & 1)];
-                        float mx = __uint_as_float(y[0]);
-#pragma unroll
-                        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(y[e]));
-                        top = fmaxf(top, fmaf(mx, fk[4 * half + g], lv[4 * half + g]));
-                    }
+                    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(y[e]));
+                    top = fmaxf(top, fmaf(mx, fk[g], lv[g]));
                 }
                 float alpha = 1.f;
                 if (top > m + kLazy) {
@@ -470,9 +470,13 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                     m = top;
                     l *= alpha;
                 }
-                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    // P_t(i - 1) V is in O_t when the step after this one has its scores
+                    ok = warp_wait(&s_full[2 * t + (buf ^ 1)], ((i + 1) >> 1) & 1, a.err, TERR_S);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {  // S_t(j) being there, P_t(j - 1) V_(j - 1) is in O_t
+                    for (int c = 0; c < D; c += 16) {
                         uint32_t o[16];
                         tmem_ld_32x32b_x16(o_col + c, o);
                         tmem_wait_ld();
@@ -483,64 +487,99 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                 }
                 const float less = m == -INFINITY ? 0.f : m - kPUp;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    // in three sweeps, so that 32 exponentials are on their way at once
-                    float y[32];
+                for (int c = 0; c < 2; ++c) {
                     uint32_t pk[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                        fma2(y[e], y[e + 1], __uint_as_float(x[c & 1][e]), __uint_as_float(x[c & 1][e + 1]), fk[2 * c + e / 16],
-                             lv[2 * c + e / 16] - less);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        if (e / 2 % 8 >= 8 - kPolyPairs) {
-                            exp2_poly(y[e], y[e + 1]);
-                        } else {
-                            y[e] = ex2_approx(y[e]);
-                            y[e + 1] = ex2_approx(y[e + 1]);
-                        }
-                    }
-#pragma unroll
                     for (int g = 0; g < 2; ++g) {
+                        const float k = fk[2 * c + g], b = lv[2 * c + g] - less;
                         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
                         for (int e = 16 * g; e < 16 * g + 16; e += 2) {
-                            fadd2(s0, s1, s0, s1, y[e], y[e + 1]);
-                            const __half2 h = __floats2half2_rn(y[e], y[e + 1]);
+                            float y0, y1;
+                            fma2(y0, y1, __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]), k, b);
+                            if (e / 2 % 8 >= 8 - kPolyPairs) {
+                                exp2_poly(y0, y1);
+                            } else {
+                                y0 = ex2_approx(y0);
+                                y1 = ex2_approx(y1);
+                            }
+                            fadd2(s0, s1, s0, s1, y0, y1);
+                            const __half2 h = __floats2half2_rn(y0, y1);
                             pk[e / 2] = *reinterpret_cast<const uint32_t *>(&h);
                         }
                         l = fmaf(s0 + s1, inv_v[2 * c + g], l);
                     }
-                    tmem_st_32x32b_x16(s_col + 16 * c, pk);
-                    if (c > 0 && c < 3) {
-                        tmem_wait_ld();
-                        pass32(x[(c + 1) & 1]);
-                    }
-                    if (c < 2) tmem_ld_32x32b_x32(s_col + 64 + 32 * c, x[c]);
+                    tmem_st_32x32b_x16(s_at + 16 * c, pk);
                 }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t]);
+                if (lane == 0) mbar_arrive(&p_full[2 * t + buf]);
             }
-            if (ok && ntiles > 0) ok = warp_wait(&s_full[t], ntiles & 1, a.err, TERR_S);
+            // the last step's O
+            if (ok && nsteps > 0) ok = warp_wait(&s_full[2 * t + ((nsteps + 1) & 1)], ((nsteps + 1) >> 1) & 1, a.err, TERR_S);
             if (ok) {
                 tc_fence_after();
-                const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key yields zeros
+                const float inv = n_split > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;  // a row that sees no key yields zeros
                 const int64_t at = (q.r0 + static_cast<int64_t>(i)) * a.ys.token + head * a.ys.head;
+                float *to = part_of(split) + (threadIdx.x & 255);  // [dimension][row]: a warp's rows lie together
 #pragma unroll
                 for (int c = 0; c < D; c += 32) {
                     uint32_t o[32];
-                    if (ntiles > 0) {
+                    if (nsteps > 0) {
                         tmem_ld_32x32b_x32(o_col + c, o);
                         tmem_wait_ld();
+                        pass32(o);
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         float v[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = ntiles > 0 ? __uint_as_float(o[e + k]) * inv : 0.f;
-                        if (live) kv_store8(a, at + c + e, v);
+                        for (int k = 0; k < 8; ++k) v[k] = nsteps > 0 ? __uint_as_float(o[e + k]) * inv : 0.f;
+                        if (n_split > 1) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) to[(c + e + k) * C::kRows] = v[k];
+                        } else if (live) {
+                            kv_store8(a, at + c + e, v);
+                        }
+                    }
+                }
+                if (n_split > 1) to[D * C::kRows] = m, to[(D + 1) * C::kRows] = l;
+            }
+            if (n_split > 1) {
+                // The last of the row tile's blocks joins the parts, in their order.  (Here and not behind the roles:
+                // the other warps have given their registers away.)
+                auto sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(nq * 128) : "memory"); };
+                sync();
+                if (threadIdx.x == 0) {
+                    __threadfence();
+                    *tmem_slot = atomicInc(a.done + group, n_split - 1) == static_cast<unsigned>(n_split - 1);
+                    __threadfence();
+                }
+                sync();
+                if (*tmem_slot && live) {
+                    const int tid = threadIdx.x;
+                    float M = -INFINITY, L = 0.f;
+                    for (int k = 0; k < n_split; ++k) M = fmaxf(M, __ldcg(part_of(k) + D * C::kRows + tid));
+                    for (int k = 0; k < n_split; ++k) {
+                        const float mk = __ldcg(part_of(k) + D * C::kRows + tid);
+                        L = fmaf(__ldcg(part_of(k) + (D + 1) * C::kRows + tid), mk == M ? 1.f : ex2_approx(mk - M), L);
+                    }
+                    const float inv = L == 0.f ? 0.f : 1.f / L;
+                    const int64_t at = (q.r0 + static_cast<int64_t>(i)) * a.ys.token + head * a.ys.head;
+                    for (int d = 0; d < D; d += 32) {
+                        float v[4][8];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e >> 3][e & 7] = 0.f;
+                        for (int k = 0; k < n_split; ++k) {
+                            const float *from = part_of(k) + tid;
+                            const float mk = __ldcg(from + D * C::kRows), f = (mk == M ? 1.f : ex2_approx(mk - M)) * inv;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                v[e >> 3][e & 7] = fmaf(__ldcg(from + (d + e) * C::kRows), f, v[e >> 3][e & 7]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) kv_store8(a, at + d + 8 * e, v[e]);
                     }
                 }
             }
@@ -553,7 +592,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
 }
 
 template <int D>
-cudaError_t launch_tc(const KvAttnArgs &a, int64_t units, cudaStream_t st) {
+cudaError_t launch_tc(const KvAttnArgs &a, cudaStream_t st) {
     using C = Tc<D>;
     if (!(*a.ready & (1u << (16 + (D == 64))))) {
         cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
@@ -564,16 +603,29 @@ cudaError_t launch_tc(const KvAttnArgs &a, int64_t units, cudaStream_t st) {
         if (f.numRegs < kRegsStart) return cudaErrorInvalidConfiguration;
         *a.ready |= 1u << (16 + (D == 64));
     }
-    kv_attn_tc_kernel<D><<<static_cast<unsigned>(units * a.c.heads), C::kThreads, C::kSmem, st>>>(a);
+    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 8) + a.b.n_seqs;
+    kv_attn_tc_kernel<D><<<static_cast<unsigned>(units * a.c.heads * a.splits), C::kThreads, C::kSmem, st>>>(a);
     return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t kv_attn_tc(const KvAttnArgs &a, cudaStream_t st) {
-    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 8) + a.b.n_seqs;
-    if (units * a.c.heads > 0x7fffffff) return cudaErrorInvalidValue;
-    return a.c.D == 64 ? launch_tc<64>(a, units, st) : launch_tc<128>(a, units, st);
+cudaError_t kv_attn_tc(KvAttnArgs a, int num_sms, cudaStream_t st) {
+    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 8) + a.b.n_seqs, groups = units * a.c.heads;
+    // Parts of the key range: the number that gives the shortest schedule of one block an SM, counted in tiles of 128
+    // tokens (about 2 us), a block's start and end as 4 of them and the join of parts as 3.
+    const int64_t span = a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len;
+    const int64_t tiles = std::max((span + 127) / 128, static_cast<int64_t>(1));
+    const int64_t most = std::min(kPartFloats / (256 * (a.c.D + 2)) / std::max(groups, static_cast<int64_t>(1)), static_cast<int64_t>(32));
+    int64_t splits = 1, least = 0x7fffffffffffffff;
+    for (int64_t n = 1; n <= std::max(most, static_cast<int64_t>(1)) && (n == 1 || 2 * n <= tiles); ++n) {
+        const int64_t cost = (groups * n + num_sms - 1) / num_sms * ((tiles + n - 1) / n + (n > 1 ? 7 : 4));
+        if (cost < least) least = cost, splits = n;
+    }
+    if (groups * splits > 0x7fffffff) return cudaErrorInvalidValue;
+    a.splits = static_cast<int>(splits);
+    a.chunk = static_cast<int>((tiles + splits - 1) / splits * 128);
+    return a.c.D == 64 ? launch_tc<64>(a, st) : launch_tc<128>(a, st);
 }
 
 }  // namespace b200
