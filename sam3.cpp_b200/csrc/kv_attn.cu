@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
         const int shares = n_rows >= 4 ? 1 : n_rows == 1 ? 4 : 2;
         float *share = reinterpret_cast<float *>(smem), *share_ml = share + kWarps * F::kRows * D;
         constexpr int kLanes = D / 4, kStep = 32 / kLanes;  // lanes a row, parts a warp and step
+        constexpr int kFlight = 8;                          // loads of a lane on their way at once
         for (int id = warp; id < n_rows * shares; id += kWarps) {
             const int i = id / shares;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -411,11 +412,11 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
                 total = total * f + l1 * f1;
                 v.x = v.x * f + x.x * f1, v.y = v.y * f + x.y * f1, v.z = v.z * f + x.z * f1, v.w = v.w * f + x.w * f1;
             };
-            for (int k0 = (id % shares) * kStep + lane / kLanes; k0 < n_split; k0 += 8 * shares * kStep) {
-                float2 y[8];
-                float4 x[8];
+            for (int k0 = (id % shares) * kStep + lane / kLanes; k0 < n_split; k0 += kFlight * shares * kStep) {
+                float2 y[kFlight];
+                float4 x[kFlight];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
+                for (int u = 0; u < kFlight; ++u) {
                     const int k = k0 + u * shares * kStep;
                     y[u] = make_float2(-INFINITY, 0.f);
                     if (k >= n_split) continue;
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
                     x[u] = __ldcg(reinterpret_cast<const float4 *>(from + static_cast<int64_t>(k) * F::kRows * D));
                 }
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
+                for (int u = 0; u < kFlight; ++u)
                     if (k0 + u * shares * kStep < n_split) add(y[u].x, y[u].y, x[u]);
             }
             if constexpr (kStep == 2) {
@@ -589,7 +590,9 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
     a.causal = causal != 0, a.window = static_cast<int>(std::min<int64_t>(window, 0x7fffffff));
     a.part = k->part, a.done = k->done, a.ready = &k->ready, a.err = k->be->err;
     DeviceScope dev(k->be->device);
-    const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= 64;
+    // us, 8 kv heads of 128, 32 rows a kv head: one sequence of 8000 tokens 39 (few) and 42, of 100000 115 and 117, 16 of
+    // 4000 79 and 71; 64 rows: 41 and 43, 189 and 118, 128 and 94
+    const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= 32;
     const cudaError_t e = few ? kv_attn_few(a, k->be->num_sms, k->be->stream) : kv_attn_tc(a, k->be->num_sms, k->be->stream);
     k->be->count();
     return cuda_ok(e, "kv_attention launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
