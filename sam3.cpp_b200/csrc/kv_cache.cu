@@ -86,12 +86,29 @@ __device__ __forceinline__ Raw8<T> raw8(const T *p) {
     return r;
 }
 
+// Largest magnitude of 8 values by the bits, as those of an f32: infinities and NaN are above all numbers and show.
+__device__ __forceinline__ uint32_t top_bits(const Raw8<float> &r) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(r.v[j])));
+    return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const Raw8<T> &r) {  // 16-bit types, two at a time
+    const uint4 w = *reinterpret_cast<const uint4 *>(&r);
+    constexpr uint32_t k = 0x7fff7fffu;
+    uint32_t m = __vmaxu2(__vmaxu2(w.x & k, w.y & k), __vmaxu2(w.z & k, w.w & k));
+    m = max(m & 0xffffu, m >> 16);
+    const uint16_t h = static_cast<uint16_t>(m);
+    return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&h)));
+}
+
 // Grid (units of one page, groups of kWarps / W slabs); slab = head + heads * (0 keys, 1 values).
 // PER: groups of 8 values that a thread holds.
 template <typename T, bool VEC, int W, int PER = 4>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteArgs a) {
     __shared__ float wmax[kWarps];
-    const int D = a.c.D;
+    const int D = a.c.D, d_log2 = D == 64 ? 6 : 7;
     if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
     KvSeq q;
@@ -117,17 +134,13 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
         const int e = first + (k * W * 32 + thread) * 8;
-        if (e < end) raw[k] = raw8<VEC>(x + static_cast<int64_t>(e / D) * a.xs[w].token + e % D);
+        if (e < end) raw[k] = raw8<VEC>(x + (e >> d_log2) * a.xs[w].token + (e & (D - 1)));
     }
     const float held = there && lo > 0 ? *scale : 0.f;
-    // largest magnitude, by its bits: infinities and NaN are above all numbers and show
     uint32_t bits = 0;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        if (first + (k * W * 32 + thread) * 8 >= end) continue;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) bits = max(bits, __float_as_uint(fabsf(to_f32(raw[k].v[j]))));
-    }
+    for (int k = 0; k < PER; ++k)
+        if (first + (k * W * 32 + thread) * 8 < end) bits = max(bits, top_bits(raw[k]));
     const bool finite = bits < 0x7f800000u;
     float amax = finite ? __uint_as_float(bits) : 0.f;
     if (!finite) {
@@ -152,21 +165,35 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
         __syncwarp();
     }
     const float to = fmaxf(held, amax < kKvSmallest ? 0.f : __fmul_rn(amax, 1.f / 127.f));
-    const float inv = to > 0.f ? __frcp_rn(to) : 0.f, top = fminf(__fmul_rn(127.f, to), kF32Max);
+    const float inv = to > 0.f ? __frcp_rn(to) : 0.f;
+    if (finite) {
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int e = first + (k * W * 32 + thread) * 8;
-        if (e >= end) continue;
-        float v[8];
-        int c[8];
+        for (int k = 0; k < PER; ++k) {
+            const int e = first + (k * W * 32 + thread) * 8;
+            if (e >= end) continue;
+            float v[8];
+            int c[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = to_f32(raw[k].v[j]);
-            if (!finite) v[j] = v[j] == v[j] ? fminf(fmaxf(v[j], -top), top) : 0.f;  // NaN is stored as 0, infinities as the ends
-            c[j] = 0;
+            for (int j = 0; j < 8; ++j) v[j] = to_f32(raw[k].v[j]), c[j] = 0;
+            if (to > 0.f) round_quotients(v, to, inv, c);
+            *reinterpret_cast<uint2 *>(codes + e) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
         }
-        if (to > 0.f) round_quotients(v, to, inv, c);
-        *reinterpret_cast<uint2 *>(codes + e) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+    } else {  // NaN is stored as 0, infinities as the ends
+        const float top = fminf(__fmul_rn(127.f, to), kF32Max);
+#pragma unroll 1
+        for (int e = first + thread * 8; e < end; e += W * 32 * 8) {
+            const Raw8<T> r = raw8<VEC>(x + (e >> d_log2) * a.xs[w].token + (e & (D - 1)));
+            float v[8];
+            int c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = to_f32(r.v[j]);
+                v[j] = v[j] == v[j] ? fminf(fmaxf(v[j], -top), top) : 0.f;
+                c[j] = 0;
+            }
+            if (to > 0.f) round_quotients(v, to, inv, c);
+            *reinterpret_cast<uint2 *>(codes + e) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+        }
     }
     if (there && thread == 0) *scale = to;
     if (to == held) return;
@@ -208,11 +235,12 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
     const int lo = static_cast<int>(max(begin - p0, static_cast<int64_t>(0)));
     const int hi = static_cast<int>(min(q.len - p0, static_cast<int64_t>(1) << a.c.page_log2));
     const int64_t row0 = q.r0 + p0 - begin;
-    const int chunks = D / 16, each = (hi - lo) * chunks;  // 16-code chunks of a slab
+    // 16-byte chunks of a slab, counted over the whole page so that shifts take a number apart
+    const int chunk_log2 = D == 64 ? 2 : 3, each_log2 = a.c.page_log2 + chunk_log2;
     const int slab0 = blockIdx.y * a.slabs, slabs = min(a.slabs, 2 * a.c.heads - slab0);
-#pragma unroll 4
-    for (int id = threadIdx.x; id < slabs * each; id += kThreads) {
-        const int slab = slab0 + id / each, at = id % each, t = lo + at / chunks, d = at % chunks * 16;
+    for (int id = threadIdx.x; id < slabs << each_log2; id += kThreads) {
+        const int slab = slab0 + (id >> each_log2), t = (id >> chunk_log2) & ((1 << a.c.page_log2) - 1), d = (id & ((1 << chunk_log2) - 1)) * 16;
+        if (t < lo || t >= hi) continue;
         const int w = slab >= a.c.heads, head = slab - w * a.c.heads;
         uint4 raw = make_uint4(0u, 0u, 0u, 0u);
         float scale = 0.f;
@@ -223,11 +251,13 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
         T *y = static_cast<T *>(a.y[w]) + head * a.ys[w].head + (row0 + t) * a.ys[w].token + d;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t u[2] = {h ? raw.z : raw.x, h ? raw.w : raw.y};
+            const uint32_t u[2] = {(h ? raw.z : raw.x) ^ 0x80808080u, (h ? raw.w : raw.y) ^ 0x80808080u};
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                v[j] = page < 0 ? 0.f : __fmul_rn(static_cast<float>(static_cast<int8_t>(u[j >> 2] >> (8 * (j & 3)))), scale);
+            for (int j = 0; j < 8; ++j) {  // 2^23 + 128 + code by its bits
+                const float m = __uint_as_float(__byte_perm(u[j >> 2], 0x4b000000u, 0x7550 | (j & 3)));
+                v[j] = __fmul_rn(__fsub_rn(m, 8388736.f), scale);
+            }
             store8<VEC>(y + 8 * h, v);
         }
     }
@@ -363,9 +393,8 @@ extern "C" int sam3b200_kv_read(sam3b200_backend *h, const sam3b200_kv_cache *ca
     if (a.b.n_seqs == 0 || a.b.n_rows == 0) return SAM3B200_STATUS_SUCCESS;
     a.err = be->err;
     DeviceScope dev(be->device);
-    // about 16 K codes a block, fewer where a page gives a call few rows
-    const int most = std::min(1 << a.c.page_log2, a.b.max_rows) * a.c.D;
-    a.slabs = std::min(std::max(16384 / std::max(most, 1), 1), 2 * a.c.heads);
+    // about 16 K codes a block
+    a.slabs = std::min(std::max(16384 / (a.c.D << a.c.page_log2), 1), 2 * a.c.heads);
     const dim3 grid((a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs, (2 * a.c.heads + a.slabs - 1) / a.slabs);
     const bool vec = a.ys[0].aligned16 && a.ys[1].aligned16;
     auto go = [&](auto t) {
