@@ -568,7 +568,7 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
         set_error("kv_attention: %lld query heads over %d kv heads (a positive multiple is needed)", (long long)n_heads, a.c.heads);
         return SAM3B200_STATUS_FAILED;
     }
-    if (!(scale >= 0.f) || !std::isfinite(scale) || window < 0 || (window && !causal)) {
+    if (!(scale >= 0.f) || !std::isfinite(scale * 1.4426950408889634f) || window < 0 || (window && !causal)) {
         set_error("kv_attention: bad scale %g or window %lld (a window needs the causal mask)", scale, (long long)window);
         return SAM3B200_STATUS_FAILED;
     }

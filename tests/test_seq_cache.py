@@ -92,7 +92,7 @@ def test_attention_arguments_are_checked(b200):
     for change, why in ((dict(q=None), "null"), (dict(y=None), "null"), (dict(type=F32), "unsupported types"),
                         (dict(y_type=BF16), "unsupported types"), (dict(q=A + 1), "unaligned"), (dict(y_type=F32, y=A + 2), "unaligned"),
                         (dict(heads=3), "query heads"), (dict(heads=0), "query heads"), (dict(heads=-2), "query heads"),
-                        (dict(scale=-1.0), "bad scale"), (dict(scale=float("nan")), "bad scale"), (dict(scale=float("inf")), "bad scale"),
+                        (dict(scale=-1.0), "bad scale"), (dict(scale=float("nan")), "bad scale"), (dict(scale=float("inf")), "bad scale"), (dict(scale=3e38), "bad scale"),
                         (dict(window=-1), "window"), (dict(causal=0, window=5), "window"),
                         (dict(y_nb=(ctypes.c_int64 * 2)(128, 128)), "strides of y"), (dict(q_nb=(ctypes.c_int64 * 2)(-5, 128)), "strides of q"),
                         ({}, "null handle")):
@@ -100,6 +100,9 @@ def test_attention_arguments_are_checked(b200):
         assert L.sam3b200_kv_attention_run(None, c, b, a["type"], a["q"], a["q_nb"], a["heads"], a["scale"], a["causal"],
                                            a["window"], a["y_type"], a["y"], a["y_nb"]) == b200.STATUS_FAILED
         assert why in b200.last_error(), (change, b200.last_error())
+    keep[1].n_rows = 1 << 27  # a kv head's rows are counted in 32 bits
+    assert L.sam3b200_kv_attention_run(None, c, b, F16, A, None, 2 * 32, 0.1, 1, 0, F16, A, None) == b200.STATUS_FAILED
+    assert "too many" in b200.last_error()
     assert not L.sam3b200_kv_attention_create(None)
     L.sam3b200_kv_attention_free(None)
     L.sam3b200_rope_free(None)
