@@ -189,13 +189,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
         for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(&sc_full[i], 4);
         fence_mbar_init();
     }
-    if (warp == 12) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
-    }
-    tc_fence_before();
     __syncthreads();
-    tc_fence_after();
     constexpr uint32_t tmem = 0;  // all columns are this block's, so they start at 0
 
     if (warp >= 8 && warp < 12) {
@@ -301,6 +295,12 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     } else if (warp >= 12) {
         // ---- MMA issuer ----
         give_regs<kRegsMma>();
+        if (warp == 12) {  // while keys and queries are on their way
+            tmem_alloc(tmem_slot, 512);
+            tmem_relinquish();
+        }
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+        tc_fence_after();
         if (warp - 12 < nq) {
             const int t = warp - 12;
             constexpr uint32_t idesc_s = idesc_f16_f32(128, 64);
@@ -392,23 +392,26 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
 #pragma unroll
                     for (int k = 0; k < kBatch; ++k) {
                         if (a.q_bf16) {
-                            float x[8], top = 0.f;
                             const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+                            float x[8];
 #pragma unroll
-                            for (int n = 0; n < 4; ++n) {
-                                x[2 * n] = __uint_as_float(u[n] << 16);
-                                x[2 * n + 1] = __uint_as_float(u[n] & 0xffff0000u);
-                                top = fmaxf(top, fmaxf(fabsf(x[2 * n]), fabsf(x[2 * n + 1])));
+                            for (int n = 0; n < 4; ++n) x[2 * n] = __uint_as_float(u[n] << 16), x[2 * n + 1] = __uint_as_float(u[n] & 0xffff0000u);
+                            // largest of the 8 by their bits; where all lanes' are in [2^-4, 2^15] f16 holds the rows as they are
+                            uint32_t most = __vmaxu2(__vmaxu2(u[0] & 0x7fff7fffu, u[1] & 0x7fff7fffu), __vmaxu2(u[2] & 0x7fff7fffu, u[3] & 0x7fff7fffu));
+                            most = max(most & 0xffffu, most >> 16);
+                            if (!__all_sync(0xffffffffu, most >= 0x3d80u && most <= 0x4700u)) {
+#pragma unroll
+                                for (int o = kLanes / 2; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                                const int e = min(static_cast<int>(most >> 7), 253);
+                                const float down = e ? __int_as_float((254 - e) << 23) : 1.f;
+                                const float up = __shfl_sync(0xffffffffu, e ? __int_as_float(e << 23) : 1.f, lane % kRowsStep * kLanes);
+                                if (lane / kRowsStep == step0 + k) row_c = up;
+#pragma unroll
+                                for (int n = 0; n < 8; ++n) x[n] *= down;
                             }
-#pragma unroll
-                            for (int o = kLanes / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            const int e = min((__float_as_int(top) >> 23) & 0xff, 253);
-                            const float down = e ? __int_as_float((254 - e) << 23) : 1.f;
-                            const float up = __shfl_sync(0xffffffffu, e ? __int_as_float(e << 23) : 1.f, lane % kRowsStep * kLanes);
-                            if (lane / kRowsStep == step0 + k) row_c = up;
                             __half2 h[4];
 #pragma unroll
-                            for (int n = 0; n < 4; ++n) h[n] = __floats2half2_rn(x[2 * n] * down, x[2 * n + 1] * down);
+                            for (int n = 0; n < 4; ++n) h[n] = __floats2half2_rn(x[2 * n], x[2 * n + 1]);
                             raw[k] = *reinterpret_cast<const uint4 *>(h);
                         }
                         const int row = (warp & 3) * 32 + (step0 + k) * kRowsStep + lane / kLanes;
@@ -486,31 +489,46 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                     }
                 }
                 const float less = m == -INFINITY ? 0.f : m - kPUp;
+                // in sweeps over 8 pairs, so that many exponentials are on their way at once
+                float bb[4], sum[4][2];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) bb[g] = lv[g] - less, sum[g][0] = sum[g][1] = 0.f;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t pk[16];
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float k = fk[2 * c + g], b = lv[2 * c + g] - less;
-                        float s0 = 0.f, s1 = 0.f;
+                    for (int e0 = 0; e0 < 16; e0 += 8) {
+                        float y[2][8];
 #pragma unroll
-                        for (int e = 16 * g; e < 16 * g + 16; e += 2) {
-                            float y0, y1;
-                            fma2(y0, y1, __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]), k, b);
-                            if (e / 2 % 8 >= 8 - kPolyPairs) {
-                                exp2_poly(y0, y1);
-                            } else {
-                                y0 = ex2_approx(y0);
-                                y1 = ex2_approx(y1);
+                        for (int e = 0; e < 8; e += 2)
+#pragma unroll
+                            for (int g = 0; g < 2; ++g)
+                                fma2(y[g][e], y[g][e + 1], __uint_as_float(x[c][16 * g + e0 + e]),
+                                     __uint_as_float(x[c][16 * g + e0 + e + 1]), fk[2 * c + g], bb[2 * c + g]);
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2)
+#pragma unroll
+                            for (int g = 0; g < 2; ++g) {
+                                if ((e0 + e) / 2 >= 8 - kPolyPairs) {
+                                    exp2_poly(y[g][e], y[g][e + 1]);
+                                } else {
+                                    y[g][e] = ex2_approx(y[g][e]);
+                                    y[g][e + 1] = ex2_approx(y[g][e + 1]);
+                                }
                             }
-                            fadd2(s0, s1, s0, s1, y0, y1);
-                            const __half2 h = __floats2half2_rn(y0, y1);
-                            pk[e / 2] = *reinterpret_cast<const uint32_t *>(&h);
-                        }
-                        l = fmaf(s0 + s1, inv_v[2 * c + g], l);
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2)
+#pragma unroll
+                            for (int g = 0; g < 2; ++g) {
+                                fadd2(sum[2 * c + g][0], sum[2 * c + g][1], sum[2 * c + g][0], sum[2 * c + g][1], y[g][e], y[g][e + 1]);
+                                const __half2 h = __floats2half2_rn(y[g][e], y[g][e + 1]);
+                                pk[8 * g + (e0 + e) / 2] = *reinterpret_cast<const uint32_t *>(&h);
+                            }
                     }
                     tmem_st_32x32b_x16(s_at + 16 * c, pk);
                 }
+#pragma unroll
+                for (int g = 0; g < 4; ++g) l = fmaf(sum[g][0] + sum[g][1], inv_v[g], l);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -571,6 +589,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                         float v[4][8];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e >> 3][e & 7] = 0.f;
+#pragma unroll 2
                         for (int k = 0; k < n_split; ++k) {
                             const float *from = part_of(k) + tid;
                             const float mk = __ldcg(from + D * C::kRows), f = (mk == M ? 1.f : ex2_approx(mk - M)) * inv;
