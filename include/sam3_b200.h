@@ -325,7 +325,9 @@ typedef struct sam3b200_kv_batch {
  * scale.  NaN is stored as 0, infinities as the ends of the range.  Codes of
  * positions >= kv_len are left as they are.  Writing the same rows again
  * changes nothing; a shorter kv_len than before (tokens taken back) is fine.
- * Two sequences of one batch may not write to the same page. */
+ * Two sequences of one batch may not write to the same page; a page that
+ * several sequences read (a common prompt) must be full, since a later token
+ * may round its codes again. */
 int sam3b200_kv_write(sam3b200_backend *be, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch, int type,
                       const void *k, const int64_t k_nb[2], const void *v, const int64_t v_nb[2]);
 

@@ -438,6 +438,59 @@ def test_attention_extreme_values(b200, backend, attend, t, rows):
         check_attention(dev, attend, store(x * 1e-30, t), t, start, lens, 2, 1e30)
 
 
+@pytest.mark.parametrize("rows", [1, 50])
+def test_sequences_share_full_pages(b200, backend, attend, rows):
+    """A common prompt's full pages stand in the tables of several sequences; each goes on in pages of its own."""
+    P, D, H = 32, 64, 2
+    table = np.array([[5, 2, 7, 0], [5, 2, 1, 3], [5, 2, 6, 4]])
+    lens = [2 * P + rows, 2 * P + rows + 3, 2 * P + 40]
+    dev = Device(b200, backend, sc.empty_cache(8, H, P, D), table)
+    rng = np.random.default_rng(9)
+    k, v = rng.normal(size=(2 * P, H, D)), rng.normal(size=(2 * P, H, D))
+    dev.write(k, v, "f16", [0, 2 * P, 2 * P, 2 * P], [2 * P] * 3)  # the first sequence's rows; the others have none
+    new = np.array(lens) - 2 * P
+    start = np.concatenate([[0], np.cumsum(new)])
+    dev.write(rng.normal(size=(start[-1], H, D)), rng.normal(size=(start[-1], H, D)), "f16", start, lens)
+    dev.same()
+    q = store(rng.normal(size=(3 * rows, 4, D)), "f16")
+    check_attention(dev, attend, q, "f16", np.arange(4) * rows, lens, 4, 0.125)
+
+
+def test_pages_behind_four_gigabytes(b200, backend, attend):
+    """Codes whose offsets pass 32 bits: written, read and attended to as in a small cache, bit for bit."""
+    P, D, H, lens = 128, 128, 8, [300, 1000]
+    small_table, n = pages_for(lens, P)
+    far = 33000  # pages of 128 KiB
+    far_table = np.where(small_table < n, small_table + far, small_table).astype(np.int32)
+    rng = np.random.default_rng(10)
+    start = np.concatenate([[0], np.cumsum(lens)])
+    k, v = (backend.upload(store(rng.normal(size=(start[-1], H, D)), "bf16")) for _ in range(2))
+    q = {r: backend.upload(store(rng.normal(size=(2 * r, 16, D)), "bf16")) for r in (1, 40)}
+    results = []
+    for pages, table in ((n, small_table), (n + far, far_table)):
+        codes, scales = [backend.alloc(pages * H * P * D) for _ in range(2)], [backend.alloc(pages * H * 4) for _ in range(2)]
+        cache = b200.KVCache(codes[0].ptr, codes[1].ptr, scales[0].ptr, scales[1].ptr, pages, H, P, D)
+        keep = [backend.upload(np.ascontiguousarray(x, np.int32)) for x in (table, start, lens)]
+        batch = b200.KVBatch(keep[0].ptr, table.shape[1], keep[1].ptr, keep[2].ptr, 2, int(start[-1]), max(lens), max(lens))
+        backend.kv_write(cache, batch, TYPES["bf16"], k.ptr, v.ptr)
+        out = [backend.alloc(int(start[-1]) * H * D * 4) for _ in range(2)]
+        backend.kv_read(cache, batch, TYPES["f32"], out[0].ptr, out[1].ptr)
+        got = [o.get((start[-1], H, D), np.float32) for o in out]
+        for r in q:
+            at = backend.upload(np.array([0, r, 2 * r], np.int32))
+            y = backend.alloc(2 * r * 16 * D * 2)
+            b = b200.KVBatch(keep[0].ptr, table.shape[1], at.ptr, keep[2].ptr, 2, 2 * r, r, max(lens))
+            attend.run(cache, b, TYPES["bf16"], q[r].ptr, 16, y.ptr, 0.09)
+            backend.synchronize()
+            got.append(y.get((2 * r, 16, D), np.uint16))
+        backend.synchronize()
+        results.append(got)
+        for x in codes + scales:
+            x.free()
+    assert all(np.array_equal(a, b) for a, b in zip(*results))
+    assert np.abs(results[0][0]).max() > 1
+
+
 def test_results_repeat_bit_for_bit(b200, backend, attend):
     lens = [9000, 100, 5000]
     dev = filled(b200, backend, lens, 32, 128, 2)
