@@ -23,6 +23,14 @@
 // product's layout to the second's by movmatrix.  The warps' partial results
 // are joined through shared memory, the parts' through the workspace by the
 // last block to finish.
+//
+// Measured (32 heads on 8 of 128): 64 sequences of 500 to 8100 tokens 111 us,
+// 4.8 TB/s; 8 heads without groups over 100 and 131 thousand tokens 93 us, 5.1
+// TB/s; one token over 700 10.2 us, 8.3 in a graph, of which 0.8 find the
+// sequence, 1.5 the pages and queries, 0.5 the part, 3 its join.  No unit is
+// full (DRAM 60 to 64 %, issue 45 %): 16 warps an SM wait on their own chains.
+// With the queries as the 16-row operand (8 of 16 rows idle, twice the
+// registers and softmax work) the first took 138 us and the second 111.
 #include <algorithm>
 #include <cmath>
 #include <new>

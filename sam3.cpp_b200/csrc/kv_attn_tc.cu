@@ -25,6 +25,19 @@
 // row's maximum rose by more than kLazy.
 // Tensor memory (512 columns): S_t(i), and P_t(i) over it, at 128 t + 64 (i % 2);
 // O_t at 256 + D t.
+//
+// Bounds, for 128 keys of a block: the products take 2048 cycles at D = 128
+// (half at 64), the exponentials 2048 on the special-function unit, 1536 with
+// a quarter of them on the FMA pipe.  Measured 2.2 us (about 4100 cycles) at
+// D = 128, 1130 TFLOP/s, and 2.0 us at 64, 620 TFLOP/s: the two softmax warps
+// of a sub-partition run in step and leave it idle half of their waits.  A
+// block's start and end cost about 10 us more (8 to its first scores, of
+// which 2 are the query rows and 4 the first keys; 3 from the last).  A whole
+// prompt of 4096 tokens, 32 heads on 8 of 128: 184 us, 745 TFLOP/s; 5184 rows
+// over 10368 tokens, 16 heads of 64: 449 us.  Not kept: two threads a row (212
+// us for the prompt then at 193), one lane polling for a warp (277), the
+// results by whole rows through shared memory (185 to 188: the loop's
+// registers).
 #include <algorithm>
 
 #include "kv_attn.cuh"
@@ -40,7 +53,9 @@ enum { TERR_Q = 1 << 8, TERR_K = 1 << 9, TERR_V = 1 << 10, TERR_FREE = 1 << 11, 
 constexpr int kRegsStart = 128, kRegsSoftmax = 168, kRegsCodes = 120, kRegsMma = 56;
 static_assert(2 * kRegsSoftmax + kRegsCodes + kRegsMma <= 4 * kRegsStart, "register shares");
 
-constexpr int kPolyPairs = 2;  // of 8 pairs of weights, those whose exponential runs on the FMA pipe
+// Of 8 pairs of weights, those whose exponential runs on the FMA pipe (us, prompt and images: 0 pairs 191 and 465, 2
+// 185 and 444, 3 186 and 451).
+constexpr int kPolyPairs = 2;
 
 template <int REGS>
 __device__ __forceinline__ void take_regs() {
