@@ -49,9 +49,13 @@ namespace {
 enum { TERR_Q = 1 << 8, TERR_K = 1 << 9, TERR_V = 1 << 10, TERR_FREE = 1 << 11, TERR_S = 1 << 12, TERR_P = 1 << 13 };
 
 // Registers a thread after the split: a block starts with 128 for each of its
-// four warpgroups, and the shares may not add up to more.
-constexpr int kRegsStart = 128, kRegsSoftmax = 168, kRegsCodes = 120, kRegsMma = 56;
+// four warpgroups, and the shares may not add up to more.  Those that give
+// may not end above the start, nor the one that takes below it: an illegal
+// instruction.
+constexpr int kRegsStart = 128, kRegsSoftmax = 176, kRegsCodes = 104, kRegsMma = 56;
 static_assert(2 * kRegsSoftmax + kRegsCodes + kRegsMma <= 4 * kRegsStart, "register shares");
+static_assert(kRegsSoftmax >= kRegsStart && kRegsCodes <= kRegsStart && kRegsMma <= kRegsStart, "register shares' directions");
+static_assert(kRegsSoftmax % 8 == 0 && kRegsCodes % 8 == 0 && kRegsMma % 8 == 0, "register shares are in eights");
 
 // Of 8 pairs of weights, those whose exponential runs on the FMA pipe (us, prompt and images: 0 pairs 191 and 465, 2
 // 185 and 444, 3 186 and 451).
