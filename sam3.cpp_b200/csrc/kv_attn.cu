@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
     // the tile's keys, and this block's part of them
     const int k_end = kv_last(a, q, i_hi) + 1, k_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
     const int range = max(k_end - k_begin, 0);
-    const int chunk = max(a.chunk, ((range + a.splits - 1) / a.splits + 63) & ~63);
+    const int chunk = max(range < a.short_range ? a.chunk_short : a.chunk, ((range + a.splits - 1) / a.splits + 63) & ~63);
     const int n_split = max((range + chunk - 1) / chunk, 1);
     if (split >= n_split) return;
     const int t_begin = k_begin + split * chunk, t_end = min(t_begin + chunk, k_end);
@@ -486,6 +486,9 @@ cudaError_t launch_few(KvAttnArgs &a, int num_sms, cudaStream_t st) {
     if (units * splits > 0x7fffffff) return cudaErrorInvalidValue;
     a.splits = static_cast<int>(splits);
     a.chunk = static_cast<int>(((span + splits - 1) / splits + 63) & ~int64_t(63));
+    // With few sequences one that is far shorter than max_len (a captured step's bound) is cut finer, into all parts.
+    a.chunk_short = static_cast<int>(2 * groups < wave ? std::min<int64_t>(least, a.chunk) : a.chunk);
+    a.short_range = static_cast<int>(span / 2);
     if (!(*a.ready & (1 << (2 * NT + (D == 64))))) {
         const cudaError_t e = cudaFuncSetAttribute(kv_attn_few_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
         if (e != cudaSuccess) return e;

@@ -17,7 +17,8 @@ struct KvAttnArgs {
     float scale_log2;     // scale * log2(e)
     int causal, window;   // window 0: none
     int splits;           // most parts of a key range
-    int chunk;            // tokens of a part (a multiple of 64, for 256 rows of 128)
+    int chunk;            // least tokens of a part (a multiple of 64, for 256 rows of 128)
+    int chunk_short, short_range;  // the same for key ranges below short_range
     float *part;          // partial results: see kPartFloats
     unsigned *done;       // parts finished, one counter a unit and kv head; 0 between calls
     int *err;

@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     // the rows' keys, and this block's part of them
     const int all_keys_end = kv_last(a, q, i_hi) + 1, all_keys_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
     const int range = max(all_keys_end - all_keys_begin, 0);
-    const int part = max(a.chunk, ((range + a.splits - 1) / a.splits + 127) & ~127);
+    const int part = max(range < a.short_range ? a.chunk_short : a.chunk, ((range + a.splits - 1) / a.splits + 127) & ~127);
     const int n_split = max((range + part - 1) / part, 1);
     if (split >= n_split) return;
     const int k_begin = all_keys_begin + split * part, k_end = min(k_begin + part, all_keys_end);
@@ -663,6 +663,9 @@ cudaError_t kv_attn_tc(KvAttnArgs a, int num_sms, cudaStream_t st) {
     if (groups * splits > 0x7fffffff) return cudaErrorInvalidValue;
     a.splits = static_cast<int>(splits);
     a.chunk = static_cast<int>((tiles + splits - 1) / splits * 128);
+    // with few row tiles a sequence far shorter than max_len is cut finer, into all parts
+    a.chunk_short = 2 * groups < num_sms ? std::min(a.chunk, 256) : a.chunk;
+    a.short_range = static_cast<int>(span / 2);
     return a.c.D == 64 ? launch_tc<64>(a, st) : launch_tc<128>(a, st);
 }
 

@@ -303,7 +303,7 @@ def filled(b200, backend, lens, P, D, H, seed=0, k_size=1.0, spread=0.0):
 
 
 def check_attention(dev, attend, q_raw, t, row_start, kv_len, n_heads, scale, causal=True, window=0, t_out=None, q_nb=None, y_nb=None,
-                    n_rows=None, q=None):
+                    n_rows=None, q=None, max_len=None):
     """Runs the call on packed or strided rows and compares every row of every sequence."""
     be, D = dev.be, dev.host["k_codes"].shape[3]
     t_out = t_out or t
@@ -312,7 +312,7 @@ def check_attention(dev, attend, q_raw, t, row_start, kv_len, n_heads, scale, ca
     qb = be.upload(q_raw)
     size = N * n_heads * D if y_nb is None else (N - 1) * y_nb[0] + (n_heads - 1) * y_nb[1] + D
     yb = be.upload(np.full(size, 77, dtype(t_out)))
-    attend.run(dev.cache, dev.batch(row_start, kv_len, n_rows=N), TYPES[t], qb.ptr, n_heads, yb.ptr, scale, causal=causal, window=window,
+    attend.run(dev.cache, dev.batch(row_start, kv_len, n_rows=N, max_len=max_len), TYPES[t], qb.ptr, n_heads, yb.ptr, scale, causal=causal, window=window,
                y_type=TYPES[t_out], q_nb=q_nb, y_nb=y_nb)
     be.synchronize()
     raw = yb.get(size, dtype(t_out))
@@ -388,6 +388,10 @@ def test_attention_long_contexts_in_parts(b200, backend, attend, rows):
     q = store(np.random.default_rng(1).normal(size=(5 * rows, 4, 128)) * 3, "bf16")
     check_attention(dev, attend, q, "bf16", start, lens, 4, 128 ** -0.5)
     check_attention(dev, attend, q, "bf16", start, lens, 4, 128 ** -0.5, window=5000)
+    # a bound far above every length, as a captured step has it, and one sequence alone under it
+    for bound in (100000, 1 << 30):
+        check_attention(dev, attend, q, "bf16", start, lens, 4, 128 ** -0.5, max_len=bound)
+        check_attention(dev, attend, q[:rows], "bf16", start[:2], lens[:1], 4, 128 ** -0.5, max_len=bound)
 
 
 @pytest.mark.parametrize("rows", [2, 150])
