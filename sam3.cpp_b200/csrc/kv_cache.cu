@@ -301,11 +301,11 @@ bool kv_views(const char *op, const sam3b200_kv_cache *c, const sam3b200_kv_batc
         set_error("%s: null argument", op);
         return false;
     }
-    if (c->n_pages < 1 || c->n_kv_heads < 1 || c->n_kv_heads > 65535 ||
+    if (c->n_pages < 1 || c->n_kv_heads < 1 || c->n_kv_heads > 32767 ||
         (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128) ||
         (c->head_dim != 64 && c->head_dim != 128)) {
         set_error("%s: unsupported cache: %d pages of %d tokens, %d kv heads of %d (pages of 16, 32, 64 or 128 tokens, "
-                  "head dims 64 and 128)",
+                  "at most 32767 heads, head dims 64 and 128)",
                   op, c->n_pages, c->page_tokens, c->n_kv_heads, c->head_dim);
         return false;
     }

@@ -28,7 +28,7 @@ def _batch(b200, **kw):
 
 
 BAD_CACHE = [(dict(k_codes=None), "null"), (dict(v_scale=None), "null"), (dict(n_pages=0), "unsupported cache"),
-             (dict(n_kv_heads=0), "unsupported cache"), (dict(page_tokens=48), "unsupported cache"),
+             (dict(n_kv_heads=0), "unsupported cache"), (dict(n_kv_heads=32768), "unsupported cache"), (dict(page_tokens=48), "unsupported cache"),
              (dict(page_tokens=256), "unsupported cache"), (dict(head_dim=96), "unsupported cache"),
              (dict(v_codes=A + 8), "16-byte"), (dict(k_scale=A + 2), "4-byte")]
 BAD_BATCH = [(dict(table=None), "null"), (dict(row_start=None), "null"), (dict(kv_len=None), "null"),
