@@ -24,10 +24,10 @@
 // are joined through shared memory, the parts' through the workspace by the
 // last block to finish.
 //
-// Measured (32 heads on 8 of 128): 64 sequences of 500 to 8100 tokens 111 us,
-// 4.8 TB/s; 8 heads without groups over 100 and 131 thousand tokens 93 us, 5.1
-// TB/s; one token over 700 10.2 us, 8.3 in a graph, of which 0.8 find the
-// sequence, 1.5 the pages and queries, 0.5 the part, 3 its join.  No unit is
+// Measured (32 heads on 8 of 128): 64 sequences of 500 to 8100 tokens 105
+// to 115 us, 5 to 4.6 TB/s; 8 heads without groups over 100 and 131 thousand
+// tokens 91 to 96 us, 5.2 to 4.9 TB/s; one token over 700 7.8 us, of which 0.8
+// find the sequence, 1.5 the pages and queries, 0.5 the part, 3 its join.  No unit is
 // full (DRAM 60 to 64 %, issue 45 %): 16 warps an SM wait on their own chains.
 // With the queries as the 16-row operand (8 of 16 rows idle, twice the
 // registers and softmax work) the first took 138 us and the second 111.
@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float s_m[kWarps][F::kRows], s_l[kWarps][F::kRows];
     __shared__ int s_last;
+    wait_for_stream();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int kv = blockIdx.y, G = a.group;
     const unsigned unit = blockIdx.x / a.splits;
@@ -495,8 +496,7 @@ cudaError_t launch_few(KvAttnArgs &a, int num_sms, cudaStream_t st) {
         *a.ready |= 1 << (2 * NT + (D == 64));
     }
     const dim3 grid(static_cast<unsigned>(units * a.splits), a.c.heads);
-    kv_attn_few_kernel<D, NT><<<grid, kWarps * 32, F::kSmem, st>>>(a);
-    return cudaGetLastError();
+    return launch_after(kv_attn_few_kernel<D, NT>, grid, kWarps * 32, F::kSmem, st, a);
 }
 
 struct KvAttention {

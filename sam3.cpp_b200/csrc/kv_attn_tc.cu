@@ -34,7 +34,7 @@
 // block's start and end cost about 10 us more (8 to its first scores, of
 // which 2 are the query rows and 4 the first keys; 3 from the last).  A whole
 // prompt of 4096 tokens, 32 heads on 8 of 128: 184 us, 745 TFLOP/s; 5184 rows
-// over 10368 tokens, 16 heads of 64: 449 us.  Not kept: two threads a row (212
+// over 10368 tokens, 16 heads of 64: 444 us.  Not kept: two threads a row (212
 // us for the prompt then at 193), one lane polling for a warp (277), the
 // results by whole rows through shared memory (185 to 188: the loop's
 // registers).
@@ -156,6 +156,7 @@ template <int D>
 __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __grid_constant__ KvAttnArgs a) {
     using C = Tc<D>;
     extern __shared__ uint8_t smem_raw[];
+    wait_for_stream();
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *q_full = reinterpret_cast<uint64_t *>(smem + C::kBars);
     uint64_t *k_full = q_full + 1;       // [2] keys of tile j in slot j % 2
@@ -642,8 +643,7 @@ cudaError_t launch_tc(const KvAttnArgs &a, cudaStream_t st) {
         *a.ready |= 1u << (16 + (D == 64));
     }
     const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 8) + a.b.n_seqs;
-    kv_attn_tc_kernel<D><<<static_cast<unsigned>(units * a.c.heads * a.splits), C::kThreads, C::kSmem, st>>>(a);
-    return cudaGetLastError();
+    return launch_after(kv_attn_tc_kernel<D>, dim3(static_cast<unsigned>(units * a.c.heads * a.splits)), C::kThreads, C::kSmem, st, a);
 }
 
 }  // namespace

@@ -20,11 +20,11 @@
 // (f16) bytes in and 1 out per value, and the other way round on reading.
 //
 // Measured: ragged prompts of 5 sequences, pages of 16, 8 heads of 128 in f16,
-// written and read back in 49 us, 3.9 TB/s (kernels 26 and 23 us: issue 61 and
+// written and read back in 44 us, 4.3 TB/s (kernels 26 and 23 us: issue 61 and
 // 47 %, about 20 and 12 instructions a value; a block's start, 2 us of
 // dependent loads, is the rest).  64 sequences of one token each, written and
-// their last pages read back: 13.4 us, of which the host's two calls take 9 to
-// 13.
+// their last pages read back: 9.7 us, on the device as on the host (two
+// launches).
 #include <algorithm>
 
 #include "kv_cache.cuh"
@@ -115,6 +115,7 @@ __device__ __forceinline__ uint32_t top_bits(const Raw8<T> &r) {  // 16-bit type
 template <typename T, bool VEC, int W, int PER = 4>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ WriteArgs a) {
     __shared__ float wmax[kWarps];
+    wait_for_stream();
     const int D = a.c.D, d_log2 = D == 64 ? 6 : 7;
     if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
@@ -228,6 +229,7 @@ struct ReadArgs {
 // Grid (units of one page, groups of a.slabs slabs); 16 codes a thread and step.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ ReadArgs a) {
+    wait_for_stream();
     const int D = a.c.D;
     if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, true, a.err);
     int64_t local;
@@ -271,16 +273,17 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
 }
 
 template <typename T, bool VEC>
-void launch_write(const WriteArgs &a, cudaStream_t st) {
+cudaError_t launch_write(const WriteArgs &a, cudaStream_t st) {
     // values that a call can put into one slab of a page, 1024 a warp
     const int most = std::min(1 << a.c.page_log2, a.b.max_rows) * a.c.D;
     const int units = (a.b.n_rows >> a.c.page_log2) + 2 * a.b.n_seqs;
     auto grid = [&](int w) { return dim3(units, (2 * a.c.heads + kWarps / w - 1) / (kWarps / w)); };
-    if (most <= 1024) kv_write_kernel<T, VEC, 1><<<grid(1), kThreads, 0, st>>>(a);
-    else if (most <= 2048) kv_write_kernel<T, VEC, 2><<<grid(2), kThreads, 0, st>>>(a);
-    else if (most <= 4096) kv_write_kernel<T, VEC, 4><<<grid(4), kThreads, 0, st>>>(a);
-    else if (most <= 8192) kv_write_kernel<T, VEC, 8><<<grid(8), kThreads, 0, st>>>(a);
-    else kv_write_kernel<T, VEC, 8, 8><<<grid(8), kThreads, 0, st>>>(a);
+    auto go = [&](auto *kernel, int w) { return launch_after(kernel, grid(w), kThreads, 0, st, a); };
+    if (most <= 1024) return go(kv_write_kernel<T, VEC, 1>, 1);
+    if (most <= 2048) return go(kv_write_kernel<T, VEC, 2>, 2);
+    if (most <= 4096) return go(kv_write_kernel<T, VEC, 4>, 4);
+    if (most <= 8192) return go(kv_write_kernel<T, VEC, 8>, 8);
+    return go(kv_write_kernel<T, VEC, 8, 8>, 8);
 }
 
 }  // namespace
@@ -366,14 +369,11 @@ extern "C" int sam3b200_kv_write(sam3b200_backend *h, const sam3b200_kv_cache *c
     const bool vec = a.xs[0].aligned16 && a.xs[1].aligned16;
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (vec) launch_write<T, true>(a, be->stream);
-        else launch_write<T, false>(a, be->stream);
+        return vec ? launch_write<T, true>(a, be->stream) : launch_write<T, false>(a, be->stream);
     };
-    if (type == SAM3B200_TYPE_F32) go(float());
-    else if (type == SAM3B200_TYPE_F16) go(__half());
-    else go(__nv_bfloat16());
+    const cudaError_t e = type == SAM3B200_TYPE_F32 ? go(float()) : type == SAM3B200_TYPE_F16 ? go(__half()) : go(__nv_bfloat16());
     be->count();
-    return cuda_ok(cudaGetLastError(), "kv_write launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
+    return cuda_ok(e, "kv_write launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
 }
 
 extern "C" int sam3b200_kv_read(sam3b200_backend *h, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch,
@@ -406,12 +406,10 @@ extern "C" int sam3b200_kv_read(sam3b200_backend *h, const sam3b200_kv_cache *ca
     const bool vec = a.ys[0].aligned16 && a.ys[1].aligned16;
     auto go = [&](auto t) {
         using T = decltype(t);
-        if (vec) kv_read_kernel<T, true><<<grid, kThreads, 0, be->stream>>>(a);
-        else kv_read_kernel<T, false><<<grid, kThreads, 0, be->stream>>>(a);
+        return vec ? launch_after(kv_read_kernel<T, true>, grid, kThreads, 0, be->stream, a)
+                   : launch_after(kv_read_kernel<T, false>, grid, kThreads, 0, be->stream, a);
     };
-    if (type == SAM3B200_TYPE_F32) go(float());
-    else if (type == SAM3B200_TYPE_F16) go(__half());
-    else go(__nv_bfloat16());
+    const cudaError_t e = type == SAM3B200_TYPE_F32 ? go(float()) : type == SAM3B200_TYPE_F16 ? go(__half()) : go(__nv_bfloat16());
     be->count();
-    return cuda_ok(cudaGetLastError(), "kv_read launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
+    return cuda_ok(e, "kv_read launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
 }

@@ -150,6 +150,35 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
     }
 }
 
+// ---- launches -----------------------------------------------------------------
+// The kernels of this family follow one another in a step's few microseconds,
+// so a launch lets its blocks be placed as the last blocks of the kernel in
+// front of it on the stream leave, without a wait for its memory first
+// (programmatic stream serialisation); each kernel begins with that wait, and
+// reads and writes nothing before it.  A chain of rotary, rotary, write, read
+// and attention in small calls: 21.3 us as a graph and 25.6 called one by one,
+// against 23.2 and 31.9 with plain launches.  Letting the next kernel in when
+// this one starts (launch_dependents) costs the gain again: its blocks then sit
+// beside these with another split of shared memory; 23.8 us.
+__device__ __forceinline__ void wait_for_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const Args &...args) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    cudaGetLastError();  // returned here, not left for the next check
+    return e;
+}
+
 // ---- host ---------------------------------------------------------------------
 
 // Makes `device` current for the scope and restores the caller's device.

@@ -15,8 +15,8 @@
 // shared memory); a thread has 8 pairs of a row in registers and walks over
 // every eighth head with 16-byte loads.  An angle costs 50 to 100
 // instructions, so it is computed once for a row and not by each thread.
-// Measured: 21037 rows of 40 heads of 128, bf16, 80 us, 5.4 TB/s; 5184 rows of
-// 32 heads of 64, f32 to f16, 14.4 us, 4.4 TB/s; 7 rows of 40 heads 2.5 us.
+// Measured: 21037 rows of 40 heads of 128, bf16, 77 us, 5.6 TB/s; 5184 rows of
+// 32 heads of 64, f32 to f16, 12.5 us, 5.1 TB/s; 7 rows of 40 heads 2.3 us.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -82,6 +82,7 @@ struct Stream8 {
 template <typename TX, typename TY, bool NEIGHBOURS>
 __global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeArgs a, int rows) {
     __shared__ float2 turn[128];
+    wait_for_stream();
     const int n = a.t.pairs, each = a.t.head_dim / 16;  // parts of a row
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows;
     const int part = threadIdx.x % each, lane = threadIdx.x / each % kHeadLanes, row_in = threadIdx.x / (each * kHeadLanes);
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeA
 // behind the turned ones, a thread.
 template <typename TX, typename TY>
 __global__ void __launch_bounds__(128) rope_any_kernel(const __grid_constant__ RopeArgs a) {
+    wait_for_stream();
     const int n = a.t.pairs, each = a.t.head_dim - n;
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x;
     const int64_t row64 = id / each;
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(128) rope_any_kernel(const __grid_constant__ R
 }
 
 template <typename TX, typename TY>
-void launch_rope(RopeArgs &a, bool wide, cudaStream_t st, int num_sms) {
+cudaError_t launch_rope(RopeArgs &a, bool wide, cudaStream_t st, int num_sms) {
     if (wide) {
         const int each = a.t.head_dim / 16, rows = std::max(16 / each, 1);  // 128 pairs at most
         const int64_t blocks = (static_cast<int64_t>(a.n_rows) + rows - 1) / rows;
@@ -176,16 +178,15 @@ void launch_rope(RopeArgs &a, bool wide, cudaStream_t st, int num_sms) {
         const int64_t split = (num_sms * int64_t(8) + blocks - 1) / blocks;
         a.heads_each = static_cast<int>((a.n_heads + split - 1) / split + kHeadLanes - 1) / kHeadLanes * kHeadLanes;
         const dim3 grid(static_cast<unsigned>(blocks), (a.n_heads + a.heads_each - 1) / a.heads_each);
-        if (a.t.neighbours) rope_kernel<TX, TY, true><<<grid, rows * each * kHeadLanes, 0, st>>>(a, rows);
-        else rope_kernel<TX, TY, false><<<grid, rows * each * kHeadLanes, 0, st>>>(a, rows);
-        return;
+        return launch_after(a.t.neighbours ? rope_kernel<TX, TY, true> : rope_kernel<TX, TY, false>, grid,
+                            rows * each * kHeadLanes, 0, st, a, rows);
     }
     // a thread walks over all heads where the rows alone fill the GPU (2048 threads an SM), else over fewer
     const int64_t threads = static_cast<int64_t>(a.n_rows) * (a.t.head_dim - a.t.pairs);
     const int64_t split = (num_sms * int64_t(2048) + threads - 1) / threads;
     a.heads_each = static_cast<int>(split >= a.n_heads ? 1 : (a.n_heads + split - 1) / split);
     const dim3 grid(static_cast<unsigned>((threads + 127) / 128), (a.n_heads + a.heads_each - 1) / a.heads_each);
-    rope_any_kernel<TX, TY><<<grid, 128, 0, st>>>(a);
+    return launch_after(rope_any_kernel<TX, TY>, grid, 128, 0, st, a);
 }
 
 }  // namespace
@@ -272,15 +273,13 @@ extern "C" int sam3b200_rope_run(sam3b200_rope *h, int x_type, const void *x, co
     // 16-byte groups of 8 pairs: whole groups, aligned rows
     const bool wide = a.xs.aligned16 && a.ys.aligned16 && a.t.pairs % 8 == 0 && a.t.head_dim % 16 == 0;
     DeviceScope dev(r->be->device);
-    auto go = [&](auto tx, auto ty) { launch_rope<decltype(tx), decltype(ty)>(a, wide, r->be->stream, r->be->num_sms); };
+    auto go = [&](auto tx, auto ty) { return launch_rope<decltype(tx), decltype(ty)>(a, wide, r->be->stream, r->be->num_sms); };
     auto from = [&](auto tx) {
-        if (y_type == SAM3B200_TYPE_F32) go(tx, float());
-        else if (y_type == SAM3B200_TYPE_F16) go(tx, __half());
-        else go(tx, __nv_bfloat16());
+        return y_type == SAM3B200_TYPE_F32 ? go(tx, float()) : y_type == SAM3B200_TYPE_F16 ? go(tx, __half()) : go(tx, __nv_bfloat16());
     };
-    if (x_type == SAM3B200_TYPE_F32) from(float());
-    else if (x_type == SAM3B200_TYPE_F16) from(__half());
-    else from(__nv_bfloat16());
+    const cudaError_t e = x_type == SAM3B200_TYPE_F32   ? from(float())
+                          : x_type == SAM3B200_TYPE_F16 ? from(__half())
+                                                        : from(__nv_bfloat16());
     r->be->count();
-    return cuda_ok(cudaGetLastError(), "rope launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
+    return cuda_ok(e, "rope launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
 }

@@ -593,3 +593,73 @@ def test_a_captured_step_replays_with_new_lengths(b200, backend):
     del graph
     for h in (own, other, rope):
         h.free()
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_wait_for_another_stream_and_are_waited_for(b200, backend, attend, captured):
+    """Every call of a chain follows a kernel of its own stream and, by an event, slow work of another stream that makes
+    its input; and the other stream's work over the results follows the chain.  Any call that started early, or any work
+    that did not see a call's results, gives other numbers."""
+    import torch
+    rng = np.random.default_rng(9)
+    H, G, D, P, S, L = 2, 2, 64, 16, 2, 200
+    width, t = H * G + 2 * H, b200.TYPE_F16
+    table, n = pages_for([L] * S, P)
+    dev = Device(b200, backend, sc.empty_cache(n, H, P, D), table)
+    rope = backend.rope(D, [32])
+    src = torch.from_numpy(rng.normal(size=(S * L, width, D)).astype(np.float16)).cuda()
+    pos = torch.arange(L, dtype=torch.int32, device="cuda").repeat(S)
+    x, out = torch.zeros_like(src), torch.zeros((S * L, H * G, D), dtype=torch.float16, device="cuda")
+    kept = torch.zeros((4, *out.shape), dtype=torch.float16, device="cuda")
+    slow, pad = torch.zeros(1 << 26, device="cuda"), torch.zeros(D, dtype=torch.float16, device="cuda")
+    batch = dev.batch([0, L, 2 * L], [L, L])
+    own, side = torch.cuda.ExternalStream(backend.stream), torch.cuda.Stream()
+    at = lambda head: x.data_ptr() + head * D * 2
+    nb = (width * D, D)
+    torch.cuda.synchronize()
+
+    def work():
+        for i in range(4):
+            side.wait_stream(own)  # the side stream keeps the last results, then makes the next input, slowly
+            with torch.cuda.stream(side):
+                if i:
+                    kept[i - 1].copy_(out)
+                slow.add_(1.0)
+                x.copy_(src).mul_(1.0 + i)
+            if i % 2 == 0:
+                rope.apply(pad.data_ptr(), t, pos.data_ptr(), 1, 1, pad.data_ptr(), t)  # a kernel in front, of no matter
+            own.wait_stream(side)
+            rope.apply(at(0), t, pos.data_ptr(), S * L, H * G + H, at(0), t, x_nb=nb, y_nb=nb)
+            backend.kv_write(dev.cache, batch, t, at(H * G), at(H * G + H), nb, nb)
+            attend.run(dev.cache, batch, t, at(0), H * G, out.data_ptr(), 0.125, q_nb=nb)
+        side.wait_stream(own)
+        with torch.cuda.stream(side):
+            kept[3].copy_(out)
+        own.wait_stream(side)
+
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=own):
+            work()
+        with torch.cuda.stream(own):
+            graph.replay()
+    else:
+        work()
+    torch.cuda.synchronize()
+    backend.synchronize()
+    got = kept.cpu().numpy()
+    # the values' scale is proportional to the input: outputs of step i are those of its own input, computed alone
+    for i in range(4):
+        x.copy_(src).mul_(1.0 + i)
+        torch.cuda.synchronize()
+        rope.apply(at(0), t, pos.data_ptr(), S * L, H * G + H, at(0), t, x_nb=nb, y_nb=nb)
+        backend.synchronize()
+        backend.kv_write(dev.cache, batch, t, at(H * G), at(H * G + H), nb, nb)
+        backend.synchronize()
+        attend.run(dev.cache, batch, t, at(0), H * G, out.data_ptr(), 0.125, q_nb=nb)
+        backend.synchronize()
+        assert np.array_equal(got[i], out.cpu().numpy())
+    assert not np.array_equal(got[0], got[1])
+    if captured:
+        del graph
+    rope.free()
