@@ -31,10 +31,11 @@
 // a quarter of them on the FMA pipe.  Measured 2.2 us (about 4100 cycles) at
 // D = 128, 1130 TFLOP/s, and 2.0 us at 64, 620 TFLOP/s: the two softmax warps
 // of a sub-partition run in step and leave it idle half of their waits.  A
-// block's start and end cost about 10 us more (8 to its first scores, of
-// which 2 are the query rows and 4 the first keys; 3 from the last).  A whole
-// prompt of 4096 tokens, 32 heads on 8 of 128: 184 us, 745 TFLOP/s; 5184 rows
-// over 10368 tokens, 16 heads of 64: 444 us.  Not kept: two threads a row (212
+// block's start and end cost about 9 us more (at D = 128 in bf16 6 to 7 to its
+// first scores, which wait for the query rows; in f16 at 64 under 5, of which 3
+// are the first keys; 3 from the last).  A whole
+// prompt of 4096 tokens, 32 heads on 8 of 128: 181 us, 759 TFLOP/s; 5184 rows
+// over 10368 tokens, 16 heads of 64: 445 us.  Not kept: two threads a row (212
 // us for the prompt then at 193), one lane polling for a warp (277), the
 // results by whole rows through shared memory (185 to 188: the loop's
 // registers).
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
             const int last = live ? kv_last(a, q, i) : -1, first = live ? kv_first(a, last) : 0;
             float row_c = 1.f;
             {  // the warp's 32 rows as f16; bf16 rows are brought to [1, 2) by a power of two, undone by row_c
-                constexpr int kLanes = D / 8, kRowsStep = 32 / kLanes, kBatch = 4;  // lanes a row, rows a step, steps a batch
+                constexpr int kLanes = D / 8, kRowsStep = 32 / kLanes, kBatch = 8;  // lanes a row, rows a step, steps a batch (4: 0.8 % slower on a whole prompt, 16: 0.5 %)
                 const int64_t at = (q.r0 + static_cast<int64_t>(i)) * a.qs.token + head * a.qs.head;
                 const int part = lane % kLanes;
                 for (int step0 = 0; step0 < 32 / kRowsStep; step0 += kBatch) {
