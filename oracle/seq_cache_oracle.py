@@ -1,4 +1,4 @@
-"""The sequence-cache operators in numpy float64, written from their definitions (checker only).
+"""The sequence-cache operators in numpy float64, written from their definitions (the oracle of their tests).
 
 rope: pairs turned by positions of several axes.  write / read: the paged 8-bit cache.  attention: softmax over the
 cached tokens.  The cache is a dict of arrays: k_codes, v_codes int8 [pages][heads][P][D], k_scale, v_scale float32
