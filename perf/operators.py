@@ -5,6 +5,10 @@ listed() and draw() give the cases, prepare() a program's data on the GPU, run()
 in its plain form (elementary torch operations) where `own` is false, by the library's calls where it is true.
 exact() is the operators' definition in 64 bits.
 
+The backend launches on a stream of its own, which waits for no other.  A program that makes its inputs with torch
+makes that stream torch's current one, as prepare() does, and everything is in order; where another stream is current
+when run() is called, the two wait for each other around the calls.  Results are ready on the current stream.
+
 The cache: codes int8 [pages][kv heads][page tokens][head dim] and one f32 scale for each page and kv head, for
 keys and for values.  A sequence's tokens [i P, (i + 1) P) lie in the page that entry i of its row of the block
 table names.  A batch gives each sequence a run of rows (row_start) and its length with these rows (kv_len): its
@@ -37,6 +41,7 @@ def _framework():
         spec.loader.exec_module(mod)
         _kept["mod"], _kept["be"] = mod, mod.Backend(torch.cuda.current_device())
         _kept["attend"] = _kept["be"].kv_attention()
+        _kept["stream"] = torch.cuda.ExternalStream(_kept["be"].stream)
     return _kept["mod"], _kept["be"]
 
 
@@ -213,6 +218,9 @@ def _prepare_cache(case, g):
 
 
 def prepare(case, seed):
+    if own:
+        _framework()
+        torch.cuda.set_stream(_kept["stream"])
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
     st = _prepare_rope(case, g) if case["op"] == "rope" else _prepare_cache(case, g)
@@ -344,25 +352,37 @@ def _plain_attend(st):
 # ---- one pass --------------------------------------------------------------------------------------------------
 
 
+def _calls(st):
+    case = st["case"]
+    mod, be = _framework()
+    types = {torch.float32: mod.TYPE_F32, torch.float16: mod.TYPE_F16, torch.bfloat16: mod.TYPE_BF16}
+    if case["op"] == "rope":
+        x, out = st["x"], st["out"]
+        st["rope"].apply(x.data_ptr(), types[x.dtype], st["pos"].data_ptr(), x.shape[0], x.shape[1], out.data_ptr(),
+                         types[out.dtype])
+        return out
+    if case["op"] == "cache":
+        k, v, k_out, v_out = st["k"], st["v"], st["k_out"], st["v_out"]
+        be.kv_write(st["cache"], st["batch"], types[k.dtype], k.data_ptr(), v.data_ptr())
+        be.kv_read(st["cache"], st["batch_read"], types[k.dtype], k_out.data_ptr(), v_out.data_ptr())
+        return k_out, v_out
+    q, out = st["q"], st["out"]
+    st["attend"].run(st["cache"], st["batch"], types[q.dtype], q.data_ptr(), q.shape[1], out.data_ptr(),
+                     scale=st["scale"], causal=case["causal"], window=case["window"])
+    return out
+
+
 def run(state):
     st, case = state, state["case"]
     if own:
-        mod, be = _framework()
-        types = {torch.float32: mod.TYPE_F32, torch.float16: mod.TYPE_F16, torch.bfloat16: mod.TYPE_BF16}
-        if case["op"] == "rope":
-            x, out = st["x"], st["out"]
-            st["rope"].apply(x.data_ptr(), types[x.dtype], st["pos"].data_ptr(), x.shape[0], x.shape[1], out.data_ptr(),
-                             types[out.dtype])
-            return out
-        if case["op"] == "cache":
-            k, v, k_out, v_out = st["k"], st["v"], st["k_out"], st["v_out"]
-            be.kv_write(st["cache"], st["batch"], types[k.dtype], k.data_ptr(), v.data_ptr())
-            be.kv_read(st["cache"], st["batch_read"], types[k.dtype], k_out.data_ptr(), v_out.data_ptr())
-            return k_out, v_out
-        q, out = st["q"], st["out"]
-        st["attend"].run(st["cache"], st["batch"], types[q.dtype], q.data_ptr(), q.shape[1], out.data_ptr(),
-                         scale=st["scale"], causal=case["causal"], window=case["window"])
-        return out
+        there = _kept["stream"]
+        here = torch.cuda.current_stream(there.device_index)
+        if here.cuda_stream == there.cuda_stream:
+            return _calls(st)
+        there.wait_stream(here)
+        result = _calls(st)
+        here.wait_stream(there)
+        return result
     if case["op"] == "rope":
         return _plain_rope(st)
     if case["op"] == "cache":
