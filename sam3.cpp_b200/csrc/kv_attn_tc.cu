@@ -131,16 +131,26 @@ __device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, f
         : "f"(a0), "f"(a1), "f"(b), "f"(c));
 }
 
+// The largest of three numbers, NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // 2^y of two numbers on the FMA pipe, for y <= 127: the magic sum splits y into an integer n and f in [-1/2, 1/2], a
-// cubic with the least largest relative error there (7.5e-5, found by Remez exchange) gives 2^f, n goes to the exponent.
-// Below -126: 2^-126.
+// cubic with nearly the least largest relative error there (7.8e-5; 7.5e-5 by Remez exchange) gives 2^f, n goes to the
+// exponent.  At the least y that is let through, -127 + 14 / 2^17, the cubic is 1 (its constant was moved by 2e-6 for
+// that), so that n takes all of its bits: the weight of a masked score is 0 exactly, and the weights of a row that sees
+// no key add up to 0.  NaN is not kept.
+constexpr float kPolyLeast = -127.f + 14.f / 131072.f;
 __device__ __forceinline__ void exp2_poly(float &y0, float &y1) {
-    y0 = fmaxf(y0, -126.f), y1 = fmaxf(y1, -126.f);
+    y0 = fmaxf(y0, kPolyLeast), y1 = fmaxf(y1, kPolyLeast);
     float n0, n1, f0, f1;
     fadd2(n0, n1, y0, y1, 12582912.f, 12582912.f);
     fadd2(f0, f1, n0, n1, -12582912.f, -12582912.f);
     fadd2(f0, f1, y0, y1, -f0, -f1);
-    float a0, a1, b0 = 0.69326097f, b1 = 0.69326097f, c0 = 0.99992806f, c1 = 0.99992806f;
+    float a0, a1, b0 = 0.69326097f, b1 = 0.69326097f, c0 = 0.999926f, c1 = 0.999926f;
     fma2(a0, a1, f0, f1, 0.05517167f, 0.24261113f);
     ffma2(b0, b1, a0, a1, f0, f1);
     ffma2(c0, c1, b0, b1, f0, f1);
@@ -485,12 +495,12 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                     const uint32_t *y = &x[g >> 1][16 * (g & 1)];
                     float mx = __uint_as_float(y[0]);
 #pragma unroll
-                    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(y[e]));
-                    top = fmaxf(top, fmaf(mx, fk[g], lv[g]));
+                    for (int e = 1; e < 15; e += 2) mx = max3(mx, __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
+                    top = max3(top, fmaf(mx, fk[g], lv[g]), fmaf(__uint_as_float(y[15]), fk[g], lv[g]));
                 }
                 float alpha = 1.f;
-                if (top > m + kLazy) {
-                    alpha = ex2_approx(m - top);
+                if (!(top <= m + kLazy)) {  // a score that is NaN or +inf makes l NaN, and the row
+                    alpha = ex2_approx(m - top) + (top - top);
                     m = top;
                     l *= alpha;
                 }

@@ -1,0 +1,73 @@
+"""Edges of the sequence-cache operators on the GPU: values far from 1, rows that see nothing beside them, queries that
+are not numbers.
+
+Tolerances are those of test_seq_cache_gpu.py; where a result has no rounding (zeros, NaN) it is asked for as it is.
+bf16 queries that the tcgen05 kernel takes as they are (every 8 elements' largest in [2^-4, 2^15]) lose at most half of
+f16's smallest step, 2^-25, that is 2^-21 of a row's largest element; scores stay below 64 here, so a weight moves by
+less than 2^-12."""
+import numpy as np
+import pytest
+
+import seq_cache_oracle as sc
+from test_seq_cache_gpu import Device, attend, check_attention, pages_for, store  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def sized(b200, backend, lens, P, D, H, size, seed=0):
+    """A cache whose values are of the given size, keys near 1."""
+    rng = np.random.default_rng(seed)
+    table, n = pages_for(lens, P, seed=seed)
+    host = sc.empty_cache(n, H, P, D, seed)
+    rows = np.concatenate([[0], np.cumsum(lens)])
+    sc.write(host, rng.normal(size=(rows[-1], H, D)), rng.normal(size=(rows[-1], H, D)) * size, table, rows, lens)
+    return Device(b200, backend, host, table)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1e4, 1e6, 1e30])
+@pytest.mark.parametrize("length", [50, 64, 128])
+def test_rows_without_keys_beside_large_values(b200, backend, attend, t, D, size, length):
+    """Six rows more than tokens: the first six see nothing and are zero whatever the values' size, in both kernels and
+    under bounds that cut long key ranges into parts."""
+    for G, n in ((4, length + 6), (1, 8)):
+        rows = [n, 3]
+        lens = [n - 6, 3]
+        dev = sized(b200, backend, lens, 16, D, 1, size)
+        q = store(np.random.default_rng(1).normal(size=(n + 3, G, D)), t)
+        for bound in (None, 100000):
+            got = check_attention(dev, attend, q, t, np.concatenate([[0], np.cumsum(rows)]), lens, G, D ** -0.5, t_out="f32", max_len=bound)
+            assert np.all(got[:6] == 0)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [4, 48])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_queries_that_are_not_numbers(b200, backend, attend, t, rows, bad):
+    """One element of every other row: NaN makes the row NaN however few tokens it sees and wherever they lie, infinities
+    what the definition makes of them."""
+    dev = sized(b200, backend, [48 + rows], 16, 64, 1, 1.0)
+    for codes in (dev.host["k_codes"], dev.host["v_codes"]):  # no zeros: the sums of infinities are the definition's
+        codes[codes == 0] = 1
+    for n in ("k_codes", "v_codes"):
+        dev.buf[n].set(dev.host[n])
+    x = np.random.default_rng(2).normal(size=(rows, 1, 64))
+    x[::2, 0, 5] = bad
+    for window in (1, 2, 4, 20, 0):
+        got = check_attention(dev, attend, store(x, t), t, [0, rows], [48 + rows], 1, 0.125, window=window)
+        if np.isnan(bad):
+            assert np.isnan(got[::2]).all()
+        assert not np.isnan(got[1::2]).any()
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("size", [1.0, 1e15, 1e20, 1e35])
+@pytest.mark.parametrize("length", [65, 70, 97, 127])
+def test_values_of_any_size_beside_unused_places(b200, backend, attend, rows, size, length):
+    """Places of a key tile that no token fills weigh nothing, however small the weights 1 / scale of the others are."""
+    for D in (64, 128):
+        dev = sized(b200, backend, [length], 16, D, 1, size)
+        q = store(np.random.default_rng(3).normal(size=(rows, 1, D)), "bf16")
+        check_attention(dev, attend, q, "bf16", [0, rows], [length], 1, D ** -0.5, t_out="f32")
+        check_attention(dev, attend, q, "bf16", [0, rows], [length], 1, D ** -0.5, t_out="f32", causal=False)
