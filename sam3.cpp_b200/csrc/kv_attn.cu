@@ -598,7 +598,8 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
     a.y_type = y_type;
     a.heads = static_cast<int>(n_heads), a.group = static_cast<int>(n_heads / a.c.heads);
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.causal = causal != 0, a.window = static_cast<int>(std::min<int64_t>(window, 0x7fffffff));
+    // a window that no length reaches is none; below 2^30 it cannot pass 32 bits where rows are more than tokens
+    a.causal = causal != 0, a.window = window < a.b.max_len ? static_cast<int>(window) : 0;
     a.part = k->part, a.done = k->done, a.ready = &k->ready, a.err = k->be->err;
     DeviceScope dev(k->be->device);
     // us, 8 kv heads of 128, 32 rows a kv head: one sequence of 8000 tokens 39 (few) and 42, of 100000 115 and 117, 16 of

@@ -1,5 +1,5 @@
 """Edges of the sequence-cache operators on the GPU: values far from 1, rows that see nothing beside them, queries that
-are not numbers.
+are not numbers, windows beyond every length.
 
 Tolerances are those of test_seq_cache_gpu.py; where a result has no rounding (zeros, NaN) it is asked for as it is.
 bf16 queries that the tcgen05 kernel takes as they are (every 8 elements' largest in [2^-4, 2^15]) lose at most half of
@@ -71,3 +71,15 @@ def test_values_of_any_size_beside_unused_places(b200, backend, attend, rows, si
         q = store(np.random.default_rng(3).normal(size=(rows, 1, D)), "bf16")
         check_attention(dev, attend, q, "bf16", [0, rows], [length], 1, D ** -0.5, t_out="f32")
         check_attention(dev, attend, q, "bf16", [0, rows], [length], 1, D ** -0.5, t_out="f32", causal=False)
+
+
+@pytest.mark.parametrize("rows,length", [(6, 3), (9, 2), (80, 20), (300, 290)])
+@pytest.mark.parametrize("window", [1 << 30, (1 << 31) - 1, 1 << 31, 1 << 62])
+def test_windows_beyond_every_length(b200, backend, attend, rows, length, window):
+    """A window that no length reaches is no window, also where the first rows see nothing."""
+    dev = sized(b200, backend, [length, 40], 16, 64, 1, 1.0)
+    q = store(np.random.default_rng(4).normal(size=(2 * rows, 1, 64)), "f16")
+    start, lens = [0, rows, 2 * rows], [length, 40]
+    for bound in (None, 5000):
+        got = check_attention(dev, attend, q, "f16", start, lens, 1, 0.125, window=window, max_len=bound)
+        assert np.array_equal(got, check_attention(dev, attend, q, "f16", start, lens, 1, 0.125, max_len=bound))
