@@ -39,6 +39,7 @@
 // bf16 packed in pairs), PV (64).
 #include "attn.cuh"
 #include "mmq.cuh"
+#include "error_bits.h"
 #include "ptx.cuh"
 #include "tmap.h"
 
@@ -79,6 +80,8 @@ enum : int {
     AERR_S_FULL = 1 << 14,
     AERR_PV_FULL = 1 << 15,
 };
+static_assert(((AERR_Q | AERR_KV_EMPTY | AERR_KV_FULL | AERR_S_EMPTY | AERR_P_FULL | AERR_PV_EMPTY | AERR_S_FULL | AERR_PV_FULL) & kErrData) == 0,
+              "bits of waits");
 
 // Row max over 32 scores (the keys past N are skipped when MASKED).
 template <bool MASKED>

@@ -28,6 +28,7 @@
 // Tensor memory (512 columns): O 0..255, S buffers 256..383, P buffers 384..447.
 #include "attn_mma.cuh"
 #include "attn_tc256.cuh"
+#include "error_bits.h"
 #include "ptx.cuh"
 #include "tmap.h"
 
@@ -56,15 +57,17 @@ struct T256 {
 constexpr float RESCALE_LOG2 = 8.0f;
 
 enum : int {
-    TERR_Q = 1 << 16,
-    TERR_K_EMPTY = 1 << 17,
-    TERR_K_FULL = 1 << 18,
-    TERR_V_EMPTY = 1 << 19,
-    TERR_V_FULL = 1 << 20,
-    TERR_S_FULL = 1 << 21,
-    TERR_P_FULL = 1 << 22,
-    TERR_PV_DONE = 1 << 23,
+    TERR_Q = 1 << 8,
+    TERR_K_EMPTY = 1 << 9,
+    TERR_K_FULL = 1 << 10,
+    TERR_V_EMPTY = 1 << 11,
+    TERR_V_FULL = 1 << 12,
+    TERR_S_FULL = 1 << 13,
+    TERR_P_FULL = 1 << 14,
+    TERR_PV_DONE = 1 << 15,
 };
+static_assert(((TERR_Q | TERR_K_EMPTY | TERR_K_FULL | TERR_V_EMPTY | TERR_V_FULL | TERR_S_FULL | TERR_P_FULL | TERR_PV_DONE) & kErrData) == 0,
+              "bits of waits");
 
 __global__ void __launch_bounds__(T256::THREADS, 1)
     attn_tc256_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,

@@ -26,6 +26,7 @@
 //               f32 output rows.
 // Tensor memory (512 columns): O 0..Dp-1, S buffers 128..383, P buffers 384..511.
 #include "attn_tcw.cuh"
+#include "error_bits.h"
 #include "ptx.cuh"
 #include "tmap.h"
 
@@ -71,6 +72,8 @@ enum : int {
     WERR_P_FULL = 1 << 29,
     WERR_PV_DONE = 1 << 30,
 };
+static_assert(((WERR_Q | WERR_K_EMPTY | WERR_K_FULL | WERR_V_EMPTY | WERR_V_FULL | WERR_S_FULL | WERR_P_FULL | WERR_PV_DONE) & kErrData) == 0,
+              "bits of waits");
 
 // grid (query tiles per window, window groups, heads).  PACK (P > 0): P
 // packed windows per group, one query tile and one key tile; otherwise (P = 0)

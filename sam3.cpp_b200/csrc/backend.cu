@@ -3,8 +3,8 @@
 // tensor-core layout, and the MUL_MAT node.
 #include "../../include/sam3_b200.h"
 #include "backend_impl.h"
+#include "error_bits.h"
 #include "gemm_f16.cuh"
-#include "kv_cache.cuh"
 #include "mmq.cuh"
 #include "vit_ops.cuh"
 
@@ -164,13 +164,18 @@ int sam3b200_backend_synchronize(sam3b200_backend *h) {
     if (!cuda_ok(cudaMemcpy(&e, be->err, sizeof(int), cudaMemcpyDeviceToHost), "read error word"))
         return SAM3B200_STATUS_FAILED;
     if (e != 0) {
-        if (e == (1 << 20))  // ops.cu: a get_rows index outside the source rows
-            set_error("get_rows: row index out of range (error word 0x%x)", e);
-        else if (e & (kErrKvPage | kErrKvBatch))
-            set_error("kv cache:%s%s (error word 0x%x)", e & kErrKvPage ? " page index out of range" : "",
-                      e & kErrKvBatch ? " row_start or kv_len contradicts the batch's sizes" : "", e);
-        else
-            set_error("kernel pipeline wait timed out (error word 0x%x)", e);
+        // kernels of several calls may have set bits: all are named
+        const struct {
+            int bits;
+            const char *what;
+        } errors[] = {{~kErrData, "kernel pipeline wait timed out"},
+                      {kErrGetRowsIndex, "get_rows: row index out of range"},
+                      {kErrKvPage, "kv cache: page index out of range"},
+                      {kErrKvBatch, "kv cache: row_start or kv_len contradicts the batch's sizes"}};
+        char text[256] = "";
+        for (const auto &x : errors)
+            if (e & x.bits) snprintf(text + strlen(text), sizeof(text) - strlen(text), "%s%s", text[0] ? "; " : "", x.what);
+        set_error("%s (error word 0x%x)", text, static_cast<unsigned>(e));
         cudaMemset(be->err, 0, sizeof(int));
         return SAM3B200_STATUS_FAILED;
     }

@@ -12,7 +12,7 @@ struct Backend {
     int device = 0;
     int num_sms = 0;
     cudaStream_t stream = nullptr;
-    int *err = nullptr;  // device error word written by bounded pipeline waits
+    int *err = nullptr;  // device error word (error_bits.h)
     int mmq_impl = 0;    // SAM3B200_MMQ_*
     int mmq_cvt = 0;     // MMQ epilogue int->float conversion (tuning: env SAM3B200_MMQ_CVT=0|1)
     int mmq_bn = 0;      // MMQ tile width: 0 = by K (tuning: env SAM3B200_MMQ_BN=64|128)

@@ -9,12 +9,14 @@
 // limit, so the failure path can be tested without breaking a real kernel.
 #include "../../include/sam3_b200.h"
 #include "backend_impl.h"
+#include "error_bits.h"
 #include "ptx.cuh"
 
 namespace b200 {
 namespace {
 
 constexpr int ERR_DIAG_WAIT = 1 << 24;
+static_assert((ERR_DIAG_WAIT & kErrData) == 0, "bit of a wait");
 
 __global__ void wait_timeout_kernel(int *err, uint64_t limit_ns) {
     __shared__ uint64_t bar;

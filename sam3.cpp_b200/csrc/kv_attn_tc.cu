@@ -48,6 +48,7 @@ namespace b200 {
 namespace {
 
 enum { TERR_Q = 1 << 8, TERR_K = 1 << 9, TERR_V = 1 << 10, TERR_FREE = 1 << 11, TERR_S = 1 << 12, TERR_P = 1 << 13 };
+static_assert(((TERR_Q | TERR_K | TERR_V | TERR_FREE | TERR_S | TERR_P) & kErrData) == 0, "bits of waits");
 
 // Registers a thread after the split: a block starts with 128 for each of its
 // four warpgroups, and the shares may not add up to more.  Those that give

@@ -10,12 +10,9 @@
 
 #include "../../include/sam3_b200.h"
 #include "backend_impl.h"
+#include "error_bits.h"
 
 namespace b200 {
-
-// Bits of the backend's error word (read by sam3b200_backend_synchronize).
-constexpr int kErrKvPage = 1 << 21;   // a block table names a page outside [0, n_pages)
-constexpr int kErrKvBatch = 1 << 22;  // row_start / kv_len contradict the batch's sizes
 
 // Pages whose largest magnitude is below this store zeros under scale 0, so
 // that reciprocals of scales stay finite.

@@ -18,6 +18,7 @@
 // That is the oracle's fma sequence, so results are bit-identical to it.
 #include "act.cuh"
 #include "mmq.cuh"
+#include "error_bits.h"
 #include "ptx.cuh"
 #include "tmap.h"
 
@@ -243,6 +244,7 @@ enum : int {
     ERR_WAIT_TFULL = 16,
     ERR_WAIT_RAW = 32,
 };
+static_assert(((ERR_WAIT_EMPTY | ERR_WAIT_FULL_MMA | ERR_WAIT_TEMPTY | ERR_WAIT_TFULL | ERR_WAIT_RAW) & kErrData) == 0, "bits of waits");
 
 // No-swizzle K-major operand descriptor for the K=16 scale MMA: core
 // matrices of 8 rows x 16 bytes, 8-row groups 128 bytes apart (SBO), the

@@ -33,6 +33,7 @@
 #include "attn.cuh"
 #include "attn_simt.cuh"
 #include "backend_impl.h"
+#include "error_bits.h"
 #include "gemm_f16.cuh"
 #include "vit_ops.cuh"
 #include "../../include/sam3_b200.h"
@@ -40,8 +41,6 @@
 
 namespace b200 {
 namespace {
-
-constexpr int kOpErrGetRowsIndex = 1 << 20;  // get_rows: an index outside [0, nrows)
 
 __host__ __device__ inline int64_t pad8(int64_t k) { return (k + 7) / 8 * 8; }
 
@@ -136,7 +135,7 @@ __global__ void get_rows_kernel(int type, const uint8_t *__restrict__ src, int64
     const int32_t r = idx[i];
     float *d = dst + i * ncols;
     if (r < 0 || r >= nrows) {
-        if (threadIdx.x == 0) atomicOr(err, kOpErrGetRowsIndex);
+        if (threadIdx.x == 0) atomicOr(err, kErrGetRowsIndex);
         for (int64_t c = threadIdx.x; c < ncols; c += blockDim.x) d[c] = 0.f;
         return;
     }

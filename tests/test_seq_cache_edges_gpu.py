@@ -1,5 +1,6 @@
 """Edges of the sequence-cache operators on the GPU: values far from 1, rows that see nothing beside them, queries that
-are not numbers, windows beyond every length.
+are not numbers, windows beyond every length, errors of two
+kinds at once.
 
 Tolerances are those of test_seq_cache_gpu.py; where a result has no rounding (zeros, NaN) it is asked for as it is.
 bf16 queries that the tcgen05 kernel takes as they are (every 8 elements' largest in [2^-4, 2^15]) lose at most half of
@@ -9,7 +10,7 @@ import numpy as np
 import pytest
 
 import seq_cache_oracle as sc
-from test_seq_cache_gpu import Device, attend, check_attention, pages_for, store  # noqa: F401
+from test_seq_cache_gpu import TYPES, Device, attend, check_attention, pages_for, store  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +84,16 @@ def test_windows_beyond_every_length(b200, backend, attend, rows, length, window
     for bound in (None, 5000):
         got = check_attention(dev, attend, q, "f16", start, lens, 1, 0.125, window=window, max_len=bound)
         assert np.array_equal(got, check_attention(dev, attend, q, "f16", start, lens, 1, 0.125, max_len=bound))
+
+
+def test_errors_of_two_kinds_are_both_named(b200, backend):
+    """A wait that ran out and a bad page before one synchronize."""
+    dev = Device(b200, backend, sc.empty_cache(2, 1, 16, 64), [[9]])
+    rows = backend.upload(np.zeros((4, 1, 64), np.float16))
+    batch = dev.batch([0, 4], [4])
+    backend.debug_wait_timeout(2_000_000)
+    backend.kv_write(dev.cache, batch, TYPES["f16"], rows.ptr, rows.ptr)
+    with pytest.raises(b200.B200Error, match="page index") as e:
+        backend.synchronize()
+    assert "timed out" in str(e.value)
+    backend.synchronize()
