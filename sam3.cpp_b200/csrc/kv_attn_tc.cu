@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
             for (int g = 0; g < 2; ++g) {
                 const int tok = k_begin + j * C::kKeys + w * 32 + g * 16;
                 r.p[g] = 0;
-                if (j < ntiles && tok < k_end) r.p[g] = __ldg(a.b.table + s * a.b.table_width + (tok >> a.c.page_log2));
+                if (j < ntiles && tok < k_end) r.p[g] = a.b.table[s * a.b.table_width + (tok >> a.c.page_log2)];
             }
             return r;
         };
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                 for (int i = 0; i < kPer / 2; ++i) {
                     uint4 &v = x[g * (kPer / 2) + i];
                     v = make_uint4(0u, 0u, 0u, 0u);
-                    if (pg.p[g] >= 0) v = __ldg(reinterpret_cast<const uint4 *>(from + i * kTokens * D));
+                    if (pg.p[g] >= 0) v = *reinterpret_cast<const uint4 *>(from + i * kTokens * D);
                 }
             }
         };

@@ -85,7 +85,7 @@ __device__ __forceinline__ Raw8<T> raw8(const T *p) {
     if constexpr (VEC) {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-            reinterpret_cast<uint4 *>(&r)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+            reinterpret_cast<uint4 *>(&r)[i] = reinterpret_cast<const uint4 *>(p)[i];
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) r.v[i] = p[i];
@@ -254,8 +254,8 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
         uint4 raw = make_uint4(0u, 0u, 0u, 0u);
         float scale = 0.f;
         if (page >= 0) {
-            raw = __ldg(reinterpret_cast<const uint4 *>(a.c.codes[w] + kv_slab(a.c, page, head) + t * D + d));
-            scale = __ldg(a.c.scale[w] + static_cast<int64_t>(page) * a.c.heads + head);
+            raw = *reinterpret_cast<const uint4 *>(a.c.codes[w] + kv_slab(a.c, page, head) + t * D + d);
+            scale = a.c.scale[w][static_cast<int64_t>(page) * a.c.heads + head];
         }
         T *y = static_cast<T *>(a.y[w]) + head * a.ys[w].head + (row0 + t) * a.ys[w].token + d;
 #pragma unroll

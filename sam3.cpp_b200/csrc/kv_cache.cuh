@@ -152,11 +152,13 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
 // so a launch lets its blocks be placed as the last blocks of the kernel in
 // front of it on the stream leave, without a wait for its memory first
 // (programmatic stream serialisation); each kernel begins with that wait, and
-// reads and writes nothing before it.  A chain of rotary, rotary, write, read
-// and attention in small calls: 21.3 us as a graph and 25.6 called one by one,
-// against 23.2 and 31.9 with plain launches.  Letting the next kernel in when
-// this one starts (launch_dependents) costs the gain again: its blocks then sit
-// beside these with another split of shared memory; 23.8 us.
+// reads and writes nothing before it.  It reads through ordinary loads: the
+// read-only ones ask for memory that nobody writes from a kernel's start, which
+// here lies before the end of the kernel in front.  A chain of rotary, rotary,
+// write, read and attention in small calls: 21.3 us as a graph and 25.6 called
+// one by one, against 23.2 and 31.9 with plain launches.  Letting the next
+// kernel in when this one starts (launch_dependents) costs the gain again: its
+// blocks then sit beside these with another split of shared memory; 23.8 us.
 __device__ __forceinline__ void wait_for_stream() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <typename... Params, typename... Args>

@@ -1,4 +1,4 @@
-"""CPU checks around the sequence-cache kernels: the backend's error word."""
+"""CPU checks around the sequence-cache kernels: the backend's error word, and loads of kernels that are placed early."""
 import glob
 import os
 import re
@@ -20,3 +20,12 @@ def test_bits_of_wrong_data_mean_nothing_else():
             (data if what.startswith("kErr") or what.startswith("kOpErr") else waits).setdefault(int(bit), []).append((name, what))
     assert not set(data) & set(waits), {b: data[b] + waits[b] for b in set(data) & set(waits)}
     assert len(data) == sum(len(v) for v in data.values()) == 3 and sum(len(v) for v in waits.values()) > 20
+
+
+def test_kernels_placed_early_read_through_coherent_loads():
+    """Kernels that wait_for_stream() are on the GPU before the kernel in front has written its results: read-only loads
+    ask for memory that nothing writes from a kernel's start to its end."""
+    files = [(name, text) for name, text in _sources() if "wait_for_stream()" in text]
+    assert len(files) >= 4
+    for name, text in files:
+        assert "__ldg" not in text and "global.nc" not in text, name
