@@ -1,6 +1,6 @@
 """Edges of the sequence-cache operators on the GPU: values far from 1, rows that see nothing beside them, queries that
 are not numbers, windows beyond every length, errors of two
-kinds at once.
+kinds at once, many sequences, results over the queries.
 
 Tolerances are those of test_seq_cache_gpu.py; where a result has no rounding (zeros, NaN) it is asked for as it is.
 bf16 queries that the tcgen05 kernel takes as they are (every 8 elements' largest in [2^-4, 2^15]) lose at most half of
@@ -97,3 +97,43 @@ def test_errors_of_two_kinds_are_both_named(b200, backend):
         backend.synchronize()
     assert "timed out" in str(e.value)
     backend.synchronize()
+
+
+@pytest.mark.parametrize("seqs", [129, 700])
+@pytest.mark.parametrize("new", [1, 40])
+def test_more_sequences_than_a_block_has_threads(b200, backend, attend, seqs, new):
+    """Sequences are found in several turns; some of them have no rows."""
+    rng = np.random.default_rng(seqs + new)
+    P, D, H, G = 16, 64, 1, 1
+    rows = rng.integers(0, new + 1, seqs)
+    rows[-1] = new
+    lens = rows + rng.integers(0, 40, seqs)
+    table, n = pages_for(lens, P)
+    dev = Device(b200, backend, sc.empty_cache(n, H, P, D), table)
+    every = np.concatenate([[0], np.cumsum(lens)])
+    start = np.concatenate([[0], np.cumsum(rows)])
+    k, v = rng.normal(size=(every[-1], H, D)), rng.normal(size=(every[-1], H, D))
+    dev.write(k, v, "f16", every, lens)
+    dev.same()
+    out = [backend.alloc(int(start[-1]) * H * D * 4) for _ in range(2)]
+    backend.kv_read(dev.cache, dev.batch(start, lens), TYPES["f32"], out[0].ptr, out[1].ptr)
+    backend.synchronize()
+    for got, want in zip(out, sc.read(dev.host, table, start, lens)):
+        assert np.array_equal(got.get(want.shape, np.float32), want.astype(np.float32))
+    q = store(rng.normal(size=(start[-1], H * G, D)), "f16")
+    check_attention(dev, attend, q, "f16", start, lens, H * G, 0.125)
+    check_attention(dev, attend, q, "f16", start, lens, H * G, 0.125, causal=False)
+
+
+@pytest.mark.parametrize("rows,length", [(1, 5000), (5, 700), (60, 5000), (300, 300)])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_results_over_the_queries(b200, backend, attend, t, rows, length):
+    """y may be q: every block reads its queries before any block of the same rows stores results."""
+    dev = sized(b200, backend, [length, 100 + rows], 64, 128, 2, 1.0)
+    start, lens = np.array([0, rows, 2 * rows]), [length, 100 + rows]
+    q = store(np.random.default_rng(5).normal(size=(2 * rows, 8, 128)), t)
+    apart = check_attention(dev, attend, q, t, start, lens, 8, 128 ** -0.5)
+    buf = backend.upload(q)
+    attend.run(dev.cache, dev.batch(start, lens), TYPES[t], buf.ptr, 8, buf.ptr, 128 ** -0.5)
+    backend.synchronize()
+    assert np.array_equal(store(apart, t), buf.get(q.shape, q.dtype))
