@@ -596,14 +596,16 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
     if (a.b.n_seqs == 0 || a.b.n_rows == 0) return SAM3B200_STATUS_SUCCESS;
     a.q_bf16 = type == SAM3B200_TYPE_BF16;
     a.y_type = y_type;
-    a.heads = static_cast<int>(n_heads), a.group = static_cast<int>(n_heads / a.c.heads);
+    a.group = static_cast<int>(n_heads / a.c.heads);
     a.scale_log2 = scale * 1.4426950408889634f;
     // a window that no length reaches is none; below 2^30 it cannot pass 32 bits where rows are more than tokens
     a.causal = causal != 0, a.window = window < a.b.max_len ? static_cast<int>(window) : 0;
     a.part = k->part, a.done = k->done, a.ready = &k->ready, a.err = k->be->err;
     DeviceScope dev(k->be->device);
-    // us, 8 kv heads of 128, 32 rows a kv head: one sequence of 8000 tokens 39 (few) and 42, of 100000 115 and 117, 16 of
-    // 4000 79 and 71; 64 rows: 41 and 43, 189 and 118, 128 and 94
+    // us in a graph, 8 kv heads, few rows and tc, for one sequence of 8000 tokens, one of 100000, 16 of 4000.  Heads of 128:
+    // 16 rows a kv head 28 and 35, 84 and 112, 51 and 67; 32 rows 36 and 35, 113 and 111, 76 and 68; 64 rows 39 and 35, 185
+    // and 112, 125 and 89.  Heads of 64: 16 rows 17 and 24, 54 and 88, 36 and 56; 32 rows 23 and 24, 77 and 89, 53 and 57;
+    // 64 rows 27 and 24, 121 and 88, 86 and 71
     const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= 32;
     const cudaError_t e = few ? kv_attn_few(a, k->be->num_sms, k->be->stream) : kv_attn_tc(a, k->be->num_sms, k->be->stream);
     k->be->count();

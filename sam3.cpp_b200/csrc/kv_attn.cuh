@@ -13,7 +13,7 @@ struct KvAttnArgs {
     RowTensor qs, ys;
     int q_bf16;           // else f16
     int y_type;           // SAM3B200_TYPE_*
-    int heads, group;     // query heads, query heads of a kv head
+    int group;            // query heads of a kv head
     float scale_log2;     // scale * log2(e)
     int causal, window;   // window 0: none
     int splits;           // most parts of a key range
@@ -27,10 +27,14 @@ struct KvAttnArgs {
 
 // 2^x scores: P = 2^(t - m + kPUp) with m within kLazy of the running
 // maximum, so f16 P reaches 2^(kPUp + kLazy) < 65504 at most, and what falls
-// below f16's smallest number is 2^-32 of the largest.
+// below f16's smallest number is 2^-32 of the largest.  P is rounded to f16
+// because the matrix instructions take the codes exactly only as f16: at
+// most 2^-11 of a weight, against 2^-8 as bf16; tf32 runs at half the rate.  The sum of the weights takes them unrounded, in f32.
 constexpr float kPUp = 7.f, kLazy = 8.f;
 
-// Scale of a value page that holds only zeros, as the softmax weights see it.
+// Scale of a value page that holds only zeros, as the softmax weights see it:
+// low, so that the other pages' weights keep their bits (scales from 2^-90
+// on), and not so low that its own leave the sum beside scales up to 2^20.
 constexpr float kZeroScaleLog2 = -80.f;
 
 // The device workspace of a handle: parts of key ranges, each [rows][D + 2] (sums, maximum, weight), of 8 or 16 rows
@@ -58,7 +62,7 @@ __device__ __forceinline__ void kv_store8(const KvAttnArgs &a, int64_t at, const
     else put(static_cast<__nv_bfloat16 *>(a.y));
 }
 
-cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st);  // kv_attn.cu: 16 rows a block
+cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st);  // kv_attn.cu: 8 or 16 rows a block
 cudaError_t kv_attn_tc(KvAttnArgs a, int num_sms, cudaStream_t st);   // kv_attn_tc.cu: 256 rows a block
 
 }  // namespace b200

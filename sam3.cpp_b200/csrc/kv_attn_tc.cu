@@ -57,6 +57,7 @@ static_assert(((TERR_Q | TERR_K | TERR_V | TERR_FREE | TERR_S | TERR_P) & kErrDa
 constexpr int kRegsStart = 128, kRegsSoftmax = 176, kRegsCodes = 104, kRegsMma = 56;
 static_assert(2 * kRegsSoftmax + kRegsCodes + kRegsMma <= 4 * kRegsStart, "register shares");
 static_assert(kRegsSoftmax >= kRegsStart && kRegsCodes <= kRegsStart && kRegsMma <= kRegsStart, "register shares' directions");
+// (ptxas spills 4 bytes of the D = 128 kernel's 128 registers and 8 of the other's; the shares were measured with that.)
 static_assert(kRegsSoftmax % 8 == 0 && kRegsCodes % 8 == 0 && kRegsMma % 8 == 0, "register shares are in eights");
 
 // Of 8 pairs of weights, those whose exponential runs on the FMA pipe (us, prompt and images: 0 pairs 191 and 465, 2
@@ -428,7 +429,8 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                             float x[8];
 #pragma unroll
                             for (int n = 0; n < 4; ++n) x[2 * n] = __uint_as_float(u[n] << 16), x[2 * n + 1] = __uint_as_float(u[n] & 0xffff0000u);
-                            // largest of the 8 by their bits; where all lanes' are in [2^-4, 2^15] f16 holds the rows as they are
+                            // largest of the 8 by their bits; where all lanes' are in [2^-4, 2^15] f16 holds the rows as they are,
+                            // to half its smallest step, 2^-25, that is 2^-21 of a row's largest element
                             uint32_t most = __vmaxu2(__vmaxu2(u[0] & 0x7fff7fffu, u[1] & 0x7fff7fffu), __vmaxu2(u[2] & 0x7fff7fffu, u[3] & 0x7fff7fffu));
                             most = max(most & 0xffffu, most >> 16);
                             if (!__all_sync(0xffffffffu, most >= 0x3d80u && most <= 0x4700u)) {

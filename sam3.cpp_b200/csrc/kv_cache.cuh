@@ -118,21 +118,6 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 
 // Eight consecutive elements; VEC: p is 16-byte aligned.
 template <bool VEC, typename T>
-__device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
-    if constexpr (VEC) {
-        uint4 raw[sizeof(T) / 2];
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = reinterpret_cast<const uint4 *>(p)[i];
-        const T *e = reinterpret_cast<const T *>(raw);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
-    }
-}
-
-template <bool VEC, typename T>
 __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
     if constexpr (VEC) {
         uint4 raw[sizeof(T) / 2];
