@@ -261,8 +261,11 @@ int sam3b200_get_rows(sam3b200_backend *be, int type, const void *src, int64_t n
  * backend stream, allocates nothing and may be captured into a CUDA graph. */
 #define SAM3B200_TYPE_BF16 30 /* enum ggml_type GGML_TYPE_BF16 */
 
-/* Rotary positions of one to four axes, as ggml_rope_ext / ggml_rope_multi
- * turn them.  Pair i of a head, i < pairs = sum of sections, is turned by
+/* Rotary positions of one to four axes: the pairings and sections of
+ * ggml_rope_ext / ggml_rope_multi, with one base and one linear scale of the
+ * positions.  Their tables of factors a frequency and their extrapolation
+ * parameters (ext_factor, attn_factor, beta_fast, beta_slow) have no
+ * counterpart here.  Pair i of a head, i < pairs = sum of sections, is turned by
  * pos_scale * pos[axis(i)] * w(i):
  *   neighbours 0: elements i and i + pairs; 1: elements 2i and 2i + 1;
  *   deal 0: the first sections[0] pairs belong to axis 0, the next to axis 1,
@@ -332,7 +335,7 @@ int sam3b200_kv_write(sam3b200_backend *be, const sam3b200_kv_cache *cache, cons
                       const void *k, const int64_t k_nb[2], const void *v, const int64_t v_nb[2]);
 
 /* The reverse: the last rows of each sequence, kv_len - rows .. kv_len - 1, as
- * code * scale rounded to `type`. */
+ * code * scale rounded to `type`.  k and v may not overlap. */
 int sam3b200_kv_read(sam3b200_backend *be, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch, int type,
                      void *k, const int64_t k_nb[2], void *v, const int64_t v_nb[2]);
 
@@ -346,12 +349,19 @@ void sam3b200_kv_attention_free(sam3b200_kv_attention *h);
 /* y = softmax(scale * q k^T + mask) v over the cached tokens, query head h
  * reading kv head h / (n_heads / n_kv_heads).  causal 1: the rows of a
  * sequence are its last tokens, row i sees tokens 0 .. kv_len - rows + i, of
- * these the last `window` if window > 0; causal 0: every row sees all kv_len
+ * these the last `window` if window > 0 (any number; one that no length reaches
+ * is none); causal 0: every row sees all kv_len
  * tokens, which need not include the rows (window 0).  A row that sees no
- * token yields zeros.  q: F16 or BF16; y: q's type or F32.  Products are
- * exact in the codes, sums and softmax statistics f32, softmax weights
- * rounded to f16: within 2^-10 of the largest cached magnitude, plus the
- * rounding to y's type.  scale >= 0. */
+ * token yields zeros, any other with a NaN in its query NaN.  q: F16 or BF16; y:
+ * q's type or F32, and it may be q (same type and strides) but not overlap it
+ * otherwise.  Products are exact in the codes, sums and softmax statistics
+ * f32, softmax weights rounded to f16, BF16 queries to f16 (2^-21 of a row's
+ * largest element): within 2^-10 of the largest cached magnitude, plus the
+ * rounding to y's type.  That holds where the value scales of the pages that a
+ * row sees lie within 2^100 of one another, beside a page of zeros between
+ * 2^-90 and 2^20 (else weights may be lost), and where scale times a page's
+ * key scale, and scale times a BF16 row's largest element, are ordinary f32
+ * numbers.  scale >= 0. */
 int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch,
                               int type, const void *q, const int64_t q_nb[2], int64_t n_heads, float scale, int causal,
                               int64_t window, int y_type, void *y, const int64_t y_nb[2]);

@@ -137,3 +137,17 @@ def test_results_over_the_queries(b200, backend, attend, t, rows, length):
     attend.run(dev.cache, dev.batch(start, lens), TYPES[t], buf.ptr, 8, buf.ptr, 128 ** -0.5)
     backend.synchronize()
     assert np.array_equal(store(apart, t), buf.get(q.shape, q.dtype))
+
+
+@pytest.mark.parametrize("rows", [1, 48])
+@pytest.mark.parametrize("sizes", [(0, 1e7), (1e7, 0), (0, 1e-25), (1e-25, 0), (1e-14, 1e14), (1e14, 1e-14)])
+def test_pages_of_far_sizes_side_by_side(b200, backend, attend, rows, sizes):
+    """Value scales at the ends of the range that the accuracy is stated for: their weights all stay in the sum."""
+    P = 64
+    table, n = pages_for([4 * P], P)
+    dev = Device(b200, backend, sc.empty_cache(n, 1, P, 64), table)
+    rng = np.random.default_rng(6)
+    size = np.repeat(np.tile(sizes, 2), P)[:, None, None]
+    dev.write(rng.normal(size=(4 * P, 1, 64)), rng.normal(size=(4 * P, 1, 64)) * size, "f32", [0, 4 * P], [4 * P])
+    q = store(rng.normal(size=(rows, 1, 64)), "f16")
+    check_attention(dev, attend, q, "f16", [0, rows], [4 * P], 1, 0.125, t_out="f32")
