@@ -35,7 +35,7 @@
 // first scores, which wait for the query rows; in f16 at 64 under 5, of which 3
 // are the first keys; 3 from the last).  A whole
 // prompt of 4096 tokens, 32 heads on 8 of 128: 181 us, 759 TFLOP/s; 5184 rows
-// over 10368 tokens, 16 heads of 64: 445 us.  Not kept: two threads a row (212
+// over 10368 tokens, 16 heads of 64: 443 us.  Not kept: two threads a row (212
 // us for the prompt then at 193), one lane polling for a warp (277), the
 // results by whole rows through shared memory (185 to 188: the loop's
 // registers).
