@@ -358,10 +358,11 @@ void sam3b200_kv_attention_free(sam3b200_kv_attention *h);
  * f32, softmax weights rounded to f16, BF16 queries to f16 (2^-21 of a row's
  * largest element): within 2^-10 of the largest cached magnitude, plus the
  * rounding to y's type.  That holds where the value scales of the pages that a
- * row sees lie within 2^100 of one another, beside a page of zeros between
- * 2^-90 and 2^20 (else weights may be lost), and where scale times a page's
- * key scale, and scale times a BF16 row's largest element, are ordinary f32
- * numbers.  scale >= 0. */
+ * row sees are 0 (a page of zeros) or at least 2^-90, and lie within 2^100 of
+ * one another, beside a page of zeros below 2^20 (else weights may leave the
+ * sum, or the sum f32's range), and where scale times a page's key scale, and
+ * scale times a BF16 row's largest element, are ordinary f32 numbers.
+ * scale >= 0. */
 int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch,
                               int type, const void *q, const int64_t q_nb[2], int64_t n_heads, float scale, int causal,
                               int64_t window, int y_type, void *y, const int64_t y_nb[2]);

@@ -151,3 +151,12 @@ def test_pages_of_far_sizes_side_by_side(b200, backend, attend, rows, sizes):
     dev.write(rng.normal(size=(4 * P, 1, 64)), rng.normal(size=(4 * P, 1, 64)) * size, "f32", [0, 4 * P], [4 * P])
     q = store(rng.normal(size=(rows, 1, 64)), "f16")
     check_attention(dev, attend, q, "f16", [0, rows], [4 * P], 1, 0.125, t_out="f32")
+
+
+@pytest.mark.parametrize("rows", [1, 48])
+@pytest.mark.parametrize("size", [1e-25, 1e35])
+def test_long_contexts_of_far_sizes(b200, backend, attend, rows, size):
+    """The sum of weights over value scales stays in f32 over a long context."""
+    dev = sized(b200, backend, [100000], 128, 64, 1, size)
+    q = store(np.random.default_rng(7).normal(size=(rows, 1, 64)), "bf16")
+    check_attention(dev, attend, q, "bf16", [0, rows], [100000], 1, 0.125, t_out="f32")
