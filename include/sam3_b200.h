@@ -184,6 +184,23 @@ int sam3b200_set_arith(sam3b200_backend *be, int arith);
 int sam3b200_mul_mat_dq16(sam3b200_backend *be, const sam3b200_weight *w, const float *x, int64_t ldx, int64_t M,
                           const float *bias, float *dst, int64_t ldd);
 
+/* GGML_OP_MUL_MAT of a few rows (1 to 16: a step of single tokens) with Q4_0
+ * or Q4_1 weights, the activations taken as they are instead of quantised:
+ *   dst[m][n] = sum_k w[n][k] * x[m][k]  (+ bias[n]),  w[n][k] the block's value.
+ * x: device rows of K elements of x_type (F32, F16, BF16), row stride ldx
+ * elements; bias: device f32 [N] or NULL; dst: device rows of y_type (F32, or
+ * x_type), row stride ldd.  Products are exact in codes and activations (F16
+ * as they are; BF16, and F32 as a sum of two, in f16 after a power of two a row:
+ * 2^-23 of an F32 element, and 2^-39 of the row's largest one where that is at
+ * least 2^-112, may be lost), a block's sum is scaled and added in f32, in an
+ * order that the shapes fix, and rounded once to y_type.  The
+ * weights are the handle's own codes, with their scales a second time in 2
+ * (Q4_1: 4) bytes a block, made by sam3b200_weight_upload.  Other weight types
+ * and more rows are refused with an error: sam3b200_mul_mat takes them.
+ * Allocates nothing.  Asynchronous on the backend stream. */
+int sam3b200_mul_mat_vec(sam3b200_backend *be, const sam3b200_weight *w, int x_type, const void *x, int64_t ldx,
+                         int64_t M, const float *bias, int y_type, void *dst, int64_t ldd);
+
 /* GGML_OP_FLASH_ATTN_EXT as the ViT blocks use it (sam3.cpp:3778: no mask,
  * max_bias 0, logit softcap 0): dst = softmax(q k^T * scale) v per (head,
  * batch).  q, k, v: device f32 ggml tensors [D, N, heads, batch], contiguous
@@ -290,6 +307,26 @@ int sam3b200_rope_run(sam3b200_rope *r, int x_type, const void *x, const int64_t
                       int64_t pos_stride, int64_t n_rows, int64_t n_heads, int inverse, int y_type, void *y,
                       const int64_t y_nb[2]);
 
+/* Queries and keys normalised for each head, then turned as sam3b200_rope_run
+ * turns them, in one pass: u = (x - mu) / sqrt(var + eps) * weight + bias over
+ * the head_dim elements of a head; layer 0 (RMS norm): mu = 0 and var the mean
+ * square; layer 1 (layer norm): the mean and the mean square around it.  The
+ * 1 to 4 sets of heads (queries, keys, ...) have weights of their own and
+ * share rows, positions and types.  All sums are f32 (elements up to f32's
+ * largest are taken; eps > 0), and y is rounded once.  A set may have no heads.
+ * y may be x of the same set (one type, the same strides); no other tensors may
+ * overlap.  Weights and biases: device [head_dim] of w_type (F32, F16, BF16). */
+typedef struct sam3b200_norm_heads {
+    const void *x;
+    const int64_t *x_nb;      /* element strides {row, head}, NULL for packed rows */
+    const void *weight, *bias; /* NULL: ones, zeros */
+    void *y;
+    const int64_t *y_nb;
+    int64_t n_heads;
+} sam3b200_norm_heads;
+int sam3b200_rope_norm_run(sam3b200_rope *r, const sam3b200_norm_heads *sets, int n_sets, int x_type, int w_type,
+                           int layer, float eps, const int32_t *pos, int64_t pos_stride, int64_t n_rows, int y_type);
+
 /* The cache: int8 codes and one f32 scale per page and kv head, value = code *
  * scale.  All memory is the caller's (sam3b200_buffer_alloc, codes 16-byte
  * aligned); nothing has to be initialised.  A page holds page_tokens (16, 32,
@@ -366,6 +403,46 @@ void sam3b200_kv_attention_free(sam3b200_kv_attention *h);
 int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b200_kv_cache *cache, const sam3b200_kv_batch *batch,
                               int type, const void *q, const int64_t q_nb[2], int64_t n_heads, float scale, int causal,
                               int64_t window, int y_type, void *y, const int64_t y_nb[2]);
+
+/* ---- The same cache in 4 bits ---------------------------------------------
+ * 4.5 bits a value instead of 8.  32 consecutive dimensions of one token's head
+ * share a bf16 scale d, value = d * (code - 8): Q4_0's rule with a scale a
+ * token, so a token's codes never change once they are written, and a page may
+ * be shared before it is full.  Batches, pages, strides and errors are those
+ * of the 8-bit cache; codes and scales are the caller's memory, 16-byte
+ * aligned, and nothing has to be initialised. */
+typedef struct sam3b200_kv4_cache {
+    void *k_codes, *v_codes; /* device uint8 [n_pages][n_kv_heads][page_tokens][head_dim / 2]: dimension 2i in the low half of byte i, 2i + 1 in the high one */
+    void *k_scale, *v_scale; /* device bf16 [n_pages][n_kv_heads][page_tokens][head_dim / 32] */
+    int32_t n_pages, n_kv_heads, page_tokens, head_dim;
+} sam3b200_kv4_cache;
+
+/* Rows into the cache, as sam3b200_kv_write.  d = top / -8 rounded to bf16, top
+ * the group's finite element of largest magnitude (the positive one of two);
+ * below 2^-100 top counts as 0.  Codes are the exact quotient x / d rounded to
+ * nearest even, cut to -8 .. 7, plus 8 (8 where d is 0).  NaN is stored as 0,
+ * infinities as the ends of the range.  Two rows of one call may not lie in
+ * the same place of a page. */
+int sam3b200_kv4_write(sam3b200_backend *be, const sam3b200_kv4_cache *cache, const sam3b200_kv_batch *batch, int type,
+                       const void *k, const int64_t k_nb[2], const void *v, const int64_t v_nb[2]);
+
+/* The reverse, as sam3b200_kv_read: d * (code - 8) rounded to `type`. */
+int sam3b200_kv4_read(sam3b200_backend *be, const sam3b200_kv4_cache *cache, const sam3b200_kv_batch *batch, int type,
+                      void *k, const int64_t k_nb[2], void *v, const int64_t v_nb[2]);
+
+/* Attention over it, with sam3b200_kv_attention_run's handle, arguments, masks
+ * and results.  Values reach the products exactly (11 bits), except that a
+ * value below 2^-10 of the largest scale of the tokens near it may lose bits, at most 2^-24
+ * of that scale; scales and softmax statistics are f32, softmax weights are
+ * rounded to f16, BF16 queries to f16 as there: within 2^-10 of the largest
+ * cached magnitude, plus the rounding to y's type.  That holds where the value
+ * scales of the tokens that a row sees are 0 or at least 2^-90 and lie within
+ * 2^100 of one another (2^20 beside a token of zeros), and where scale times a
+ * key scale, and scale times a BF16 row's largest element, are ordinary f32
+ * numbers.  Tokens that no row sees need not have been written. */
+int sam3b200_kv4_attention_run(sam3b200_kv_attention *h, const sam3b200_kv4_cache *cache, const sam3b200_kv_batch *batch,
+                               int type, const void *q, const int64_t q_nb[2], int64_t n_heads, float scale, int causal,
+                               int64_t window, int y_type, void *y, const int64_t y_nb[2]);
 
 /* ---- Graph level: the backend's supports_op and graph_compute -------------
  * ggml_backend_graph_compute (sam3.cpp:1023-1028) hands a backend the nodes

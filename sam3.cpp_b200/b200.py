@@ -275,6 +275,7 @@ def lib() -> ctypes.CDLL:
         "sam3b200_set_mmq_impl": (i32, [vp, i32]),
         "sam3b200_set_arith": (i32, [vp, i32]),
         "sam3b200_mul_mat_dq16": (i32, [vp, vp, vp, i64, i64, vp, vp, i64]),
+        "sam3b200_mul_mat_vec": (i32, [vp, vp, i32, vp, i64, i64, vp, i32, vp, i64]),
         "sam3b200_vit_create": (vp, [vp, vp]),
         "sam3b200_vit_free": (None, [vp]),
         "sam3b200_vit_set_tensor": (i32, [vp, ctypes.c_char_p, i32, vp, vp]),
@@ -298,11 +299,15 @@ def lib() -> ctypes.CDLL:
         "sam3b200_rope_create": (vp, [vp, vp]),
         "sam3b200_rope_free": (None, [vp]),
         "sam3b200_rope_run": (i32, [vp, i32, vp, vp, vp, i64, i64, i64, i32, i32, vp, vp]),
+        "sam3b200_rope_norm_run": (i32, [vp, vp, i32, i32, i32, i32, ctypes.c_float, vp, i64, i64, i32]),
         "sam3b200_kv_write": (i32, [vp, vp, vp, i32, vp, vp, vp, vp]),
         "sam3b200_kv_read": (i32, [vp, vp, vp, i32, vp, vp, vp, vp]),
         "sam3b200_kv_attention_create": (vp, [vp]),
         "sam3b200_kv_attention_free": (None, [vp]),
         "sam3b200_kv_attention_run": (i32, [vp, vp, vp, i32, vp, vp, i64, ctypes.c_float, i32, i64, i32, vp, vp]),
+        "sam3b200_kv4_write": (i32, [vp, vp, vp, i32, vp, vp, vp, vp]),
+        "sam3b200_kv4_read": (i32, [vp, vp, vp, i32, vp, vp, vp, vp]),
+        "sam3b200_kv4_attention_run": (i32, [vp, vp, vp, i32, vp, vp, i64, ctypes.c_float, i32, i64, i32, vp, vp]),
         "sam3b200_supports_op": (i32, [ctypes.POINTER(GraphTensor)]),
         "sam3b200_select_memory_frames": (i32, [i32, i32, vp, i32]),
         "sam3b200_extract_obj_ptr": (i32, [i32, i32, vp, ctypes.c_float, vp, vp, vp, vp]),
@@ -469,10 +474,14 @@ class DeviceBuffer:
 
 
 class Weight:
-    def __init__(self, be: "Backend", qtype: int, blocks: np.ndarray, K: int, N: int):
-        blocks = np.ascontiguousarray(blocks)
+    """A weight on the backend (sam3b200_weight_upload) from ggml's blocks: an array, or the address of blocks in host
+    memory or in device memory of the backend's GPU (ready when this is called)."""
+
+    def __init__(self, be: "Backend", qtype: int, blocks: np.ndarray | int, K: int, N: int):
+        if not isinstance(blocks, int):
+            blocks = np.ascontiguousarray(blocks)
         self.be, self.qtype, self.K, self.N = be, qtype, K, N
-        self.h = lib().sam3b200_weight_upload(be.h, qtype, blocks.ctypes.data, K, N)
+        self.h = lib().sam3b200_weight_upload(be.h, qtype, blocks if isinstance(blocks, int) else blocks.ctypes.data, K, N)
         if not self.h:
             raise B200Error(f"weight_upload failed: {last_error()}")
 
@@ -1197,6 +1206,12 @@ class KVBatch(ctypes.Structure):
                 ("max_rows", ctypes.c_int32), ("max_len", ctypes.c_int64)]
 
 
+class KV4Cache(ctypes.Structure):
+    """sam3b200_kv4_cache (include/sam3_b200.h): the caller's device memory of a paged 4-bit key/value cache, with
+    KVCache's fields."""
+    _fields_ = list(KVCache._fields_)
+
+
 def _strides(nb):
     return None if nb is None else (ctypes.c_int64 * 2)(*[int(x) for x in nb])
 
@@ -1206,6 +1221,19 @@ class RopeHparams(ctypes.Structure):
     _fields_ = [("head_dim", ctypes.c_int32), ("n_axes", ctypes.c_int32), ("sections", ctypes.c_int32 * 4),
                 ("neighbours", ctypes.c_int32), ("deal", ctypes.c_int32), ("restart", ctypes.c_int32),
                 ("base", ctypes.c_double), ("pos_scale", ctypes.c_double)]
+
+
+class NormHeads(ctypes.Structure):
+    """sam3b200_norm_heads (include/sam3_b200.h): one set of heads of Rope.norm.  Addresses of device memory; *_nb are
+    element strides (row, head), None for packed rows; no weight is ones, no bias zeros."""
+    _fields_ = [("x", ctypes.c_void_p), ("x_nb", ctypes.POINTER(ctypes.c_int64)), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_nb", ctypes.POINTER(ctypes.c_int64)),
+                ("n_heads", ctypes.c_int64)]
+
+    def __init__(self, x: int, n_heads: int, weight: int | None, y: int, bias: int | None = None, x_nb=None, y_nb=None):
+        super().__init__(x=x, weight=weight, bias=bias, y=y, n_heads=n_heads)
+        self._nb = (_strides(x_nb), _strides(y_nb))  # what the pointers show lives as long as this
+        self.x_nb, self.y_nb = (ctypes.cast(nb, ctypes.POINTER(ctypes.c_int64)) if nb is not None else None for nb in self._nb)
 
 
 class Rope:
@@ -1223,12 +1251,20 @@ class Rope:
         if not self.h:
             raise B200Error(f"rope_create failed: {last_error()}")
         self._run = lib().sam3b200_rope_run  # looked up once: a step of single tokens is a few microseconds
+        self._norm = lib().sam3b200_rope_norm_run
 
     def apply(self, x: int, x_type: int, pos: int, n_rows: int, n_heads: int, y: int, y_type: int, inverse: bool = False,
               x_nb=None, y_nb=None, pos_stride: int | None = None) -> None:
         """y = x turned by its positions; x, pos, y are device addresses, *_nb element strides (row, head)."""
         _check(self._run(self.h, x_type, x, _strides(x_nb), pos, n_rows if pos_stride is None else pos_stride,
                          n_rows, n_heads, 1 if inverse else 0, y_type, y, _strides(y_nb)), "rope")
+
+    def norm(self, sets, x_type: int, pos: int, n_rows: int, y_type: int, w_type: int = TYPE_F32, eps: float = 1e-6,
+             layer: bool = False, pos_stride: int | None = None) -> None:
+        """Each of one to four NormHeads: its heads normalised (RMS, or layer norm) and turned by their positions."""
+        sets = list(sets)
+        _check(self._norm(self.h, (NormHeads * len(sets))(*sets), len(sets), x_type, w_type, 1 if layer else 0, eps, pos,
+                          n_rows if pos_stride is None else pos_stride, n_rows, y_type), "rope_norm")
 
     def free(self) -> None:
         if self.h:
@@ -1237,7 +1273,7 @@ class Rope:
 
 
 class KVAttention:
-    """Attention over a KVCache (sam3b200_kv_attention: the workspace of its calls)."""
+    """Attention over a KVCache or KV4Cache (sam3b200_kv_attention: the workspace of its calls)."""
 
     def __init__(self, be: "Backend"):
         self.be = be
@@ -1245,12 +1281,14 @@ class KVAttention:
         if not self.h:
             raise B200Error(f"kv_attention_create failed: {last_error()}")
         self._run = lib().sam3b200_kv_attention_run
+        self._run4 = lib().sam3b200_kv4_attention_run
 
-    def run(self, cache: KVCache, batch: KVBatch, q_type: int, q: int, n_heads: int, y: int, scale: float,
+    def run(self, cache: KVCache | KV4Cache, batch: KVBatch, q_type: int, q: int, n_heads: int, y: int, scale: float,
             causal: bool = True, window: int = 0, y_type: int | None = None, q_nb=None, y_nb=None) -> None:
         """y = softmax(scale q k^T + mask) v; q and y are device addresses of [rows][n_heads][head_dim]."""
-        _check(self._run(self.h, ctypes.addressof(cache), ctypes.addressof(batch), q_type, q, _strides(q_nb), n_heads, scale,
-                         1 if causal else 0, window, q_type if y_type is None else y_type, y, _strides(y_nb)), "kv_attention")
+        run = self._run4 if isinstance(cache, KV4Cache) else self._run
+        _check(run(self.h, ctypes.addressof(cache), ctypes.addressof(batch), q_type, q, _strides(q_nb), n_heads, scale,
+                   1 if causal else 0, window, q_type if y_type is None else y_type, y, _strides(y_nb)), "kv_attention")
 
     def free(self) -> None:
         if self.h:
@@ -1356,7 +1394,7 @@ class Backend:
         buf.set(arr)
         return buf
 
-    def weight(self, qtype: int, blocks: np.ndarray, K: int, N: int) -> Weight:
+    def weight(self, qtype: int, blocks: np.ndarray | int, K: int, N: int) -> Weight:
         return Weight(self, qtype, blocks, K, N)
 
     def set_mmq_impl(self, impl: int) -> int:
@@ -1385,6 +1423,12 @@ class Backend:
         the library's fixed device array (for callers that cannot allocate)."""
         st = lib().sam3b200_mul_mat_noalloc(self.h, w.h, x.ptr, w.K, M, bias.ptr if bias else None, y.ptr, w.N)
         _check(st, "mul_mat_noalloc")
+
+    def mul_mat_vec(self, w: Weight, x: int, x_type: int, M: int, y: int, y_type: int, bias: int | None = None,
+                    ldx: int | None = None, ldy: int | None = None) -> None:
+        """sam3b200_mul_mat_vec: 1 to 16 rows with Q4_0 / Q4_1 weights, activations as they are (device addresses)."""
+        _check(lib().sam3b200_mul_mat_vec(self.h, w.h, x_type, x, w.K if ldx is None else ldx, M, bias, y_type, y,
+                                          w.N if ldy is None else ldy), "mul_mat_vec")
 
     def mul_mat_block_dots(self, w: Weight, x: DeviceBuffer, M: int) -> np.ndarray:
         nb = w.K // 32
@@ -1441,6 +1485,16 @@ class Backend:
         """sam3b200_kv_read: the last rows of each sequence back from the cache."""
         _check(lib().sam3b200_kv_read(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
                                       v, _strides(v_nb)), "kv_read")
+
+    def kv4_write(self, cache: KV4Cache, batch: KVBatch, ttype: int, k: int, v: int, k_nb=None, v_nb=None) -> None:
+        """sam3b200_kv4_write: rows of k and v (device addresses) quantised into the 4-bit cache."""
+        _check(lib().sam3b200_kv4_write(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
+                                        v, _strides(v_nb)), "kv4_write")
+
+    def kv4_read(self, cache: KV4Cache, batch: KVBatch, ttype: int, k: int, v: int, k_nb=None, v_nb=None) -> None:
+        """sam3b200_kv4_read: the last rows of each sequence back from the 4-bit cache."""
+        _check(lib().sam3b200_kv4_read(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
+                                       v, _strides(v_nb)), "kv4_read")
 
     def kv_attention(self) -> KVAttention:
         return KVAttention(self)

@@ -316,6 +316,9 @@ sam3b200_weight *sam3b200_weight_upload(sam3b200_backend *h, int type, const voi
                      "weight upload") &&
              cuda_ok(repack_weight_blocks(type, raw, N, K, w->codes, w->quads, w->ld, be->stream, w->mins),
                      "weight repack") &&
+             (type == SAM3B200_TYPE_Q8_0 ||
+              (cuda_ok(cudaMalloc(&w->vec_scales, vec_scale_bytes(type, N, K)), "cudaMalloc(weight scales)") &&
+               cuda_ok(pack_vec_scales(type, raw, N, K, w->vec_scales, be->stream), "weight scales"))) &&
              cuda_ok(cudaStreamSynchronize(be->stream), "weight upload sync");
     }
     if (raw) cudaFree(raw);
@@ -324,6 +327,7 @@ sam3b200_weight *sam3b200_weight_upload(sam3b200_backend *h, int type, const voi
         if (w->quads) cudaFree(w->quads);
         if (w->mins) cudaFree(w->mins);
         if (w->dense) cudaFree(w->dense);
+        if (w->vec_scales) cudaFree(w->vec_scales);
         delete w;
         return nullptr;
     }
@@ -343,6 +347,7 @@ void sam3b200_weight_free(sam3b200_backend *h, sam3b200_weight *wh) {
     cudaFree(w->mins);
     cudaFree(w->dense);
     cudaFree(w->w16);
+    cudaFree(w->vec_scales);
     delete w;
 }
 

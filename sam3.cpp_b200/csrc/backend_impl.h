@@ -18,6 +18,7 @@ struct Backend {
     int mmq_bn = 0;      // MMQ tile width: 0 = by K (tuning: env SAM3B200_MMQ_BN=64|128)
     int mmq_arith = 1;   // SAM3B200_ARITH_*: the encoder runners' linear-layer arithmetic (env SAM3B200_ARITH)
     char name[320] = {0};
+    unsigned vec_ready = 0;  // mul_mat_vec kernels whose attributes are set on the device
     // scratch for the quantised activations of the current MUL_MAT
     void *act_codes = nullptr;
     size_t act_codes_bytes = 0;
@@ -47,6 +48,7 @@ struct Weight {
     void *mins = nullptr;   // Q4_1: block minima as fp16 records [K/32][ld][8] (slot b % 8)
     void *dense = nullptr;  // F16 / F32 weights: fp16 [N][K] for the fp16 tensor-core GEMM
     void *w16 = nullptr;    // Q8_0 / Q4_0: the blocks dequantised to fp16 [N][K], made by the first mul_mat_dq16
+    void *vec_scales = nullptr;  // Q4_0 / Q4_1: the scales (and minima) as mul_mat_vec reads them
 };
 
 void set_error(const char *fmt, ...);
@@ -54,6 +56,11 @@ bool cuda_ok(cudaError_t e, const char *what);
 
 int run_mul_mat(Backend *be, const Weight *w, const float *x, int64_t ldx, int64_t M, const float *bias, float *dst,
                 int64_t ldd, int32_t *dump);
+
+// mul_mat_vec.cu: the scales of Q4_0 / Q4_1 blocks as its kernel reads them, f16 [N / 16][K / 128][16 rows][4 blocks] (Q4_1:
+// scales, then minima, of each 16 x 4)
+size_t vec_scale_bytes(int type, int N, int K);
+cudaError_t pack_vec_scales(int type, const void *blocks, int N, int K, void *out, cudaStream_t s);
 
 // sam_dec.cu: a decoder mask's logits [S][S] resized to out_w x out_h (bilinear) and binarised at 0 -> 255 / 0
 cudaError_t launch_mask_resize(const float *src, int S, int out_w, int out_h, uint8_t *dst, cudaStream_t s);

@@ -35,40 +35,10 @@
 #include <cmath>
 #include <new>
 
-#include "kv_attn.cuh"
-#include "ptx.cuh"
+#include "kv_attn_few.cuh"
 
 namespace b200 {
 namespace {
-
-constexpr int kWarps = 4;
-constexpr int kMaxSplits = 256;  // most parts of a key range
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// d += a b: a 16 x 16 (rows), b 16 x 8, f16 in, f32 sums.
-__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// An 8 x 8 matrix of f16, a row's pair of columns a lane, transposed.
-__device__ __forceinline__ uint32_t transposed(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
 
 // Bytes i and j of w (codes + 128) as f16: 0x64uu is 1024 + u, exactly.
 template <int SEL>
@@ -76,11 +46,6 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
     const uint32_t h = __byte_perm(w, 0x64646464u, SEL);
     const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&h), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t *>(&r);
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // Four consecutive query elements (d a multiple of 4), as they come, and the j-th of them.
@@ -116,7 +81,7 @@ struct Few {
         if (D == 128) return t * 128 + (c ^ (t & 6) ^ ((t & 1) << 2)) * 16;
         return (t >> 1) * 128 + ((((t & 1) << 2) | c) ^ (t & 6)) * 16;
     }
-    static __device__ __forceinline__ int padded(int d) { return d + d / kLane * 4; }
+    static __device__ __forceinline__ int column(int d) { return d + d / kLane * 4; }
 };
 
 template <int D, int NT>
@@ -124,27 +89,13 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
     using F = Few<D, NT>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float s_m[kWarps][F::kRows], s_l[kWarps][F::kRows];
-    __shared__ int s_last;
     wait_for_stream();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int kv = blockIdx.y, G = a.group;
-    const unsigned unit = blockIdx.x / a.splits;
-    const int split = blockIdx.x % a.splits;
-    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, false, a.err);
-    int64_t local;
-    KvSeq q;
-    if (!kv_find(a.b, unit, G, NT == 1 ? 3 : 4, 1, a.c.page_log2, q, local)) return;
-    const int R = q.n * G;  // the host keeps n_rows * G below 2^31
-    if (local * F::kRows >= R) return;
-    const int row0 = static_cast<int>(local) * F::kRows, i_lo = row0 / G, i_hi = (min(row0 + F::kRows, R) - 1) / G;
-
-    // the tile's keys, and this block's part of them
-    const int k_end = kv_last(a, q, i_hi) + 1, k_begin = kv_first(a, kv_last(a, q, i_lo)) & ~15;
-    const int range = max(k_end - k_begin, 0);
-    const int chunk = max(range < a.short_range ? a.chunk_short : a.chunk, ((range + a.splits - 1) / a.splits + 63) & ~63);
-    const int n_split = max((range + chunk - 1) / chunk, 1);
-    if (split >= n_split) return;
-    const int t_begin = k_begin + split * chunk, t_end = min(t_begin + chunk, k_end);
+    FewTile tile;
+    if (!few_tile<NT>(a, tile)) return;
+    const KvSeq &q = tile.q;
+    const int row0 = tile.row0, i_lo = tile.i_lo, i_hi = tile.i_hi, R = tile.R, t_begin = tile.t_begin, t_end = tile.t_end;
     const int n_blocks = t_end > t_begin ? (t_end - t_begin + 15) / 16 : 0;
     const int mine = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;  // blocks warp, warp + 4, ...
 
@@ -358,160 +309,26 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], x);
             if (g == 0) s_m[warp][row] = m[n][k], s_l[warp][row] = l[n][k];
-            float *to = rows + (warp * F::kRows + row) * F::kRowFloats + F::padded(g * F::kLane);
+            float *to = rows + (warp * F::kRows + row) * F::kRowFloats + F::column(g * F::kLane);
 #pragma unroll
             for (int i = 0; i < D / 16; i += 2)
                 *reinterpret_cast<float4 *>(to + 2 * i) = make_float4(o[n][i][k], o[n][i][k + 2], o[n][i + 1][k], o[n][i + 1][k + 2]);
         }
     __syncthreads();
-    constexpr int kEach = F::kEach, kPer = D / kEach;  // threads a row
-    const int row = threadIdx.x / kPer, d0 = threadIdx.x % kPer * kEach;
-    const int r = row0 + row;
-    const bool live = row < F::kRows && r < R;
-    float M = -INFINITY, L = 0.f, sum[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
-    if (live) {
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][row]);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float f = s_m[w][row] == M ? 1.f : ex2_approx(s_m[w][row] - M);
-            L = fmaf(s_l[w][row], f, L);
-            const float *from = rows + (w * F::kRows + row) * F::kRowFloats;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) sum[i] = fmaf(from[F::padded(d0 + i)], f, sum[i]);
-        }
-    }
-    if (n_split > 1) {
-        const int64_t group = static_cast<int64_t>(unit) * a.c.heads + kv;
-        float *base = a.part + group * a.splits * F::kRows * (D + 2);
-        float *ml = base + static_cast<int64_t>(a.splits) * F::kRows * D;
-        if (live) {
-            float *to = base + (static_cast<int64_t>(split) * F::kRows + row) * D + d0;
-#pragma unroll
-            for (int i = 0; i < kEach; i += 4)
-                *reinterpret_cast<float4 *>(to + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
-            if (d0 == 0) *reinterpret_cast<float2 *>(ml + (split * F::kRows + row) * 2) = make_float2(M, L);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            __threadfence();
-            s_last = atomicInc(a.done + group, n_split - 1) == static_cast<unsigned>(n_split - 1);
-            __threadfence();
-        }
-        __syncthreads();
-        if (!s_last) return;
-        // Join the parts, in a fixed order: a warp takes a row, or with fewer than 4 rows a share of one's parts, its
-        // lanes along the dimensions; then the shares are joined.
-        const int n_rows = min(R - row0, F::kRows);
-        const int shares = n_rows >= 4 ? 1 : n_rows == 1 ? 4 : 2;
-        float *share = reinterpret_cast<float *>(smem), *share_ml = share + kWarps * F::kRows * D;
-        constexpr int kLanes = D / 4, kStep = 32 / kLanes;  // lanes a row, parts a warp and step
-        constexpr int kFlight = 8;                          // loads of a lane on their way at once
-        for (int id = warp; id < n_rows * shares; id += kWarps) {
-            const int i = id / shares;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            float top = -INFINITY, total = 0.f;
-            const float *from = base + static_cast<int64_t>(i) * D + lane % kLanes * 4;
-            auto add = [&](float m1, float l1, const float4 &x) {
-                const float to = fmaxf(top, m1);
-                const float f = top == to ? 1.f : ex2_approx(top - to), f1 = m1 == to ? 1.f : ex2_approx(m1 - to);
-                top = to;
-                total = total * f + l1 * f1;
-                v.x = v.x * f + x.x * f1, v.y = v.y * f + x.y * f1, v.z = v.z * f + x.z * f1, v.w = v.w * f + x.w * f1;
-            };
-            for (int k0 = (id % shares) * kStep + lane / kLanes; k0 < n_split; k0 += kFlight * shares * kStep) {
-                float2 y[kFlight];
-                float4 x[kFlight];
-#pragma unroll
-                for (int u = 0; u < kFlight; ++u) {
-                    const int k = k0 + u * shares * kStep;
-                    y[u] = make_float2(-INFINITY, 0.f);
-                    if (k >= n_split) continue;
-                    y[u] = __ldcg(reinterpret_cast<const float2 *>(ml + (k * F::kRows + i) * 2));
-                    x[u] = __ldcg(reinterpret_cast<const float4 *>(from + static_cast<int64_t>(k) * F::kRows * D));
-                }
-#pragma unroll
-                for (int u = 0; u < kFlight; ++u)
-                    if (k0 + u * shares * kStep < n_split) add(y[u].x, y[u].y, x[u]);
-            }
-            if constexpr (kStep == 2) {
-                const float4 x = make_float4(__shfl_xor_sync(0xffffffffu, v.x, 16), __shfl_xor_sync(0xffffffffu, v.y, 16),
-                                             __shfl_xor_sync(0xffffffffu, v.z, 16), __shfl_xor_sync(0xffffffffu, v.w, 16));
-                const float m1 = __shfl_xor_sync(0xffffffffu, top, 16), l1 = __shfl_xor_sync(0xffffffffu, total, 16);
-                add(m1, l1, x);
-            }
-            if (lane < kLanes) *reinterpret_cast<float4 *>(share + id * D + lane * 4) = v;
-            if (lane == 0) share_ml[2 * id] = top, share_ml[2 * id + 1] = total;
-        }
-        __syncthreads();
-        if (!live) return;
-        M = -INFINITY, L = 0.f;
-        for (int w = row * shares; w < (row + 1) * shares; ++w) M = fmaxf(M, share_ml[2 * w]);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
-        for (int w = row * shares; w < (row + 1) * shares; ++w) {
-            const float f = share_ml[2 * w] == M ? 1.f : ex2_approx(share_ml[2 * w] - M);
-            L = fmaf(share_ml[2 * w + 1], f, L);
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) sum[i] = fmaf(share[w * D + d0 + i], f, sum[i]);
-        }
-    }
-    if (!live) return;
-    const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees no key yields zeros
-    const int64_t at = (q.r0 + static_cast<int64_t>(r / G)) * a.ys.token + (kv * static_cast<int64_t>(G) + r % G) * a.ys.head + d0;
-#pragma unroll
-    for (int i = 0; i < kEach; i += 8) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = sum[i + k] * inv;
-        kv_store8(a, at + i, v);
-    }
+    few_finish<F, D>(a, tile, smem, s_m, s_l);
 }
 
 template <int D, int NT>
-cudaError_t launch_few(KvAttnArgs &a, int num_sms, cudaStream_t st) {
-    using F = Few<D, NT>;
-    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> (NT == 1 ? 3 : 4)) + a.b.n_seqs;
-    // parts for two waves where there are few sequences and heads, for four where the lengths of many have to even out
-    const int64_t wave = F::kBlocks * static_cast<int64_t>(num_sms), groups = units * a.c.heads;
-    const int64_t span =
-        std::max(a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len, int64_t(1));
-    int64_t splits = 2 * groups < wave ? (2 * wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
-    // a block's least part: 64 tokens, one turn of its warps, while the blocks fit in one wave, else 256
-    const int64_t least = groups * ((span + 63) / 64) <= wave ? 64 : 256;
-    splits = std::min(splits, (span + least - 1) / least);
-    splits = std::min(splits, std::min(static_cast<int64_t>(kMaxParts) / groups, static_cast<int64_t>(kMaxSplits)));
-    splits = std::max(splits, static_cast<int64_t>(1));
-    if (units * splits > 0x7fffffff) return cudaErrorInvalidValue;
-    a.splits = static_cast<int>(splits);
-    a.chunk = static_cast<int>(((span + splits - 1) / splits + 63) & ~int64_t(63));
-    // With few sequences one that is far shorter than max_len (a captured step's bound) is cut finer, into all parts.
-    a.chunk_short = static_cast<int>(2 * groups < wave ? std::min<int64_t>(least, a.chunk) : a.chunk);
-    a.short_range = static_cast<int>(span / 2);
-    if (!(*a.ready & (1 << (2 * NT + (D == 64))))) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_attn_few_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
-        if (e != cudaSuccess) return e;
-        *a.ready |= 1 << (2 * NT + (D == 64));
-    }
-    const dim3 grid(static_cast<unsigned>(units * a.splits), a.c.heads);
-    return launch_after(kv_attn_few_kernel<D, NT>, grid, kWarps * 32, F::kSmem, st, a);
+cudaError_t launch(KvAttnArgs &a, int num_sms, cudaStream_t st) {
+    return few_launch<Few<D, NT>, NT>(kv_attn_few_kernel<D, NT>, a, kReadyFew + 2 * (NT - 1) + (D == 64), num_sms, st);
 }
-
-struct KvAttention {
-    Backend *be = nullptr;
-    unsigned ready = 0;  // kernels whose attributes are set on this handle's device
-    float *part = nullptr;
-    unsigned *done = nullptr;
-};
 
 }  // namespace
 
 cudaError_t kv_attn_few(KvAttnArgs a, int num_sms, cudaStream_t st) {
     const bool one = static_cast<int64_t>(a.b.max_rows) * a.group <= 8;
-    if (a.c.D == 64) return one ? launch_few<64, 1>(a, num_sms, st) : launch_few<64, 2>(a, num_sms, st);
-    return one ? launch_few<128, 1>(a, num_sms, st) : launch_few<128, 2>(a, num_sms, st);
+    if (a.c.D == 64) return one ? launch<64, 1>(a, num_sms, st) : launch<64, 2>(a, num_sms, st);
+    return one ? launch<128, 1>(a, num_sms, st) : launch<128, 2>(a, num_sms, st);
 }
 
 }  // namespace b200
@@ -559,48 +376,10 @@ extern "C" int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b20
                                          const int64_t *y_nb) {
     auto *k = reinterpret_cast<KvAttention *>(h);
     KvAttnArgs a;
-    if (!kv_views("kv_attention", cache, batch, a.c, a.b)) return SAM3B200_STATUS_FAILED;
-    if (!q || !y) {
-        set_error("kv_attention: null argument");
+    bool empty;
+    if (!kv_attn_args("kv_attention", k, cache, batch, type, q, q_nb, n_heads, scale, causal, window, y_type, y, y_nb, a, empty))
         return SAM3B200_STATUS_FAILED;
-    }
-    const int yb = type_bytes(y_type);
-    if ((type != SAM3B200_TYPE_F16 && type != SAM3B200_TYPE_BF16) || (y_type != type && y_type != SAM3B200_TYPE_F32) ||
-        reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(y) % yb) {
-        set_error("kv_attention: unsupported types %d -> %d (q F16=1 or BF16=30, y q's type or F32=0) or unaligned data", type,
-                  y_type);
-        return SAM3B200_STATUS_FAILED;
-    }
-    if (n_heads >= 1 && a.b.n_rows * (n_heads / a.c.heads) > 0x7fffff00) {
-        set_error("kv_attention: %d rows of %lld query heads over %d kv heads are too many", a.b.n_rows, (long long)n_heads, a.c.heads);
-        return SAM3B200_STATUS_FAILED;
-    }
-    if (n_heads < 1 || n_heads > 65535 || n_heads % a.c.heads != 0) {
-        set_error("kv_attention: %lld query heads over %d kv heads (a positive multiple is needed)", (long long)n_heads, a.c.heads);
-        return SAM3B200_STATUS_FAILED;
-    }
-    if (!(scale >= 0.f) || !std::isfinite(scale * 1.4426950408889634f) || window < 0 || (window && !causal)) {
-        set_error("kv_attention: bad scale %g or window %lld (a window needs the causal mask)", scale, (long long)window);
-        return SAM3B200_STATUS_FAILED;
-    }
-    a.q = q, a.y = y;
-    a.qs = row_tensor(q, type, q_nb, n_heads, a.c.D);
-    a.ys = row_tensor(y, y_type, y_nb, n_heads, a.c.D);
-    if (!rows_ok("kv_attention", "q", a.qs, a.b.n_rows, n_heads, a.c.D, false) ||
-        !rows_ok("kv_attention", "y", a.ys, a.b.n_rows, n_heads, a.c.D, true))
-        return SAM3B200_STATUS_FAILED;
-    if (!k) {
-        set_error("kv_attention: null handle");
-        return SAM3B200_STATUS_FAILED;
-    }
-    if (a.b.n_seqs == 0 || a.b.n_rows == 0) return SAM3B200_STATUS_SUCCESS;
-    a.q_bf16 = type == SAM3B200_TYPE_BF16;
-    a.y_type = y_type;
-    a.group = static_cast<int>(n_heads / a.c.heads);
-    a.scale_log2 = scale * 1.4426950408889634f;
-    // a window that no length reaches is none; below 2^30 it cannot pass 32 bits where rows are more than tokens
-    a.causal = causal != 0, a.window = window < a.b.max_len ? static_cast<int>(window) : 0;
-    a.part = k->part, a.done = k->done, a.ready = &k->ready, a.err = k->be->err;
+    if (empty) return SAM3B200_STATUS_SUCCESS;
     DeviceScope dev(k->be->device);
     // us in a graph, 8 kv heads, few rows and tc, for one sequence of 8000 tokens, one of 100000, 16 of 4000.  Heads of 128:
     // 16 rows a kv head 28 and 35, 84 and 112, 51 and 67; 32 rows 36 and 35, 113 and 111, 76 and 68; 64 rows 39 and 35, 185

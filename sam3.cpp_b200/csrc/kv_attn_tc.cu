@@ -1,5 +1,5 @@
-// kv_attn_tc.cu -- attention over the paged 8-bit cache for many query rows a
-// kv head (prompts, parts of prompts, cross attention), on the
+// kv_attn_tc.cu -- attention over the paged caches of 8 and 4 bits for many
+// query rows a kv head (prompts, parts of prompts, cross attention), on the
 // 5th-generation tensor cores.
 //
 // A block owns 256 query rows of one kv head (the group's query heads times
@@ -23,6 +23,13 @@
 // kv_attn.cu), so the scales of 16 tokens enter as one multiply-add in front
 // of the exponential.  O stays in tensor memory; it is rescaled only where a
 // row's maximum rose by more than kLazy.
+// The 4-bit cache's scales, one for 32 dimensions of a token, are multiplied
+// in while its codes are widened: of 16 tokens the power of two of the largest
+// scale takes the place of the page's scale, and what is left of each, in
+// [0, 2), times a code is exact in f16 (8 + 3 bits) down to 2^-10 of it.  Its
+// nibbles come out in pairs (0, 4), (1, 5), (2, 6), (3, 7) of 8 dimensions:
+// keys and values stay in that order, the queries are staged in it, and the
+// results are put back where they are read from tensor memory.
 // Tensor memory (512 columns): S_t(i), and P_t(i) over it, at 128 t + 64 (i % 2);
 // O_t at 256 + D t.
 //
@@ -40,8 +47,10 @@
 // results by whole rows through shared memory (185 to 188: the loop's
 // registers).
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_attn.cuh"
+#include "kv4_codes.cuh"
 #include "ptx.cuh"
 
 namespace b200 {
@@ -160,14 +169,20 @@ __device__ __forceinline__ void exp2_poly(float &y0, float &y1) {
     y1 = __int_as_float((__float_as_int(n1) << 23) + __float_as_int(c1));
 }
 
+// 8 elements in the order (0, 4, 1, 5, 2, 6, 3, 7).
+__device__ __forceinline__ uint4 paired(const uint4 &x) {
+    return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+}
+
 // The softmax constants of 16 tokens: ks scale log2(e), log2(vs), 1 / vs.
 struct Scales {
     float k, lv, inv_v, pad;
 };
 
-template <int D>
-__global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __grid_constant__ KvAttnArgs a) {
+template <int D, typename Args>
+__global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __grid_constant__ Args a) {
     using C = Tc<D>;
+    constexpr bool kFour = std::is_same<Args, Kv4AttnArgs>::value;
     extern __shared__ uint8_t smem_raw[];
     wait_for_stream();
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -230,19 +245,6 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
         give_regs<kRegsCodes>();
         // warp w widens tokens 32 w ... 32 w + 31 of each tile: two runs of 16, each in one page
         const int w = warp - 8;
-        constexpr int kChunks = D / 16, kPer = C::kKeys * kChunks / 128;  // 16-code chunks a token, a thread
-        constexpr int kTokens = 32 / kChunks;                             // tokens a step
-        // Lane bits: 0-1 the chunk within 64 dimensions, 2 the token's lowest bit, 3 (D = 128) the half, the rest
-        // more of the token.  8 lanes that store together are then 2 neighbouring tokens of one half, whose swizzled
-        // chunks have different banks; a token's 128 bytes are still read by lanes of one load.
-        const int half = D == 128 ? (lane >> 3) & 1 : 0;
-        const int token0 = ((lane >> 2) & 1) + (D == 128 ? (lane >> 4) * 2 : (lane >> 3) * 2);  // of the step's kTokens
-        const int chunk = half * 4 + (lane & 3);
-        // where this lane's first chunk goes: token t's row, chunk c of it at c ^ (t & 7)
-        const uint32_t at0 = half * C::kHalf + (w * 32 + token0) * 128 + ((2 * (lane & 3)) ^ (token0 & 7)) * 16;
-        const int64_t own = static_cast<int64_t>(token0) * D + chunk * 16;
-        uint4 kx[kPer], vx[kPer];
-        float ks = 0.f, vs = 0.f;  // lanes 0, 1: the scales of the two runs
         struct Pages {
             int p[2];  // -1 behind the end
         };
@@ -269,61 +271,156 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
             }
             return r;
         };
-        auto fetch = [&](int which, int j, const Pages &pg, uint4 (&x)[kPer]) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int in_page = (k_begin + j * C::kKeys + w * 32 + g * 16) & ((1 << a.c.page_log2) - 1);
-                const int8_t *from = a.c.codes[which] + kv_slab(a.c, max(pg.p[g], 0), kv) + static_cast<int64_t>(in_page) * D + own;
-#pragma unroll
-                for (int i = 0; i < kPer / 2; ++i) {
-                    uint4 &v = x[g * (kPer / 2) + i];
-                    v = make_uint4(0u, 0u, 0u, 0u);
-                    if (pg.p[g] >= 0) v = *reinterpret_cast<const uint4 *>(from + i * kTokens * D);
-                }
-            }
-        };
-        auto fetch_scales = [&](const Pages &pg) {
-            if (lane >= 2) return;
-            const int page = lane ? pg.p[1] : pg.p[0];
-            const int64_t h = static_cast<int64_t>(max(page, 0)) * a.c.heads + kv;
-            ks = page < 0 ? 0.f : a.c.scale[0][h];
-            vs = page < 0 ? 0.f : a.c.scale[1][h];
-        };
-        auto put = [&](uint8_t *tile, const uint4 (&x)[kPer]) {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)  // a step of 4 tokens (D = 128) flips bit 2 of t & 7
-                put_codes(tile, (kTokens == 4 && (i & 1) ? at0 ^ 64 : at0) + i * kTokens * 128, x[i]);
-        };
-        auto put_scales = [&](int j) {
-            if (lane >= 2) return;
-            Scales v{ks * a.scale_log2, vs > 0.f ? __log2f(vs) : kZeroScaleLog2, 0.f, 0.f};
-            v.inv_v = ex2_approx(-v.lv);
-            reinterpret_cast<Scales *>(smem + C::kScales)[(j % C::kScaleSlots) * 8 + w * 2 + lane] = v;
-        };
         auto publish = [&](uint64_t *bar) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        // Codes and scales are loaded a tile ahead, table entries two.
-        Pages pg_next = checked(0, lookup(0)), raw = lookup(1);
-        fetch(0, 0, pg_next, kx);
-        fetch_scales(pg_next);
-        fetch(1, 0, pg_next, vx);
-        for (int j = 0; j < ntiles; ++j) {
-            pg_next = checked(j + 1, raw);
-            raw = lookup(j + 2);
-            if (j >= 2 && !warp_wait(&k_free[j & 1], ((j >> 1) - 1) & 1, a.err, TERR_FREE)) break;
-            put(smem + C::kK + (j & 1) * C::kTile, kx);
-            put_scales(j);
-            publish(&k_full[j & 1]);
-            if (lane == 0) mbar_arrive(&sc_full[j % C::kScaleSlots]);
-            fetch(0, j + 1, pg_next, kx);
+        if constexpr (kFour) {
+            constexpr int kGroups = D / 32, kTokens = 32 / kGroups, kPer = 32 / kTokens;  // tokens a step, steps a tile
+            // A lane takes one group of a token a step: 16 bytes of codes, contiguous over the warp, and 64 bytes of f16.
+            const int grp = lane % kGroups, token0 = lane / kGroups, half = grp >> 1;
+            // Chunk c of token t's row goes to c ^ (t & 7); lanes of the upper half store chunks 2, 3, 0, 1, so that the 8
+            // lanes that store together have different banks.
+            const uint32_t at0 = half * C::kHalf + (w * 32 + token0) * 128;
+            const int first_any = kv_first(a, kv_last(a, q, i_lo));  // tokens in front of it need not hold numbers
+            uint4 kx[kPer], vx[kPer];
+            uint16_t kd[kPer], vd[kPer];  // scales
+            auto fetch = [&](int which, int j, const Pages &pg, uint4 (&x)[kPer], uint16_t (&d)[kPer]) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int tok = k_begin + j * C::kKeys + w * 32 + g * 16 + token0;
+                    const int64_t at = ((static_cast<int64_t>(max(pg.p[g], 0)) * a.c.heads + kv) << a.c.page_log2) + (tok & ((1 << a.c.page_log2) - 1));
+#pragma unroll
+                    for (int i = 0; i < kPer / 2; ++i) {
+                        const int k = g * (kPer / 2) + i, t = tok + i * kTokens;
+                        x[k] = make_uint4(0u, 0u, 0u, 0u);
+                        d[k] = 0;
+                        if (pg.p[g] < 0 || t >= k_end || t < first_any) continue;
+                        x[k] = *reinterpret_cast<const uint4 *>(a.c.codes[which] + (at + i * kTokens) * (D / 2) + grp * 16);
+                        d[k] = reinterpret_cast<const uint16_t *>(a.c.scale[which])[(at + i * kTokens) * kGroups + grp];
+                    }
+                }
+            };
+            // biased exponents of the largest scales of the two runs, in the halves of a word
+            auto exponents = [&](const uint16_t (&d)[kPer]) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) top = __vmaxu2(top, static_cast<uint32_t>(d[k] & 0x7fff) << (k < kPer / 2 ? 0 : 16));
+#pragma unroll
+                for (int o = 16; o; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+                return (top >> 7) & 0x00ff00ffu;
+            };
+            auto put = [&](uint8_t *tile, const uint4 (&x)[kPer], const uint16_t (&d)[kPer], uint32_t e) {
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    const int er = min(static_cast<int>(k < kPer / 2 ? e & 0xffffu : e >> 16), 253);
+                    const float less = er ? __int_as_float((254 - er) << 23) : 0.f;
+                    const __half2 by = __float2half2_rn(__uint_as_float(static_cast<uint32_t>(d[k]) << 16) * less);
+                    const uint32_t words[4] = {half ? x[k].z : x[k].x, half ? x[k].w : x[k].y, half ? x[k].x : x[k].z, half ? x[k].y : x[k].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t p[4];
+                        codes4(words[i], p);
+                        __half2 v[4];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) v[n] = __hmul2(*reinterpret_cast<const __half2 *>(&p[n]), by);
+                        const int chunk = (grp & 1) * 4 + (i ^ (2 * half));
+                        *reinterpret_cast<uint4 *>(tile + at0 + k * kTokens * 128 + ((chunk ^ (token0 & 7)) * 16)) = *reinterpret_cast<const uint4 *>(v);
+                    }
+                }
+            };
+            auto put_scales = [&](int j, uint32_t ke, uint32_t ve) {
+                if (lane >= 2) return;
+                const int k = min(static_cast<int>(lane ? ke >> 16 : ke & 0xffffu), 253), v = min(static_cast<int>(lane ? ve >> 16 : ve & 0xffffu), 253);
+                Scales z{__int_as_float(k << 23) * a.scale_log2, v ? static_cast<float>(v - 127) : kZeroScaleLog2, 0.f, 0.f};
+                z.inv_v = ex2_approx(-z.lv);
+                reinterpret_cast<Scales *>(smem + C::kScales)[(j % C::kScaleSlots) * 8 + w * 2 + lane] = z;
+            };
+            // Codes and scales are loaded a tile ahead, table entries two.
+            Pages pg_next = checked(0, lookup(0)), raw = lookup(1);
+            fetch(0, 0, pg_next, kx, kd);
+            fetch(1, 0, pg_next, vx, vd);
+            for (int j = 0; j < ntiles; ++j) {
+                pg_next = checked(j + 1, raw);
+                raw = lookup(j + 2);
+                const uint32_t ke = exponents(kd), ve = exponents(vd);
+                if (j >= 2 && !warp_wait(&k_free[j & 1], ((j >> 1) - 1) & 1, a.err, TERR_FREE)) break;
+                put(smem + C::kK + (j & 1) * C::kTile, kx, kd, ke);
+                put_scales(j, ke, ve);
+                publish(&k_full[j & 1]);
+                if (lane == 0) mbar_arrive(&sc_full[j % C::kScaleSlots]);
+                fetch(0, j + 1, pg_next, kx, kd);
+                if (j >= 2 && !warp_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, a.err, TERR_FREE)) break;
+                put(smem + C::kV + (j & 1) * C::kTile, vx, vd, ve);
+                publish(&v_full[j & 1]);
+                fetch(1, j + 1, pg_next, vx, vd);
+            }
+        } else {
+            constexpr int kChunks = D / 16, kPer = C::kKeys * kChunks / 128;  // 16-code chunks a token, a thread
+            constexpr int kTokens = 32 / kChunks;                             // tokens a step
+            // Lane bits: 0-1 the chunk within 64 dimensions, 2 the token's lowest bit, 3 (D = 128) the half, the rest
+            // more of the token.  8 lanes that store together are then 2 neighbouring tokens of one half, whose swizzled
+            // chunks have different banks; a token's 128 bytes are still read by lanes of one load.
+            const int half = D == 128 ? (lane >> 3) & 1 : 0;
+            const int token0 = ((lane >> 2) & 1) + (D == 128 ? (lane >> 4) * 2 : (lane >> 3) * 2);  // of the step's kTokens
+            const int chunk = half * 4 + (lane & 3);
+            // where this lane's first chunk goes: token t's row, chunk c of it at c ^ (t & 7)
+            const uint32_t at0 = half * C::kHalf + (w * 32 + token0) * 128 + ((2 * (lane & 3)) ^ (token0 & 7)) * 16;
+            const int64_t own = static_cast<int64_t>(token0) * D + chunk * 16;
+            uint4 kx[kPer], vx[kPer];
+            float ks = 0.f, vs = 0.f;  // lanes 0, 1: the scales of the two runs
+            auto fetch = [&](int which, int j, const Pages &pg, uint4 (&x)[kPer]) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int in_page = (k_begin + j * C::kKeys + w * 32 + g * 16) & ((1 << a.c.page_log2) - 1);
+                    const int8_t *from = a.c.codes[which] + kv_slab(a.c, max(pg.p[g], 0), kv) + static_cast<int64_t>(in_page) * D + own;
+#pragma unroll
+                    for (int i = 0; i < kPer / 2; ++i) {
+                        uint4 &v = x[g * (kPer / 2) + i];
+                        v = make_uint4(0u, 0u, 0u, 0u);
+                        if (pg.p[g] >= 0) v = *reinterpret_cast<const uint4 *>(from + i * kTokens * D);
+                    }
+                }
+            };
+            auto fetch_scales = [&](const Pages &pg) {
+                if (lane >= 2) return;
+                const int page = lane ? pg.p[1] : pg.p[0];
+                const int64_t h = static_cast<int64_t>(max(page, 0)) * a.c.heads + kv;
+                ks = page < 0 ? 0.f : a.c.scale[0][h];
+                vs = page < 0 ? 0.f : a.c.scale[1][h];
+            };
+            auto put = [&](uint8_t *tile, const uint4 (&x)[kPer]) {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)  // a step of 4 tokens (D = 128) flips bit 2 of t & 7
+                    put_codes(tile, (kTokens == 4 && (i & 1) ? at0 ^ 64 : at0) + i * kTokens * 128, x[i]);
+            };
+            auto put_scales = [&](int j) {
+                if (lane >= 2) return;
+                Scales v{ks * a.scale_log2, vs > 0.f ? __log2f(vs) : kZeroScaleLog2, 0.f, 0.f};
+                v.inv_v = ex2_approx(-v.lv);
+                reinterpret_cast<Scales *>(smem + C::kScales)[(j % C::kScaleSlots) * 8 + w * 2 + lane] = v;
+            };
+            // Codes and scales are loaded a tile ahead, table entries two.
+            Pages pg_next = checked(0, lookup(0)), raw = lookup(1);
+            fetch(0, 0, pg_next, kx);
             fetch_scales(pg_next);
-            if (j >= 2 && !warp_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, a.err, TERR_FREE)) break;
-            put(smem + C::kV + (j & 1) * C::kTile, vx);
-            publish(&v_full[j & 1]);
-            fetch(1, j + 1, pg_next, vx);
+            fetch(1, 0, pg_next, vx);
+            for (int j = 0; j < ntiles; ++j) {
+                pg_next = checked(j + 1, raw);
+                raw = lookup(j + 2);
+                if (j >= 2 && !warp_wait(&k_free[j & 1], ((j >> 1) - 1) & 1, a.err, TERR_FREE)) break;
+                put(smem + C::kK + (j & 1) * C::kTile, kx);
+                put_scales(j);
+                publish(&k_full[j & 1]);
+                if (lane == 0) mbar_arrive(&sc_full[j % C::kScaleSlots]);
+                fetch(0, j + 1, pg_next, kx);
+                fetch_scales(pg_next);
+                if (j >= 2 && !warp_wait(&v_free[j & 1], ((j >> 1) - 1) & 1, a.err, TERR_FREE)) break;
+                put(smem + C::kV + (j & 1) * C::kTile, vx);
+                publish(&v_full[j & 1]);
+                fetch(1, j + 1, pg_next, vx);
+            }
         }
     } else if (warp >= 12) {
         // ---- MMA issuer ----
@@ -448,6 +545,7 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                             for (int n = 0; n < 4; ++n) h[n] = __floats2half2_rn(x[2 * n], x[2 * n + 1]);
                             raw[k] = *reinterpret_cast<const uint4 *>(h);
                         }
+                        if constexpr (kFour) raw[k] = paired(raw[k]);
                         const int row = (warp & 3) * 32 + (step0 + k) * kRowsStep + lane / kLanes;
                         *reinterpret_cast<uint4 *>(smem + C::kQ + t * C::kTile + (part >> 3) * C::kHalf + row * 128 +
                                                    ((part & 7) ^ (row & 7)) * 16) = raw[k];
@@ -587,7 +685,8 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                     for (int e = 0; e < 32; e += 8) {
                         float v[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = nsteps > 0 ? __uint_as_float(o[e + k]) * inv : 0.f;
+                        for (int k = 0; k < 8; ++k)
+                            v[kFour ? (k >> 1) + (k & 1) * 4 : k] = nsteps > 0 ? __uint_as_float(o[e + k]) * inv : 0.f;
                         if (n_split > 1) {
 #pragma unroll
                             for (int k = 0; k < 8; ++k) to[(c + e + k) * C::kRows] = v[k];
@@ -644,25 +743,26 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
     if (warp == 12) tmem_dealloc(tmem, 512);
 }
 
-template <int D>
-cudaError_t launch_tc(const KvAttnArgs &a, cudaStream_t st) {
+template <int D, typename Args>
+cudaError_t launch_tc(const Args &a, cudaStream_t st) {
     using C = Tc<D>;
-    if (!(*a.ready & (1u << (16 + (D == 64))))) {
-        cudaError_t e = cudaFuncSetAttribute(kv_attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    void (*const kernel)(Args) = kv_attn_tc_kernel<D, Args>;
+    const unsigned bit = 1u << ((std::is_same<Args, Kv4AttnArgs>::value ? kReadyTc4 : kReadyTc) + (D == 64));
+    if (!(*a.ready & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
         if (e != cudaSuccess) return e;
         cudaFuncAttributes f;  // the register shares draw on what the block starts with
-        e = cudaFuncGetAttributes(&f, kv_attn_tc_kernel<D>);
+        e = cudaFuncGetAttributes(&f, kernel);
         if (e != cudaSuccess) return e;
         if (f.numRegs < kRegsStart) return cudaErrorInvalidConfiguration;
-        *a.ready |= 1u << (16 + (D == 64));
+        *a.ready |= bit;
     }
     const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 8) + a.b.n_seqs;
-    return launch_after(kv_attn_tc_kernel<D>, dim3(static_cast<unsigned>(units * a.c.heads * a.splits)), C::kThreads, C::kSmem, st, a);
+    return launch_after(kernel, dim3(static_cast<unsigned>(units * a.c.heads * a.splits)), C::kThreads, C::kSmem, st, a);
 }
 
-}  // namespace
-
-cudaError_t kv_attn_tc(KvAttnArgs a, int num_sms, cudaStream_t st) {
+template <typename Args>
+cudaError_t run(Args &a, int num_sms, cudaStream_t st) {
     const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> 8) + a.b.n_seqs, groups = units * a.c.heads;
     // Parts of the key range: the number that gives the shortest schedule of one block an SM, counted in tiles of 128
     // tokens (about 2 us), a block's start and end as 4 of them and the join of parts as 3.
@@ -682,5 +782,10 @@ cudaError_t kv_attn_tc(KvAttnArgs a, int num_sms, cudaStream_t st) {
     a.short_range = static_cast<int>(span / 2);
     return a.c.D == 64 ? launch_tc<64>(a, st) : launch_tc<128>(a, st);
 }
+
+}  // namespace
+
+cudaError_t kv_attn_tc(KvAttnArgs a, int num_sms, cudaStream_t st) { return run(a, num_sms, st); }
+cudaError_t kv_attn_tc(Kv4AttnArgs a, int num_sms, cudaStream_t st) { return run(a, num_sms, st); }
 
 }  // namespace b200

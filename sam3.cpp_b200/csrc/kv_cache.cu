@@ -26,37 +26,12 @@
 // their last pages read back: 9.7 us, on the device as on the host (two
 // launches).
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.cuh"
 
 namespace b200 {
 namespace {
-
-constexpr float kF32Max = 3.402823466e38f;
-
-// round(x / s), ties to even, for finite |x| <= 127.5 s, s a normal f32, as
-// the low bytes of c.  The magic sum rounds x * inv (inv ~ 1 / s) to an
-// integer q that is at most one off; r = x - q s is exact wherever |r| is near
-// s / 2 (x and q s are multiples of the smaller of their units, and r needs no
-// more bits than s), so comparing it with s / 2 tells on which side of the
-// border x lies.  The largest |r| of 8 values decides whether any is looked
-// at again.
-__device__ __forceinline__ void round_quotients(const float (&x)[8], float s, float inv, int (&c)[8]) {
-    float far = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float m = __fmaf_rn(x[j], inv, 12582912.f);
-        c[j] = __float_as_int(m);
-        far = fmaxf(far, fabsf(__fmaf_rn(-__fsub_rn(m, 12582912.f), s, x[j])));
-    }
-    const float h = 0.5f * s;
-    if (far < h) return;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float r = __fmaf_rn(-__fsub_rn(__int_as_float(c[j]), 12582912.f), s, x[j]);
-        if (fabsf(r) > h || (fabsf(r) == h && (c[j] & 1))) c[j] += r > 0.f ? 1 : -1;
-    }
-}
 
 // The low bytes of four numbers.
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
@@ -72,26 +47,6 @@ struct WriteArgs {
     RowTensor xs[2];
     int *err;
 };
-
-// 8 values as they come.
-template <typename T>
-struct alignas(16) Raw8 {
-    T v[8];
-};
-
-template <bool VEC, typename T>
-__device__ __forceinline__ Raw8<T> raw8(const T *p) {
-    Raw8<T> r;
-    if constexpr (VEC) {
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-            reinterpret_cast<uint4 *>(&r)[i] = reinterpret_cast<const uint4 *>(p)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.v[i] = p[i];
-    }
-    return r;
-}
 
 // Largest magnitude of 8 values by the bits, as those of an f32: infinities and NaN are above all numbers and show.
 __device__ __forceinline__ uint32_t top_bits(const Raw8<float> &r) {
@@ -299,7 +254,11 @@ bool rows_ok(const char *op, const char *what, const RowTensor &t, int64_t rows,
     return false;
 }
 
-bool kv_views(const char *op, const sam3b200_kv_cache *c, const sam3b200_kv_batch *b, KvView &cv, KvRows &bv) {
+namespace {
+
+// The checks that the two caches share.
+template <typename Cache, typename View>
+bool views(const char *op, const Cache *c, const sam3b200_kv_batch *b, View &cv, KvRows &bv) {
     if (!c || !b || !c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale || !b->table || !b->row_start || !b->kv_len) {
         set_error("%s: null argument", op);
         return false;
@@ -317,6 +276,12 @@ bool kv_views(const char *op, const sam3b200_kv_cache *c, const sam3b200_kv_batc
             set_error("%s: cache codes must be 16-byte aligned", op);
             return false;
         }
+    constexpr bool four = std::is_same<View, Kv4View>::value;
+    for (const void *p : {static_cast<const void *>(c->k_scale), static_cast<const void *>(c->v_scale)})
+        if (four && reinterpret_cast<uintptr_t>(p) % 16) {
+            set_error("%s: the scales of a 4-bit cache must be 16-byte aligned", op);
+            return false;
+        }
     for (const void *p : {static_cast<const void *>(c->k_scale), static_cast<const void *>(c->v_scale),
                           static_cast<const void *>(b->table), static_cast<const void *>(b->row_start),
                           static_cast<const void *>(b->kv_len)})
@@ -332,10 +297,21 @@ bool kv_views(const char *op, const sam3b200_kv_cache *c, const sam3b200_kv_batc
     }
     int lg = 4;
     while ((1 << lg) < c->page_tokens) ++lg;
-    cv = KvView{{static_cast<int8_t *>(c->k_codes), static_cast<int8_t *>(c->v_codes)},
-                {c->k_scale, c->v_scale}, c->n_pages, c->n_kv_heads, lg, c->head_dim};
+    using Code = typename std::remove_reference<decltype(*cv.codes[0])>::type;
+    using Scale = typename std::remove_reference<decltype(*cv.scale[0])>::type;
+    cv = View{{static_cast<Code *>(c->k_codes), static_cast<Code *>(c->v_codes)},
+              {static_cast<Scale *>(c->k_scale), static_cast<Scale *>(c->v_scale)}, c->n_pages, c->n_kv_heads, lg, c->head_dim};
     bv = KvRows{b->table, b->row_start, b->kv_len, b->table_width, b->n_seqs, b->n_rows, b->max_rows, b->max_len};
     return true;
+}
+
+}  // namespace
+
+bool kv_views(const char *op, const sam3b200_kv_cache *c, const sam3b200_kv_batch *b, KvView &cv, KvRows &bv) {
+    return views(op, c, b, cv, bv);
+}
+bool kv_views(const char *op, const sam3b200_kv4_cache *c, const sam3b200_kv_batch *b, Kv4View &cv, KvRows &bv) {
+    return views(op, c, b, cv, bv);
 }
 
 }  // namespace b200

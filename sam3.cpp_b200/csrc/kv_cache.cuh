@@ -1,6 +1,7 @@
-// kv_cache.cuh -- the paged 8-bit key/value cache as its kernels see it: the
-// device views of sam3b200_kv_cache and sam3b200_kv_batch, how a kernel finds
-// its sequence, and the host checks shared by the entry points.
+// kv_cache.cuh -- the paged key/value caches of 8 and 4 bits as their kernels
+// see them: the device views of sam3b200_kv_cache, sam3b200_kv4_cache and
+// sam3b200_kv_batch, how a kernel finds its sequence, and the host checks
+// shared by the entry points.
 #pragma once
 
 #include <cstdint>
@@ -17,10 +18,17 @@ namespace b200 {
 // Pages whose largest magnitude is below this store zeros under scale 0, so
 // that reciprocals of scales stay finite.
 constexpr float kKvSmallest = 7.888609052210118e-31f;  // 2^-100
+constexpr float kF32Max = 3.402823466e38f;
 
 struct KvView {
     int8_t *codes[2];  // keys, values: [n_pages][heads][1 << page_log2][D]
     float *scale[2];   // [n_pages][heads]
+    int n_pages, heads, page_log2, D;
+};
+
+struct Kv4View {
+    uint8_t *codes[2];         // keys, values: [n_pages][heads][1 << page_log2][D / 2]
+    __nv_bfloat16 *scale[2];   // [n_pages][heads][1 << page_log2][D / 32]
     int n_pages, heads, page_log2, D;
 };
 
@@ -91,7 +99,8 @@ __device__ __forceinline__ bool kv_find(const KvRows &b, int64_t u, int m, int u
 
 // The page of tokens [i << page_log2, ...) of sequence s; a bad entry is
 // recorded and reads as -1.
-__device__ __forceinline__ int kv_page(const KvView &c, const KvRows &b, int s, int64_t i, int *err) {
+template <typename View>
+__device__ __forceinline__ int kv_page(const View &c, const KvRows &b, int s, int64_t i, int *err) {
     const int p = b.table[s * b.table_width + i];
     if (p >= 0 && p < c.n_pages) return p;
     atomicOr(err, kErrKvPage);
@@ -129,6 +138,50 @@ __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = from_f32<T>(x[i]);
+    }
+}
+
+// 8 values as they come.
+template <typename T>
+struct alignas(16) Raw8 {
+    T v[8];
+};
+
+template <bool VEC, typename T>
+__device__ __forceinline__ Raw8<T> raw8(const T *p) {
+    Raw8<T> r;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+            reinterpret_cast<uint4 *>(&r)[i] = reinterpret_cast<const uint4 *>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = p[i];
+    }
+    return r;
+}
+
+// round(x / s), ties to even, for finite |x| <= 127.5 s, s a normal f32, as
+// the low bytes of c.  The magic sum rounds x * inv (inv ~ 1 / s) to an
+// integer q that is at most one off; r = x - q s is exact wherever |r| is near
+// s / 2 (x and q s are multiples of the smaller of their units, and r needs no
+// more bits than s), so comparing it with s / 2 tells on which side of the
+// border x lies.  The largest |r| of 8 values decides whether any is looked
+// at again.
+__device__ __forceinline__ void round_quotients(const float (&x)[8], float s, float inv, int (&c)[8]) {
+    float far = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float m = __fmaf_rn(x[j], inv, 12582912.f);
+        c[j] = __float_as_int(m);
+        far = fmaxf(far, fabsf(__fmaf_rn(-__fsub_rn(m, 12582912.f), s, x[j])));
+    }
+    const float h = 0.5f * s;
+    if (far < h) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float r = __fmaf_rn(-__fsub_rn(__int_as_float(c[j]), 12582912.f), s, x[j]);
+        if (fabsf(r) > h || (fabsf(r) == h && (c[j] & 1))) c[j] += r > 0.f ? 1 : -1;
     }
 }
 
@@ -200,5 +253,6 @@ inline RowTensor row_tensor(const void *p, int type, const int64_t *nb, int64_t 
 bool rows_ok(const char *op, const char *what, const RowTensor &t, int64_t rows, int64_t heads, int64_t D, bool written);
 // Host checks of a cache and a batch; on failure the message names `op`.
 bool kv_views(const char *op, const sam3b200_kv_cache *c, const sam3b200_kv_batch *b, KvView &cv, KvRows &bv);
+bool kv_views(const char *op, const sam3b200_kv4_cache *c, const sam3b200_kv_batch *b, Kv4View &cv, KvRows &bv);
 
 }  // namespace b200

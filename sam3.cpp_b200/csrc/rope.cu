@@ -21,23 +21,10 @@
 #include <cmath>
 #include <new>
 
-#include "kv_cache.cuh"
+#include "rope.cuh"
 
 namespace b200 {
 namespace {
-
-constexpr int kMaxPairs = 128;
-
-struct RopeTable {
-    double turns[kMaxPairs];  // w / 2 pi
-    uint8_t axis[kMaxPairs];
-    int head_dim, pairs, n_axes, neighbours;
-};
-
-struct Rope {
-    Backend *be;
-    RopeTable t;
-};
 
 struct RopeArgs {
     RopeTable t;
@@ -48,32 +35,6 @@ struct RopeArgs {
     int64_t pos_stride;
     int n_rows, n_heads, heads_each;  // heads a thread walks over
     float sign;
-};
-
-__device__ __forceinline__ void angle(const RopeArgs &a, int i, const int (&p)[4], float &c, float &s) {
-    const int ax = a.t.axis[i];
-    const int at = ax == 0 ? p[0] : ax == 1 ? p[1] : ax == 2 ? p[2] : p[3];
-    const double turns = at * a.t.turns[i];
-    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-    s *= a.sign;
-}
-
-__device__ __forceinline__ void positions(const RopeArgs &a, int row, int (&p)[4]) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) p[k] = k < a.t.n_axes ? a.pos[k * a.pos_stride + row] : 0;
-}
-
-constexpr int kHeadLanes = 8;  // threads that share a row's 8 pairs, over heads
-
-// 8 elements as they come, read past the L1 and soon to be evicted from the L2: nothing is read twice.
-template <typename T>
-struct Stream8 {
-    uint4 raw[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T *p) {
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
-    }
-    __device__ __forceinline__ float operator[](int i) const { return to_f32(reinterpret_cast<const T *>(raw)[i]); }
 };
 
 // Blocks of `rows` rows; a thread: 8 pairs, or 16 elements behind the turned ones, of every eighth head, one at a time:
@@ -99,8 +60,8 @@ __global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeA
         const int64_t r = row0 + id / n;
         if (r >= a.n_rows) break;
         int p[4];
-        positions(a, static_cast<int>(r), p);
-        angle(a, id % n, p, turn[id].x, turn[id].y);
+        positions(a.t, a.pos, a.pos_stride, static_cast<int>(r), p);
+        angle(a.t, a.sign, id % n, p, turn[id].x, turn[id].y);
     }
     __syncthreads();
     float c[8], s[8];
@@ -158,9 +119,9 @@ __global__ void __launch_bounds__(128) rope_any_kernel(const __grid_constant__ R
         return;
     }
     int p[4];
-    positions(a, row, p);
+    positions(a.t, a.pos, a.pos_stride, row, p);
     float c, s;
-    angle(a, part, p, c, s);
+    angle(a.t, a.sign, part, p, c, s);
     const int d0 = a.t.neighbours ? 2 * part : part, d1 = a.t.neighbours ? 2 * part + 1 : part + n;
     for (int h = h0; h < h1; ++h) {
         const float x0 = to_f32(x[h * a.xs.head + d0]), x1 = to_f32(x[h * a.xs.head + d1]);
