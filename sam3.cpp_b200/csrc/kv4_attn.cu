@@ -9,19 +9,22 @@
 //   O(d) = sum over tokens of (p dv(token, g(d))) cv
 // The first takes a multiply-add in f32 a token and group behind two 16-wide
 // products.  The second takes one softmax weight a group: p dv is rounded to
-// f16 (2^-11 of it).  With m the running maximum of t + log2(max over g of
-// |dv|), t = score scale log2(e), the weights p = 2^(t - m) stay in f32 and
-// p dv stays in [-1, 1] for f16 whatever the scales are; O and the sum of p
-// have the same reference, so y = O / l.
+// f16 (2^-11 of it).  With m the running maximum of t + log2(|dv|), t = score
+// scale log2(e) and |dv| the largest of the scales next to it, the weights
+// p = 2^(t - m) stay in f32 and p dv stays in [-1, 1] for f16 whatever the
+// scales are; O and the sum of p have the same reference, so y = O / l.
 //
 // The kernel is kv_attn.cu's otherwise: one block of 4 warps per (8 or 16
-// query rows of a kv head, part of the key range), blocks of 16 tokens through
+// query rows of a kv head, part of the key range), blocks of 32 tokens (two of 16, each in one page) through
 // a warp's own ring of shared memory, codes as the 16-row operand.  A lane's
 // codes come by ldmatrix: plain for keys, word c of each group of token g (8
 // dimensions), and transposed for values, 4 dimensions of tokens 2c and 2c + 1
 // side by side, so a nibble and the one 16 bits above it are the pair that the
 // instruction wants, in either product, and widening is a mask and a
-// subtraction for a pair.
+// subtraction for a pair.  Half of the subtractions (of 72, where a code comes
+// as 64 + code) are left to the products: for keys as what a group's sum starts
+// from, -72 times the sum of its queries, for values as one more product of the
+// weights with -72 a group.
 #include <algorithm>
 #include <cmath>
 
@@ -34,6 +37,27 @@ namespace {
 __device__ __forceinline__ float low_bf16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
+__device__ __forceinline__ float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The largest of three numbers (NaN is none), and of their magnitudes.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+    return d;
+}
+__device__ __forceinline__ float max3_abs(float x, float y, float z) {
+    float d;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
+    return d;
+}
+
+constexpr float kZeroScale = 8.271806125530277e-25f;  // 2^-80: what tokens of zeros count as (2^kZeroScaleLog2)
+static_assert(kZeroScaleLog2 == -80.f, "its logarithm");
+
 // The scales of one token, D / 32 bf16 numbers.
 template <int G>
 __device__ __forceinline__ void scales_of(const uint8_t *from, float (&d)[G]) {
@@ -45,6 +69,24 @@ __device__ __forceinline__ void scales_of(const uint8_t *from, float (&d)[G]) {
         d[0] = low_bf16(w), d[1] = high_bf16(w);
     }
 }
+
+// The words that a lane's rows of four matrices give it, for 16 tokens: w[r][k] of group k and tokens 8 r ... .
+template <int D, bool TRANS>
+__device__ __forceinline__ void load_half(uint32_t (&w)[2][D / 32], uint32_t from) {
+    uint32_t r[4];
+    ldmatrix4<TRANS>(r, from);
+    if constexpr (D == 128) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[0][k] = r[k];
+        ldmatrix4<TRANS>(r, from + 8 * 64);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[1][k] = r[k];
+    } else {
+        w[0][0] = r[0], w[0][1] = r[1], w[1][0] = r[2], w[1][1] = r[3];
+    }
+}
+
+constexpr uint32_t kMinus72 = 0xd480d480u;  // a pair of f16
 
 // Eight consecutive query elements, as they come, and the j-th of them.
 __device__ __forceinline__ uint4 load_q8(const Kv4AttnArgs &a, int64_t at) {
@@ -66,19 +108,20 @@ __device__ __forceinline__ float q_value(const Kv4AttnArgs &a, const uint4 &x, i
 template <int D, int NT>
 struct Few4 {
     static constexpr int kRows = 8 * NT, kGroups = D / 32;
-    static constexpr int kStages = 4, kBlocks = NT == 1 ? 4 : 3;   // stages of a warp, blocks an SM
+    static constexpr int kStages = D == 128 ? 3 : 4, kBlocks = NT == 1 ? 4 : 3;  // stages of a warp, blocks an SM
     static constexpr int kCodeBytes = 16 * D / 2;                  // of 16 tokens
     static constexpr int kScaleBytes = 16 * kGroups * 2;
-    static constexpr int kScaleAt = 2 * kCodeBytes;
-    static constexpr int kStageBytes = 2 * (kCodeBytes + kScaleBytes);
+    // a stage: for each half its keys' and values' codes, then for each half their scales
+    static constexpr int kHalfBytes = 2 * kCodeBytes, kScaleAt = 2 * kHalfBytes, kStageBytes = kScaleAt + 4 * kScaleBytes;
+    static constexpr bool kFoldKeys = false;
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kRowFloats = D + 4;                       // a joined row, padded against bank conflicts
     static constexpr int kJoin = kWarps * kRows * kRowFloats * 4;
     static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
     static_assert(kSmem >= kWarps * kRows * (D + 2) * 4, "shares of the parts");
     static constexpr int kEach = D * kRows / 128 > 8 ? D * kRows / 128 : 8;  // dimensions of a thread that joins
-    // Byte of group c of token t within 16 staged tokens, turned so that 8 consecutive tokens' 16 bytes have different
-    // banks.  Token t + 8 lies 8 tokens further.
+    // Byte of group c of token t within 16 staged tokens, turned so that 8 consecutive tokens' 16 bytes have
+    // different banks.  Token t + 8 lies 8 tokens further.
     static __device__ __forceinline__ uint32_t at(int t, int c) {
         if (D == 128) return t * 64 + (c ^ ((t >> 1) & 3)) * 16;
         return t * 32 + (c ^ ((t >> 2) & 1)) * 16;
@@ -99,7 +142,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
     if (!few_tile<NT>(a, tile)) return;
     const KvSeq &q = tile.q;
     const int row0 = tile.row0, i_lo = tile.i_lo, i_hi = tile.i_hi, R = tile.R, t_begin = tile.t_begin, t_end = tile.t_end;
-    const int n_blocks = t_end > t_begin ? (t_end - t_begin + 15) / 16 : 0;
+    const int n_blocks = t_end > t_begin ? (t_end - t_begin + 31) / 32 : 0;          // of 32 tokens, as two halves
     const int mine = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;  // blocks warp, warp + 4, ...
 
     // the queries are on their way while the first pages are looked up: row 8 n + g, dimensions 8 c ... of each group
@@ -117,35 +160,41 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
     }
 
     uint8_t *ring = smem + warp * F::kStages * F::kStageBytes;
-    // this lane's bytes within a stage: the copy of chunk lane (of 32 a step), and its row of the matrices that it loads
+    // this lane's bytes within a half of a stage: the copy of chunk lane (of 32 a step), and its row of the matrices that it loads
     const uint32_t put0 = F::at(lane / kGroups, lane % kGroups);
     const uint32_t get0 = D == 128 ? F::at(lane & 7, lane >> 3) : F::at((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1);
-    int page_now = 0, page_next = 0;  // lane j: the page of block 32 b + j of this warp, for batches b and b + 1
-    auto load_page = [&](int j) -> int {
-        if (j >= mine) return 0;
-        const int p = kv_page(a.c, a.b, q.s, (t_begin + (j * kWarps + warp) * 16) >> a.c.page_log2, a.err);
-        return max(p, 0);
+    // what this lane copies, for token 0 of the cache's slabs: tokens are counted over all of them, in 32 bits (see kv_views)
+    const uint8_t *own_k = a.c.codes[0] + lane * 16, *own_v = a.c.codes[1] + lane * 16;
+    constexpr int kScaleChunks = F::kScaleBytes / 16;
+    const uint8_t *own_scale = reinterpret_cast<const uint8_t *>(a.c.scale[lane >= kScaleChunks]) + lane % kScaleChunks * 16;
+    const uint32_t ring_at = smem_u32(ring), put_at = ring_at + put0, put_scale_at = ring_at + F::kScaleAt + lane * 16;
+    // lane 2 j + h: where half h of block 16 b + j of this warp begins, for batches b and b + 1
+    uint32_t at_now = 0, at_next = 0;
+    auto look_up = [&](int j) -> uint32_t {
+        const int tok = t_begin + ((j >> 1) * kWarps + warp) * 32 + (j & 1) * 16;
+        if ((j >> 1) >= mine || tok >= t_end) return 0;
+        const int page = max(kv_page(a.c, a.b, q.s, tok >> a.c.page_log2, a.err), 0);
+        return ((static_cast<uint32_t>(page) * a.c.heads + kv) << a.c.page_log2) + (tok & ((1 << a.c.page_log2) - 1));
     };
-    page_next = load_page(lane);
+    at_next = look_up(lane);
+    const int halves = mine ? 2 * mine - (t_begin + ((mine - 1) * kWarps + warp) * 32 + 16 >= t_end) : 0;
     auto issue = [&](int j, int slot) {  // block j of this warp into a slot
-        if (j < mine) {
-            if ((j & 31) == 0) {
-                page_now = page_next;
-                page_next = load_page(j + 32 + lane);
+        if (2 * j < halves) {
+            if ((j & 15) == 0) {
+                at_now = at_next;
+                at_next = look_up(2 * (j + 16) + lane);
             }
-            const int page = __shfl_sync(0xffffffffu, page_now, j & 31);
-            const int tok = t_begin + (j * kWarps + warp) * 16;
-            const int64_t at = ((static_cast<int64_t>(page) * a.c.heads + kv) << a.c.page_log2) + (tok & ((1 << a.c.page_log2) - 1));
-            const uint32_t dst = smem_u32(ring + slot * F::kStageBytes);
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
+            for (int h = 0; h < 2; ++h) {
+                const uint64_t at = __shfl_sync(0xffffffffu, at_now, 2 * (j & 15) + h);
+                if (2 * j + h >= halves) break;
+                const uint32_t to = slot * F::kStageBytes;
 #pragma unroll
-                for (int k = 0; k < F::kCodeBytes / 512; ++k)  // a step of 8 (D = 128) or 16 tokens
-                    cp16(dst + w * F::kCodeBytes + put0 + k * 512, a.c.codes[w] + at * (D / 2) + lane * 16 + k * 512);
-            constexpr int kChunks = F::kScaleBytes / 16;
-            if (lane < 2 * kChunks) {
-                const int w = lane / kChunks, k = lane % kChunks;
-                cp16(dst + F::kScaleAt + lane * 16, a.c.scale[w] + at * kGroups + k * 8);
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int k = 0; k < F::kCodeBytes / 512; ++k)  // a step of 8 (D = 128) or 16 tokens
+                        cp16(put_at + to + h * F::kHalfBytes + w * F::kCodeBytes + k * 512, (w ? own_v : own_k) + at * (D / 2) + k * 512);
+                if (lane < 2 * kScaleChunks) cp16(put_scale_at + to + 2 * h * F::kScaleBytes, own_scale + at * (D / 16));
             }
         }
         cp_commit();
@@ -155,6 +204,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 
     // queries as f16: for a group's two products the pairs of dimensions that codes4 gives
     uint32_t qf[NT][kGroups][4];
+    float from[NT][kGroups][2];
     float row_c[NT][2];  // for rows 8 n + 2 c, + 1: scale log2(e), and what the power of two below took
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -173,17 +223,29 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 qf[n][k][j] = pack_f16(q_value(a, qraw[n][k], j) * down, q_value(a, qraw[n][k], j + 4) * down);
+        if (F::kFoldKeys) {  // what a group's sums start from: -72 for each code that keeps its 64 + 8
 #pragma unroll
-        for (int j = 0; j < 2; ++j) row_c[n][j] = __shfl_sync(0xffffffffu, up, (2 * c + j) * 4);
+            for (int k = 0; k < kGroups; ++k) {
+                const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(&qf[n][k][1])), v = __half22float2(*reinterpret_cast<const __half2 *>(&qf[n][k][3]));
+                float sum = (u.x + u.y) + (v.x + v.y);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) from[n][k][j] = -72.f * __shfl_sync(0xffffffffu, sum, (2 * c + j) * 4);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)  // a factor of 0 would make NaN of -inf; a tiny one leaves 0 of the scores
+            row_c[n][j] = fmaxf(__shfl_sync(0xffffffffu, up, (2 * c + j) * 4), 1e-37f);
     }
     // tokens that some row of the tile does not see, and those that none sees (they need not hold numbers)
     const int seen_by_all = kv_last(a, q, i_lo), window_end = kv_first(a, kv_last(a, q, i_hi)), first_any = kv_first(a, seen_by_all);
 
     float o[NT][D / 16][4];
-    float m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2], high[NT][2], less[NT][2];  // high, less: what follows from m for the next scores
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+        m[n][0] = m[n][1] = high[n][0] = high[n][1] = -INFINITY, l[n][0] = l[n][1] = less[n][0] = less[n][1] = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
@@ -194,131 +256,126 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
         __syncwarp();  // block j is there for all lanes, and block j - 1 is read by all
         issue(j + F::kStages - 1, slot_in);
         const uint8_t *st = ring + slot * F::kStageBytes;
-        const uint32_t st_at = smem_u32(st);
+        const uint32_t st_at = ring_at + slot * F::kStageBytes;
         slot_in = slot;
         slot = slot + 1 == F::kStages ? 0 : slot + 1;
-        const int tok = t_begin + (j * kWarps + warp) * 16;
+        const int tok = t_begin + (j * kWarps + warp) * 32;
 
-        // scores of tokens g (t[n][0], [1]) and g + 8 ([2], [3]) for rows 8 n + 2 c, + 1
-        float t[NT][4];
-        {
+        // scores of tokens 16 h + g (t[h][n][0], [1]) and 16 h + g + 8 ([2], [3]) for rows 8 n + 2 c, + 1
+        float t[2][NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
             uint32_t w[2][kGroups];  // word c of each group of tokens g and g + 8
-            uint32_t r[4];
-            ldmatrix4<false>(r, st_at + get0);
-            if constexpr (D == 128) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[0][k] = r[k];
-                ldmatrix4<false>(r, st_at + get0 + 8 * 64);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[1][k] = r[k];
-            } else {
-                w[0][0] = r[0], w[0][1] = r[1], w[1][0] = r[2], w[1][1] = r[3];
-            }
+            load_half<D, false>(w, st_at + h * F::kHalfBytes + get0);
             float d0[kGroups], d1[kGroups];
-            scales_of<kGroups>(st + F::kScaleAt + g * (2 * kGroups), d0);
-            scales_of<kGroups>(st + F::kScaleAt + (g + 8) * (2 * kGroups), d1);
+            scales_of<kGroups>(st + F::kScaleAt + 2 * h * F::kScaleBytes + g * (2 * kGroups), d0);
+            scales_of<kGroups>(st + F::kScaleAt + 2 * h * F::kScaleBytes + (g + 8) * (2 * kGroups), d1);
 #pragma unroll
             for (int k = 0; k < kGroups; ++k) {
                 uint32_t u[4], v[4];
-                codes4(w[0][k], u);
-                codes4(w[1][k], v);
+                codes4<8, F::kFoldKeys>(w[0][k], u);
+                codes4<8, F::kFoldKeys>(w[1][k], v);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float s[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma16816(s, u[0], v[0], u[1], v[1], qf[n][k][0], qf[n][k][1]);
+                    float s[4];
+                    if (F::kFoldKeys) mma16816_from(s, u[0], v[0], u[1], v[1], qf[n][k][0], qf[n][k][1], from[n][k][0], from[n][k][1]);
+                    else mma16816_first(s, u[0], v[0], u[1], v[1], qf[n][k][0], qf[n][k][1]);
                     mma16816(s, u[2], v[2], u[3], v[3], qf[n][k][2], qf[n][k][3]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float d = i < 2 ? d0[k] : d1[k];
-                        t[n][i] = k ? fmaf(s[i], d, t[n][i]) : s[i] * d;
+                        t[h][n][i] = k ? fmaf(s[i], d, t[h][n][i]) : s[i] * d;
                     }
                 }
             }
         }
-        float d0[kGroups], d1[kGroups];  // the values' scales of tokens g and g + 8
-        scales_of<kGroups>(st + F::kScaleAt + F::kScaleBytes + g * (2 * kGroups), d0);
-        scales_of<kGroups>(st + F::kScaleAt + F::kScaleBytes + (g + 8) * (2 * kGroups), d1);
-        if (tok + 15 >= t_end || tok < first_any) {
-            const bool out0 = tok + g >= t_end || tok + g < first_any, out1 = tok + g + 8 >= t_end || tok + g + 8 < first_any;
+        float dv[2][2][kGroups], top_d = kZeroScale;  // the values' scales of tokens 16 h + 8 r + g
 #pragma unroll
-            for (int k = 0; k < kGroups; ++k) d0[k] = out0 ? 0.f : d0[k], d1[k] = out1 ? 0.f : d1[k];
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) scales_of<kGroups>(st + F::kScaleAt + (2 * h + 1) * F::kScaleBytes + (8 * r + g) * (2 * kGroups), dv[h][r]);
+        if (tok + 31 >= t_end || tok < first_any) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int at = tok + 16 * h + 8 * r + g;
+#pragma unroll
+                    for (int k = 0; k < kGroups; ++k) dv[h][r][k] = at >= t_end || at < first_any ? 0.f : dv[h][r][k];
+                }
         }
-        float top0 = 0.f, top1 = 0.f;
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) top0 = fmaxf(top0, fabsf(d0[k])), top1 = fmaxf(top1, fabsf(d1[k]));
-        const float lv0 = fmaxf(__log2f(top0), kZeroScaleLog2), lv1 = fmaxf(__log2f(top1), kZeroScaleLog2);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) t[n][k] *= row_c[n][k & 1];
-        if (tok + 15 > seen_by_all || tok < window_end) {
+            for (int k = 0; k < kGroups; ++k) top_d = max3_abs(top_d, dv[h][0][k], dv[h][1][k]);
+        const float lv = lg2_approx(top_d);
+        if (tok + 31 > seen_by_all || tok < window_end) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const int last = kv_last(a, q, i_lo + (rest0 + 8 * n + 2 * c + k) / G), first = kv_first(a, last);
-                    if (tok + g > last || tok + g < first) t[n][k] = -INFINITY;
-                    if (tok + g + 8 > last || tok + g + 8 < first) t[n][k + 2] = -INFINITY;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const int at = tok + 16 * h + 8 * r + g;
+                            if (at > last || at < first) t[h][n][2 * r + k] = -INFINITY;
+                        }
                 }
         }
+        auto most = [&](int n, int k) { return fmaf(fmaxf(max3(t[0][n][k], t[0][n][k + 2], t[1][n][k]), t[1][n][k + 2]), row_c[n][k], lv); };
         bool rise = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) rise |= fmaxf(t[n][k] + lv0, t[n][k + 2] + lv1) > m[n][k] + kLazy;
+            for (int k = 0; k < 2; ++k) rise |= most(n, k) > high[n][k];
         if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    float top = fmaxf(t[n][k] + lv0, t[n][k + 2] + lv1);
+                    float top = most(n, k);
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                     const float to = fmaxf(m[n][k], top);
                     const float alpha = m[n][k] == to ? 1.f : ex2_approx(m[n][k] - to);
                     m[n][k] = to;
+                    high[n][k] = to + kLazy;
+                    less[n][k] = to == -INFINITY ? 0.f : to - kPUp;
                     l[n][k] *= alpha;
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) o[n][i][k] *= alpha, o[n][i][k + 2] *= alpha;
                 }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const float less = m[n][k] == -INFINITY ? 0.f : m[n][k] - kPUp;
-                t[n][k] = ex2_approx(t[n][k] - less);
-                t[n][k + 2] = ex2_approx(t[n][k + 2] - less);
-                l[n][k] += t[n][k] + t[n][k + 2];
-            }
-
-        // values: of each group 4 dimensions (4 g ...) of tokens 2c, 2c + 1 and of 8 + 2c, 9 + 2c
-        uint32_t w[2][kGroups];
-        {
-            uint32_t r[4];
-            ldmatrix4<true>(r, st_at + F::kCodeBytes + get0);
-            if constexpr (D == 128) {
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[0][k] = r[k];
-                ldmatrix4<true>(r, st_at + F::kCodeBytes + get0 + 8 * 64);
+                for (int k = 0; k < 2; ++k) {
+                    t[h][n][k] = ex2_approx(fmaf(t[h][n][k], row_c[n][k], -less[n][k]));
+                    t[h][n][k + 2] = ex2_approx(fmaf(t[h][n][k + 2], row_c[n][k], -less[n][k]));
+                    l[n][k] += t[h][n][k] + t[h][n][k + 2];
+                }
+            // values: of each group 4 dimensions (4 g ...) of tokens 2c, 2c + 1 and of 8 + 2c, 9 + 2c
+            uint32_t w[2][kGroups];
+            load_half<D, true>(w, st_at + h * F::kHalfBytes + F::kCodeBytes + get0);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[1][k] = r[k];
-            } else {
-                w[0][0] = r[0], w[0][1] = r[1], w[1][0] = r[2], w[1][1] = r[3];
-            }
-        }
+            for (int k = 0; k < kGroups; ++k) {
+                uint32_t u[4], v[4];
+                codes4<8, true>(w[0][k], u);
+                codes4<8, true>(w[1][k], v);
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
-            uint32_t u[4], v[4];
-            codes4(w[0][k], u);
-            codes4(w[1][k], v);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint32_t p0 = transposed(pack_f16(t[n][0] * d0[k], t[n][1] * d0[k]));
-                const uint32_t p1 = transposed(pack_f16(t[n][2] * d1[k], t[n][3] * d1[k]));
-                // dimensions 4 g, + 1 of the group are rows g, g + 8 of one product, + 2, + 3 of the next
-                mma16816(o[n][2 * k], u[0], u[1], v[0], v[1], p0, p1);
-                mma16816(o[n][2 * k + 1], u[2], u[3], v[2], v[3], p0, p1);
+                for (int n = 0; n < NT; ++n) {
+                    const uint32_t p0 = transposed(pack_f16(t[h][n][0] * dv[h][0][k], t[h][n][1] * dv[h][0][k]));
+                    const uint32_t p1 = transposed(pack_f16(t[h][n][2] * dv[h][1][k], t[h][n][3] * dv[h][1][k]));
+                    // dimensions 4 g, 4 g + 2 of the group are rows g, g + 8 of one product, 4 g + 1, 4 g + 3 of the next,
+                    // whose codes keep their 64 + 8
+                    mma16816(o[n][2 * k], u[0], u[2], v[0], v[2], p0, p1);
+                    mma16816(o[n][2 * k + 1], u[1], u[3], v[1], v[3], p0, p1);
+                    mma16816(o[n][2 * k + 1], kMinus72, kMinus72, kMinus72, kMinus72, p0, p1);
+                }
             }
         }
     }
@@ -338,7 +395,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
             float *to = rows + (warp * F::kRows + row) * F::kRowFloats + 4 * g;
 #pragma unroll
             for (int i = 0; i < D / 16; i += 2)
-                *reinterpret_cast<float4 *>(to + 16 * i) = make_float4(o[n][i][k], o[n][i][k + 2], o[n][i + 1][k], o[n][i + 1][k + 2]);
+                *reinterpret_cast<float4 *>(to + 16 * i) = make_float4(o[n][i][k], o[n][i + 1][k], o[n][i][k + 2], o[n][i + 1][k + 2]);
         }
     __syncthreads();
     few_finish<F, D>(a, tile, smem, s_m, s_l);

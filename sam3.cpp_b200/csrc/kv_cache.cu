@@ -277,6 +277,11 @@ bool views(const char *op, const Cache *c, const sam3b200_kv_batch *b, View &cv,
             return false;
         }
     constexpr bool four = std::is_same<View, Kv4View>::value;
+    // kernels count the slabs' tokens in 32 bits (155 GB at head dim 64, twice that at 128)
+    if (four && static_cast<uint64_t>(c->n_pages) * c->n_kv_heads * c->page_tokens > uint64_t(1) << 31) {
+        set_error("%s: unsupported cache: %d pages of %d tokens for %d heads are too many", op, c->n_pages, c->page_tokens, c->n_kv_heads);
+        return false;
+    }
     for (const void *p : {static_cast<const void *>(c->k_scale), static_cast<const void *>(c->v_scale)})
         if (four && reinterpret_cast<uintptr_t>(p) % 16) {
             set_error("%s: the scales of a 4-bit cache must be 16-byte aligned", op);

@@ -1,20 +1,21 @@
 // mul_mat_vec.cu -- MUL_MAT of 1 to 16 rows with Q4_0 / Q4_1 weights, the
 // activations as they are.
 //
-//   y[m][n] = sum over blocks b of d[n][b] (sum_k (code - 8) x[m][k])
-//             (+ (mn[n][b] + 8 d[n][b]) (sum_k x[m][k]) for Q4_1)  + bias[n]
+//   y[m][n] = sum over blocks b of d[n][b] (sum_k (code - 8) x[m][k])  + bias[n]         Q4_0
+//   y[m][n] = sum over b of d[n][b] (sum_k code x[m][k]) + mn[n][b] (sum_k x[m][k])  + bias[n]  Q4_1
 //
-// Bound by memory: 18 bytes a block of 32 weights, read once.  A tile is 16 rows
-// of the weights; W of a block's 8 warps share it, each with every W-th chunk
-// of 128 k, which it copies by cp.async into its own ring of shared memory.  The
-// products run on mma.m16n8k16 f16 with f32 sums: the codes are its 16-row
-// operand (exact in f16), the rows of x its 8 columns, so up to 8 rows cost what
-// one does, and the legacy matrix instruction is wide enough for what memory
-// delivers.  Word t of each weight row's block (elements 4t ... and 16 + 4t ...)
-// comes to a lane by ldmatrix, a nibble and the one 16 bits above it are one
-// operand register after a mask and a subtraction, and x is staged in shared
-// memory in the same order.  A block's sum is scaled in f32, 4 multiply-adds a
-// lane for 16 x 8 results.
+// Bound by memory: 18 bytes a block of 32 weights, read once.  A block of 16
+// warps an SM keeps x in shared memory; W of its warps share a tile of 16 or 32
+// rows of the weights, each with every W-th chunk of 128 k, which it copies by
+// cp.async into its own ring of shared memory.  The products run on mma.m16n8k16
+// f16 with f32 sums: the codes are its 16-row operand (exact in f16), the rows of
+// x its 8 columns, so up to 8 rows cost what one does, and the legacy matrix
+// instruction is wide enough for what memory delivers; widening the codes and
+// scaling the sums, some 130 instructions for 1 KB of codes, is what comes next.
+// Word t of each weight row's block (elements 4t ... and 16 + 4t ...) comes to a
+// lane by ldmatrix, a nibble and the one 16 bits above it are one operand
+// register after a mask and a subtraction, and x is staged in the same order.  A
+// block's sum is scaled in f32, 4 multiply-adds a lane for 16 x 8 results.
 // x as f16: F16 as it is; BF16 after a power of two a row that brings the
 // largest element to [2^14, 2^15), exact down to 2^-31 of it, and to 2^-39 of it
 // below; F32 the same way as a sum of two f16 numbers in two columns (2^-23 of an
@@ -30,11 +31,9 @@
 namespace b200 {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32, kStages = 4;
+constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kMaxRows = 16;
-constexpr int kCodeBytes = 16 * 64;  // a chunk: 16 rows of 4 blocks
-constexpr int kScaleBytes = 16 * 4 * 2;
-constexpr int kXBytes = 64 << 10;    // most shared memory for x: with more k, x comes in phases
+constexpr int kSmem = 226 << 10;  // of a block, one an SM
 
 struct VecArgs {
     const uint8_t *codes, *scales;
@@ -44,8 +43,19 @@ struct VecArgs {
     void *y;
     int M, N, K, cols;           // cols: columns of x, M or 2 M
     int tiles, chunks, w_log2;   // warps of a tile
-    int phase;                   // chunks of x in shared memory at once, a multiple of 8 or all
+    int phase;                   // chunks of x in shared memory at once, a multiple of the warps of a tile, or all
     int y_type, aligned;         // aligned: four elements of x at once
+};
+
+// NT: tiles of 8 columns; RT: tiles of 16 weight rows that a warp has at once.
+template <int NT, int RT, bool MINS>
+struct Vec {
+    static constexpr int kStages = RT == 1 ? 4 : 3;
+    static constexpr int kCodeBytes = 16 * 64;  // a chunk of 16 rows: 4 blocks each
+    static constexpr int kScaleBytes = 16 * 4 * 2, kRecord = MINS ? 2 * kScaleBytes : kScaleBytes;
+    static constexpr int kStageBytes = RT * (kCodeBytes + kRecord);
+    static constexpr int kRed = 2 * kWarps * NT * RT * 512;
+    static constexpr int kX = kRed + kWarps * kStages * kStageBytes;  // where x begins
 };
 
 // f16 of v; `rest`: what it leaves (0 of an infinity or NaN).
@@ -55,56 +65,91 @@ __device__ __forceinline__ float f16_of(float v, float &rest) {
     return h;
 }
 
+// Four elements as they come.
 template <typename T>
-__device__ __forceinline__ void load4(const T *p, bool aligned, float *v) {
-    T e[4];
-    if (aligned) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(p);
-        else *reinterpret_cast<uint2 *>(e) = *reinterpret_cast<const uint2 *>(p);
-    } else {
+struct alignas(4 * sizeof(T)) Raw4 {
+    T v[4];
+    __device__ __forceinline__ void load(const T *p, bool aligned) {
+        if (aligned) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
+            else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = p[i];
+            for (int i = 0; i < 4; ++i) v[i] = p[i];
+        }
     }
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = to_f32(e[i]);
-}
+        for (int i = 0; i < 4; ++i) v[i] = from_f32<T>(0.f);
+    }
+};
 
-// NT: tiles of 8 columns.
-template <int NT, bool MINS, typename TX>
-__global__ void __launch_bounds__(kThreads, (NT == 1 ? 4 : NT == 2 ? 3 : 2)) mul_mat_vec_kernel(const __grid_constant__ VecArgs a) {
+template <int NT, int RT, bool MINS, typename TX>
+__global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_constant__ VecArgs a) {
+    using V = Vec<NT, RT, MINS>;
+    constexpr int kStages = V::kStages, kStageBytes = V::kStageBytes;
     constexpr int kParts = sizeof(TX) == 4 ? 2 : 1;  // columns of a row
     constexpr bool kScaled = !std::is_same<TX, __half>::value;
-    constexpr int kRecord = MINS ? 2 * kScaleBytes : kScaleBytes, kStageBytes = kCodeBytes + kRecord;
+    constexpr int kFlight = 4;  // rows of x that a thread has on their way at once
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float s_up[kMaxRows], s_down[kMaxRows];
+    __shared__ unsigned s_top[kMaxRows];
+    __shared__ uint4 zeros[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int W = 1 << a.w_log2, group = warp >> a.w_log2, w_in = warp & (W - 1), groups = kWarps >> a.w_log2;
     const int rounds = (a.tiles + gridDim.x * groups - 1) / (gridDim.x * groups), blocks = a.K / 32;
-    float4 *red = reinterpret_cast<float4 *>(smem);                                   // [2][kWarps][NT][32]
-    uint8_t *ring = smem + 2 * kWarps * NT * 512 + warp * (kStages * kStageBytes);
-    uint4 *xs = reinterpret_cast<uint4 *>(smem + kWarps * (2 * NT * 512 + kStages * kStageBytes));  // [block][column][4]
-    float *sums = reinterpret_cast<float *>(xs + a.phase * 4 * a.cols * 4);           // MINS: [block][8 NT]
+    float4 *red = reinterpret_cast<float4 *>(smem);                          // [2][kWarps][RT][NT][32]
+    const uint8_t *ring = smem + V::kRed + warp * (kStages * kStageBytes);
+    uint4 *xs = reinterpret_cast<uint4 *>(smem + V::kX);                     // [block][column][4]
+    float *sums = reinterpret_cast<float *>(xs + a.phase * 4 * a.cols * 4);  // MINS: [block][8 NT]
     auto tile_of = [&](int round) { return (round * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)) * groups + group; };
 
-    // chunk next_c of tile next_tile into a slot; zeros behind the weights' rows and blocks
+    // The copies of a warp's chunks in their order: a lane's rows of codes and its part of the scales; zeros behind the
+    // weights' rows and blocks.
     const int put_row = lane >> 2, put_part = lane & 3;
-    int next_round = 0, next_c = w_in;
-    auto issue = [&](int slot) {
+    const uint32_t ring_at = smem_u32(ring);
+    const uint32_t put0 = put_row * 64 + ((put_part ^ ((put_row >> 1) & 3)) * 16);  // row + 8: 512 further
+    const int64_t eight = static_cast<int64_t>(a.K / 2) * 8;                        // rows, in bytes
+    int next_round = 0, next_c = 0, next_n = 0;
+    const uint8_t *from = nullptr, *from_scales = nullptr;
+    bool more = false;
+    auto to_tile = [&] {
         const int tile = tile_of(next_round);
-        if (next_round < rounds && tile < a.tiles) {
-            const uint32_t dst = smem_u32(ring + slot * kStageBytes);
-            const int b = next_c * 4 + put_part;
+        more = next_round < rounds && tile < a.tiles;
+        if (!more) return;
+        next_n = tile * 16 * RT;
+        next_c = w_in;
+        from = a.codes + static_cast<int64_t>(next_n + put_row) * (a.K / 2) + (w_in * 4 + put_part) * 16;
+        from_scales = a.scales + (static_cast<int64_t>(tile) * RT * a.chunks + w_in) * V::kRecord + lane * 16;
+    };
+    to_tile();
+    auto issue = [&](int slot) {
+        if (more) {
+            const uint32_t dst = ring_at + slot * kStageBytes;
+            if (next_n + 16 * RT <= a.N && next_c * 4 + 4 <= blocks) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int row = put_row + 8 * k, n = tile * 16 + row;
-                const bool there = n < a.N && b < blocks;
-                const uint8_t *from = a.codes + (there ? static_cast<int64_t>(n) * (a.K / 2) + b * 16 : 0);
-                cp16_or_zero(dst + row * 64 + ((put_part ^ ((row >> 1) & 3)) * 16), from, there);
+                for (int k = 0; k < 2 * RT; ++k) cp16(dst + put0 + k * 512, from + k * eight);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2 * RT; ++k) {
+                    const bool there = next_n + put_row + 8 * k < a.N && next_c * 4 + put_part < blocks;
+                    cp16_or_zero(dst + put0 + k * 512, there ? from + k * eight : a.codes, there);
+                }
             }
-            if (lane < kRecord / 16)
-                cp16(dst + kCodeBytes + lane * 16, a.scales + (static_cast<int64_t>(tile) * a.chunks + next_c) * kRecord + lane * 16);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const uint32_t to = dst + RT * V::kCodeBytes + r * V::kRecord + lane * 16;
+                if (lane < V::kRecord / 16) {
+                    if (r == 0 || next_n + 16 * r < a.N) cp16(to, from_scales + static_cast<int64_t>(r) * a.chunks * V::kRecord);
+                    else cp16_or_zero(to, a.scales, false);
+                }
+            }
+            from += W * 64, from_scales += W * V::kRecord;
             next_c += W;
-            if (next_c >= a.chunks) next_c = w_in, ++next_round;
+            if (next_c >= a.chunks) {
+                ++next_round;
+                to_tile();
+            }
         }
         cp_commit();
     };
@@ -114,56 +159,87 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? 4 : NT == 2 ? 3 : 2)) mul
     wait_for_stream();
 
     if (kScaled) {  // the power of two of each row, from its largest finite element
-        for (int m = warp; m < a.M; m += kWarps) {
-            const TX *x = static_cast<const TX *>(a.x) + m * a.ldx;
-            float top = 0.f;
-            for (int k = lane * 4; k < a.K; k += 128) {
-                float v[4];
-                load4(x + k, a.aligned, v);
+        if (threadIdx.x < kMaxRows) s_top[threadIdx.x] = 0;
+        __syncthreads();
+        for (int m0 = 0; m0 < a.M; m0 += kFlight) {
+            const TX *x = static_cast<const TX *>(a.x) + m0 * a.ldx;
+            unsigned top[kFlight];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[i]) <= kF32Max ? fabsf(v[i]) : 0.f);
+            for (int m = 0; m < kFlight; ++m) top[m] = 0;
+            for (int k = threadIdx.x * 4; k < a.K; k += kThreads * 4) {
+                Raw4<TX> raw[kFlight];
+#pragma unroll
+                for (int m = 0; m < kFlight; ++m) {
+                    raw[m].zero();
+                    if (m0 + m < a.M) raw[m].load(x + m * a.ldx + k, a.aligned);
+                }
+#pragma unroll
+                for (int m = 0; m < kFlight; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned bits = __float_as_uint(fabsf(to_f32(raw[m].v[i])));
+                        top[m] = max(top[m], bits < 0x7f800000u ? bits : 0u);
+                    }
             }
 #pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = top > 0.f ? min(268 - ((__float_as_int(top) >> 23) & 0xff), 253) : 127;
-            if (lane == 0) s_down[m] = __int_as_float(e << 23), s_up[m] = __int_as_float((254 - e) << 23);
+            for (int m = 0; m < kFlight; ++m) {
+                top[m] = __reduce_max_sync(0xffffffffu, top[m]);
+                if (lane == m && m0 + m < a.M) atomicMax(&s_top[m0 + m], top[m]);
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x < a.M) {
+            const unsigned top = s_top[threadIdx.x];
+            const int e = top ? min(268 - static_cast<int>(top >> 23), 253) : 127;
+            s_down[threadIdx.x] = __int_as_float(e << 23), s_up[threadIdx.x] = __int_as_float((254 - e) << 23);
         }
         __syncthreads();
     }
+    if (threadIdx.x < 4) zeros[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
     auto stage_x = [&](int c0) {  // chunks c0 ... of x
-        const int n_blocks = min(a.phase, a.chunks - c0) * 4, items = n_blocks * a.M * 4;
+        const int n_blocks = min(a.phase, a.chunks - c0) * 4, items = n_blocks * 4;
         for (int id0 = 0; id0 < items; id0 += kThreads) {  // all lanes: four neighbours share a block
-            const int id = id0 + threadIdx.x, t = id & 3, m = (id >> 2) % a.M, b = (id >> 2) / a.M;
-            float v[8];
+            const int id = id0 + threadIdx.x, t = id & 3, b = id >> 2;
+            const bool there = id < items && c0 * 4 + b < blocks;
+            for (int m0 = 0; m0 < a.M; m0 += kFlight) {
+                const TX *x = static_cast<const TX *>(a.x) + m0 * a.ldx + c0 * 128 + b * 32 + 4 * t;
+                Raw4<TX> raw[kFlight][2];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            if (id < items && c0 * 4 + b < blocks) {
-                const TX *x = static_cast<const TX *>(a.x) + m * a.ldx + (c0 * 4 + b) * 32 + 4 * t;
-                load4(x, a.aligned, v);
-                load4(x + 16, a.aligned, v + 4);
-                if (kScaled) {
-                    const float by = s_down[m];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] *= by;
+                for (int m = 0; m < kFlight; ++m) {
+                    raw[m][0].zero();
+                    raw[m][1].zero();
+                    if (there && m0 + m < a.M) {
+                        raw[m][0].load(x + m * a.ldx, a.aligned);
+                        raw[m][1].load(x + m * a.ldx + 16, a.aligned);
+                    }
                 }
-            }
 #pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-                float h[8], sum = 0.f;
+                for (int m = 0; m < kFlight; ++m) {
+                    if (m0 + m >= a.M) break;
+                    const float by = kScaled ? s_down[m0 + m] : 1.f;
+                    float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float rest;
-                    h[i] = f16_of(v[i], rest);
-                    v[i] = rest;
-                    sum += h[i];
-                }
-                const int col = m * kParts + part;
-                if (id < items)
-                    xs[(b * a.cols + col) * 4 + t] = make_uint4(pack_f16(h[0], h[2]), pack_f16(h[4], h[6]), pack_f16(h[1], h[3]), pack_f16(h[5], h[7]));
-                if (MINS) {
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                    if (id < items && t == 0) sums[b * 8 * NT + col] = sum;
+                    for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[m][i >> 2].v[i & 3]) * by;
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) {
+                        float h[8], sum = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float rest;
+                            h[i] = f16_of(v[i], rest);
+                            v[i] = rest;
+                            sum += h[i];
+                        }
+                        const int col = (m0 + m) * kParts + part;
+                        if (id < items)
+                            xs[(b * a.cols + col) * 4 + t] =
+                                make_uint4(pack_f16(h[0], h[2]), pack_f16(h[4], h[6]), pack_f16(h[1], h[3]), pack_f16(h[5], h[7]));
+                        if (MINS) {
+                            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                            if (id < items && t == 0) sums[b * 8 * NT + col] = sum;
+                        }
+                    }
                 }
             }
         }
@@ -172,14 +248,24 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? 4 : NT == 2 ? 3 : 2)) mul
                 if (id % (8 * NT) >= a.cols) sums[id] = 0.f;
     };
 
-    const uint32_t get0 = ((lane & 7) + (lane >> 3 & 1) * 8) * 64, get_turn = (lane & 7) >> 1, get_part = lane >> 4;
+    const uint32_t get0 = ((lane & 7) + (lane >> 3 & 1) * 8) * 64 + (((lane >> 4) ^ ((lane & 7) >> 1)) * 16);  // blocks 2, 3: ^ 32
+    // where this lane's column of x lies, and its step from block to block: columns of no row read zeros
+    uint32_t x_at[NT], x_step[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const bool there = n * 8 + g < a.cols;
+        x_at[n] = there ? smem_u32(xs) + ((n * 8 + g) * 4 + c) * 16 : smem_u32(zeros) + c * 16;
+        x_step[n] = there ? a.cols * 64 : 0;
+    }
     int slot = 0, slot_in = kStages - 1;
 #pragma unroll 1
     for (int round = 0; round < rounds; ++round) {
         const int tile = tile_of(round);
-        float acc[NT][4];
+        float acc[RT][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.f;
 #pragma unroll 1
         for (int p0 = 0; p0 < a.chunks; p0 += a.phase) {
             if (round == 0 || a.phase < a.chunks) {
@@ -189,75 +275,95 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? 4 : NT == 2 ? 3 : 2)) mul
             }
             if (tile >= a.tiles) continue;
             const int end = min(p0 + a.phase, a.chunks);
+            uint32_t x_now[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x_now[n] = x_at[n] + w_in * 4 * x_step[n];
 #pragma unroll 1
             for (int ch = p0 + w_in; ch < end; ch += W) {
                 cp_wait<kStages - 2>();
                 __syncwarp();  // the chunk is there for all lanes, and the one before is read by all
                 issue(slot_in);
                 const uint8_t *st = ring + slot * kStageBytes;
-                const uint32_t st_at = smem_u32(st);
+                const uint32_t st_at = ring_at + slot * kStageBytes;
                 slot_in = slot;
                 slot = slot + 1 == kStages ? 0 : slot + 1;
-                const uint2 da = *reinterpret_cast<const uint2 *>(st + kCodeBytes + g * 8), db = *reinterpret_cast<const uint2 *>(st + kCodeBytes + g * 8 + 64);
-                uint2 ma = make_uint2(0u, 0u), mb = ma;
-                if (MINS) {
-                    ma = *reinterpret_cast<const uint2 *>(st + kCodeBytes + kScaleBytes + g * 8);
-                    mb = *reinterpret_cast<const uint2 *>(st + kCodeBytes + kScaleBytes + g * 8 + 64);
-                }
-                auto half_of = [](const uint2 &w, int b) {
-                    const uint32_t x = b < 2 ? w.x : w.y;
-                    return __half2float(__ushort_as_half(static_cast<uint16_t>(b & 1 ? x >> 16 : x)));
-                };
-                const uint4 *xb = xs + static_cast<int64_t>(ch - p0) * 4 * a.cols * 4;
-                uint32_t w[2][4];  // rows g and g + 8, word c of each block
+                __half2 d[RT][2][2], mn[RT][2][2];  // rows g and g + 8, blocks 0, 1 and 2, 3
+                uint32_t w[RT][2][4];               // rows g and g + 8, word c of each block
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    uint32_t r[4];
-                    ldmatrix4<false>(r, st_at + get0 + (((2 * k + get_part) ^ get_turn) * 16));
-                    w[0][2 * k] = r[0], w[1][2 * k] = r[1], w[0][2 * k + 1] = r[2], w[1][2 * k + 1] = r[3];
+                for (int r = 0; r < RT; ++r) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint8_t *at = st + RT * V::kCodeBytes + r * V::kRecord + (g + 8 * h) * 8;
+                        *reinterpret_cast<uint2 *>(d[r][h]) = *reinterpret_cast<const uint2 *>(at);
+                        if (MINS) *reinterpret_cast<uint2 *>(mn[r][h]) = *reinterpret_cast<const uint2 *>(at + V::kScaleBytes);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t z[4];
+                        ldmatrix4<false>(z, st_at + r * V::kCodeBytes + (get0 ^ (32 * k)));
+                        w[r][0][2 * k] = z[0], w[r][1][2 * k] = z[1], w[r][0][2 * k + 1] = z[2], w[r][1][2 * k + 1] = z[3];
+                    }
                 }
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    uint32_t u[4], v[4];
-                    codes4(w[0][b], u);
-                    codes4(w[1][b], v);
-                    const float d0 = half_of(da, b), d1 = half_of(db, b);
+                    uint4 y[NT];
+                    float2 x[NT];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        uint4 y = make_uint4(0u, 0u, 0u, 0u);
-                        if (n * 8 + g < a.cols) y = xb[(b * a.cols + n * 8 + g) * 4 + c];
-                        float s[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma16816(s, u[0], v[0], u[1], v[1], y.x, y.y);
-                        mma16816(s, u[2], v[2], u[3], v[3], y.z, y.w);
-                        acc[n][0] = fmaf(s[0], d0, acc[n][0]), acc[n][1] = fmaf(s[1], d0, acc[n][1]);
-                        acc[n][2] = fmaf(s[2], d1, acc[n][2]), acc[n][3] = fmaf(s[3], d1, acc[n][3]);
-                        if (MINS) {
-                            const float2 x = *reinterpret_cast<const float2 *>(sums + ((ch - p0) * 4 + b) * 8 * NT + n * 8 + 2 * c);
-                            const float m0 = fmaf(8.f, d0, half_of(ma, b)), m1 = fmaf(8.f, d1, half_of(mb, b));
-                            acc[n][0] = fmaf(x.x, m0, acc[n][0]), acc[n][1] = fmaf(x.y, m0, acc[n][1]);
-                            acc[n][2] = fmaf(x.x, m1, acc[n][2]), acc[n][3] = fmaf(x.y, m1, acc[n][3]);
+                        y[n] = lds128(x_now[n]);
+                        x_now[n] += x_step[n];
+                        if (MINS) x[n] = *reinterpret_cast<const float2 *>(sums + ((ch - p0) * 4 + b) * 8 * NT + n * 8 + 2 * c);
+                    }
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        uint32_t u[4], v[4];
+                        codes4<MINS ? 0 : 8>(w[r][0][b], u);
+                        codes4<MINS ? 0 : 8>(w[r][1][b], v);
+                        float ds[2], ms[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            ds[h] = b & 1 ? __high2float(d[r][h][b >> 1]) : __low2float(d[r][h][b >> 1]);
+                            if (MINS) ms[h] = b & 1 ? __high2float(mn[r][h][b >> 1]) : __low2float(mn[r][h][b >> 1]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float s[4];
+                            mma16816_first(s, u[0], v[0], u[1], v[1], y[n].x, y[n].y);
+                            mma16816(s, u[2], v[2], u[3], v[3], y[n].z, y[n].w);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                acc[r][n][i] = fmaf(s[i], ds[i >> 1], acc[r][n][i]);
+                                if (MINS) acc[r][n][i] = fmaf(i & 1 ? x[n].y : x[n].x, ms[i >> 1], acc[r][n][i]);
+                            }
                         }
                     }
                 }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) x_now[n] += (W - 1) * 4 * x_step[n];
             }
         }
         if (tile >= a.tiles) continue;
         if (W > 1) {
             // Two buffers in turn: a round's is written again behind the barrier of the round between.
-            float4 *to = red + ((round & 1) * kWarps + group * W) * NT * 32;
+            float4 *to = red + ((round & 1) * kWarps + group * W) * RT * NT * 32;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) to[(w_in * NT + n) * 32 + lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    to[((w_in * RT + r) * NT + n) * 32 + lane] = make_float4(acc[r][n][0], acc[r][n][1], acc[r][n][2], acc[r][n][3]);
             asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(W * 32) : "memory");
             if (w_in != (round & (W - 1))) continue;  // the warps take turns to finish a tile
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float4 s = to[n * 32 + lane];
-                for (int k = 1; k < W; ++k) {
-                    const float4 x = to[(k * NT + n) * 32 + lane];
-                    s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float4 s = to[(r * NT + n) * 32 + lane];
+                    for (int k = 1; k < W; ++k) {
+                        const float4 x = to[((k * RT + r) * NT + n) * 32 + lane];
+                        s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+                    }
+                    acc[r][n][0] = s.x, acc[r][n][1] = s.y, acc[r][n][2] = s.z, acc[r][n][3] = s.w;
                 }
-                acc[n][0] = s.x, acc[n][1] = s.y, acc[n][2] = s.z, acc[n][3] = s.w;
-            }
         }
         auto store = [&](int m, int n, float v) {
             if (m >= a.M || n >= a.N) return;
@@ -268,17 +374,19 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? 4 : NT == 2 ? 3 : 2)) mul
             else static_cast<TX *>(a.y)[at] = from_f32<TX>(v);
         };
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int out = tile * 16 + g + 8 * r;
-                if (kParts == 2) {
-                    store(n * 4 + c, out, acc[n][2 * r] + acc[n][2 * r + 1]);
-                } else {
-                    store(n * 8 + 2 * c, out, acc[n][2 * r]);
-                    store(n * 8 + 2 * c + 1, out, acc[n][2 * r + 1]);
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int out = (tile * RT + r) * 16 + g + 8 * h;
+                    if (kParts == 2) {
+                        store(n * 4 + c, out, acc[r][n][2 * h] + acc[r][n][2 * h + 1]);
+                    } else {
+                        store(n * 8 + 2 * c, out, acc[r][n][2 * h]);
+                        store(n * 8 + 2 * c + 1, out, acc[r][n][2 * h + 1]);
+                    }
                 }
-            }
     }
     cp_wait<0>();
 }
@@ -300,33 +408,43 @@ __global__ void vec_scales_kernel(const uint8_t *blocks, int N, int nblk, int mi
     if (mins) out[record * 128 + 64 + (id & 63)] = __ushort_as_half(m);
 }
 
-template <int NT, bool MINS, typename TX>
+template <int NT, int RT, bool MINS, typename TX>
 cudaError_t launch(Backend *be, VecArgs &a) {
-    constexpr int kRecord = MINS ? 2 * kScaleBytes : kScaleBytes;
+    using V = Vec<NT, RT, MINS>;
+    a.tiles = (a.N + 16 * RT - 1) / (16 * RT);
     const int per_chunk = 4 * (a.cols * 64 + (MINS ? 8 * NT * 4 : 0));
-    a.phase = a.chunks * per_chunk <= kXBytes ? a.chunks : std::max(kXBytes / per_chunk / 8, 1) * 8;
-    const int smem = kWarps * (2 * NT * 512 + kStages * (kCodeBytes + kRecord)) + a.phase * per_chunk;
-    void (*const kernel)(VecArgs) = mul_mat_vec_kernel<NT, MINS, TX>;
-    constexpr int kSmemMost = kWarps * (2 * NT * 512 + kStages * (kCodeBytes + kRecord)) + std::max(kXBytes, 8 * 4 * 8 * NT * (64 + 4));
-    static_assert(kSmemMost + 1024 <= 227 << 10, "shared memory");
-    constexpr unsigned kBit = 1u << (NT + 4 * MINS + 8 * (sizeof(TX) == 4 ? 0 : std::is_same<TX, __half>::value ? 1 : 2));
+    static_assert((kSmem - V::kX) / (4 * 8 * NT * (64 + (MINS ? 4 : 0))) >= 8, "phases of several chunks");
+    const int most = (kSmem - V::kX) / per_chunk;
+    const bool phases = a.chunks > most;
+    void (*const kernel)(VecArgs) = mul_mat_vec_kernel<NT, RT, MINS, TX>;
+    constexpr unsigned kBit = 1u << (((NT == 4 ? 4 : 2 * (NT - 1) + RT - 1) + 5 * MINS) + 10 * (sizeof(TX) == 4 ? 0 : std::is_same<TX, __half>::value ? 1 : 2));
     if (!(be->vec_ready & kBit)) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return e;
         be->vec_ready |= kBit;
     }
-    const int resident = std::min(NT == 1 ? 4 : NT == 2 ? 3 : 2, (227 << 10) / (smem + 1024 + 256));
-    // warps a tile: the number that gives the fewest steps of a warp, a tile's end counted as one
+    // warps a tile: the number that gives the fewest steps of a warp, a tile's end counted as one, and x that comes again
+    // for every tile by its instructions
     int64_t least = 0x7fffffffffffffff;
-    const int64_t fit = static_cast<int64_t>(be->num_sms) * resident;
-    for (int lg = 0; lg <= 3 && (1 << lg) <= a.chunks; ++lg) {
-        const int64_t tiles_round = fit * (kWarps >> lg);
-        const int64_t cost = (a.tiles + tiles_round - 1) / tiles_round * ((a.chunks + (1 << lg) - 1) / (1 << lg) + 1);
+    for (int lg = 0; lg <= 4 && (1 << lg) <= std::min(a.chunks, most); ++lg) {
+        const int64_t tiles_round = static_cast<int64_t>(be->num_sms) * (kWarps >> lg);
+        const int64_t steps = (a.chunks + (1 << lg) - 1) / (1 << lg) + 1 + (phases ? a.chunks * a.cols / 64 : 0);
+        const int64_t cost = (a.tiles + tiles_round - 1) / tiles_round * steps;
         if (cost <= least) least = cost, a.w_log2 = lg;
     }
+    a.phase = phases ? most >> a.w_log2 << a.w_log2 : a.chunks;
+    const int smem = V::kX + a.phase * per_chunk;
     const int groups = kWarps >> a.w_log2;
-    const int64_t grid = std::min<int64_t>(fit, (a.tiles + groups - 1) / groups);
+    const int64_t grid = std::min<int64_t>(be->num_sms, (a.tiles + groups - 1) / groups);
     return launch_after(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, be->stream, a);
+}
+
+// Tiles of 32 rows where there are enough of them: x is read from shared memory once for both halves.
+template <int NT, bool MINS, typename TX>
+cudaError_t launch(Backend *be, VecArgs &a) {
+    if constexpr (NT < 4)
+        if (a.N >= be->num_sms * 32) return launch<NT, 2, MINS, TX>(be, a);
+    return launch<NT, 1, MINS, TX>(be, a);
 }
 
 }  // namespace
@@ -376,7 +494,7 @@ extern "C" int sam3b200_mul_mat_vec(sam3b200_backend *h, const sam3b200_weight *
     a.x = x, a.ldx = ldx, a.ldy = ldd, a.bias = bias, a.y = dst;
     a.M = static_cast<int>(M), a.N = w->N, a.K = w->K;
     a.cols = a.M * (x_type == SAM3B200_TYPE_F32 ? 2 : 1);
-    a.tiles = (a.N + 15) / 16, a.chunks = (a.K + 127) / 128;
+    a.tiles = 0, a.chunks = (a.K + 127) / 128;
     a.w_log2 = 0, a.phase = a.chunks;
     a.y_type = y_type;
     a.aligned = reinterpret_cast<uintptr_t>(x) % (4 * xb) == 0 && ldx % 4 == 0;
