@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <type_traits>
 
 #include "../../include/sam3_b200.h"
 #include "backend_impl.h"
@@ -130,9 +131,16 @@ template <bool VEC, typename T>
 __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
     if constexpr (VEC) {
         uint4 raw[sizeof(T) / 2];
-        T *e = reinterpret_cast<T *>(raw);
+        if constexpr (std::is_same<T, __half>::value) {  // two in one conversion
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+            for (int i = 0; i < 4; ++i) reinterpret_cast<__half2 *>(raw)[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<__nv_bfloat162 *>(raw)[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) reinterpret_cast<T *>(raw)[i] = x[i];
+        }
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4 *>(p)[i] = raw[i];
     } else {

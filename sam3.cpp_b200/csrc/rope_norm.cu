@@ -14,12 +14,18 @@
 #include <algorithm>
 #include <cmath>
 
+#include "ptx.cuh"
 #include "rope.cuh"
 
 namespace b200 {
 namespace {
 
 constexpr int kMaxSets = 4;
+// Blocks an SM that the registers are cut for (us, a video prompt of 40 heads of 128 in bf16: 5 blocks 101, 6 92, 8 88; an
+// image of 32 heads of 64, f32 to f16: 5 blocks 19.6, 6 20.0, 8 21.4).
+template <typename TX>
+constexpr int kBlocks = sizeof(TX) == 2 ? 8 : 6;
+constexpr float kEpsLeast = 1.17549435e-38f;
 constexpr float kSumMost = 3e38f;               // sums of squares above this are taken again, of elements
 constexpr float kShrink = 8.470329472543003e-22f;  // 2^-70 times as large
 
@@ -36,8 +42,8 @@ struct RopeNormArgs {
     const int32_t *pos;
     int64_t pos_stride;
     int n_sets, n_rows, heads_each;  // heads that a block walks over
-    int w_type;
-    float eps;
+    int w_type, layer;
+    float eps, inv_dim;
 };
 
 __device__ __forceinline__ float weight_at(const void *w, int type, int i, float none) {
@@ -47,63 +53,110 @@ __device__ __forceinline__ float weight_at(const void *w, int type, int i, float
     return to_f32(static_cast<const __nv_bfloat16 *>(w)[i]);
 }
 
-// The N elements of this lane become (x - mean) / sqrt(var + eps) over the elements of its group of lanes (a power of
-// two of them); lanes without elements of the head bring zeros and live = false.
-template <bool LAYER, int N>
-__device__ __forceinline__ void normalise(float (&f)[N], bool live, int lanes, float dim, float eps) {
-    auto total = [&](float s) {
-        for (int o = lanes >> 1; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        return s;
-    };
-    auto squares = [&] {
-        if (LAYER) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) s += f[i];
-            const float mean = total(s) / dim;
-#pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = live ? f[i] - mean : 0.f;
-        }
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) s = fmaf(f[i], f[i], s);
-        return total(s);
-    };
-    float x[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = f[i];
-    float sum = squares();
-    if (__any_sync(0xffffffffu, !(sum <= kSumMost))) {  // elements above 2^60 or so
-        const float by = sum <= kSumMost ? 1.f : kShrink;
-#pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = x[i] * by;
-        sum = squares();
-        eps *= by * by;
-    }
-    const float r = __frsqrt_rn(sum / dim + eps);
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] *= r;
+__device__ __forceinline__ float rsqrt_approx(float x) {
+    float y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-// Blocks of `rows` rows; 8 pairs, or 16 elements behind the turned ones, of every eighth head a thread (see rope.cu).
-// lanes: threads of a head, head_dim / 16 rounded up to a power of two.
-template <typename TX, typename TY, bool NEIGHBOURS, bool LAYER>
-__global__ void __launch_bounds__(128) rope_norm_kernel(const __grid_constant__ RopeNormArgs a, int rows, int lanes) {
-    __shared__ float2 turn[128];
-    extern __shared__ __align__(16) float weights[];  // [set][weight, bias][head_dim]
+// Over the 16 elements of this lane and those of its group of lanes (a power of two of them; `mine`: this one has
+// elements of the head): what is taken off each element, and what it is multiplied by, (x - mean) / sqrt(var + eps).
+// Where the squares pass f32 the elements become 2^-70 times as large first.
+template <bool CENTER>
+__device__ __forceinline__ void moments(float (&f)[16], bool mine, int lanes, float inv_dim, float eps, float &mean, float &by) {
+    auto total = [&](float s) {
+        s = mine ? s : 0.f;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            const float x = __shfl_xor_sync(0xffffffffu, s, o);
+            if (o < lanes) s += x;
+        }
+        return s;
+    };
+    auto variance = [&] {
+        mean = 0.f;
+        if (CENTER) {
+            float s0 = f[0], s1 = f[1];
+#pragma unroll
+            for (int i = 2; i < 16; i += 2) fadd2(s0, s1, s0, s1, f[i], f[i + 1]);
+            mean = total(s0 + s1) * inv_dim;
+        }
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            float d0 = f[i], d1 = f[i + 1];
+            if (CENTER) fadd2(d0, d1, d0, d1, -mean, -mean);
+            ffma2(s0, s1, d0, d1, d0, d1);
+        }
+        return total(s0 + s1);
+    };
+    float sum = variance();
+    if (__any_sync(0xffffffffu, !(sum <= kSumMost))) {  // elements above 2^60 or so
+        if (!(sum <= kSumMost)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] *= kShrink;
+            eps *= kShrink * kShrink;
+        }
+        sum = variance();
+    }
+    by = rsqrt_approx(fmaf(sum, inv_dim, eps));
+}
+
+// Blocks of `rows` rows; a thread: 8 pairs, or 16 elements behind the turned ones, of every eighth head (see rope.cu), the
+// next head's on their way while one is worked on.  lanes: threads of a head, head_dim / 16 rounded up to a power of two.
+// PLAIN: an RMS norm without biases.
+template <typename TX, typename TY, bool NEIGHBOURS, bool PLAIN>
+__global__ void __launch_bounds__(128, kBlocks<TX>) rope_norm_kernel(const __grid_constant__ RopeNormArgs a, int rows, int lanes) {
+    __shared__ __align__(16) float2 turn[128];
+    extern __shared__ __align__(16) float weights[];
     wait_for_stream();
-    const int n = a.t.pairs, D = a.t.head_dim;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows;
-    const int part = threadIdx.x & (lanes - 1), lane = threadIdx.x / lanes % kHeadLanes, row_in = threadIdx.x / (lanes * kHeadLanes);
-    const int64_t row = row0 + row_in;
-    const bool turned = part < n / 8, mine = part < D / 16 && row < a.n_rows;
-    int d0, d1;  // first elements of the two groups of 8
-    if (NEIGHBOURS || !turned) d0 = part * 16, d1 = d0 + 8;
+    const int n = a.t.pairs, D = a.t.head_dim, lanes_log2 = 31 - __clz(lanes);
+    const int part = threadIdx.x & (lanes - 1), lane = (threadIdx.x >> lanes_log2) % kHeadLanes, row_in = threadIdx.x >> lanes_log2 >> 3;
+    static_assert(kHeadLanes == 8, "row_in");
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows, row = min(row0 + row_in, static_cast<int64_t>(a.n_rows) - 1);
+    const bool turned = part < n / 8, mine = part < D / 16, here = mine && row0 + row_in < a.n_rows;
+    int d0, d1;  // first elements of the two groups of 8; threads without any look at the first ones
+    if (NEIGHBOURS || !turned) d0 = mine ? part * 16 : 0, d1 = d0 + 8;
     else d0 = part * 8, d1 = n + part * 8;
+
+    const int h_end = min(static_cast<int>(blockIdx.y + 1) * a.heads_each, a.set[a.n_sets - 1].end);
+    int h = blockIdx.y * a.heads_each + lane;  // this lane's head, counted over all sets
+    // A walk over this lane's heads of x, and another of y: the set, its end, the head's elements, the way to the next head.
+    int x_set = -1, x_end = 0, y_set = -1, y_end = 0;
+    const TX *x = nullptr;
+    TY *y = nullptr;
+    int64_t x_step = 0, y_step = 0;
+    auto seek = [&](int at, int &set, int &end) {
+        int first = 0;
+        do {
+            ++set;
+            first = set ? a.set[set - 1].end : 0;
+            end = a.set[set].end;
+        } while (at >= end);
+        return at - first;
+    };
+    auto x_seek = [&](int at) {
+        const int k = seek(at, x_set, x_end);
+        const HeadSet &q = a.set[x_set];
+        x = static_cast<const TX *>(q.x) + row * q.xs.token + k * q.xs.head, x_step = kHeadLanes * q.xs.head;
+    };
+    auto y_seek = [&](int at) {
+        const int k = seek(at, y_set, y_end);
+        const HeadSet &q = a.set[y_set];
+        y = static_cast<TY *>(q.y) + row * q.ys.token + k * q.ys.head, y_step = kHeadLanes * q.ys.head;
+    };
+    x_seek(min(h, h_end - 1));  // (lanes behind the end look at the last head)
+    Stream8<TX> u, v;
+    u.load(x + d0);
+    v.load(x + d1);
+    // weights in the order in which the threads of a head read them, 4 at a time: [set][weight, bias][4 of a thread's 16][thread]
     for (int id = threadIdx.x; id < a.n_sets * D; id += blockDim.x) {
-        const int s = id / D, i = id % D;
-        weights[2 * s * D + i] = weight_at(a.set[s].weight, a.w_type, i, 1.f);
-        weights[(2 * s + 1) * D + i] = weight_at(a.set[s].bias, a.w_type, i, 0.f);
+        const int k = id / D, i = id % D;
+        const bool half = !NEIGHBOURS && i < 2 * n;
+        const int of = half ? i % n / 8 : i / 16, e = half ? i % n % 8 + i / n * 8 : i % 16;
+        float *to = weights + ((2 * k * 4 + e / 4) * lanes + of) * 4 + e % 4;
+        *to = weight_at(a.set[k].weight, a.w_type, i, 1.f);
+        if (!PLAIN) to[16 * lanes] = weight_at(a.set[k].bias, a.w_type, i, 0.f);
     }
     for (int id = threadIdx.x; id < rows * n; id += blockDim.x) {
         const int64_t r = row0 + id / n;
@@ -113,65 +166,60 @@ __global__ void __launch_bounds__(128) rope_norm_kernel(const __grid_constant__ 
         angle(a.t, 1.f, id % n, p, turn[id].x, turn[id].y);
     }
     __syncthreads();
+    // f[j] and f[j + 8] are pair j: of the 16 elements the halves, or the even and the odd ones
+    auto place = [](int e) { return NEIGHBOURS ? (e & 1) * 8 + (e >> 1) : e; };
     float c[8], s[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float2 z = turned && mine ? turn[row_in * n + part * 8 + j] : make_float2(1.f, 0.f);
-        c[j] = z.x, s[j] = z.y;
+    for (int j = 0; j < 8; j += 2) {
+        float4 z = make_float4(1.f, 0.f, 1.f, 0.f);
+        if (turned) z = *reinterpret_cast<const float4 *>(&turn[row_in * n + part * 8 + j]);
+        c[j] = z.x, s[j] = z.y, c[j + 1] = z.z, s[j + 1] = z.w;
     }
-    const int h_begin = blockIdx.y * a.heads_each, h_end = h_begin + a.heads_each;
 #pragma unroll 1
-    for (int i = 0, first = 0; i < a.n_sets; first = a.set[i].end, ++i) {
-        const HeadSet &q = a.set[i];
-        const int lo = max(h_begin, first), hi = min(h_end, q.end);
-        if (lo >= hi) continue;
-        float w[16], b[16];
+    for (int k = blockIdx.y * a.heads_each; k < h_end; k += kHeadLanes, h += kHeadLanes) {  // all lanes, for the shuffles
+        float f[16], mean = 0.f, by;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            w[j] = mine ? weights[2 * i * D + d0 + j] : 0.f, w[j + 8] = mine ? weights[2 * i * D + d1 + j] : 0.f;
-            b[j] = mine ? weights[(2 * i + 1) * D + d0 + j] : 0.f, b[j + 8] = mine ? weights[(2 * i + 1) * D + d1 + j] : 0.f;
+        for (int j = 0; j < 8; ++j) f[place(j)] = u[j], f[place(j + 8)] = v[j];
+        if (h + kHeadLanes < h_end) {
+            if (h + kHeadLanes < x_end) x += x_step;
+            else x_seek(h + kHeadLanes);
+            u.load(x + d0);
+            v.load(x + d1);
         }
-        const TX *x = static_cast<const TX *>(q.x) + row * q.xs.token;
-        TY *y = static_cast<TY *>(q.y) + row * q.ys.token;
-#pragma unroll 1
-        for (int h0 = lo; h0 < hi; h0 += kHeadLanes) {  // all lanes, for the shuffles
-            const int h = h0 + lane - first;
-            const bool live = mine && h0 + lane < hi;
-            float f[16];
+        if (PLAIN || !a.layer) moments<false>(f, mine, lanes, a.inv_dim, a.eps, mean, by);
+        else moments<true>(f, mine, lanes, a.inv_dim, a.eps, mean, by);
+        if (!here || h >= h_end) continue;
+        if (h < y_end) y += y_step;
+        else y_seek(h);
+        // (weights stay in shared memory: their registers are worth more as blocks an SM)
+        const float *w = weights + (8 * y_set * lanes + part) * 4;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] = 0.f;
-            if (live) {
-                Stream8<TX> u, v;
-                u.load(x + h * q.xs.head + d0);
-                v.load(x + h * q.xs.head + d1);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = u[j], f[j + 8] = v[j];
-            }
-            normalise<LAYER>(f, live, lanes, static_cast<float>(D), a.eps);
-            if (!live) continue;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] = fmaf(f[j], w[j], b[j]);
-            float lo8[8], hi8[8];
-            if (turned) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {  // pair j: elements j and j + 8 of the 16, or 2 j and 2 j + 1
-                    const int e0 = NEIGHBOURS ? 2 * j : j, e1 = NEIGHBOURS ? 2 * j + 1 : j + 8;
-                    const float x0 = f[e0], x1 = f[e1];
-                    f[e0] = x0 * c[j] - x1 * s[j];
-                    f[e1] = x1 * c[j] + x0 * s[j];
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) lo8[j] = f[j], hi8[j] = f[j + 8];
-            store8<true>(y + h * q.ys.head + d0, lo8);
-            store8<true>(y + h * q.ys.head + d1, hi8);
+        for (int e = 0; e < 16; e += 4) {
+            const float4 z = *reinterpret_cast<const float4 *>(w + e * lanes);
+            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!PLAIN) b = *reinterpret_cast<const float4 *>(w + (16 + e) * lanes);
+            f[place(e)] = fmaf((f[place(e)] - mean) * by, z.x, b.x), f[place(e + 1)] = fmaf((f[place(e + 1)] - mean) * by, z.y, b.y);
+            f[place(e + 2)] = fmaf((f[place(e + 2)] - mean) * by, z.z, b.z), f[place(e + 3)] = fmaf((f[place(e + 3)] - mean) * by, z.w, b.w);
         }
+        if (turned) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x0 = f[j], x1 = f[j + 8];
+                f[j] = x0 * c[j] - x1 * s[j];
+                f[j + 8] = x1 * c[j] + x0 * s[j];
+            }
+        }
+        float lo8[8], hi8[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lo8[j] = f[place(j)], hi8[j] = f[place(j + 8)];
+        store8<true>(y + d0, lo8);
+        store8<true>(y + d1, hi8);
     }
 }
 
 // Any head dim, pair count, stride and alignment: a warp a row and share of its heads, one head at a time through
 // shared memory, the angles of its row in registers.
-template <typename TX, typename TY, bool LAYER>
+template <typename TX, typename TY>
 __global__ void __launch_bounds__(128) rope_norm_any_kernel(const __grid_constant__ RopeNormArgs a) {
     __shared__ float head[4][2 * kMaxPairs];
     wait_for_stream();
@@ -200,11 +248,11 @@ __global__ void __launch_bounds__(128) rope_norm_any_kernel(const __grid_constan
             float by = 1.f, sum;
             for (int turn = 0;; ++turn) {
                 float u[8], mean = 0.f;
-                if (LAYER) {
+                if (a.layer) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k) mean += f[k] * by;
                     for (int o = 16; o; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
-                    mean /= static_cast<float>(D);
+                    mean *= a.inv_dim;
                 }
                 sum = 0.f;
 #pragma unroll
@@ -220,7 +268,7 @@ __global__ void __launch_bounds__(128) rope_norm_any_kernel(const __grid_constan
                 }
                 by = kShrink;
             }
-            const float r = __frsqrt_rn(sum / static_cast<float>(D) + a.eps * by * by);
+            const float r = rsqrt_approx(fmaf(sum, a.inv_dim, a.eps * by * by));
             __syncwarp();  // the head before is read
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -243,8 +291,8 @@ __global__ void __launch_bounds__(128) rope_norm_any_kernel(const __grid_constan
     }
 }
 
-template <typename TX, typename TY, bool LAYER>
-cudaError_t launch_rope_norm(RopeNormArgs &a, bool wide, cudaStream_t st, int num_sms) {
+template <typename TX, typename TY>
+cudaError_t launch_rope_norm(RopeNormArgs &a, bool wide, bool plain, cudaStream_t st, int num_sms) {
     const int n_heads = a.set[a.n_sets - 1].end;
     auto split_heads = [&](int64_t blocks, int64_t want, int step) {  // heads are split over blocks where the rows give fewer than wanted
         const int64_t split = (want + blocks - 1) / blocks;
@@ -255,13 +303,13 @@ cudaError_t launch_rope_norm(RopeNormArgs &a, bool wide, cudaStream_t st, int nu
         int lanes = 1;
         while (lanes * 16 < a.t.head_dim) lanes *= 2;
         const int rows = std::max(16 / lanes, 1);  // 128 pairs at most
-        const int64_t blocks = (static_cast<int64_t>(a.n_rows) + rows - 1) / rows;
-        const dim3 grid = split_heads(blocks, num_sms * int64_t(8), kHeadLanes);
-        return launch_after(a.t.neighbours ? rope_norm_kernel<TX, TY, true, LAYER> : rope_norm_kernel<TX, TY, false, LAYER>, grid,
-                            rows * lanes * kHeadLanes, a.n_sets * 2 * a.t.head_dim * sizeof(float), st, a, rows, lanes);
+        const dim3 grid = split_heads((static_cast<int64_t>(a.n_rows) + rows - 1) / rows, num_sms * int64_t(8), kHeadLanes);
+        auto *const kernel = plain ? (a.t.neighbours ? rope_norm_kernel<TX, TY, true, true> : rope_norm_kernel<TX, TY, false, true>)
+                                   : (a.t.neighbours ? rope_norm_kernel<TX, TY, true, false> : rope_norm_kernel<TX, TY, false, false>);
+        return launch_after(kernel, grid, rows * lanes * kHeadLanes, a.n_sets * 2 * 16 * lanes * sizeof(float), st, a, rows, lanes);
     }
     const dim3 grid = split_heads((static_cast<int64_t>(a.n_rows) + 3) / 4, num_sms * int64_t(16), 1);
-    return launch_after(rope_norm_any_kernel<TX, TY, LAYER>, grid, 128, 0, st, a);
+    return launch_after(rope_norm_any_kernel<TX, TY>, grid, 128, 0, st, a);
 }
 
 }  // namespace
@@ -281,8 +329,8 @@ extern "C" int sam3b200_rope_norm_run(sam3b200_rope *h, const sam3b200_norm_head
         set_error("rope_norm: unsupported types %d -> %d, weights %d (F32=0, F16=1, BF16=30) or unaligned positions", x_type, y_type, w_type);
         return SAM3B200_STATUS_FAILED;
     }
-    if (n_sets < 1 || n_sets > kMaxSets || !(eps > 0.f) || !std::isfinite(eps)) {
-        set_error("rope_norm: %d sets of heads (1 to %d), eps %g (above 0)", n_sets, kMaxSets, eps);
+    if (n_sets < 1 || n_sets > kMaxSets || !(eps >= kEpsLeast) || !std::isfinite(eps)) {
+        set_error("rope_norm: %d sets of heads (1 to %d), eps %g (a normal number above 0)", n_sets, kMaxSets, eps);
         return SAM3B200_STATUS_FAILED;
     }
     if (n_rows < 0 || n_rows > (1 << 27) || pos_stride < 0 || (r->t.n_axes > 1 && pos_stride < n_rows)) {
@@ -294,6 +342,7 @@ extern "C" int sam3b200_rope_norm_run(sam3b200_rope *h, const sam3b200_norm_head
     const int D = a.t.head_dim;
     // 16-byte groups of 8 pairs: whole groups, aligned rows
     bool wide = a.t.pairs % 8 == 0 && D % 16 == 0;
+    bool plain = !layer;
     int64_t heads = 0;
     a.n_sets = 0;
     for (int i = 0; i < n_sets; ++i) {
@@ -324,18 +373,15 @@ extern "C" int sam3b200_rope_norm_run(sam3b200_rope *h, const sam3b200_norm_head
         }
         heads += s.n_heads;
         q.end = static_cast<int>(heads);
-        wide = wide && q.xs.aligned16 && q.ys.aligned16;
+        wide = wide && q.xs.aligned16 && q.ys.aligned16, plain = plain && !q.bias;
     }
     if (n_rows == 0 || heads == 0) return SAM3B200_STATUS_SUCCESS;
     a.pos = pos, a.pos_stride = pos_stride;
     a.n_rows = static_cast<int>(n_rows);
-    a.w_type = w_type, a.eps = eps;
+    a.w_type = w_type, a.layer = layer != 0, a.eps = eps, a.inv_dim = 1.f / D;
     DeviceScope dev(r->be->device);
     auto go = [&](auto tx, auto ty) {
-        using TX = decltype(tx);
-        using TY = decltype(ty);
-        return layer ? launch_rope_norm<TX, TY, true>(a, wide, r->be->stream, r->be->num_sms)
-                     : launch_rope_norm<TX, TY, false>(a, wide, r->be->stream, r->be->num_sms);
+        return launch_rope_norm<decltype(tx), decltype(ty)>(a, wide, plain, r->be->stream, r->be->num_sms);
     };
     auto from = [&](auto tx) {
         return y_type == SAM3B200_TYPE_F32 ? go(tx, float()) : y_type == SAM3B200_TYPE_F16 ? go(tx, __half()) : go(tx, __nv_bfloat16());
