@@ -419,7 +419,8 @@ typedef struct sam3b200_kv4_cache {
 
 /* Rows into the cache, as sam3b200_kv_write.  d = top / -8 rounded to bf16, top
  * the group's finite element of largest magnitude (the positive one of two);
- * below 2^-100 top counts as 0.  Codes are the exact quotient x / d rounded to
+ * below 2^-100 top counts as 0, and d is at most (2 - 2^-7) * 2^124, so that all
+ * values are finite.  Codes are the exact quotient x / d rounded to
  * nearest even, cut to -8 .. 7, plus 8 (8 where d is 0).  NaN is stored as 0,
  * infinities as the ends of the range.  Two rows of one call may not lie in
  * the same place of a page. */

@@ -57,7 +57,8 @@ def kv4_quantise(x):
     finite = np.where(np.isfinite(y), y, 0.0)
     high, low = finite.max(-1), finite.min(-1)
     top = np.where(high >= -low, high, low)
-    bits = bf16_bits(np.where(np.abs(top) < SMALL, 0.0, top / -8 + 0.0).astype(np.float32))
+    most = (2 - 2.0 ** -7) * 2.0 ** 124
+    bits = bf16_bits(np.where(np.abs(top) < SMALL, 0.0, np.clip(top / -8, -most, most)).astype(np.float32))
     bits = np.where(np.abs(top) < SMALL, np.uint16(0), bits)
     d = bf16_value(bits)[..., None]
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):

@@ -225,6 +225,25 @@ def test_kv4_write_and_read(b200, backend, t, P, D, H):
         assert np.all(got_k[-8:] == 77) and np.all(got_v[-8:] == 77)
 
 
+@pytest.mark.parametrize("D,H,t", [(64, 3, "bf16"), (128, 1, "f16"), (64, 1, "f32"), (128, 20, "bf16")])
+@pytest.mark.parametrize("rows", [1, 2, 17])
+def test_kv4_many_sequences(b200, backend, D, H, t, rows):
+    """Hundreds of sequences with a few rows each: blocks of all slabs, heads that do not fill a block's turns."""
+    rng = np.random.default_rng(rows)
+    S, P = 700 // rows + 500, 16
+    lens = rng.integers(rows, rows + 40, S)
+    table, n = pages_for(lens, P)
+    dev = Device(b200, backend, do.kv4_empty(n, H, P, D), table)
+    start = np.arange(S + 1) * rows
+    dev.write(rng.normal(size=(S * rows, H, D)), rng.normal(size=(S * rows, H, D)) * 5, t, start, lens)
+    dev.same()
+    want = do.kv4_read(dev.host, table, start, lens)
+    out = [backend.alloc(S * rows * H * D * 4) for _ in range(2)]
+    backend.kv4_read(dev.cache, dev.batch(start, lens), TYPES["f32"], out[0].ptr, out[1].ptr)
+    backend.synchronize()
+    assert all(np.array_equal(o.get(w.shape, np.float32), w.astype(np.float32)) for o, w in zip(out, want))
+
+
 def test_kv4_write_rounds_the_exact_quotient(b200, backend):
     """Values on and next to the borders between two codes, largest magnitudes of both signs at once, NaN, infinities,
     zeros, subnormal and huge magnitudes."""
@@ -243,9 +262,32 @@ def test_kv4_write_rounds_the_exact_quotient(b200, backend):
         v = (rng.normal(size=(P, H, D)) * np.float64(amax) / 4).clip(-top, top).astype(np.float32)
         v[3, 0, 5], v[4, 0, 6], v[5, 0, 7] = np.nan, np.inf, -np.inf
         v[6, 0, :32], v[7, 0, 32:64], v[8, 0] = np.nan, np.inf, 0.0
-        dev = Device(b200, backend, do.kv4_empty(3, H, P, D), [[1]])
-        dev.write(k, v, "f32", [0, P], [P])
+        for t in ("f32", "bf16") if amax > 65504 or amax < 1e-4 else ("f32", "bf16", "f16"):
+            dev = Device(b200, backend, do.kv4_empty(3, H, P, D), [[1]])
+            dev.write(k, v, t, [0, P], [P])
+            dev.same()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_kv4_write_of_every_16_bit_number(b200, backend, t):
+    """Each number of the type next to largest ones of many sizes: every quotient that the type can make, ties among them."""
+    P, D, H = 128, 128, 4
+    every = np.arange(1 << 16, dtype=np.uint16).view(np.float16) if t == "f16" else np.arange(1 << 16, dtype=np.uint16)
+    x = value(every, t)
+    x = np.sort(np.where(np.isfinite(x), x, 0.0))
+    rng = np.random.default_rng(7)
+    for shift in range(3):  # a group's 32 numbers: of one size, from -7 steps to the largest
+        base = np.abs(rng.choice(x[np.abs(x) > 2.0 ** -10], (P * H * D // 32 * 4, 1))).clip(2.0 ** -9, 2.0 ** 14)
+        group = base * (np.arange(-16, 16) / 16 + (shift / 64 if shift else 0)) + base * rng.choice([0, 2.0 ** -9, -2.0 ** -9], (len(base), 32))
+        group[np.arange(len(group)), rng.integers(0, 32, len(group))] = base[:, 0] * rng.choice([-1, 1], len(group))
+        k, v = group[:2 * P * H * D // 32].reshape(2 * P, H, D), group[2 * P * H * D // 32:].reshape(2 * P, H, D)
+        dev = Device(b200, backend, do.kv4_empty(3, H, P, D), [[2, 0]])
+        dev.write(k, v, t, [0, 2 * P], [2 * P])
         dev.same()
+    pages = len(x) // (P * D)  # and all of them in order
+    dev = Device(b200, backend, do.kv4_empty(pages, 1, P, D), [list(range(pages))])
+    dev.write(x.reshape(-1, 1, D), x[::-1].reshape(-1, 1, D), t, [0, pages * P], [pages * P])
+    dev.same()
 
 
 def test_kv4_views_and_broadcast_rows(b200, backend):
