@@ -42,8 +42,8 @@ struct VecArgs {
     const float *bias;
     void *y;
     int M, N, K, cols;           // cols: columns of x, M or 2 M
-    int tiles, chunks, w_log2;   // warps of a tile
-    int phase;                   // chunks of x in shared memory at once, a multiple of the warps of a tile, or all
+    int tiles, chunks;
+    int phase, w_log2;           // chunks of x in shared memory at once: all, or a multiple of the 1 << w_log2 warps of a tile
     int y_type, aligned;         // aligned: four elements of x at once
 };
 
@@ -96,43 +96,50 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
     __shared__ unsigned s_top[kMaxRows];
     __shared__ uint4 zeros[4];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int W = 1 << a.w_log2, group = warp >> a.w_log2, w_in = warp & (W - 1), groups = kWarps >> a.w_log2;
-    const int rounds = (a.tiles + gridDim.x * groups - 1) / (gridDim.x * groups), blocks = a.K / 32;
-    float4 *red = reinterpret_cast<float4 *>(smem);                          // [2][kWarps][RT][NT][32]
+    const int blocks = a.K / 32;
+    float4 *red = reinterpret_cast<float4 *>(smem);                          // [kWarps][2][RT][NT][32]
     const uint8_t *ring = smem + V::kRed + warp * (kStages * kStageBytes);
     uint4 *xs = reinterpret_cast<uint4 *>(smem + V::kX);                     // [block][column][4]
     float *sums = reinterpret_cast<float *>(xs + a.phase * 4 * a.cols * 4);  // MINS: [block][8 NT]
-    auto tile_of = [&](int round) { return (round * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x)) * groups + group; };
 
-    // The copies of a warp's chunks in their order: a lane's rows of codes and its part of the scales; zeros behind the
+    // The steps of a warp, each one chunk of one tile.  Where all of x fits, the block has consecutive tiles [t0, t1), whose
+    // chunks in a row are cut into 16 equal parts, so that a warp begins and ends within a tile but needs no other warp before
+    // the end.  Else W warps share a tile, chunk by chunk, and the block takes 16 / W tiles after the other through all of x.
+    const bool whole = a.phase >= a.chunks;
+    const int W = 1 << a.w_log2, w_in = warp & (W - 1), batch = kWarps >> a.w_log2;
+    const int t0 = static_cast<int>(static_cast<int64_t>(blockIdx.x) * a.tiles / gridDim.x);
+    const int t1 = static_cast<int>((static_cast<int64_t>(blockIdx.x) + 1) * a.tiles / gridDim.x);
+    const int total = (t1 - t0) * a.chunks;
+    auto part = [&](int w) { return static_cast<int>(static_cast<int64_t>(w) * total / kWarps); };
+    const int first_step = part(warp), n_steps = part(warp + 1) - first_step;
+    const int first_tile = whole ? t0 + first_step / a.chunks : t0 + (warp >> a.w_log2), first_chunk = whole ? first_step % a.chunks : w_in;
+
+    // The copies of those steps in their order: a lane's rows of codes and its part of the scales; zeros behind the
     // weights' rows and blocks.
     const int put_row = lane >> 2, put_part = lane & 3;
     const uint32_t ring_at = smem_u32(ring);
     const uint32_t put0 = put_row * 64 + ((put_part ^ ((put_row >> 1) & 3)) * 16);  // row + 8: 512 further
     const int64_t eight = static_cast<int64_t>(a.K / 2) * 8;                        // rows, in bytes
-    int next_round = 0, next_c = 0, next_n = 0;
+    const int stride = whole ? 1 : W, tile_stride = whole ? 1 : batch;
+    int left = whole ? n_steps : first_tile < t1 ? ((t1 - first_tile - 1) / batch + 1) * ((a.chunks - w_in + W - 1) >> a.w_log2) : 0;
+    int next_tile = first_tile, next_c = first_chunk;
     const uint8_t *from = nullptr, *from_scales = nullptr;
-    bool more = false;
-    auto to_tile = [&] {
-        const int tile = tile_of(next_round);
-        more = next_round < rounds && tile < a.tiles;
-        if (!more) return;
-        next_n = tile * 16 * RT;
-        next_c = w_in;
-        from = a.codes + static_cast<int64_t>(next_n + put_row) * (a.K / 2) + (w_in * 4 + put_part) * 16;
-        from_scales = a.scales + (static_cast<int64_t>(tile) * RT * a.chunks + w_in) * V::kRecord + lane * 16;
+    auto seek = [&] {
+        from = a.codes + static_cast<int64_t>(next_tile * 16 * RT + put_row) * (a.K / 2) + (next_c * 4 + put_part) * 16;
+        from_scales = a.scales + (static_cast<int64_t>(next_tile) * RT * a.chunks + next_c) * V::kRecord + lane * 16;
     };
-    to_tile();
+    seek();
     auto issue = [&](int slot) {
-        if (more) {
+        if (left > 0) {
             const uint32_t dst = ring_at + slot * kStageBytes;
-            if (next_n + 16 * RT <= a.N && next_c * 4 + 4 <= blocks) {
+            const int n = next_tile * 16 * RT;
+            if (n + 16 * RT <= a.N && next_c * 4 + 4 <= blocks) {
 #pragma unroll
                 for (int k = 0; k < 2 * RT; ++k) cp16(dst + put0 + k * 512, from + k * eight);
             } else {
 #pragma unroll
                 for (int k = 0; k < 2 * RT; ++k) {
-                    const bool there = next_n + put_row + 8 * k < a.N && next_c * 4 + put_part < blocks;
+                    const bool there = n + put_row + 8 * k < a.N && next_c * 4 + put_part < blocks;
                     cp16_or_zero(dst + put0 + k * 512, there ? from + k * eight : a.codes, there);
                 }
             }
@@ -140,15 +147,17 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
             for (int r = 0; r < RT; ++r) {
                 const uint32_t to = dst + RT * V::kCodeBytes + r * V::kRecord + lane * 16;
                 if (lane < V::kRecord / 16) {
-                    if (r == 0 || next_n + 16 * r < a.N) cp16(to, from_scales + static_cast<int64_t>(r) * a.chunks * V::kRecord);
+                    if (r == 0 || n + 16 * r < a.N) cp16(to, from_scales + static_cast<int64_t>(r) * a.chunks * V::kRecord);
                     else cp16_or_zero(to, a.scales, false);
                 }
             }
-            from += W * 64, from_scales += W * V::kRecord;
-            next_c += W;
+            --left;
+            from += stride * 64, from_scales += stride * V::kRecord;
+            next_c += stride;
             if (next_c >= a.chunks) {
-                ++next_round;
-                to_tile();
+                next_tile += tile_stride;
+                next_c = whole ? 0 : w_in;
+                seek();
             }
         }
         cp_commit();
@@ -258,121 +267,107 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
         x_step[n] = there ? a.cols * 64 : 0;
     }
     int slot = 0, slot_in = kStages - 1;
+    float acc[RT][NT][4];
+    // Chunks first, first + by, ... below end (counted from the first one in shared memory) of a tile.
+    auto run = [&](int first, int end, int by) {
+        uint32_t x_now[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) x_now[n] = x_at[n] + first * 4 * x_step[n];
 #pragma unroll 1
-    for (int round = 0; round < rounds; ++round) {
-        const int tile = tile_of(round);
-        float acc[RT][NT][4];
+        for (int ch = first; ch < end; ch += by) {
+            cp_wait<kStages - 2>();
+            __syncwarp();  // the chunk is there for all lanes, and the one before is read by all
+            issue(slot_in);
+            const uint8_t *st = ring + slot * kStageBytes;
+            const uint32_t st_at = ring_at + slot * kStageBytes;
+            slot_in = slot;
+            slot = slot + 1 == kStages ? 0 : slot + 1;
+            __half2 d[RT][2][2], mn[RT][2][2];  // rows g and g + 8, blocks 0, 1 and 2, 3
+            uint32_t w[RT][2][4];               // rows g and g + 8, word c of each block
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint8_t *at = st + RT * V::kCodeBytes + r * V::kRecord + (g + 8 * h) * 8;
+                    *reinterpret_cast<uint2 *>(d[r][h]) = *reinterpret_cast<const uint2 *>(at);
+                    if (MINS) *reinterpret_cast<uint2 *>(mn[r][h]) = *reinterpret_cast<const uint2 *>(at + V::kScaleBytes);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t z[4];
+                    ldmatrix4<false>(z, st_at + r * V::kCodeBytes + (get0 ^ (32 * k)));
+                    w[r][0][2 * k] = z[0], w[r][1][2 * k] = z[1], w[r][0][2 * k + 1] = z[2], w[r][1][2 * k + 1] = z[3];
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                uint4 y[NT];
+                float2 x[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    y[n] = lds128(x_now[n]);
+                    x_now[n] += x_step[n];
+                    if (MINS) x[n] = *reinterpret_cast<const float2 *>(sums + (ch * 4 + b) * 8 * NT + n * 8 + 2 * c);
+                }
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    uint32_t u[4], v[4];
+                    codes4<MINS ? 0 : 8>(w[r][0][b], u);
+                    codes4<MINS ? 0 : 8>(w[r][1][b], v);
+                    float ds[2], ms[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        ds[h] = b & 1 ? __high2float(d[r][h][b >> 1]) : __low2float(d[r][h][b >> 1]);
+                        if (MINS) ms[h] = b & 1 ? __high2float(mn[r][h][b >> 1]) : __low2float(mn[r][h][b >> 1]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float s[4];
+                        mma16816_first(s, u[0], v[0], u[1], v[1], y[n].x, y[n].y);
+                        mma16816(s, u[2], v[2], u[3], v[3], y[n].z, y[n].w);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            acc[r][n][i] = fmaf(s[i], ds[i >> 1], acc[r][n][i]);
+                            if (MINS) acc[r][n][i] = fmaf(i & 1 ? x[n].y : x[n].x, ms[i >> 1], acc[r][n][i]);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x_now[n] += (by - 1) * 4 * x_step[n];
+        }
+    };
+    auto clear = [&] {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.f;
-#pragma unroll 1
-        for (int p0 = 0; p0 < a.chunks; p0 += a.phase) {
-            if (round == 0 || a.phase < a.chunks) {
-                if (round || p0) __syncthreads();  // the phase before is read
-                stage_x(p0);
-                __syncthreads();
+    };
+    auto place = [&](int w, int k) { return red + (w * 2 + k) * RT * NT * 32 + lane; };  // warp w's sums, k: of its first tile or its last
+    auto put = [&](float4 *to) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) to[(r * NT + n) * 32] = make_float4(acc[r][n][0], acc[r][n][1], acc[r][n][2], acc[r][n][3]);
+    };
+    auto add = [&](const float4 *x) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float4 v = x[(r * NT + n) * 32];
+                acc[r][n][0] += v.x, acc[r][n][1] += v.y, acc[r][n][2] += v.z, acc[r][n][3] += v.w;
             }
-            if (tile >= a.tiles) continue;
-            const int end = min(p0 + a.phase, a.chunks);
-            uint32_t x_now[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) x_now[n] = x_at[n] + w_in * 4 * x_step[n];
-#pragma unroll 1
-            for (int ch = p0 + w_in; ch < end; ch += W) {
-                cp_wait<kStages - 2>();
-                __syncwarp();  // the chunk is there for all lanes, and the one before is read by all
-                issue(slot_in);
-                const uint8_t *st = ring + slot * kStageBytes;
-                const uint32_t st_at = ring_at + slot * kStageBytes;
-                slot_in = slot;
-                slot = slot + 1 == kStages ? 0 : slot + 1;
-                __half2 d[RT][2][2], mn[RT][2][2];  // rows g and g + 8, blocks 0, 1 and 2, 3
-                uint32_t w[RT][2][4];               // rows g and g + 8, word c of each block
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint8_t *at = st + RT * V::kCodeBytes + r * V::kRecord + (g + 8 * h) * 8;
-                        *reinterpret_cast<uint2 *>(d[r][h]) = *reinterpret_cast<const uint2 *>(at);
-                        if (MINS) *reinterpret_cast<uint2 *>(mn[r][h]) = *reinterpret_cast<const uint2 *>(at + V::kScaleBytes);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        uint32_t z[4];
-                        ldmatrix4<false>(z, st_at + r * V::kCodeBytes + (get0 ^ (32 * k)));
-                        w[r][0][2 * k] = z[0], w[r][1][2 * k] = z[1], w[r][0][2 * k + 1] = z[2], w[r][1][2 * k + 1] = z[3];
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    uint4 y[NT];
-                    float2 x[NT];
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        y[n] = lds128(x_now[n]);
-                        x_now[n] += x_step[n];
-                        if (MINS) x[n] = *reinterpret_cast<const float2 *>(sums + ((ch - p0) * 4 + b) * 8 * NT + n * 8 + 2 * c);
-                    }
-#pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        uint32_t u[4], v[4];
-                        codes4<MINS ? 0 : 8>(w[r][0][b], u);
-                        codes4<MINS ? 0 : 8>(w[r][1][b], v);
-                        float ds[2], ms[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            ds[h] = b & 1 ? __high2float(d[r][h][b >> 1]) : __low2float(d[r][h][b >> 1]);
-                            if (MINS) ms[h] = b & 1 ? __high2float(mn[r][h][b >> 1]) : __low2float(mn[r][h][b >> 1]);
-                        }
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float s[4];
-                            mma16816_first(s, u[0], v[0], u[1], v[1], y[n].x, y[n].y);
-                            mma16816(s, u[2], v[2], u[3], v[3], y[n].z, y[n].w);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                acc[r][n][i] = fmaf(s[i], ds[i >> 1], acc[r][n][i]);
-                                if (MINS) acc[r][n][i] = fmaf(i & 1 ? x[n].y : x[n].x, ms[i >> 1], acc[r][n][i]);
-                            }
-                        }
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) x_now[n] += (W - 1) * 4 * x_step[n];
-            }
-        }
-        if (tile >= a.tiles) continue;
-        if (W > 1) {
-            // Two buffers in turn: a round's is written again behind the barrier of the round between.
-            float4 *to = red + ((round & 1) * kWarps + group * W) * RT * NT * 32;
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    to[((w_in * RT + r) * NT + n) * 32 + lane] = make_float4(acc[r][n][0], acc[r][n][1], acc[r][n][2], acc[r][n][3]);
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(W * 32) : "memory");
-            if (w_in != (round & (W - 1))) continue;  // the warps take turns to finish a tile
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float4 s = to[(r * NT + n) * 32 + lane];
-                    for (int k = 1; k < W; ++k) {
-                        const float4 x = to[((k * RT + r) * NT + n) * 32 + lane];
-                        s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
-                    }
-                    acc[r][n][0] = s.x, acc[r][n][1] = s.y, acc[r][n][2] = s.z, acc[r][n][3] = s.w;
-                }
-        }
-        auto store = [&](int m, int n, float v) {
-            if (m >= a.M || n >= a.N) return;
-            if (kScaled) v *= s_up[m];
-            if (a.bias) v += a.bias[n];
-            const int64_t at = m * a.ldy + n;
-            if (a.y_type == SAM3B200_TYPE_F32) static_cast<float *>(a.y)[at] = v;
-            else static_cast<TX *>(a.y)[at] = from_f32<TX>(v);
-        };
+    };
+    auto store = [&](int m, int n, float v) {
+        if (m >= a.M || n >= a.N) return;
+        if (kScaled) v *= s_up[m];
+        if (a.bias) v += a.bias[n];
+        const int64_t at = m * a.ldy + n;
+        if (a.y_type == SAM3B200_TYPE_F32) static_cast<float *>(a.y)[at] = v;
+        else static_cast<TX *>(a.y)[at] = from_f32<TX>(v);
+    };
+    auto finish = [&](int tile) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -387,6 +382,48 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
                         store(n * 8 + 2 * c + 1, out, acc[r][n][2 * h + 1]);
                     }
                 }
+    };
+
+    if (whole) {
+        stage_x(0);
+        __syncthreads();
+        int tile = first_tile, ch = first_chunk;
+        for (int steps = n_steps; steps > 0; ++tile, ch = 0) {
+            const int end = min(ch + steps, a.chunks);
+            clear();
+            run(ch, end, 1);
+            steps -= end - ch;
+            if (end - ch == a.chunks) finish(tile);
+            else put(place(warp, tile != first_tile));
+        }
+        __syncthreads();
+        for (tile = t0 + warp; tile < t1; tile += kWarps) {  // tiles that several warps have parts of
+            const int64_t begin = static_cast<int64_t>(tile - t0) * a.chunks;
+            const int w0 = static_cast<int>(((begin + 1) * kWarps - 1) / total), w1 = static_cast<int>(((begin + a.chunks) * kWarps - 1) / total);
+            if (w0 == w1) continue;
+            clear();
+            for (int w = w0; w <= w1; ++w)
+                if (part(w + 1) > part(w)) add(place(w, tile != t0 + part(w) / a.chunks));
+            finish(tile);
+        }
+    } else {
+        for (int tile0 = t0; tile0 < t1; tile0 += batch) {
+            const int tile = tile0 + (warp >> a.w_log2);
+            clear();
+            for (int p0 = 0; p0 < a.chunks; p0 += a.phase) {
+                if (tile0 != t0 || p0) __syncthreads();  // the phase before is read
+                stage_x(p0);
+                __syncthreads();
+                if (tile < t1) run(w_in, min(a.phase, a.chunks - p0), W);
+            }
+            if (W > 1) {
+                if (w_in && tile < t1) put(place(warp, 0));
+                __syncthreads();
+                if (w_in == 0 && tile < t1)
+                    for (int w = warp + 1; w < warp + W; ++w) add(place(w, 0));
+            }
+            if (w_in == 0 && tile < t1) finish(tile);
+        }
     }
     cp_wait<0>();
 }
@@ -423,27 +460,35 @@ cudaError_t launch(Backend *be, VecArgs &a) {
         if (e != cudaSuccess) return e;
         be->vec_ready |= kBit;
     }
-    // warps a tile: the number that gives the fewest steps of a warp, a tile's end counted as one, and x that comes again
-    // for every tile by its instructions
-    int64_t least = 0x7fffffffffffffff;
-    for (int lg = 0; lg <= 4 && (1 << lg) <= std::min(a.chunks, most); ++lg) {
-        const int64_t tiles_round = static_cast<int64_t>(be->num_sms) * (kWarps >> lg);
-        const int64_t steps = (a.chunks + (1 << lg) - 1) / (1 << lg) + 1 + (phases ? a.chunks * a.cols / 64 : 0);
-        const int64_t cost = (a.tiles + tiles_round - 1) / tiles_round * steps;
-        if (cost <= least) least = cost, a.w_log2 = lg;
+    a.w_log2 = 0, a.phase = a.chunks;
+    if (phases) {
+        // warps a tile: the number that gives the fewest steps of a warp, with x that comes again for every batch of tiles by
+        // its instructions
+        int64_t least = 0x7fffffffffffffff;
+        const int64_t own = (a.tiles + be->num_sms - 1) / be->num_sms;  // tiles of a block
+        for (int lg = 0; lg <= 4 && (1 << lg) <= most; ++lg) {
+            const int64_t batches = (own * (1 << lg) + kWarps - 1) / kWarps;
+            const int64_t cost = batches * ((a.chunks + (1 << lg) - 1) / (1 << lg) + 1 + a.chunks * static_cast<int64_t>(a.cols) / 64);
+            if (cost <= least) least = cost, a.w_log2 = lg;
+        }
+        a.phase = most >> a.w_log2 << a.w_log2;
     }
-    a.phase = phases ? most >> a.w_log2 << a.w_log2 : a.chunks;
     const int smem = V::kX + a.phase * per_chunk;
-    const int groups = kWarps >> a.w_log2;
-    const int64_t grid = std::min<int64_t>(be->num_sms, (a.tiles + groups - 1) / groups);
+    const int grid = std::min(be->num_sms, a.tiles);
     return launch_after(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, be->stream, a);
 }
 
-// Tiles of 32 rows where there are enough of them: x is read from shared memory once for both halves.
+// Tiles of 16 or of 32 rows, where x is read from shared memory once for both halves: by the steps of a warp, one of 32
+// counted as 1.8 of 16 (us, PLACEHOLDER).
 template <int NT, bool MINS, typename TX>
 cudaError_t launch(Backend *be, VecArgs &a) {
-    if constexpr (NT < 4)
-        if (a.N >= be->num_sms * 32) return launch<NT, 2, MINS, TX>(be, a);
+    if constexpr (NT < 4) {
+        auto steps = [&](int64_t rows) {
+            const int64_t tiles = ((a.N + rows - 1) / rows + be->num_sms - 1) / be->num_sms;  // of a block
+            return (tiles * a.chunks + kWarps - 1) / kWarps;
+        };
+        if (18 * steps(32) <= 10 * steps(16)) return launch<NT, 2, MINS, TX>(be, a);
+    }
     return launch<NT, 1, MINS, TX>(be, a);
 }
 
