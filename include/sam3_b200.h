@@ -191,7 +191,7 @@ int sam3b200_mul_mat_dq16(sam3b200_backend *be, const sam3b200_weight *w, const 
  * elements; bias: device f32 [N] or NULL; dst: device rows of y_type (F32, or
  * x_type), row stride ldd.  Products are exact in codes and activations (F16
  * as they are; BF16, and F32 as a sum of two, in f16 after a power of two a row:
- * 2^-23 of an F32 element, and 2^-39 of the row's largest one where that is at
+ * 2^-23 of an F32 element, and 2^-26 of the row's largest one where that is at
  * least 2^-112, may be lost), a block's sum is scaled and added in f32, in an
  * order that the shapes fix, and rounded once to y_type.  The
  * weights are the handle's own codes, with their scales a second time in 2

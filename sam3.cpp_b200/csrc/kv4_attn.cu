@@ -21,10 +21,7 @@
 // dimensions), and transposed for values, 4 dimensions of tokens 2c and 2c + 1
 // side by side, so a nibble and the one 16 bits above it are the pair that the
 // instruction wants, in either product, and widening is a mask and a
-// subtraction for a pair.  Half of the subtractions (of 72, where a code comes
-// as 64 + code) are left to the products: for keys as what a group's sum starts
-// from, -72 times the sum of its queries, for values as one more product of the
-// weights with -72 a group.
+// subtraction for a pair.
 #include <algorithm>
 #include <cmath>
 
@@ -86,8 +83,6 @@ __device__ __forceinline__ void load_half(uint32_t (&w)[2][D / 32], uint32_t fro
     }
 }
 
-constexpr uint32_t kMinus72 = 0xd480d480u;  // a pair of f16
-
 // Eight consecutive query elements, as they come, and the j-th of them.
 __device__ __forceinline__ uint4 load_q8(const Kv4AttnArgs &a, int64_t at) {
     const uint16_t *p = static_cast<const uint16_t *>(a.q) + at;
@@ -108,12 +103,11 @@ __device__ __forceinline__ float q_value(const Kv4AttnArgs &a, const uint4 &x, i
 template <int D, int NT>
 struct Few4 {
     static constexpr int kRows = 8 * NT, kGroups = D / 32;
-    static constexpr int kStages = D == 128 ? 3 : 4, kBlocks = NT == 1 ? 4 : 3;  // stages of a warp, blocks an SM
+    static constexpr int kStages = D == 128 ? 3 : 4, kBlocks = NT == 1 ? 4 : 2;  // stages of a warp, blocks an SM
     static constexpr int kCodeBytes = 16 * D / 2;                  // of 16 tokens
     static constexpr int kScaleBytes = 16 * kGroups * 2;
     // a stage: for each half its keys' and values' codes, then for each half their scales
     static constexpr int kHalfBytes = 2 * kCodeBytes, kScaleAt = 2 * kHalfBytes, kStageBytes = kScaleAt + 4 * kScaleBytes;
-    static constexpr bool kFoldKeys = false;
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kRowFloats = D + 4;                       // a joined row, padded against bank conflicts
     static constexpr int kJoin = kWarps * kRows * kRowFloats * 4;
@@ -204,7 +198,6 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 
     // queries as f16: for a group's two products the pairs of dimensions that codes4 gives
     uint32_t qf[NT][kGroups][4];
-    float from[NT][kGroups][2];
     float row_c[NT][2];  // for rows 8 n + 2 c, + 1: scale log2(e), and what the power of two below took
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -223,17 +216,6 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 qf[n][k][j] = pack_f16(q_value(a, qraw[n][k], j) * down, q_value(a, qraw[n][k], j + 4) * down);
-        if (F::kFoldKeys) {  // what a group's sums start from: -72 for each code that keeps its 64 + 8
-#pragma unroll
-            for (int k = 0; k < kGroups; ++k) {
-                const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(&qf[n][k][1])), v = __half22float2(*reinterpret_cast<const __half2 *>(&qf[n][k][3]));
-                float sum = (u.x + u.y) + (v.x + v.y);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) from[n][k][j] = -72.f * __shfl_sync(0xffffffffu, sum, (2 * c + j) * 4);
-            }
-        }
 #pragma unroll
         for (int j = 0; j < 2; ++j)  // a factor of 0 would make NaN of -inf; a tiny one leaves 0 of the scores
             row_c[n][j] = fmaxf(__shfl_sync(0xffffffffu, up, (2 * c + j) * 4), 1e-37f);
@@ -273,13 +255,12 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 #pragma unroll
             for (int k = 0; k < kGroups; ++k) {
                 uint32_t u[4], v[4];
-                codes4<8, F::kFoldKeys>(w[0][k], u);
-                codes4<8, F::kFoldKeys>(w[1][k], v);
+                codes4(w[0][k], u);
+                codes4(w[1][k], v);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float s[4];
-                    if (F::kFoldKeys) mma16816_from(s, u[0], v[0], u[1], v[1], qf[n][k][0], qf[n][k][1], from[n][k][0], from[n][k][1]);
-                    else mma16816_first(s, u[0], v[0], u[1], v[1], qf[n][k][0], qf[n][k][1]);
+                    mma16816_first(s, u[0], v[0], u[1], v[1], qf[n][k][0], qf[n][k][1]);
                     mma16816(s, u[2], v[2], u[3], v[3], qf[n][k][2], qf[n][k][3]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -364,17 +345,15 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 #pragma unroll
             for (int k = 0; k < kGroups; ++k) {
                 uint32_t u[4], v[4];
-                codes4<8, true>(w[0][k], u);
-                codes4<8, true>(w[1][k], v);
+                codes4(w[0][k], u);
+                codes4(w[1][k], v);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const uint32_t p0 = transposed(pack_f16(t[h][n][0] * dv[h][0][k], t[h][n][1] * dv[h][0][k]));
                     const uint32_t p1 = transposed(pack_f16(t[h][n][2] * dv[h][1][k], t[h][n][3] * dv[h][1][k]));
-                    // dimensions 4 g, 4 g + 2 of the group are rows g, g + 8 of one product, 4 g + 1, 4 g + 3 of the next,
-                    // whose codes keep their 64 + 8
-                    mma16816(o[n][2 * k], u[0], u[2], v[0], v[2], p0, p1);
-                    mma16816(o[n][2 * k + 1], u[1], u[3], v[1], v[3], p0, p1);
-                    mma16816(o[n][2 * k + 1], kMinus72, kMinus72, kMinus72, kMinus72, p0, p1);
+                    // dimensions 4 g, + 1 of the group are rows g, g + 8 of one product, + 2, + 3 of the next
+                    mma16816(o[n][2 * k], u[0], u[1], v[0], v[1], p0, p1);
+                    mma16816(o[n][2 * k + 1], u[2], u[3], v[2], v[3], p0, p1);
                 }
             }
         }
@@ -395,7 +374,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
             float *to = rows + (warp * F::kRows + row) * F::kRowFloats + 4 * g;
 #pragma unroll
             for (int i = 0; i < D / 16; i += 2)
-                *reinterpret_cast<float4 *>(to + 16 * i) = make_float4(o[n][i][k], o[n][i + 1][k], o[n][i][k + 2], o[n][i + 1][k + 2]);
+                *reinterpret_cast<float4 *>(to + 16 * i) = make_float4(o[n][i][k], o[n][i][k + 2], o[n][i + 1][k], o[n][i + 1][k + 2]);
         }
     __syncthreads();
     few_finish<F, D>(a, tile, smem, s_m, s_l);

@@ -16,10 +16,9 @@
 // lane by ldmatrix, a nibble and the one 16 bits above it are one operand
 // register after a mask and a subtraction, and x is staged in the same order.  A
 // block's sum is scaled in f32, 4 multiply-adds a lane for 16 x 8 results.
-// x as f16: F16 as it is; BF16 after a power of two a row that brings the
-// largest element to [2^14, 2^15), exact down to 2^-31 of it, and to 2^-39 of it
-// below; F32 the same way as a sum of two f16 numbers in two columns (2^-23 of an
-// element at most is lost).
+// x as f16: F16 as it is; BF16 after a power of two (see kUsual) that keeps all
+// but 2^-26 of a row's largest element; F32 the same way as a sum of two f16 numbers
+// in two columns (2^-23 of an element at most is lost, too).
 // Warps' sums of a tile are added in their order: results repeat bit for bit.
 #include <algorithm>
 #include <type_traits>
@@ -57,6 +56,16 @@ struct Vec {
     static constexpr int kRed = 2 * kWarps * NT * RT * 512;
     static constexpr int kX = kRed + kWarps * kStages * kStageBytes;  // where x begins
 };
+
+// Rows whose largest element lies in [2^-5, 2^9) are multiplied by 2^6, so that their largest has at least f16's 1: what f16
+// then loses is at most 2^-26 of it, and no look over the row has to come first (us, 6 rows of 4096 in bf16: PLACEHOLDER).
+constexpr float kUsual = 64.f, kUsualLeast = 0.03125f, kUsualMost = 512.f;
+
+// The bits of v's magnitude, 0 for an infinity or NaN.
+__device__ __forceinline__ unsigned finite_bits(float v) {
+    const unsigned bits = __float_as_uint(fabsf(v));
+    return bits < 0x7f800000u ? bits : 0u;
+}
 
 // f16 of v; `rest`: what it leaves (0 of an infinity or NaN).
 __device__ __forceinline__ float f16_of(float v, float &rest) {
@@ -167,45 +176,49 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
     for (int j = 0; j < kStages - 1; ++j) issue(j);
     wait_for_stream();
 
-    if (kScaled) {  // the power of two of each row, from its largest finite element
-        if (threadIdx.x < kMaxRows) s_top[threadIdx.x] = 0;
-        __syncthreads();
-        for (int m0 = 0; m0 < a.M; m0 += kFlight) {
-            const TX *x = static_cast<const TX *>(a.x) + m0 * a.ldx;
-            unsigned top[kFlight];
-#pragma unroll
-            for (int m = 0; m < kFlight; ++m) top[m] = 0;
-            for (int k = threadIdx.x * 4; k < a.K; k += kThreads * 4) {
-                Raw4<TX> raw[kFlight];
-#pragma unroll
-                for (int m = 0; m < kFlight; ++m) {
-                    raw[m].zero();
-                    if (m0 + m < a.M) raw[m].load(x + m * a.ldx + k, a.aligned);
-                }
-#pragma unroll
-                for (int m = 0; m < kFlight; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const unsigned bits = __float_as_uint(fabsf(to_f32(raw[m].v[i])));
-                        top[m] = max(top[m], bits < 0x7f800000u ? bits : 0u);
-                    }
-            }
-#pragma unroll
-            for (int m = 0; m < kFlight; ++m) {
-                top[m] = __reduce_max_sync(0xffffffffu, top[m]);
-                if (lane == m && m0 + m < a.M) atomicMax(&s_top[m0 + m], top[m]);
-            }
-        }
-        __syncthreads();
+    // The power of two of each row, from the bits of its largest finite element.
+    auto scale_rows = [&] {
         if (threadIdx.x < a.M) {
             const unsigned top = s_top[threadIdx.x];
             const int e = top ? min(268 - static_cast<int>(top >> 23), 253) : 127;
             s_down[threadIdx.x] = __int_as_float(e << 23), s_up[threadIdx.x] = __int_as_float((254 - e) << 23);
         }
         __syncthreads();
+    };
+    if (kScaled) {
+        if (threadIdx.x < kMaxRows) s_top[threadIdx.x] = 0, s_down[threadIdx.x] = kUsual, s_up[threadIdx.x] = 1.f / kUsual;
+        __syncthreads();
+        if (!whole) {  // x will come in phases, so its largest elements are looked for first
+            for (int m0 = 0; m0 < a.M; m0 += kFlight) {
+                const TX *x = static_cast<const TX *>(a.x) + m0 * a.ldx;
+                unsigned top[kFlight];
+#pragma unroll
+                for (int m = 0; m < kFlight; ++m) top[m] = 0;
+                for (int k = threadIdx.x * 4; k < a.K; k += kThreads * 4) {
+                    Raw4<TX> raw[kFlight];
+#pragma unroll
+                    for (int m = 0; m < kFlight; ++m) {
+                        raw[m].zero();
+                        if (m0 + m < a.M) raw[m].load(x + m * a.ldx + k, a.aligned);
+                    }
+#pragma unroll
+                    for (int m = 0; m < kFlight; ++m)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) top[m] = max(top[m], finite_bits(to_f32(raw[m].v[i])));
+                }
+#pragma unroll
+                for (int m = 0; m < kFlight; ++m) {
+                    top[m] = __reduce_max_sync(0xffffffffu, top[m]);
+                    if (lane == m && m0 + m < a.M) atomicMax(&s_top[m0 + m], top[m]);
+                }
+            }
+            __syncthreads();
+            scale_rows();
+        }
     }
     if (threadIdx.x < 4) zeros[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
-    auto stage_x = [&](int c0) {  // chunks c0 ... of x
+    // Chunks c0 ... of x; `look`: the rows' largest elements are noted.
+    auto stage_x = [&](int c0, bool look) {
         const int n_blocks = min(a.phase, a.chunks - c0) * 4, items = n_blocks * 4;
         for (int id0 = 0; id0 < items; id0 += kThreads) {  // all lanes: four neighbours share a block
             const int id = id0 + threadIdx.x, t = id & 3, b = id >> 2;
@@ -227,6 +240,13 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
                     if (m0 + m >= a.M) break;
                     const float by = kScaled ? s_down[m0 + m] : 1.f;
                     float v[8];
+                    if (kScaled && look) {
+                        unsigned top = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) top = max(top, finite_bits(to_f32(raw[m][i >> 2].v[i & 3])));
+                        top = __reduce_max_sync(0xffffffffu, top);
+                        if (lane == 0) atomicMax(&s_top[m0 + m], top);
+                    }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = to_f32(raw[m][i >> 2].v[i & 3]) * by;
 #pragma unroll
@@ -385,8 +405,17 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
     };
 
     if (whole) {
-        stage_x(0);
+        stage_x(0, true);
         __syncthreads();
+        if (kScaled) {  // rows of another size than usual get a power of two of their own
+            bool usual = true;
+            for (int m = 0; m < a.M; ++m) usual = usual && s_top[m] < __float_as_uint(kUsualMost) && (s_top[m] >= __float_as_uint(kUsualLeast) || s_top[m] == 0);
+            if (!usual) {
+                scale_rows();
+                stage_x(0, false);
+                __syncthreads();
+            }
+        }
         int tile = first_tile, ch = first_chunk;
         for (int steps = n_steps; steps > 0; ++tile, ch = 0) {
             const int end = min(ch + steps, a.chunks);
@@ -412,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
             clear();
             for (int p0 = 0; p0 < a.chunks; p0 += a.phase) {
                 if (tile0 != t0 || p0) __syncthreads();  // the phase before is read
-                stage_x(p0);
+                stage_x(p0, false);
                 __syncthreads();
                 if (tile < t1) run(w_in, min(a.phase, a.chunks - p0), W);
             }
