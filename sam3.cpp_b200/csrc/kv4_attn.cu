@@ -408,7 +408,10 @@ extern "C" int sam3b200_kv4_attention_run(sam3b200_kv_attention *h, const sam3b2
         return SAM3B200_STATUS_FAILED;
     if (empty) return SAM3B200_STATUS_SUCCESS;
     DeviceScope dev(k->be->device);
-    const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= 32;
+    // us in a graph, 8 kv heads, few rows and tc, for one sequence of 8000 tokens, one of 100000, 16 of 4000.  Heads of 128:
+    // 16 rows a kv head 25 and 34, 59 and 116, 50 and 62; 32 rows 31 and 34, 116 and 114, 77 and 62.  Heads of 64: 32 rows 21
+    // and 24, 72 and 91, 52 and 58; 48 rows 23 and 24, 89 and 91, 69 and 71; 64 rows 23 and 24, 106 and 91, 82 and 72
+    const bool few = static_cast<int64_t>(a.b.max_rows) * a.group <= (a.c.D == 128 ? 16 : 48);
     const cudaError_t e = few ? kv_attn_few(a, k->be->num_sms, k->be->stream) : kv_attn_tc(a, k->be->num_sms, k->be->stream);
     k->be->count();
     return cuda_ok(e, "kv4_attention launch") ? SAM3B200_STATUS_SUCCESS : SAM3B200_STATUS_FAILED;
