@@ -478,10 +478,13 @@ class Weight:
     memory or in device memory of the backend's GPU (ready when this is called)."""
 
     def __init__(self, be: "Backend", qtype: int, blocks: np.ndarray | int, K: int, N: int):
-        if not isinstance(blocks, int):
+        if isinstance(blocks, (int, np.integer)):
+            at = int(blocks)
+        else:
             blocks = np.ascontiguousarray(blocks)
+            at = blocks.ctypes.data
         self.be, self.qtype, self.K, self.N = be, qtype, K, N
-        self.h = lib().sam3b200_weight_upload(be.h, qtype, blocks if isinstance(blocks, int) else blocks.ctypes.data, K, N)
+        self.h = lib().sam3b200_weight_upload(be.h, qtype, at, K, N)
         if not self.h:
             raise B200Error(f"weight_upload failed: {last_error()}")
 

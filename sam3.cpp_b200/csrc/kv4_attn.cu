@@ -15,8 +15,8 @@
 // scales are; O and the sum of p have the same reference, so y = O / l.
 //
 // The kernel is kv_attn.cu's otherwise: one block of 4 warps per (8 or 16
-// query rows of a kv head, part of the key range), blocks of 32 tokens (two of 16, each in one page) through
-// a warp's own ring of shared memory, codes as the 16-row operand.  A lane's
+// query rows of a kv head, part of the key range), blocks of 32 tokens (heads of 64: 64; in
+// sixteens, each in one page) through a warp's own ring of shared memory, codes as the 16-row operand.  A lane's
 // codes come by ldmatrix: plain for keys, word c of each group of token g (8
 // dimensions), and transposed for values, 4 dimensions of tokens 2c and 2c + 1
 // side by side, so a nibble and the one 16 bits above it are the pair that the
@@ -104,10 +104,12 @@ template <int D, int NT>
 struct Few4 {
     static constexpr int kRows = 8 * NT, kGroups = D / 32;
     static constexpr int kStages = D == 128 ? 3 : 4, kBlocks = NT == 1 ? 4 : 2;  // stages of a warp, blocks an SM
+    static constexpr int kTurn = 128;                              // least tokens of a part (one token over 900: 64 8.4 us, 128 7.6)
     static constexpr int kCodeBytes = 16 * D / 2;                  // of 16 tokens
     static constexpr int kScaleBytes = 16 * kGroups * 2;
-    // a stage: for each half its keys' and values' codes, then for each half their scales
-    static constexpr int kHalfBytes = 2 * kCodeBytes, kScaleAt = 2 * kHalfBytes, kStageBytes = kScaleAt + 4 * kScaleBytes;
+    // a stage: for each 16 tokens their keys' and values' codes, then for each 16 their scales
+    static constexpr int kSixteens = 256 / D, kTokens = 16 * kSixteens;
+    static constexpr int kHalfBytes = 2 * kCodeBytes, kScaleAt = kSixteens * kHalfBytes, kStageBytes = kScaleAt + 2 * kSixteens * kScaleBytes;
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kRowFloats = D + 4;                       // a joined row, padded against bank conflicts
     static constexpr int kJoin = kWarps * kRows * kRowFloats * 4;
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
     if (!few_tile<NT>(a, tile)) return;
     const KvSeq &q = tile.q;
     const int row0 = tile.row0, i_lo = tile.i_lo, i_hi = tile.i_hi, R = tile.R, t_begin = tile.t_begin, t_end = tile.t_end;
-    const int n_blocks = t_end > t_begin ? (t_end - t_begin + 31) / 32 : 0;          // of 32 tokens, as two halves
+    const int n_blocks = t_end > t_begin ? (t_end - t_begin + F::kTokens - 1) / F::kTokens : 0;
     const int mine = n_blocks > warp ? (n_blocks - warp + kWarps - 1) / kWarps : 0;  // blocks warp, warp + 4, ...
 
     // the queries are on their way while the first pages are looked up: row 8 n + g, dimensions 8 c ... of each group
@@ -162,26 +164,28 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
     constexpr int kScaleChunks = F::kScaleBytes / 16;
     const uint8_t *own_scale = reinterpret_cast<const uint8_t *>(a.c.scale[lane >= kScaleChunks]) + lane % kScaleChunks * 16;
     const uint32_t ring_at = smem_u32(ring), put_at = ring_at + put0, put_scale_at = ring_at + F::kScaleAt + lane * 16;
-    // lane 2 j + h: where half h of block 16 b + j of this warp begins, for batches b and b + 1
+    // lane kSixteens j + h: where the h-th 16 tokens of block kBatch b + j of this warp lie, for batches b and b + 1
+    constexpr int kBatch = 32 / F::kSixteens;
     uint32_t at_now = 0, at_next = 0;
     auto look_up = [&](int j) -> uint32_t {
-        const int tok = t_begin + ((j >> 1) * kWarps + warp) * 32 + (j & 1) * 16;
-        if ((j >> 1) >= mine || tok >= t_end) return 0;
+        const int tok = t_begin + (j / F::kSixteens * kWarps + warp) * F::kTokens + j % F::kSixteens * 16;
+        if (j / F::kSixteens >= mine || tok >= t_end) return 0;
         const int page = max(kv_page(a.c, a.b, q.s, tok >> a.c.page_log2, a.err), 0);
         return ((static_cast<uint32_t>(page) * a.c.heads + kv) << a.c.page_log2) + (tok & ((1 << a.c.page_log2) - 1));
     };
     at_next = look_up(lane);
-    const int halves = mine ? 2 * mine - (t_begin + ((mine - 1) * kWarps + warp) * 32 + 16 >= t_end) : 0;
+    const int last_at = t_begin + ((mine - 1) * kWarps + warp) * F::kTokens;
+    const int sixteens = mine ? F::kSixteens * (mine - 1) + min((t_end - last_at + 15) / 16, F::kSixteens) : 0;  // that this warp copies
     auto issue = [&](int j, int slot) {  // block j of this warp into a slot
-        if (2 * j < halves) {
-            if ((j & 15) == 0) {
+        if (F::kSixteens * j < sixteens) {
+            if (j % kBatch == 0) {
                 at_now = at_next;
-                at_next = look_up(2 * (j + 16) + lane);
+                at_next = look_up(F::kSixteens * (j + kBatch) + lane);
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint64_t at = __shfl_sync(0xffffffffu, at_now, 2 * (j & 15) + h);
-                if (2 * j + h >= halves) break;
+            for (int h = 0; h < F::kSixteens; ++h) {
+                const uint64_t at = __shfl_sync(0xffffffffu, at_now, F::kSixteens * (j % kBatch) + h);
+                if (F::kSixteens * j + h >= sixteens) break;
                 const uint32_t to = slot * F::kStageBytes;
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
@@ -241,12 +245,12 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
         const uint32_t st_at = ring_at + slot * F::kStageBytes;
         slot_in = slot;
         slot = slot + 1 == F::kStages ? 0 : slot + 1;
-        const int tok = t_begin + (j * kWarps + warp) * 32;
+        const int tok = t_begin + (j * kWarps + warp) * F::kTokens;
 
         // scores of tokens 16 h + g (t[h][n][0], [1]) and 16 h + g + 8 ([2], [3]) for rows 8 n + 2 c, + 1
-        float t[2][NT][4];
+        float t[F::kSixteens][NT][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < F::kSixteens; ++h) {
             uint32_t w[2][kGroups];  // word c of each group of tokens g and g + 8
             load_half<D, false>(w, st_at + h * F::kHalfBytes + get0);
             float d0[kGroups], d1[kGroups];
@@ -270,14 +274,14 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
                 }
             }
         }
-        float dv[2][2][kGroups], top_d = kZeroScale;  // the values' scales of tokens 16 h + 8 r + g
+        float dv[F::kSixteens][2][kGroups], top_d = kZeroScale;  // the values' scales of tokens 16 h + 8 r + g
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < F::kSixteens; ++h)
 #pragma unroll
             for (int r = 0; r < 2; ++r) scales_of<kGroups>(st + F::kScaleAt + (2 * h + 1) * F::kScaleBytes + (8 * r + g) * (2 * kGroups), dv[h][r]);
-        if (tok + 31 >= t_end || tok < first_any) {
+        if (tok + F::kTokens - 1 >= t_end || tok < first_any) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < F::kSixteens; ++h)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     const int at = tok + 16 * h + 8 * r + g;
@@ -286,18 +290,18 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
                 }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < F::kSixteens; ++h)
 #pragma unroll
             for (int k = 0; k < kGroups; ++k) top_d = max3_abs(top_d, dv[h][0][k], dv[h][1][k]);
         const float lv = lg2_approx(top_d);
-        if (tok + 31 > seen_by_all || tok < window_end) {
+        if (tok + F::kTokens - 1 > seen_by_all || tok < window_end) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const int last = kv_last(a, q, i_lo + (rest0 + 8 * n + 2 * c + k) / G), first = kv_first(a, last);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int h = 0; h < F::kSixteens; ++h)
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
                             const int at = tok + 16 * h + 8 * r + g;
@@ -305,7 +309,12 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
                         }
                 }
         }
-        auto most = [&](int n, int k) { return fmaf(fmaxf(max3(t[0][n][k], t[0][n][k + 2], t[1][n][k]), t[1][n][k + 2]), row_c[n][k], lv); };
+        auto most = [&](int n, int k) {
+            float x = fmaxf(t[0][n][k], t[0][n][k + 2]);
+#pragma unroll
+            for (int h = 1; h < F::kSixteens; ++h) x = max3(x, t[h][n][k], t[h][n][k + 2]);
+            return fmaf(x, row_c[n][k], lv);
+        };
         bool rise = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -330,7 +339,7 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
                 }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < F::kSixteens; ++h) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll

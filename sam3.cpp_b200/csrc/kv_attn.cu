@@ -65,6 +65,7 @@ template <int D, int NT>
 struct Few {
     static constexpr int kRows = 8 * NT;
     static constexpr int kStages = NT == 1 ? 3 : 4, kBlocks = NT == 1 ? 4 : 3;  // stages of a warp, blocks an SM
+    static constexpr int kTurn = 64;                                 // tokens of a turn of the warps: least tokens of a part
     static constexpr int kBlockBytes = 16 * D;                       // codes of 16 tokens
     static constexpr int kStageBytes = 2 * kBlockBytes + 16;         // keys, values, their two scales
     static constexpr int kRing = kWarps * kStages * kStageBytes;

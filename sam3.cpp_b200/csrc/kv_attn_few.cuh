@@ -173,8 +173,8 @@ cudaError_t few_launch(void (*kernel)(Args), Args &a, unsigned bit, int num_sms,
     const int64_t span =
         std::max(a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len, int64_t(1));
     int64_t splits = 2 * groups < wave ? (2 * wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
-    // a block's least part: 64 tokens, one turn of its warps, while the blocks fit in one wave, else 256
-    const int64_t least = groups * ((span + 63) / 64) <= wave ? 64 : 256;
+    // a block's least part: a turn of its warps while the blocks fit in one wave, else 256
+    const int64_t least = groups * ((span + F::kTurn - 1) / F::kTurn) <= wave ? F::kTurn : 256;
     splits = std::min(splits, (span + least - 1) / least);
     splits = std::min(splits, std::min(static_cast<int64_t>(kMaxParts) / groups, static_cast<int64_t>(kMaxSplits)));
     splits = std::max(splits, static_cast<int64_t>(1));

@@ -21,10 +21,10 @@ namespace b200 {
 namespace {
 
 constexpr int kMaxSets = 4;
-// Blocks an SM that the registers are cut for (us, a video prompt of 40 heads of 128 in bf16: 5 blocks 101, 6 92, 8 88; an
-// image of 32 heads of 64, f32 to f16: 5 blocks 19.6, 6 20.0, 8 21.4).
+// Blocks an SM that the registers are cut for (us, a video prompt of 40 heads of 128 in bf16: 6 blocks 92, 7 87.8, 8 90; an
+// image of 32 heads of 64, f32 to f16: 4 blocks 19.5, 5 16.8, 6 17.6).
 template <typename TX>
-constexpr int kBlocks = sizeof(TX) == 2 ? 8 : 6;
+constexpr int kBlocks = sizeof(TX) == 2 ? 7 : 5;
 constexpr float kEpsLeast = 1.17549435e-38f;
 constexpr float kSumMost = 3e38f;               // sums of squares above this are taken again, of elements
 constexpr float kShrink = 8.470329472543003e-22f;  // 2^-70 times as large
@@ -67,10 +67,8 @@ __device__ __forceinline__ void moments(float (&f)[16], bool mine, int lanes, fl
     auto total = [&](float s) {
         s = mine ? s : 0.f;
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            const float x = __shfl_xor_sync(0xffffffffu, s, o);
-            if (o < lanes) s += x;
-        }
+        for (int o = 1; o < 16; o <<= 1)
+            if (o < lanes) s += __shfl_xor_sync(0xffffffffu, s, o);  // (the block's threads agree)
         return s;
     };
     auto variance = [&] {

@@ -521,6 +521,49 @@ def test_kv4_attention_extreme_values(b200, backend, attend, t, rows, size):
         check_attention(dev, attend, store(x * 1e-30, t), t, start, lens, 2, 1e30, **kw)
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [4, 48])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_kv4_queries_that_are_not_numbers(b200, backend, attend, t, rows, bad):
+    """One element of every other row: NaN makes the row NaN however few tokens it sees, infinities what the definition
+    makes of them; the rows between are as without."""
+    dev = filled(b200, backend, [48 + rows], 16, 64, 1)
+    for n in ("k_codes", "v_codes"):  # no zeros: the sums of infinities are the definition's
+        x = dev.host[n]
+        x[:] = np.where(x & 15 == 8, x + 1, x)
+        x[:] = np.where(x >> 4 == 8, x + 16, x)
+    dev.put()
+    x = np.random.default_rng(2).normal(size=(rows, 1, 64))
+    x[::2, 0, 5] = bad
+    for window in (1, 2, 4, 20, 0):
+        got = check_attention(dev, attend, store(x, t), t, [0, rows], [48 + rows], 1, 0.125, window=window)
+        assert not np.isnan(got[1::2]).any()
+        if np.isnan(bad):
+            assert np.isnan(got[::2]).all()
+
+
+def test_kv4_and_8_bit_calls_share_a_handle(b200, backend, attend):
+    """Calls over both caches, in parts, in turn with one handle: the same numbers as each alone."""
+    from test_seq_cache_gpu import filled as filled8
+    lens = [5000, 700]
+    dev4, dev8 = filled(b200, backend, lens, 32, 128, 2), filled8(b200, backend, lens, 32, 128, 2)
+    alone, own = {}, backend.kv_attention()
+    for rows in (1, 40):
+        q = backend.upload(store(np.random.default_rng(rows).normal(size=(2 * rows, 8, 128)), "f16"))
+        for round_ in range(3):
+            for name, dev in (("4", dev4), ("8", dev8)):
+                y = backend.alloc(2 * rows * 8 * 128 * 2)
+                (own if round_ == 0 else attend).run(dev.cache, dev.batch(np.arange(3) * rows, lens), TYPES["f16"], q.ptr, 8, y.ptr, 0.1)
+                if round_ == 0:
+                    backend.synchronize()
+                alone.setdefault((name, rows), []).append(y)
+    backend.synchronize()
+    for (name, rows), ys in alone.items():
+        first, *others = [y.get((2 * rows, 8, 128), np.uint16) for y in ys]
+        assert all(np.array_equal(first, x) for x in others)
+    own.free()
+
+
 @pytest.mark.parametrize("rows", [1, 50])
 def test_kv4_sequences_share_pages(b200, backend, attend, rows):
     """A common prompt's pages, a page that is not full among them, stand in the tables of several sequences; the first
@@ -728,6 +771,19 @@ def test_vec_beside_the_other_products(b200, backend, model):
     assert np.array_equal(runs[0], runs[1]) and np.array_equal(runs[0], runs[2])
     assert np.abs(runs[0] - exact).max() <= 2.0 ** -19 * (np.abs(x).astype(np.float64) @ np.abs(do.weight(raw, "q4_0", N, K)).T).max()
     w.free()
+
+
+def test_vec_weights_from_device_memory(b200, backend):
+    """Blocks that lie on the GPU, by address, are the same weight."""
+    rng = np.random.default_rng(6)
+    N, K = 70, 192
+    for kind in ("q4_0", "q4_1"):
+        raw = do.blocks(rng, kind, N, K)
+        buf = backend.upload(raw)
+        for at in (buf.ptr, np.int64(buf.ptr)):
+            w = backend.weight(b200.TYPE_Q4_0 if kind == "q4_0" else b200.TYPE_Q4_1, at, K, N)
+            check_vec(b200, backend, raw, kind, N, K, store(rng.normal(size=(2, K)), "f32"), "f32", "f32", handle=w)
+            w.free()
 
 
 def test_vec_refusals(b200, backend):
