@@ -21,7 +21,21 @@
 // dimensions), and transposed for values, 4 dimensions of tokens 2c and 2c + 1
 // side by side, so a nibble and the one 16 bits above it are the pair that the
 // instruction wants, in either product, and widening is a mask and a
-// subtraction for a pair.
+// subtraction for a pair.  Each warp first widens its block's scales, a lane a
+// token, and leaves them in shared memory as pairs of equal f32 numbers: every
+// lane then has those of its tokens by one 16-byte load for two groups, ready
+// for arithmetic on pairs, in place of two conversions a token and group.
+//
+// What bounds it: instructions, some 650 a warp for 32 tokens of heads of 128
+// (4.6 KB; the issue slots are taken in two cycles of three), not the bytes.
+// Measured: 64 sequences of 1000 ... 16100 tokens, 8 kv heads of 128, 4 query
+// heads each, 161 us (677 MB, 4.2 TB/s; the 8-bit cache takes 213); one sequence
+// of 900 7.2 us; 3 ... 5 tokens of each of 4 sequences of 30000 ... 70000, 8
+// heads of 64, 43.4 us.  Scales taken from the stage by each lane: 169, 7.6 and
+// 45.4 us.  Copies by the bulk engine in place of 16-byte ones: 177 us, since the
+// waits take more instructions than the copies; 5 blocks an SM: 195 us, for lack
+// of registers; 3 blocks: 162 us, and 46 us with heads of 64.  Two stages (heads
+// of 64: three), since 4 blocks with the widened scales have room for no more.
 #include <algorithm>
 #include <cmath>
 
@@ -40,18 +54,12 @@ __device__ __forceinline__ float lg2_approx(float x) {
     return y;
 }
 
-// The largest of three numbers (NaN is none), and of their magnitudes.
+// The largest of three numbers (NaN is none).
 __device__ __forceinline__ float max3(float x, float y, float z) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
     return d;
 }
-__device__ __forceinline__ float max3_abs(float x, float y, float z) {
-    float d;
-    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(x), "f"(y), "f"(z));
-    return d;
-}
-
 constexpr float kZeroScale = 8.271806125530277e-25f;  // 2^-80: what tokens of zeros count as (2^kZeroScaleLog2)
 static_assert(kZeroScaleLog2 == -80.f, "its logarithm");
 
@@ -103,14 +111,16 @@ __device__ __forceinline__ float q_value(const Kv4AttnArgs &a, const uint4 &x, i
 template <int D, int NT>
 struct Few4 {
     static constexpr int kRows = 8 * NT, kGroups = D / 32;
-    static constexpr int kStages = D == 128 ? 3 : 4, kBlocks = NT == 1 ? 4 : 2;  // stages of a warp, blocks an SM
+    static constexpr int kStages = D == 128 ? 2 : 3, kBlocks = NT == 1 ? 4 : 2;  // stages of a warp, blocks an SM
     static constexpr int kTurn = 128;                              // least tokens of a part (one token over 900: 64 8.4 us, 128 7.6)
     static constexpr int kCodeBytes = 16 * D / 2;                  // of 16 tokens
     static constexpr int kScaleBytes = 16 * kGroups * 2;
     // a stage: for each 16 tokens their keys' and values' codes, then for each 16 their scales
     static constexpr int kSixteens = 256 / D, kTokens = 16 * kSixteens;
     static constexpr int kHalfBytes = 2 * kCodeBytes, kScaleAt = kSixteens * kHalfBytes, kStageBytes = kScaleAt + 2 * kSixteens * kScaleBytes;
-    static constexpr int kRing = kWarps * kStages * kStageBytes;
+    // the block's scales as f32, each twice, a pair of groups in 16 bytes: [keys, values][kGroups / 2][kTokens]
+    static constexpr int kWideAt = kWarps * kStages * kStageBytes, kWideBytes = kGroups * kTokens * 16;
+    static constexpr int kRing = kWideAt + kWarps * kWideBytes;
     static constexpr int kRowFloats = D + 4;                       // a joined row, padded against bank conflicts
     static constexpr int kJoin = kWarps * kRows * kRowFloats * 4;
     static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
@@ -163,21 +173,20 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
     const uint8_t *own_k = a.c.codes[0] + lane * 16, *own_v = a.c.codes[1] + lane * 16;
     constexpr int kScaleChunks = F::kScaleBytes / 16;
     const uint8_t *own_scale = reinterpret_cast<const uint8_t *>(a.c.scale[lane >= kScaleChunks]) + lane % kScaleChunks * 16;
+    float4 *wide = reinterpret_cast<float4 *>(smem + F::kWideAt + warp * F::kWideBytes);
     const uint32_t ring_at = smem_u32(ring), put_at = ring_at + put0, put_scale_at = ring_at + F::kScaleAt + lane * 16;
     // lane kSixteens j + h: where the h-th 16 tokens of block kBatch b + j of this warp lie, for batches b and b + 1
     constexpr int kBatch = 32 / F::kSixteens;
     uint32_t at_now = 0, at_next = 0;
     auto look_up = [&](int j) -> uint32_t {
         const int tok = t_begin + (j / F::kSixteens * kWarps + warp) * F::kTokens + j % F::kSixteens * 16;
-        if (j / F::kSixteens >= mine || tok >= t_end) return 0;
+        if (j / F::kSixteens >= mine || tok >= t_end) return 0;  // (copied all the same, and seen by no row)
         const int page = max(kv_page(a.c, a.b, q.s, tok >> a.c.page_log2, a.err), 0);
         return ((static_cast<uint32_t>(page) * a.c.heads + kv) << a.c.page_log2) + (tok & ((1 << a.c.page_log2) - 1));
     };
     at_next = look_up(lane);
-    const int last_at = t_begin + ((mine - 1) * kWarps + warp) * F::kTokens;
-    const int sixteens = mine ? F::kSixteens * (mine - 1) + min((t_end - last_at + 15) / 16, F::kSixteens) : 0;  // that this warp copies
     auto issue = [&](int j, int slot) {  // block j of this warp into a slot
-        if (F::kSixteens * j < sixteens) {
+        if (j < mine) {
             if (j % kBatch == 0) {
                 at_now = at_next;
                 at_next = look_up(F::kSixteens * (j + kBatch) + lane);
@@ -185,7 +194,6 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 #pragma unroll
             for (int h = 0; h < F::kSixteens; ++h) {
                 const uint64_t at = __shfl_sync(0xffffffffu, at_now, F::kSixteens * (j % kBatch) + h);
-                if (F::kSixteens * j + h >= sixteens) break;
                 const uint32_t to = slot * F::kStageBytes;
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
@@ -247,17 +255,36 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
         slot = slot + 1 == F::kStages ? 0 : slot + 1;
         const int tok = t_begin + (j * kWarps + warp) * F::kTokens;
 
+        // the scales: a lane a token (heads of 64: two); those of values that no row sees are 0
+        unsigned top_bits = __float_as_uint(kZeroScale);
+#pragma unroll
+        for (int u = 0; u < F::kTokens / 32; ++u) {
+            const int k = lane + 32 * u;
+            const uint8_t *from = st + F::kScaleAt + k / 16 * (2 * F::kScaleBytes) + k % 16 * (2 * kGroups);
+            float dk[kGroups], dv[kGroups];
+            scales_of<kGroups>(from, dk);
+            scales_of<kGroups>(from + F::kScaleBytes, dv);
+            const bool out = tok + k >= t_end || tok + k < first_any;
+#pragma unroll
+            for (int i = 0; i < kGroups; i += 2) {
+                if (out) dv[i] = dv[i + 1] = 0.f;
+                top_bits = max(top_bits, max(__float_as_uint(fabsf(dv[i])), __float_as_uint(fabsf(dv[i + 1]))));
+                wide[i / 2 * F::kTokens + k] = make_float4(dk[i], dk[i], dk[i + 1], dk[i + 1]);
+                wide[(kGroups + i) / 2 * F::kTokens + k] = make_float4(dv[i], dv[i], dv[i + 1], dv[i + 1]);
+            }
+        }
+        const float top_d = __uint_as_float(__reduce_max_sync(0xffffffffu, top_bits));
+        __syncwarp();
+
         // scores of tokens 16 h + g (t[h][n][0], [1]) and 16 h + g + 8 ([2], [3]) for rows 8 n + 2 c, + 1
         float t[F::kSixteens][NT][4];
 #pragma unroll
         for (int h = 0; h < F::kSixteens; ++h) {
             uint32_t w[2][kGroups];  // word c of each group of tokens g and g + 8
             load_half<D, false>(w, st_at + h * F::kHalfBytes + get0);
-            float d0[kGroups], d1[kGroups];
-            scales_of<kGroups>(st + F::kScaleAt + 2 * h * F::kScaleBytes + g * (2 * kGroups), d0);
-            scales_of<kGroups>(st + F::kScaleAt + 2 * h * F::kScaleBytes + (g + 8) * (2 * kGroups), d1);
 #pragma unroll
             for (int k = 0; k < kGroups; ++k) {
+                const float4 d0 = wide[k / 2 * F::kTokens + 16 * h + g], d1 = wide[k / 2 * F::kTokens + 16 * h + 8 + g];
                 uint32_t u[4], v[4];
                 codes4(w[0][k], u);
                 codes4(w[1][k], v);
@@ -266,33 +293,17 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
                     float s[4];
                     mma16816_first(s, u[0], v[0], u[1], v[1], qf[n][k][0], qf[n][k][1]);
                     mma16816(s, u[2], v[2], u[3], v[3], qf[n][k][2], qf[n][k][3]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float d = i < 2 ? d0[k] : d1[k];
-                        t[h][n][i] = k ? fmaf(s[i], d, t[h][n][i]) : s[i] * d;
+                    float *x = t[h][n];
+                    if (k == 0) {
+                        fmul2(x[0], x[1], s[0], s[1], d0.x, d0.y);
+                        fmul2(x[2], x[3], s[2], s[3], d1.x, d1.y);
+                    } else {
+                        ffma2(x[0], x[1], s[0], s[1], k & 1 ? d0.z : d0.x, k & 1 ? d0.w : d0.y);
+                        ffma2(x[2], x[3], s[2], s[3], k & 1 ? d1.z : d1.x, k & 1 ? d1.w : d1.y);
                     }
                 }
             }
         }
-        float dv[F::kSixteens][2][kGroups], top_d = kZeroScale;  // the values' scales of tokens 16 h + 8 r + g
-#pragma unroll
-        for (int h = 0; h < F::kSixteens; ++h)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) scales_of<kGroups>(st + F::kScaleAt + (2 * h + 1) * F::kScaleBytes + (8 * r + g) * (2 * kGroups), dv[h][r]);
-        if (tok + F::kTokens - 1 >= t_end || tok < first_any) {
-#pragma unroll
-            for (int h = 0; h < F::kSixteens; ++h)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int at = tok + 16 * h + 8 * r + g;
-#pragma unroll
-                    for (int k = 0; k < kGroups; ++k) dv[h][r][k] = at >= t_end || at < first_any ? 0.f : dv[h][r][k];
-                }
-        }
-#pragma unroll
-        for (int h = 0; h < F::kSixteens; ++h)
-#pragma unroll
-            for (int k = 0; k < kGroups; ++k) top_d = max3_abs(top_d, dv[h][0][k], dv[h][1][k]);
         const float lv = lg2_approx(top_d);
         if (tok + F::kTokens - 1 > seen_by_all || tok < window_end) {
 #pragma unroll
@@ -353,13 +364,17 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
             load_half<D, true>(w, st_at + h * F::kHalfBytes + F::kCodeBytes + get0);
 #pragma unroll
             for (int k = 0; k < kGroups; ++k) {
+                const float4 d0 = wide[(kGroups + k) / 2 * F::kTokens + 16 * h + g], d1 = wide[(kGroups + k) / 2 * F::kTokens + 16 * h + 8 + g];
                 uint32_t u[4], v[4];
                 codes4(w[0][k], u);
                 codes4(w[1][k], v);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const uint32_t p0 = transposed(pack_f16(t[h][n][0] * dv[h][0][k], t[h][n][1] * dv[h][0][k]));
-                    const uint32_t p1 = transposed(pack_f16(t[h][n][2] * dv[h][1][k], t[h][n][3] * dv[h][1][k]));
+                    const float *y = t[h][n];
+                    float x[4];
+                    fmul2(x[0], x[1], y[0], y[1], k & 1 ? d0.z : d0.x, k & 1 ? d0.w : d0.y);
+                    fmul2(x[2], x[3], y[2], y[3], k & 1 ? d1.z : d1.x, k & 1 ? d1.w : d1.y);
+                    const uint32_t p0 = transposed(pack_f16(x[0], x[1])), p1 = transposed(pack_f16(x[2], x[3]));
                     // dimensions 4 g, + 1 of the group are rows g, g + 8 of one product, + 2, + 3 of the next
                     mma16816(o[n][2 * k], u[0], u[1], v[0], v[1], p0, p1);
                     mma16816(o[n][2 * k + 1], u[2], u[3], v[2], v[3], p0, p1);
