@@ -29,7 +29,7 @@
 // What bounds it: instructions, some 650 a warp for 32 tokens of heads of 128
 // (4.6 KB; the issue slots are taken in two cycles of three), not the bytes.
 // Measured: 64 sequences of 1000 ... 16100 tokens, 8 kv heads of 128, 4 query
-// heads each, 161 us (677 MB, 4.2 TB/s; the 8-bit cache takes 213); one sequence
+// heads each, 161 us (666 MB, 4.1 TB/s; the 8-bit cache takes 213); one sequence
 // of 900 7.2 us; 3 ... 5 tokens of each of 4 sequences of 30000 ... 70000, 8
 // heads of 64, 43.4 us.  Scales taken from the stage by each lane: 169, 7.6 and
 // 45.4 us.  Copies by the bulk engine in place of 16-byte ones: 177 us, since the

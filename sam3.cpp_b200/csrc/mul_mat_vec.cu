@@ -11,7 +11,11 @@
 // f16 with f32 sums: the codes are its 16-row operand (exact in f16), the rows of
 // x its 8 columns, so up to 8 rows cost what one does, and the legacy matrix
 // instruction is wide enough for what memory delivers; widening the codes and
-// scaling the sums, some 130 instructions for 1 KB of codes, is what comes next.
+// scaling the sums, 162 instructions a warp for 1 KB of codes (62 % of the issue
+// slots), is what comes next.  Measured: 49408 x 4096 Q4_0 by one row of f16 25.8
+// us (114 MB, 4.4 TB/s), 14339 x 4096 Q4_1 by 6 rows of bf16 15 us, of which the
+// launch and the staging of x are some 5.  Chunks dealt to the warps of a tile
+// in turn, joined tile by tile, took 28.7 us in place of 25.8.
 // Word t of each weight row's block (elements 4t ... and 16 + 4t ...) comes to a
 // lane by ldmatrix, a nibble and the one 16 bits above it are one operand
 // register after a mask and a subtraction, and x is staged in the same order.  A
@@ -58,7 +62,8 @@ struct Vec {
 };
 
 // Rows whose largest element lies in [2^-5, 2^9) are multiplied by 2^6, so that their largest has at least f16's 1: what f16
-// then loses is at most 2^-26 of it, and no look over the row has to come first (us, 6 rows of 4096 in bf16: PLACEHOLDER).
+// then loses is at most 2^-26 of it, and no look over the row has to come first (6 rows of 4096 in bf16 by 14339 Q4_0 weight
+// rows, in a graph: 15.1 us with the look, 13.5 without; Q4_1 17.1 and 15.0; one row 12.4 and 11.2).
 constexpr float kUsual = 64.f, kUsualLeast = 0.03125f, kUsualMost = 512.f;
 
 // The bits of v's magnitude, 0 for an infinity or NaN.
@@ -508,7 +513,8 @@ cudaError_t launch(Backend *be, VecArgs &a) {
 }
 
 // Tiles of 16 or of 32 rows, where x is read from shared memory once for both halves: by the steps of a warp, one of 32
-// counted as 1.8 of 16 (us, PLACEHOLDER).
+// counted as 1.8 of 16.  Us for tiles of 16 and of 32, 4096 columns: 49408 weight rows and one of x 27.8 and 25.8; 14339 rows
+// of Q4_1 and 6 of x 17.4 and 18.1; 1024 columns by 4096 and one row 6.2 and 6.6.
 template <int NT, bool MINS, typename TX>
 cudaError_t launch(Backend *be, VecArgs &a) {
     if constexpr (NT < 4) {

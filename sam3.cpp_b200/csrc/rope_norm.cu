@@ -11,6 +11,12 @@
 // threads a head), so the sums of a head are 16 terms in a thread and one
 // to four shuffles.  Up to four sets of heads (queries and keys, each with
 // its weights) share a launch and the angles of a row.
+// Measured: 21037 rows of 32 + 8 heads of 128 in bf16 87.8 us, 4.9 TB/s (the
+// rotation alone 77), with 70 % of the issue slots taken: a head costs the sums,
+// the shuffles and two conversions an element on top of the turn.  5184 rows of
+// 32 heads of 64, f32 to f16, 16.8 us (64 MB; floor 9.8): one wave of blocks.
+// Weights kept in registers for arithmetic on pairs: 124 us, for lack of them;
+// several row turns a block in place of one: 105.
 #include <algorithm>
 #include <cmath>
 
