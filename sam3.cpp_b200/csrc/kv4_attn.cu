@@ -36,6 +36,9 @@
 // waits take more instructions than the copies; 5 blocks an SM: 195 us, for lack
 // of registers; 3 blocks: 162 us, and 46 us with heads of 64.  Two stages (heads
 // of 64: three), since 4 blocks with the widened scales have room for no more.
+// One wave of blocks with equal stretches of all sequences' work, cut on the
+// device, in place of a grid of parts: 182 us, and 115 in place of 82 for 200
+// sequences of 100 ... 2500, whose starts and joins then follow one another.
 #include <algorithm>
 #include <cmath>
 

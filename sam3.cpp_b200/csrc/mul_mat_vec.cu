@@ -12,10 +12,12 @@
 // x its 8 columns, so up to 8 rows cost what one does, and the legacy matrix
 // instruction is wide enough for what memory delivers; widening the codes and
 // scaling the sums, 162 instructions a warp for 1 KB of codes (62 % of the issue
-// slots), is what comes next.  Measured: 49408 x 4096 Q4_0 by one row of f16 25.8
-// us (114 MB, 4.4 TB/s), 14339 x 4096 Q4_1 by 6 rows of bf16 15 us, of which the
-// launch and the staging of x are some 5.  Chunks dealt to the warps of a tile
-// in turn, joined tile by tile, took 28.7 us in place of 25.8.
+// slots), is what comes next.  Measured: 49408 x 4096 Q4_0 by one row of f16 25.1
+// us (114 MB, 4.5 TB/s; 25.8 with blocks cut at whole tiles), 14339 x 4096 Q4_1 by
+// 6 rows of bf16 15.5 us, of which the launch, the staging of x and the end are
+// some 6.  Chunks dealt to the warps of a tile in turn, joined tile by tile, took
+// 28.7 us in place of 25.8; scales widened once
+// a warp through shared memory, for arithmetic on pairs, 26.6 (Q4_1 17 for 15.2).
 // Word t of each weight row's block (elements 4t ... and 16 + 4t ...) comes to a
 // lane by ldmatrix, a nibble and the one 16 bits above it are one operand
 // register after a mask and a subtraction, and x is staged in the same order.  A
@@ -45,7 +47,7 @@ struct VecArgs {
     const float *bias;
     void *y;
     int M, N, K, cols;           // cols: columns of x, M or 2 M
-    int tiles, chunks;
+    int sixteens, chunks;        // of weight rows; of 128 columns
     int phase, w_log2;           // chunks of x in shared memory at once: all, or a multiple of the 1 << w_log2 warps of a tile
     int y_type, aligned;         // aligned: four elements of x at once
 };
@@ -72,13 +74,6 @@ __device__ __forceinline__ unsigned finite_bits(float v) {
     return bits < 0x7f800000u ? bits : 0u;
 }
 
-// f16 of v; `rest`: what it leaves (0 of an infinity or NaN).
-__device__ __forceinline__ float f16_of(float v, float &rest) {
-    const float h = __half2float(__float2half_rn(v));
-    rest = fabsf(h) <= 65504.f ? v - h : 0.f;
-    return h;
-}
-
 // Four elements as they come.
 template <typename T>
 struct alignas(4 * sizeof(T)) Raw4 {
@@ -98,13 +93,39 @@ struct alignas(4 * sizeof(T)) Raw4 {
     }
 };
 
+// The largest of them for eight elements.
+__device__ __forceinline__ unsigned finite_bits(const Raw4<float> (&raw)[2]) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, finite_bits(raw[i >> 2].v[i & 3]));
+    return top;
+}
+__device__ __forceinline__ unsigned finite_bits(const Raw4<__half> (&)[2]) { return 0; }
+__device__ __forceinline__ unsigned finite_bits(const Raw4<__nv_bfloat16> (&raw)[2]) {
+    // pairs: magnitude + 0x80 is a positive 16-bit number if it is finite, else a negative one
+    uint32_t top = 0x00800080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = (reinterpret_cast<const uint32_t *>(raw[i >> 1].v)[i & 1] & 0x7fff7fffu) + 0x00800080u;
+        asm("max.s16x2 %0, %0, %1;" : "+r"(top) : "r"(w));
+    }
+    return (max(top >> 16, top & 0xffffu) - 0x80u) << 16;
+}
+
+// f16 of v; `rest`: what it leaves (0 of an infinity or NaN).
+__device__ __forceinline__ float f16_of(float v, float &rest) {
+    const float h = __half2float(__float2half_rn(v));
+    rest = fabsf(h) <= 65504.f ? v - h : 0.f;
+    return h;
+}
+
 template <int NT, int RT, bool MINS, typename TX>
 __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_constant__ VecArgs a) {
     using V = Vec<NT, RT, MINS>;
     constexpr int kStages = V::kStages, kStageBytes = V::kStageBytes;
     constexpr int kParts = sizeof(TX) == 4 ? 2 : 1;  // columns of a row
     constexpr bool kScaled = !std::is_same<TX, __half>::value;
-    constexpr int kFlight = 4;  // rows of x that a thread has on their way at once
+    constexpr int kFlight = 4;  // rows of x that a thread has on their way at once (us, 8 rows of 14336: 2 34.9, 3 31, 4 28, 8 30.7)
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float s_up[kMaxRows], s_down[kMaxRows];
     __shared__ unsigned s_top[kMaxRows];
@@ -116,17 +137,19 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
     uint4 *xs = reinterpret_cast<uint4 *>(smem + V::kX);                     // [block][column][4]
     float *sums = reinterpret_cast<float *>(xs + a.phase * 4 * a.cols * 4);  // MINS: [block][8 NT]
 
-    // The steps of a warp, each one chunk of one tile.  Where all of x fits, the block has consecutive tiles [t0, t1), whose
+    // The steps of a warp, each one chunk of one tile.  Where all of x fits, the block has tiles 0 ... t1 - 1 of 16 RT rows, whose
     // chunks in a row are cut into 16 equal parts, so that a warp begins and ends within a tile but needs no other warp before
     // the end.  Else W warps share a tile, chunk by chunk, and the block takes 16 / W tiles after the other through all of x.
     const bool whole = a.phase >= a.chunks;
     const int W = 1 << a.w_log2, w_in = warp & (W - 1), batch = kWarps >> a.w_log2;
-    const int t0 = static_cast<int>(static_cast<int64_t>(blockIdx.x) * a.tiles / gridDim.x);
-    const int t1 = static_cast<int>((static_cast<int64_t>(blockIdx.x) + 1) * a.tiles / gridDim.x);
-    const int total = (t1 - t0) * a.chunks;
+    // Blocks are cut at 16 rows, so that a block's last tile may be half of one.
+    const int u0 = static_cast<int>(static_cast<int64_t>(blockIdx.x) * a.sixteens / gridDim.x);
+    const int u1 = static_cast<int>((static_cast<int64_t>(blockIdx.x) + 1) * a.sixteens / gridDim.x);
+    const int row_end = min(u1 * 16, a.N), t1 = (u1 - u0 + RT - 1) / RT;
+    const int total = t1 * a.chunks;
     auto part = [&](int w) { return static_cast<int>(static_cast<int64_t>(w) * total / kWarps); };
     const int first_step = part(warp), n_steps = part(warp + 1) - first_step;
-    const int first_tile = whole ? t0 + first_step / a.chunks : t0 + (warp >> a.w_log2), first_chunk = whole ? first_step % a.chunks : w_in;
+    const int first_tile = whole ? first_step / a.chunks : warp >> a.w_log2, first_chunk = whole ? first_step % a.chunks : w_in;
 
     // The copies of those steps in their order: a lane's rows of codes and its part of the scales; zeros behind the
     // weights' rows and blocks.
@@ -139,21 +162,21 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
     int next_tile = first_tile, next_c = first_chunk;
     const uint8_t *from = nullptr, *from_scales = nullptr;
     auto seek = [&] {
-        from = a.codes + static_cast<int64_t>(next_tile * 16 * RT + put_row) * (a.K / 2) + (next_c * 4 + put_part) * 16;
-        from_scales = a.scales + (static_cast<int64_t>(next_tile) * RT * a.chunks + next_c) * V::kRecord + lane * 16;
+        from = a.codes + static_cast<int64_t>((u0 + next_tile * RT) * 16 + put_row) * (a.K / 2) + (next_c * 4 + put_part) * 16;
+        from_scales = a.scales + ((u0 + static_cast<int64_t>(next_tile) * RT) * a.chunks + next_c) * V::kRecord + lane * 16;
     };
     seek();
     auto issue = [&](int slot) {
         if (left > 0) {
             const uint32_t dst = ring_at + slot * kStageBytes;
-            const int n = next_tile * 16 * RT;
-            if (n + 16 * RT <= a.N && next_c * 4 + 4 <= blocks) {
+            const int n = (u0 + next_tile * RT) * 16;
+            if (n + 16 * RT <= row_end && next_c * 4 + 4 <= blocks) {
 #pragma unroll
                 for (int k = 0; k < 2 * RT; ++k) cp16(dst + put0 + k * 512, from + k * eight);
             } else {
 #pragma unroll
                 for (int k = 0; k < 2 * RT; ++k) {
-                    const bool there = n + put_row + 8 * k < a.N && next_c * 4 + put_part < blocks;
+                    const bool there = n + put_row + 8 * k < row_end && next_c * 4 + put_part < blocks;
                     cp16_or_zero(dst + put0 + k * 512, there ? from + k * eight : a.codes, there);
                 }
             }
@@ -161,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
             for (int r = 0; r < RT; ++r) {
                 const uint32_t to = dst + RT * V::kCodeBytes + r * V::kRecord + lane * 16;
                 if (lane < V::kRecord / 16) {
-                    if (r == 0 || n + 16 * r < a.N) cp16(to, from_scales + static_cast<int64_t>(r) * a.chunks * V::kRecord);
+                    if (r == 0 || n + 16 * r < row_end) cp16(to, from_scales + static_cast<int64_t>(r) * a.chunks * V::kRecord);
                     else cp16_or_zero(to, a.scales, false);
                 }
             }
@@ -246,10 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
                     const float by = kScaled ? s_down[m0 + m] : 1.f;
                     float v[8];
                     if (kScaled && look) {
-                        unsigned top = 0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) top = max(top, finite_bits(to_f32(raw[m][i >> 2].v[i & 3])));
-                        top = __reduce_max_sync(0xffffffffu, top);
+                        const unsigned top = __reduce_max_sync(0xffffffffu, finite_bits(raw[m]));
                         if (lane == 0) atomicMax(&s_top[m0 + m], top);
                     }
 #pragma unroll
@@ -385,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
             }
     };
     auto store = [&](int m, int n, float v) {
-        if (m >= a.M || n >= a.N) return;
+        if (m >= a.M || n >= row_end) return;
         if (kScaled) v *= s_up[m];
         if (a.bias) v += a.bias[n];
         const int64_t at = m * a.ldy + n;
@@ -399,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int out = (tile * RT + r) * 16 + g + 8 * h;
+                    const int out = (u0 + tile * RT + r) * 16 + g + 8 * h;
                     if (kParts == 2) {
                         store(n * 4 + c, out, acc[r][n][2 * h] + acc[r][n][2 * h + 1]);
                     } else {
@@ -410,16 +430,14 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
     };
 
     if (whole) {
-        stage_x(0, true);
-        __syncthreads();
-        if (kScaled) {  // rows of another size than usual get a power of two of their own
+        for (bool look = kScaled;; look = false) {  // (one place, so that the code stays small)
+            stage_x(0, look);
+            __syncthreads();
+            if (!look) break;
             bool usual = true;
             for (int m = 0; m < a.M; ++m) usual = usual && s_top[m] < __float_as_uint(kUsualMost) && (s_top[m] >= __float_as_uint(kUsualLeast) || s_top[m] == 0);
-            if (!usual) {
-                scale_rows();
-                stage_x(0, false);
-                __syncthreads();
-            }
+            if (usual) break;
+            scale_rows();  // rows of another size than usual get a power of two of their own
         }
         int tile = first_tile, ch = first_chunk;
         for (int steps = n_steps; steps > 0; ++tile, ch = 0) {
@@ -431,21 +449,21 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
             else put(place(warp, tile != first_tile));
         }
         __syncthreads();
-        for (tile = t0 + warp; tile < t1; tile += kWarps) {  // tiles that several warps have parts of
-            const int64_t begin = static_cast<int64_t>(tile - t0) * a.chunks;
+        for (tile = warp; tile < t1; tile += kWarps) {  // tiles that several warps have parts of
+            const int64_t begin = static_cast<int64_t>(tile) * a.chunks;
             const int w0 = static_cast<int>(((begin + 1) * kWarps - 1) / total), w1 = static_cast<int>(((begin + a.chunks) * kWarps - 1) / total);
             if (w0 == w1) continue;
             clear();
             for (int w = w0; w <= w1; ++w)
-                if (part(w + 1) > part(w)) add(place(w, tile != t0 + part(w) / a.chunks));
+                if (part(w + 1) > part(w)) add(place(w, tile != part(w) / a.chunks));
             finish(tile);
         }
     } else {
-        for (int tile0 = t0; tile0 < t1; tile0 += batch) {
+        for (int tile0 = 0; tile0 < t1; tile0 += batch) {
             const int tile = tile0 + (warp >> a.w_log2);
             clear();
             for (int p0 = 0; p0 < a.chunks; p0 += a.phase) {
-                if (tile0 != t0 || p0) __syncthreads();  // the phase before is read
+                if (tile0 || p0) __syncthreads();  // the phase before is read
                 stage_x(p0, false);
                 __syncthreads();
                 if (tile < t1) run(w_in, min(a.phase, a.chunks - p0), W);
@@ -482,7 +500,7 @@ __global__ void vec_scales_kernel(const uint8_t *blocks, int N, int nblk, int mi
 template <int NT, int RT, bool MINS, typename TX>
 cudaError_t launch(Backend *be, VecArgs &a) {
     using V = Vec<NT, RT, MINS>;
-    a.tiles = (a.N + 16 * RT - 1) / (16 * RT);
+    const int tiles = (a.sixteens + RT - 1) / RT;
     const int per_chunk = 4 * (a.cols * 64 + (MINS ? 8 * NT * 4 : 0));
     static_assert((kSmem - V::kX) / (4 * 8 * NT * (64 + (MINS ? 4 : 0))) >= 8, "phases of several chunks");
     const int most = (kSmem - V::kX) / per_chunk;
@@ -499,7 +517,7 @@ cudaError_t launch(Backend *be, VecArgs &a) {
         // warps a tile: the number that gives the fewest steps of a warp, with x that comes again for every batch of tiles by
         // its instructions
         int64_t least = 0x7fffffffffffffff;
-        const int64_t own = (a.tiles + be->num_sms - 1) / be->num_sms;  // tiles of a block
+        const int64_t own = ((a.sixteens + be->num_sms - 1) / be->num_sms + RT - 1) / RT;  // tiles of a block
         for (int lg = 0; lg <= 4 && (1 << lg) <= most; ++lg) {
             const int64_t batches = (own * (1 << lg) + kWarps - 1) / kWarps;
             const int64_t cost = batches * ((a.chunks + (1 << lg) - 1) / (1 << lg) + 1 + a.chunks * static_cast<int64_t>(a.cols) / 64);
@@ -508,7 +526,7 @@ cudaError_t launch(Backend *be, VecArgs &a) {
         a.phase = most >> a.w_log2 << a.w_log2;
     }
     const int smem = V::kX + a.phase * per_chunk;
-    const int grid = std::min(be->num_sms, a.tiles);
+    const int grid = std::min(be->num_sms, tiles);
     return launch_after(kernel, dim3(static_cast<unsigned>(grid)), kThreads, smem, be->stream, a);
 }
 
@@ -518,11 +536,11 @@ cudaError_t launch(Backend *be, VecArgs &a) {
 template <int NT, bool MINS, typename TX>
 cudaError_t launch(Backend *be, VecArgs &a) {
     if constexpr (NT < 4) {
-        auto steps = [&](int64_t rows) {
-            const int64_t tiles = ((a.N + rows - 1) / rows + be->num_sms - 1) / be->num_sms;  // of a block
+        auto steps = [&](int64_t rt) {
+            const int64_t tiles = ((a.sixteens + be->num_sms - 1) / be->num_sms + rt - 1) / rt;  // of a block
             return (tiles * a.chunks + kWarps - 1) / kWarps;
         };
-        if (18 * steps(32) <= 10 * steps(16)) return launch<NT, 2, MINS, TX>(be, a);
+        if (18 * steps(2) <= 10 * steps(1)) return launch<NT, 2, MINS, TX>(be, a);
     }
     return launch<NT, 1, MINS, TX>(be, a);
 }
@@ -574,7 +592,7 @@ extern "C" int sam3b200_mul_mat_vec(sam3b200_backend *h, const sam3b200_weight *
     a.x = x, a.ldx = ldx, a.ldy = ldd, a.bias = bias, a.y = dst;
     a.M = static_cast<int>(M), a.N = w->N, a.K = w->K;
     a.cols = a.M * (x_type == SAM3B200_TYPE_F32 ? 2 : 1);
-    a.tiles = 0, a.chunks = (a.K + 127) / 128;
+    a.sixteens = (a.N + 15) / 16, a.chunks = (a.K + 127) / 128;
     a.w_log2 = 0, a.phase = a.chunks;
     a.y_type = y_type;
     a.aligned = reinterpret_cast<uintptr_t>(x) % (4 * xb) == 0 && ldx % 4 == 0;
