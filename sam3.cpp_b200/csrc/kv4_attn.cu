@@ -29,16 +29,20 @@
 // What bounds it: instructions, some 650 a warp for 32 tokens of heads of 128
 // (4.6 KB; the issue slots are taken in two cycles of three), not the bytes.
 // Measured: 64 sequences of 1000 ... 16100 tokens, 8 kv heads of 128, 4 query
-// heads each, 161 us (666 MB, 4.1 TB/s; the 8-bit cache takes 213); one sequence
-// of 900 7.2 us; 3 ... 5 tokens of each of 4 sequences of 30000 ... 70000, 8
-// heads of 64, 43.4 us.  Scales taken from the stage by each lane: 169, 7.6 and
-// 45.4 us.  Copies by the bulk engine in place of 16-byte ones: 177 us, since the
-// waits take more instructions than the copies; 5 blocks an SM: 195 us, for lack
-// of registers; 3 blocks: 162 us, and 46 us with heads of 64.  Two stages (heads
-// of 64: three), since 4 blocks with the widened scales have room for no more.
-// One wave of blocks with equal stretches of all sequences' work, cut on the
-// device, in place of a grid of parts: 182 us, and 115 in place of 82 for 200
-// sequences of 100 ... 2500, whose starts and joins then follow one another.
+// heads each, 157 us (666 MB, 4.2 TB/s; the 8-bit cache takes 213); one sequence
+// of 900 7.9 us; 3 ... 5 tokens of each of 4 sequences of 30000 ... 70000, 8
+// heads of 64, 36 us.  Scales taken from the stage by each lane: 169 for 161 of
+// the first.  Copies by the bulk engine in place of 16-byte ones: 177, since the
+// waits take more instructions than the copies; 5 blocks an SM: 195, for lack of
+// registers; two stages, since 4 blocks with the widened scales have room for no
+// more.
+// The parts are cut on the device, from all lengths (few_part): cut by the host
+// from the largest length, the last took 45 us, 24 sequences of 3000 ... 30000
+// 131 in place of 109, the first 161; the look at all lengths costs one sequence
+// of 900 0.7 us, and 64 of one length 157 in place of 149.  One wave of blocks
+// with equal stretches of all the work, a block taking the end of one part and
+// the start of the next: 182 us, and 115 in place of 82 for 200 sequences of 100
+// ... 2500, whose starts and joins then follow one another.
 #include <algorithm>
 #include <cmath>
 
@@ -114,8 +118,8 @@ __device__ __forceinline__ float q_value(const Kv4AttnArgs &a, const uint4 &x, i
 template <int D, int NT>
 struct Few4 {
     static constexpr int kRows = 8 * NT, kGroups = D / 32;
-    static constexpr int kStages = D == 128 ? 2 : 3, kBlocks = NT == 1 ? 4 : 2;  // stages of a warp, blocks an SM
-    static constexpr int kTurn = 128;                              // least tokens of a part (one token over 900: 64 8.4 us, 128 7.6)
+    static constexpr int kStages = 2, kBlocks = NT == 1 ? 4 : 2;  // stages of a warp, blocks an SM
+    static constexpr int kTurn = 128;                              // least tokens of a part (one token over 900: 64 tokens 8.4 us, 128 7.6, with parts cut by the host)
     static constexpr int kCodeBytes = 16 * D / 2;                  // of 16 tokens
     static constexpr int kScaleBytes = 16 * kGroups * 2;
     // a stage: for each 16 tokens their keys' and values' codes, then for each 16 their scales
@@ -138,6 +142,103 @@ struct Few4 {
     static __device__ __forceinline__ int column(int d) { return d; }
 };
 
+// A sequence's numbers, cut to the sizes, its tiles (of every kv head), and the keys of each in steps of 64.
+template <typename F>
+__device__ __forceinline__ void few_seq(const Kv4AttnArgs &a, int s, KvSeq &q, int &tiles, int &steps) {
+    const int r0 = a.b.row_start[s], r1 = a.b.row_start[s + 1], len = a.b.kv_len[s];
+    const int64_t cap = min(a.b.table_width << a.c.page_log2, a.b.max_len);
+    q.s = s;
+    q.r0 = min(max(r0, 0), a.b.n_rows);
+    q.n = min(min(max(r1, q.r0), a.b.n_rows) - q.r0, a.b.max_rows);
+    q.len = static_cast<int>(min(static_cast<int64_t>(max(len, 0)), cap));
+    tiles = (q.n * a.group + F::kRows - 1) / F::kRows * a.c.heads;
+    steps = max((q.len - (kv_first(a, kv_last(a, q, 0)) & ~15) + 63) / 64, 1);
+}
+
+// This block's tile and part, from all sequences' lengths.  With T tiles of W steps in all, parts of W / (S - T) steps
+// are at most S in all; S is a.splits, some waves of blocks.  Blocks 0, 1, ... take the parts in the order of the sequences,
+// their tiles and kv heads.  Sums are cut where only arrays that contradict the sizes take them.  The
+// part found is one for the block, not one for each warp, so that its numbers are held once a warp (39 us in place of 36 for
+// 3 to 5 tokens with heads of 64 otherwise).  Every thread of the block calls this; false if there is nothing to do.
+template <typename F>
+__device__ __forceinline__ bool few_part(const Kv4AttnArgs &a, FewTile &t) {
+    constexpr unsigned kCut = 1u << 24;  // 128 threads' sums stay in 32 bits
+    __shared__ unsigned s_tiles[kWarps], s_parts[kWarps];
+    __shared__ uint64_t s_steps[kWarps];
+    __shared__ KvSeq s_q;
+    __shared__ unsigned s_local;  // the part's number within the sequence
+    __shared__ int s_split;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int each = (a.b.n_seqs - 1) / (kWarps * 32) + 1;  // consecutive sequences of a thread
+    const int s0 = min(static_cast<int>(threadIdx.x) * each, a.b.n_seqs), s1 = s0 + min(each, a.b.n_seqs - s0);
+    if (blockIdx.x == gridDim.x - 1) kv_check(a.b, a.c.page_log2, false, a.err);
+    KvSeq q;
+    int tiles = 0, steps = 1;
+    uint64_t T = 0, W = 0;
+    for (int s = s0; s < s1; ++s) {
+        few_seq<F>(a, s, q, tiles, steps);
+        T += tiles, W += static_cast<uint64_t>(tiles) * steps;
+    }
+    const unsigned tw = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(min(T, static_cast<uint64_t>(kCut))));
+    const unsigned low = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(W & 0xffffu));
+    const unsigned high = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(min(W >> 16, static_cast<uint64_t>(kCut))));
+    if (lane == 0) s_tiles[warp] = tw, s_steps[warp] = (static_cast<uint64_t>(high) << 16) + low;
+    __syncthreads();
+    T = W = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) T += s_tiles[w], W += s_steps[w];
+    const unsigned S = a.splits, room = max(T < S ? S - static_cast<unsigned>(T) : 0u, S / 4);
+    W += room - 1;
+    const unsigned most = W >> 32 ? static_cast<unsigned>(W / room) : static_cast<unsigned>(W) / room;
+    const int chunk = a.chunk ? a.chunk : static_cast<int>(max(min(most, 1u << 25), F::kTurn / 64u));
+    uint64_t count = 0;
+    if (each == 1) count = static_cast<uint64_t>(tiles) * ((steps + chunk - 1) / chunk);
+    else
+        for (int s = s0; s < s1; ++s) {
+            few_seq<F>(a, s, q, tiles, steps);
+            count += static_cast<uint64_t>(tiles) * ((steps + chunk - 1) / chunk);
+        }
+    const unsigned own = static_cast<unsigned>(min(count, static_cast<uint64_t>(kCut)));
+    unsigned front = own;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, front, i);
+        if (lane >= i) front += x;
+    }
+    if (lane == 31) s_parts[warp] = front;
+    __syncthreads();
+    front -= own;
+    unsigned parts = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) front += s_parts[w];
+        parts += s_parts[w];
+    }
+    const unsigned block = blockIdx.x;
+    if (block >= parts) return false;
+    if (front <= block && block < front + own) {
+        for (int s = s0; each > 1 && s < s1; ++s) {
+            few_seq<F>(a, s, q, tiles, steps);
+            const uint64_t n = static_cast<uint64_t>(tiles) * ((steps + chunk - 1) / chunk);
+            if (block < front + n) break;
+            front += static_cast<unsigned>(n);
+        }
+        s_q = q, s_local = block - front, s_split = (steps + chunk - 1) / chunk;
+    }
+    __syncthreads();
+    t.q = s_q, t.n_split = s_split;
+    const int tile = static_cast<int>(s_local / static_cast<unsigned>(t.n_split));
+    t.split = static_cast<int>(s_local) - tile * t.n_split;
+    t.slot = static_cast<int64_t>(block) - t.split;
+    t.kv = tile % a.c.heads;
+    t.R = t.q.n * a.group;
+    t.row0 = tile / a.c.heads * F::kRows, t.i_lo = t.row0 / a.group, t.i_hi = (min(t.row0 + F::kRows, t.R) - 1) / a.group;
+    const int k_end = kv_last(a, t.q, t.i_hi) + 1, k_begin = kv_first(a, kv_last(a, t.q, t.i_lo)) & ~15;
+    t.t_begin = static_cast<int>(min(k_begin + static_cast<int64_t>(t.split) * chunk * 64, static_cast<int64_t>(max(k_end, 0))));
+    t.t_end = static_cast<int>(min(t.t_begin + static_cast<int64_t>(chunk) * 64, static_cast<int64_t>(k_end)));
+    return true;
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_few_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using F = Few4<D, NT>;
@@ -146,9 +247,10 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
     __shared__ float s_m[kWarps][F::kRows], s_l[kWarps][F::kRows];
     wait_for_stream();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int kv = blockIdx.y, G = a.group;
+    const int G = a.group;
     FewTile tile;
-    if (!few_tile<NT>(a, tile)) return;
+    if (!few_part<F>(a, tile)) return;
+    const int kv = tile.kv;
     const KvSeq &q = tile.q;
     const int row0 = tile.row0, i_lo = tile.i_lo, i_hi = tile.i_hi, R = tile.R, t_begin = tile.t_begin, t_end = tile.t_end;
     const int n_blocks = t_end > t_begin ? (t_end - t_begin + F::kTokens - 1) / F::kTokens : 0;
@@ -409,7 +511,33 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 
 template <int D, int NT>
 cudaError_t launch(Kv4AttnArgs &a, int num_sms, cudaStream_t st) {
-    return few_launch<Few4<D, NT>, NT>(kv4_attn_few_kernel<D, NT>, a, kReadyFew4 + 2 * (NT - 1) + (D == 64), num_sms, st);
+    using F = Few4<D, NT>;
+    constexpr unsigned kBit = 1u << (kReadyFew4 + 2 * (NT - 1) + (D == 64));
+    const int64_t tiles = a.c.heads * std::min(static_cast<int64_t>(a.b.n_rows) * a.group / F::kRows + a.b.n_seqs,
+                                               (static_cast<int64_t>(a.b.max_rows) * a.group + F::kRows - 1) / F::kRows * a.b.n_seqs);
+    const int64_t wave = F::kBlocks * static_cast<int64_t>(num_sms);
+    const int64_t span = std::max(a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len, int64_t(1));
+    // Waves of blocks: more even out lengths (see few_part: the parts of w waves have W / (w wave - T) steps), each costs about
+    // 10 steps of 64 tokens.  W from half of the longest, the lengths being on the device.  Measured, heads of 128, 1 and 2
+    // waves: 24 sequences of 3000 ... 30000 by 8 heads 133 and 109 us; heads of 64, 16 of 900 ... 6000 16.7 and 25.7.
+    const double work = static_cast<double>(tiles) * static_cast<double>(span) / 128;
+    int64_t waves = 1;
+    double least = 0;
+    for (int64_t w = 1; w <= 4; ++w) {
+        const double cost = static_cast<double>(w) * (work / static_cast<double>(std::max(w * wave - tiles, w * wave / 4)) + 10);
+        if (w == 1 || cost < least) least = cost, waves = w;
+    }
+    int64_t grid = std::max(waves * wave, waves * wave / 4 + tiles);
+    a.splits = static_cast<int>(waves * wave), a.chunk = 0;
+    if (grid > kMaxParts) grid = tiles, a.chunk = 1 << 25;  // no parts
+    grid = std::min(grid, tiles * ((span + F::kTurn - 1) / F::kTurn));
+    if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+    if (!(*a.ready & kBit)) {
+        const cudaError_t e = cudaFuncSetAttribute(kv4_attn_few_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+        if (e != cudaSuccess) return e;
+        *a.ready |= kBit;
+    }
+    return launch_after(kv4_attn_few_kernel<D, NT>, dim3(static_cast<unsigned>(grid)), kWarps * 32, F::kSmem, st, a);
 }
 
 }  // namespace

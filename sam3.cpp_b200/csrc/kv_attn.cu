@@ -85,6 +85,32 @@ struct Few {
     static __device__ __forceinline__ int column(int d) { return d + d / kLane * 4; }
 };
 
+// Every thread of the block calls this; false if there is nothing to do.
+template <int NT>
+__device__ __forceinline__ bool few_tile(const KvAttnArgs &a, FewTile &t) {
+    constexpr int kRows = 8 * NT;
+    const int G = a.group;
+    const unsigned unit = blockIdx.x / a.splits;
+    t.split = blockIdx.x % a.splits;
+    t.kv = blockIdx.y;
+    t.slot = (static_cast<int64_t>(unit) * a.c.heads + t.kv) * a.splits;
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, false, a.err);
+    int64_t local;
+    if (!kv_find(a.b, unit, G, NT == 1 ? 3 : 4, 1, a.c.page_log2, t.q, local)) return false;
+    t.R = t.q.n * G;  // the host keeps n_rows * G below 2^31
+    if (local * kRows >= t.R) return false;
+    t.row0 = static_cast<int>(local) * kRows, t.i_lo = t.row0 / G, t.i_hi = (min(t.row0 + kRows, t.R) - 1) / G;
+
+    // the tile's keys, and this block's part of them
+    const int k_end = kv_last(a, t.q, t.i_hi) + 1, k_begin = kv_first(a, kv_last(a, t.q, t.i_lo)) & ~15;
+    const int range = max(k_end - k_begin, 0);
+    const int chunk = max(range < a.short_range ? a.chunk_short : a.chunk, ((range + a.splits - 1) / a.splits + 63) & ~63);
+    t.n_split = max((range + chunk - 1) / chunk, 1);
+    if (t.split >= t.n_split) return false;
+    t.t_begin = k_begin + t.split * chunk, t.t_end = min(t.t_begin + chunk, k_end);
+    return true;
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_few_kernel(const __grid_constant__ KvAttnArgs a) {
     using F = Few<D, NT>;
@@ -317,6 +343,37 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
         }
     __syncthreads();
     few_finish<F, D>(a, tile, smem, s_m, s_l);
+}
+
+constexpr int kMaxSplits = 256;  // most parts of a key range
+
+// The parts of a key range and the launch; `bit`: the kernel's of a.ready.
+template <typename F, int NT>
+cudaError_t few_launch(void (*kernel)(KvAttnArgs), KvAttnArgs &a, unsigned bit, int num_sms, cudaStream_t st) {
+    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> (NT == 1 ? 3 : 4)) + a.b.n_seqs;
+    // parts for two waves where there are few sequences and heads, for four where the lengths of many have to even out
+    const int64_t wave = F::kBlocks * static_cast<int64_t>(num_sms), groups = units * a.c.heads;
+    const int64_t span =
+        std::max(a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len, int64_t(1));
+    int64_t splits = 2 * groups < wave ? (2 * wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
+    // a block's least part: a turn of its warps while the blocks fit in one wave, else 256
+    const int64_t least = groups * ((span + F::kTurn - 1) / F::kTurn) <= wave ? F::kTurn : 256;
+    splits = std::min(splits, (span + least - 1) / least);
+    splits = std::min(splits, std::min(static_cast<int64_t>(kMaxParts) / groups, static_cast<int64_t>(kMaxSplits)));
+    splits = std::max(splits, static_cast<int64_t>(1));
+    if (units * splits > 0x7fffffff) return cudaErrorInvalidValue;
+    a.splits = static_cast<int>(splits);
+    a.chunk = static_cast<int>(((span + splits - 1) / splits + 63) & ~int64_t(63));
+    // With few sequences one that is far shorter than max_len (a captured step's bound) is cut finer, into all parts.
+    a.chunk_short = static_cast<int>(2 * groups < wave ? std::min<int64_t>(least, a.chunk) : a.chunk);
+    a.short_range = static_cast<int>(span / 2);
+    if (!(*a.ready & (1u << bit))) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+        if (e != cudaSuccess) return e;
+        *a.ready |= 1u << bit;
+    }
+    const dim3 grid(static_cast<unsigned>(units * a.splits), a.c.heads);
+    return launch_after(kernel, grid, kWarps * 32, F::kSmem, st, a);
 }
 
 template <int D, int NT>

@@ -11,40 +11,16 @@
 namespace b200 {
 
 constexpr int kWarps = 4;
-constexpr int kMaxSplits = 256;  // most parts of a key range
 
 // A block's rows and keys.
 struct FewTile {
     KvSeq q;
-    unsigned unit;
-    int split, n_split;
+    int kv;
+    int split, n_split;       // which part of the tile's keys this is, of how many
+    int64_t slot;             // the tile's first part in the workspace, and its counter
     int R, row0, i_lo, i_hi;  // rows of the sequence, this tile's first, its first and last token
     int t_begin, t_end;       // this block's part of the tile's keys
 };
-
-// Every thread of the block calls this; false if there is nothing to do.
-template <int NT, typename Args>
-__device__ __forceinline__ bool few_tile(const Args &a, FewTile &t) {
-    constexpr int kRows = 8 * NT;
-    const int G = a.group;
-    t.unit = blockIdx.x / a.splits;
-    t.split = blockIdx.x % a.splits;
-    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) kv_check(a.b, a.c.page_log2, false, a.err);
-    int64_t local;
-    if (!kv_find(a.b, t.unit, G, NT == 1 ? 3 : 4, 1, a.c.page_log2, t.q, local)) return false;
-    t.R = t.q.n * G;  // the host keeps n_rows * G below 2^31
-    if (local * kRows >= t.R) return false;
-    t.row0 = static_cast<int>(local) * kRows, t.i_lo = t.row0 / G, t.i_hi = (min(t.row0 + kRows, t.R) - 1) / G;
-
-    // the tile's keys, and this block's part of them
-    const int k_end = kv_last(a, t.q, t.i_hi) + 1, k_begin = kv_first(a, kv_last(a, t.q, t.i_lo)) & ~15;
-    const int range = max(k_end - k_begin, 0);
-    const int chunk = max(range < a.short_range ? a.chunk_short : a.chunk, ((range + a.splits - 1) / a.splits + 63) & ~63);
-    t.n_split = max((range + chunk - 1) / chunk, 1);
-    if (t.split >= t.n_split) return false;
-    t.t_begin = k_begin + t.split * chunk, t.t_end = min(t.t_begin + chunk, k_end);
-    return true;
-}
 
 // The end of a block: its warps' rows (sums in `smem` as [warp][row][F::kRowFloats], dimension d at F::column(d);
 // maxima and sums of weights in s_m and s_l) are joined, the parts of the key range by the last block to finish, and
@@ -53,9 +29,8 @@ template <typename F, int D, typename Args>
 __device__ __forceinline__ void few_finish(const Args &a, const FewTile &t, uint8_t *smem, const float (&s_m)[kWarps][F::kRows],
                                            const float (&s_l)[kWarps][F::kRows]) {
     __shared__ int s_last;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = blockIdx.y, G = a.group;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kv = t.kv, G = a.group;
     const int row0 = t.row0, R = t.R, split = t.split, n_split = t.n_split;
-    const unsigned unit = t.unit;
     const KvSeq &q = t.q;
     float *rows = reinterpret_cast<float *>(smem);
     constexpr int kEach = F::kEach, kPer = D / kEach;  // threads a row
@@ -78,9 +53,8 @@ __device__ __forceinline__ void few_finish(const Args &a, const FewTile &t, uint
         }
     }
     if (n_split > 1) {
-        const int64_t group = static_cast<int64_t>(unit) * a.c.heads + kv;
-        float *base = a.part + group * a.splits * F::kRows * (D + 2);
-        float *ml = base + static_cast<int64_t>(a.splits) * F::kRows * D;
+        float *base = a.part + t.slot * F::kRows * (D + 2);
+        float *ml = base + static_cast<int64_t>(n_split) * F::kRows * D;
         if (live) {
             float *to = base + (static_cast<int64_t>(split) * F::kRows + row) * D + d0;
 #pragma unroll
@@ -91,7 +65,7 @@ __device__ __forceinline__ void few_finish(const Args &a, const FewTile &t, uint
         __syncthreads();
         if (threadIdx.x == 0) {
             __threadfence();
-            s_last = atomicInc(a.done + group, n_split - 1) == static_cast<unsigned>(n_split - 1);
+            s_last = atomicInc(a.done + t.slot, n_split - 1) == static_cast<unsigned>(n_split - 1);
             __threadfence();
         }
         __syncthreads();
@@ -162,35 +136,6 @@ __device__ __forceinline__ void few_finish(const Args &a, const FewTile &t, uint
         for (int k = 0; k < 8; ++k) v[k] = sum[i + k] * inv;
         kv_store8(a, at + i, v);
     }
-}
-
-// The parts of a key range and the launch; `bit`: the kernel's of a.ready.
-template <typename F, int NT, typename Args>
-cudaError_t few_launch(void (*kernel)(Args), Args &a, unsigned bit, int num_sms, cudaStream_t st) {
-    const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> (NT == 1 ? 3 : 4)) + a.b.n_seqs;
-    // parts for two waves where there are few sequences and heads, for four where the lengths of many have to even out
-    const int64_t wave = F::kBlocks * static_cast<int64_t>(num_sms), groups = units * a.c.heads;
-    const int64_t span =
-        std::max(a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len, int64_t(1));
-    int64_t splits = 2 * groups < wave ? (2 * wave + groups - 1) / groups : (4 * wave + groups - 1) / groups;
-    // a block's least part: a turn of its warps while the blocks fit in one wave, else 256
-    const int64_t least = groups * ((span + F::kTurn - 1) / F::kTurn) <= wave ? F::kTurn : 256;
-    splits = std::min(splits, (span + least - 1) / least);
-    splits = std::min(splits, std::min(static_cast<int64_t>(kMaxParts) / groups, static_cast<int64_t>(kMaxSplits)));
-    splits = std::max(splits, static_cast<int64_t>(1));
-    if (units * splits > 0x7fffffff) return cudaErrorInvalidValue;
-    a.splits = static_cast<int>(splits);
-    a.chunk = static_cast<int>(((span + splits - 1) / splits + 63) & ~int64_t(63));
-    // With few sequences one that is far shorter than max_len (a captured step's bound) is cut finer, into all parts.
-    a.chunk_short = static_cast<int>(2 * groups < wave ? std::min<int64_t>(least, a.chunk) : a.chunk);
-    a.short_range = static_cast<int>(span / 2);
-    if (!(*a.ready & (1u << bit))) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
-        if (e != cudaSuccess) return e;
-        *a.ready |= 1u << bit;
-    }
-    const dim3 grid(static_cast<unsigned>(units * a.splits), a.c.heads);
-    return launch_after(kernel, grid, kWarps * 32, F::kSmem, st, a);
 }
 
 }  // namespace b200
