@@ -475,6 +475,23 @@ def test_kv4_attention_long_contexts_in_parts(b200, backend, attend, rows):
         check_attention(dev, attend, q[:rows], "bf16", start[:2], lens[:1], 4, 128 ** -0.5, max_len=bound)
 
 
+@pytest.mark.parametrize("S,H,D,rows", [(129, 2, 128, 1), (300, 1, 64, 3), (1200, 8, 64, 2), (257, 3, 128, 9)])
+def test_kv4_attention_many_sequences(b200, backend, attend, S, H, D, rows):
+    """More sequences than a block has threads, some without rows, one far longer than the others, so that most blocks
+    have parts of it; more tiles than the workspace has parts."""
+    rng = np.random.default_rng(S)
+    lens = rng.integers(0, 40, S)
+    lens[S // 2], lens[-1] = 9000, 3000
+    n = rng.integers(0, rows + 1, S)
+    n[[0, S // 2, S - 1]] = 0, rows, 1
+    start = np.concatenate([[0], np.cumsum(n)])
+    dev = filled(b200, backend, lens, 16, D, H)
+    q = store(rng.normal(size=(start[-1], H, D)) * 2, "f16")
+    check_attention(dev, attend, q, "f16", start, lens, H, D ** -0.5)
+    check_attention(dev, attend, q, "f16", start, lens, H, D ** -0.5, window=700)
+    check_attention(dev, attend, q, "f16", start, lens, H, D ** -0.5, max_len=1 << 30)
+
+
 @pytest.mark.parametrize("rows", [2, 150])
 def test_kv4_attention_views_and_rows_outside_sequences(b200, backend, attend, rows):
     """Queries inside a fused projection's rows, outputs with heads outside, unaligned data; rows in front of the first and
