@@ -20,11 +20,12 @@ struct KvAttnArgsOf {
     int group;            // query heads of a kv head
     float scale_log2;     // scale * log2(e)
     int causal, window;   // window 0: none
-    int splits;           // most parts of a key range
-    int chunk;            // least tokens of a part (a multiple of 64, for 256 rows of 128)
+    int splits;           // most parts of a key range (few rows over 4 bits: of all key ranges)
+    int chunk;            // least tokens of a part (a multiple of 64, for 256 rows of 128; few rows over 4 bits: steps of
+                          // 64 tokens, 0: the kernel's choice)
     int chunk_short, short_range;  // the same for key ranges below short_range
     float *part;          // partial results: see kPartFloats
-    unsigned *done;       // parts finished, one counter a unit and kv head; 0 between calls
+    unsigned *done;       // parts finished, one counter for each set of parts; 0 between calls
     int *err;
     unsigned *ready;      // host: kernels whose attributes are set on the device
 };

@@ -1,6 +1,6 @@
 // kv_attn_few.cuh -- what the kernels for few query rows a kv head share over
-// the caches of 8 and 4 bits: which rows and keys a block has, how its warps'
-// partial results and the parts of a key range are joined, and the launch.
+// the caches of 8 and 4 bits: how a block's warps' partial results and the
+// parts of a key range are joined.
 #pragma once
 
 #include <algorithm>
