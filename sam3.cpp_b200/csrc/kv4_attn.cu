@@ -513,8 +513,9 @@ template <int D, int NT>
 cudaError_t launch(Kv4AttnArgs &a, int num_sms, cudaStream_t st) {
     using F = Few4<D, NT>;
     constexpr unsigned kBit = 1u << (kReadyFew4 + 2 * (NT - 1) + (D == 64));
-    const int64_t tiles = a.c.heads * std::min(static_cast<int64_t>(a.b.n_rows) * a.group / F::kRows + a.b.n_seqs,
-                                               (static_cast<int64_t>(a.b.max_rows) * a.group + F::kRows - 1) / F::kRows * a.b.n_seqs);
+    // (a batch without rows has one too: its arrays are checked)
+    const int64_t most = (static_cast<int64_t>(a.b.max_rows) * a.group + F::kRows - 1) / F::kRows * a.b.n_seqs;
+    const int64_t tiles = a.c.heads * std::max(std::min(static_cast<int64_t>(a.b.n_rows) * a.group / F::kRows + a.b.n_seqs, most), int64_t(1));
     const int64_t wave = F::kBlocks * static_cast<int64_t>(num_sms);
     const int64_t span = std::max(a.window ? std::min(a.b.max_len, static_cast<int64_t>(a.window) + a.b.max_rows + 16) : a.b.max_len, int64_t(1));
     // Waves of blocks: more even out lengths (see few_part: the parts of w waves have W / (w wave - T) steps), each costs about

@@ -475,6 +475,21 @@ def test_kv4_attention_long_contexts_in_parts(b200, backend, attend, rows):
         check_attention(dev, attend, q[:rows], "bf16", start[:2], lens[:1], 4, 128 ** -0.5, max_len=bound)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_kv4_attention_batches_without_rows(b200, backend, attend, D):
+    """Rows that no sequence owns stay as they are; the arrays are checked all the same."""
+    dev = filled(b200, backend, [30, 5], 16, D, 2)
+    q, y = backend.upload(np.zeros((4, 2, D), np.float16)), backend.upload(np.full((4, 2, D), 7, np.float16))
+    attend.run(dev.cache, dev.batch([0, 0, 0], [30, 5], n_rows=4), TYPES["f16"], q.ptr, 2, y.ptr, 0.1)
+    backend.synchronize()
+    assert np.all(y.get((4, 2, D), np.float16) == 7)
+    b = dev.batch([0, 1, 1], [30, 5], n_rows=4)
+    b.max_rows = 0
+    attend.run(dev.cache, b, TYPES["f16"], q.ptr, 2, y.ptr, 0.1)
+    with pytest.raises(b200.B200Error, match="contradicts"):
+        backend.synchronize()
+
+
 @pytest.mark.parametrize("S,H,D,rows", [(129, 2, 128, 1), (300, 1, 64, 3), (1200, 8, 64, 2), (257, 3, 128, 9)])
 def test_kv4_attention_many_sequences(b200, backend, attend, S, H, D, rows):
     """More sequences than a block has threads, some without rows, one far longer than the others, so that most blocks
