@@ -344,7 +344,8 @@ typedef struct sam3b200_kv_cache {
  * contents); the sizes are the host's bounds on them.  Contents that
  * contradict the sizes, or a page outside [0, n_pages), make the next
  * sam3b200_backend_synchronize fail; nothing is then accessed out of range,
- * and the results of the sequences concerned are undefined.  Rows in front of
+ * the results of the sequences concerned (of the whole batch where row_start
+ * falls) are undefined, and handles stay as they were.  Rows in front of
  * row_start[0] and behind row_start[n_seqs] are not touched. */
 typedef struct sam3b200_kv_batch {
     const int32_t *table;     /* device [n_seqs][table_width] */

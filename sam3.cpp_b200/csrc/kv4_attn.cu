@@ -157,7 +157,10 @@ __device__ __forceinline__ void few_seq(const Kv4AttnArgs &a, int s, KvSeq &q, i
 
 // This block's tile and part, from all sequences' lengths.  With T tiles of W steps in all, parts of W / (S - T) steps
 // are at most S in all; S is a.splits, some waves of blocks.  Blocks 0, 1, ... take the parts in the order of the sequences,
-// their tiles and kv heads.  Sums are cut where only arrays that contradict the sizes take them.  The
+// their tiles and kv heads.  Sums are cut where only arrays that contradict the sizes take them.  Runs of rows that follow one
+// another make no more tiles than the host counted, so that the parts are at most the blocks; where row_start falls they
+// can be more, and then no block does anything, since a tile of which only some parts ran would leave its counter above 0 for
+// the calls to come.  The
 // part found is one for the block, not one for each warp, so that its numbers are held once a warp (39 us in place of 36 for
 // 3 to 5 tokens with heads of 64 otherwise).  Every thread of the block calls this; false if there is nothing to do.
 template <typename F>
@@ -215,7 +218,7 @@ __device__ __forceinline__ bool few_part(const Kv4AttnArgs &a, FewTile &t) {
         parts += s_parts[w];
     }
     const unsigned block = blockIdx.x;
-    if (block >= parts) return false;
+    if (block >= parts || parts > gridDim.x) return false;  // (kv_check names the starts that fall)
     if (front <= block && block < front + own) {
         for (int s = s0; each > 1 && s < s1; ++s) {
             few_seq<F>(a, s, q, tiles, steps);

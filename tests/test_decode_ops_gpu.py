@@ -490,6 +490,63 @@ def test_kv4_attention_batches_without_rows(b200, backend, attend, D):
         backend.synchronize()
 
 
+def handle_is_whole(b200, backend, handle, D):
+    """Valid calls whose key ranges are cut into 2 and 3 parts, which between them use the first hundred counters of a
+    handle as the first of a tile: each against the oracle."""
+    rng = np.random.default_rng(D)
+    for lens in ([200] * 50, [100] + [200] * 50, [300] * 34, [100] + [300] * 34, [200] + [300] * 34):
+        dev = filled(b200, backend, lens, 16, D, 1)
+        q = store(rng.normal(size=(len(lens), 1, D)), "f16")
+        check_attention(dev, handle, q, "f16", np.arange(len(lens) + 1), lens, 1, 0.1)
+
+
+@pytest.mark.parametrize("lens", [[200] + [300] * 11, [200] * 6 + [300] * 6])
+def test_kv4_falling_starts_leave_the_handle_whole(b200, backend, lens):
+    """Runs of rows that lie over one another, which make more parts than the host counted on: an error, and the calls
+    behind it find every counter as it was."""
+    D, rows = 64, 48
+    dev = filled(b200, backend, lens, 16, D, 1)
+    handle = backend.kv_attention()
+    b = dev.batch([0, 16] + [0, rows] * 5 + [0], lens, n_rows=rows)
+    b.max_rows = rows
+    q, y = backend.upload(np.zeros((rows, 1, D), np.float16)), backend.upload(np.full((rows + 8, 1, D), 7, np.float16))
+    for _ in range(2):
+        handle.run(dev.cache, b, TYPES["f16"], q.ptr, 1, y.ptr, 0.1)
+        with pytest.raises(b200.B200Error, match="contradicts"):
+            backend.synchronize()
+        handle_is_whole(b200, backend, handle, D)
+    assert np.all(y.get((rows + 8, 1, D), np.float16)[rows:] == 7)
+    handle.free()
+
+
+@pytest.mark.parametrize("D,G,most", [(64, 1, 5), (64, 2, 24), (128, 2, 8)])
+def test_kv4_bad_batches_of_few_rows(b200, backend, D, G, most):
+    """The bad tables, lengths and starts by as few rows as the few-row kernel takes, over several parts: each is reported,
+    nothing outside is touched, and the handle goes on."""
+    P, rows = 16, 64
+    host = do.kv4_empty(40, 1, P, D)
+    good = np.arange(40).reshape(2, 20)
+    bad = good.copy()
+    bad[0, 3], bad[1, 19] = 40, -1
+    handle = backend.kv_attention()
+    q, y = backend.upload(np.zeros((rows, G, D), np.float16)), backend.upload(np.full((rows + 8, G, D), 7, np.float16))
+    for table, row_start, kv_len, why in ((bad, [0, 5, 10], [320, 320], "page index"), (good, [0, most, most + 2], [320, 2000], "contradicts"),
+                                          (good, [0, 3, 5], [-3, 300], "contradicts"), (good, [-4, 5, 9], [320, 300], "contradicts"),
+                                          (good, [0, 5, 400], [320, 320], "contradicts"), (good, [0, 5, 2], [320, 320], "contradicts"),
+                                          (good, [60, 5, 64], [320, 310], "contradicts"), (good, [0, most + 1, most + 2], [320, 200], "contradicts")):
+        dev = Device(b200, backend, host, table)
+        b = dev.batch(row_start, kv_len, n_rows=rows, max_len=320)
+        b.max_rows = most
+        for window in (0, 30):
+            handle.run(dev.cache, b, TYPES["f16"], q.ptr, G, y.ptr, 0.1, window=window)
+            with pytest.raises(b200.B200Error, match=why):
+                backend.synchronize()
+            backend.synchronize()
+        handle_is_whole(b200, backend, handle, D)
+    assert np.all(y.get((rows + 8, G, D), np.float16)[rows:] == 7)
+    handle.free()
+
+
 @pytest.mark.parametrize("S,H,D,rows", [(129, 2, 128, 1), (300, 1, 64, 3), (1200, 8, 64, 2), (257, 3, 128, 9)])
 def test_kv4_attention_many_sequences(b200, backend, attend, S, H, D, rows):
     """More sequences than a block has threads, some without rows, one far longer than the others, so that most blocks
