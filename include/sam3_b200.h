@@ -193,7 +193,8 @@ int sam3b200_mul_mat_dq16(sam3b200_backend *be, const sam3b200_weight *w, const 
  * as they are; BF16, and F32 as a sum of two, in f16 after a power of two a row:
  * 2^-23 of an F32 element, and 2^-26 of the row's largest one where that is at
  * least 2^-112, may be lost), a block's sum is scaled and added in f32, in an
- * order that the shapes fix, and rounded once to y_type.  The
+ * order that the shapes fix, and rounded once to y_type.  Infinities and NaN
+ * give what the sum of their products with w[n][k] is.  The
  * weights are the handle's own codes, with their scales a second time in 2
  * (Q4_1: 4) bytes a block, made by sam3b200_weight_upload.  Other weight types
  * and more rows are refused with an error: sam3b200_mul_mat takes them.

@@ -14,7 +14,7 @@
 // scaling the sums, 162 instructions a warp for 1 KB of codes (62 % of the issue
 // slots), is what comes next.  Measured: 49408 x 4096 Q4_0 by one row of f16 25.1
 // us (114 MB, 4.5 TB/s; 25.8 with blocks cut at whole tiles), 14339 x 4096 Q4_1 by
-// 6 rows of bf16 15.5 us, of which the launch, the staging of x and the end are
+// 6 rows of bf16 15.8 us, of which the launch, the staging of x and the end are
 // some 6.  Chunks dealt to the warps of a tile in turn, joined tile by tile, took
 // 28.7 us in place of 25.8; scales widened once
 // a warp through shared memory, for arithmetic on pairs, 26.6 (Q4_1 17 for 15.2).
@@ -117,6 +117,32 @@ __device__ __forceinline__ float f16_of(float v, float &rest) {
     const float h = __half2float(__float2half_rn(v));
     rest = fabsf(h) <= 65504.f ? v - h : 0.f;
     return h;
+}
+
+// The results of rows of x with infinities and NaN for rows n0 ... n1 - 1 of Q4_1 weights: what these elements' products with
+// d code + m add up to, infinite or NaN, whatever the finite elements are.  Called by a block.
+template <typename TX>
+__device__ __noinline__ void odd_rows(const VecArgs &a, int n0, int n1) {
+    for (int id = threadIdx.x; id < (n1 - n0) * a.M; id += kThreads) {
+        const int m = id / (n1 - n0), n = n0 + id % (n1 - n0);
+        const TX *x = static_cast<const TX *>(a.x) + m * a.ldx;
+        const uint8_t *codes = a.codes + static_cast<int64_t>(n) * (a.K / 2);
+        const __half *scales = reinterpret_cast<const __half *>(a.scales) + static_cast<int64_t>(n >> 4) * a.chunks * 128 + (n & 15) * 4;
+        bool any = false;
+        float sum = 0.f;
+        for (int k = 0; k < a.K; ++k) {
+            const float v = to_f32(x[k]);
+            if (fabsf(v) <= kF32Max) continue;
+            const int b = k >> 5, code = codes[b * 16 + (k & 15)] >> (k & 16 ? 4 : 0) & 15;
+            const __half *d = scales + (b >> 2) * 128 + (b & 3);
+            sum += fmaf(to_f32(d[0]), static_cast<float>(code), to_f32(d[64])) * v;  // d code is exact, so the sign and 0 are right
+            any = true;
+        }
+        if (!any) continue;
+        if (a.bias) sum += a.bias[n];
+        if (a.y_type == SAM3B200_TYPE_F32) static_cast<float *>(a.y)[m * a.ldy + n] = sum;
+        else static_cast<TX *>(a.y)[m * a.ldy + n] = from_f32<TX>(sum);
+    }
 }
 
 template <int NT, int RT, bool MINS, typename TX>
@@ -404,9 +430,11 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
                 acc[r][n][0] += v.x, acc[r][n][1] += v.y, acc[r][n][2] += v.z, acc[r][n][3] += v.w;
             }
     };
+    bool odd = false;  // this thread has a result that is no finite number
     auto store = [&](int m, int n, float v) {
         if (m >= a.M || n >= row_end) return;
         if (kScaled) v *= s_up[m];
+        if (MINS) odd = odd || !(fabsf(v) <= kF32Max);
         if (a.bias) v += a.bias[n];
         const int64_t at = m * a.ldy + n;
         if (a.y_type == SAM3B200_TYPE_F32) static_cast<float *>(a.y)[at] = v;
@@ -478,6 +506,10 @@ __global__ void __launch_bounds__(kThreads, 1) mul_mat_vec_kernel(const __grid_c
         }
     }
     cp_wait<0>();
+    // An infinity or NaN in a row of x makes all its results infinite or NaN (and no other row's), but d (sum code x) +
+    // m (sum x) not those of (d code + m) x: a code of 0 makes NaN of an infinity, and so do unlike signs of d code and m.  So
+    // the results are looked at (6 rows by 14339 x 4096 15.75 us for 15.55; a look at x as it is staged: 16.5).
+    if (MINS && __syncthreads_or(odd)) odd_rows<TX>(a, u0 * 16, row_end);
 }
 
 // ggml blocks -> the scales (Q4_1: and minima) of 16 rows by 4 blocks side by side, zeros behind the weights.

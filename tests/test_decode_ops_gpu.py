@@ -843,6 +843,60 @@ def test_vec_extreme_values(b200, backend, kind, t):
         check_vec(b200, backend, raw, kind, N, K, store(x, t), t, "f32")
 
 
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("t,t_out", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("N,K,M", [(50, 256, 3), (301, 4128, 9), (33, 16384 + 96, 16)])
+def test_vec_elements_that_are_not_numbers(b200, backend, kind, t, t_out, N, K, M):
+    """Infinities alone, several of one sign and of both, NaN, beside finite elements of usual size and not, with weights
+    above, below and exactly 0: the result is the definition's, sign and all, and rows without any are as ever."""
+    rng = np.random.default_rng(K)
+    raw = do.blocks(rng, kind, N, K)
+    if kind == "q4_1":  # minima that are a whole number of steps, so that some weights are exactly 0
+        d = np.float16(2.0) ** rng.integers(-6, -2, len(raw)).astype(np.float16) * rng.choice([-1, 1], len(raw)).astype(np.float16)
+        raw[:, :2] = d[:, None].view(np.uint8)
+        raw[:, 2:4] = (d * rng.integers(-15, 1, len(raw)).astype(np.float16))[:, None].view(np.uint8)
+    assert (do.weight(raw, kind, N, K) == 0).any()
+    w = backend.weight(b200.TYPE_Q4_0 if kind == "q4_0" else b200.TYPE_Q4_1, raw, K, N)
+    plain = store(rng.normal(size=(M, K)), t)
+    bias = rng.normal(size=N).astype(np.float32)
+    usual = check_vec(b200, backend, raw, kind, N, K, plain, t, t_out, bias=bias, handle=w)
+    for size in (1.0,) if t == "f16" else (1.0, 1e20):
+        x = rng.normal(size=(M, K)) * size
+        places = [rng.choice(K, 12, replace=False) for _ in range(3)]
+        x[0, places[0][0]] = np.inf
+        x[M - 1, places[1][:2]] = -np.inf
+        x[M // 2, places[2][:6]] = rng.choice([np.inf, -np.inf], 6)
+        got = check_vec(b200, backend, raw, kind, N, K, store(x, t), t, t_out, bias=bias, handle=w)
+        with np.errstate(invalid="ignore"):
+            want = value(store(x, t), t) @ do.weight(raw, kind, N, K).T
+        odd = [0, M // 2, M - 1]
+        assert np.isinf(want[0]).any() and np.isnan(want[0]).any()
+        assert np.array_equal(value(got, t_out)[odd], want[odd], equal_nan=True)
+        x = rng.normal(size=(M, K))
+        x[:, 3] = np.nan
+        x[0], x[1] = value(plain, t)[0], np.inf
+        got = check_vec(b200, backend, raw, kind, N, K, store(x, t), t, t_out, bias=bias, handle=w)
+        assert np.array_equal(got[0], usual[0]) and np.isnan(value(got, t_out)[2:]).all()
+    w.free()
+
+
+@pytest.mark.parametrize("kind", ["q4_0", "q4_1"])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_vec_sums_past_the_range(b200, backend, kind, t):
+    """Finite elements whose sum no f32 holds give infinities of its sign."""
+    N, K = 40, 128
+    raw = do.blocks(np.random.default_rng(8), kind, N, K, size=0.5)
+    sign = np.sign(do.weight(raw, kind, N, K))
+    x = store(np.stack([sign[3], -sign[7], sign[0] * 1e-38]) * 3e38, t)
+    xb, yb, w = backend.upload(x), backend.alloc(3 * N * 4), backend.weight(b200.TYPE_Q4_0 if kind == "q4_0" else b200.TYPE_Q4_1, raw, K, N)
+    backend.mul_mat_vec(w, xb.ptr, TYPES[t], 3, yb.ptr, b200.TYPE_F32)
+    backend.synchronize()
+    got, want = yb.get((3, N), np.float32), value(x, t) @ do.weight(raw, kind, N, K).T
+    past, within = np.abs(want) > 2.0 ** 128, np.abs(want) < 2.0 ** 127
+    assert past[0, 3] and past[1, 7] and np.array_equal(got[past], np.sign(want[past]) * np.inf) and np.isfinite(got[within]).all()
+    w.free()
+
+
 def test_vec_beside_the_other_products(b200, backend, model):
     """One handle serves mul_mat, mul_mat_dq16 and mul_mat_vec; activations that Q8_0 holds exactly give the same sums up to
     f32; results repeat bit for bit."""
