@@ -9,10 +9,11 @@
 //   O(d) = sum over tokens of (p dv(token, g(d))) cv
 // The first takes a multiply-add in f32 a token and group behind two 16-wide
 // products.  The second takes one softmax weight a group: p dv is rounded to
-// f16 (2^-11 of it).  With m the running maximum of t + log2(|dv|), t = score
-// scale log2(e) and |dv| the largest of the scales next to it, the weights
-// p = 2^(t - m) stay in f32 and p dv stays in [-1, 1] for f16 whatever the
-// scales are; O and the sum of p have the same reference, so y = O / l.
+// f16 (2^-11 of it).  With t = score scale log2(e), 2^e the power of two above
+// the largest |dv| of a block of tokens, and m the running maximum of t + e, the
+// weights p = 2^(t + e - m) and the scales dv / 2^e stay within [-1, 1] for f16
+// whatever the scales are, and only tokens that count for nothing leave them;
+// the sum of the weights l takes p / 2^e, so it has the reference of O, and y = O / l.
 //
 // The kernel is kv_attn.cu's otherwise: one block of 4 warps per (8 or 16
 // query rows of a kv head, part of the key range), blocks of 32 tokens (heads of 64: 64; in
@@ -54,12 +55,6 @@ namespace {
 
 __device__ __forceinline__ float low_bf16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-
-__device__ __forceinline__ float lg2_approx(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // The largest of three numbers (NaN is none).
 __device__ __forceinline__ float max3(float x, float y, float z) {
@@ -365,23 +360,32 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
 
         // the scales: a lane a token (heads of 64: two); those of values that no row sees are 0
         unsigned top_bits = __float_as_uint(kZeroScale);
+        float dv[F::kTokens / 32][kGroups];
 #pragma unroll
         for (int u = 0; u < F::kTokens / 32; ++u) {
             const int k = lane + 32 * u;
             const uint8_t *from = st + F::kScaleAt + k / 16 * (2 * F::kScaleBytes) + k % 16 * (2 * kGroups);
-            float dk[kGroups], dv[kGroups];
+            float dk[kGroups];
             scales_of<kGroups>(from, dk);
-            scales_of<kGroups>(from + F::kScaleBytes, dv);
+            scales_of<kGroups>(from + F::kScaleBytes, dv[u]);
             const bool out = tok + k >= t_end || tok + k < first_any;
 #pragma unroll
             for (int i = 0; i < kGroups; i += 2) {
-                if (out) dv[i] = dv[i + 1] = 0.f;
-                top_bits = max(top_bits, max(__float_as_uint(fabsf(dv[i])), __float_as_uint(fabsf(dv[i + 1]))));
+                if (out) dv[u][i] = dv[u][i + 1] = 0.f;
+                top_bits = max(top_bits, max(__float_as_uint(fabsf(dv[u][i])), __float_as_uint(fabsf(dv[u][i + 1]))));
                 wide[i / 2 * F::kTokens + k] = make_float4(dk[i], dk[i], dk[i + 1], dk[i + 1]);
-                wide[(kGroups + i) / 2 * F::kTokens + k] = make_float4(dv[i], dv[i], dv[i + 1], dv[i + 1]);
             }
         }
-        const float top_d = __uint_as_float(__reduce_max_sync(0xffffffffu, top_bits));
+        // 2^e above all of them, and 2^-e
+        const int top_e = min(static_cast<int>(__reduce_max_sync(0xffffffffu, top_bits) >> 23), 252);
+        const float lv = static_cast<float>(top_e - 126), down = __int_as_float((253 - top_e) << 23);
+#pragma unroll
+        for (int u = 0; u < F::kTokens / 32; ++u)
+#pragma unroll
+            for (int i = 0; i < kGroups; i += 2) {
+                const float x = dv[u][i] * down, y = dv[u][i + 1] * down;
+                wide[(kGroups + i) / 2 * F::kTokens + lane + 32 * u] = make_float4(x, x, y, y);
+            }
         __syncwarp();
 
         // scores of tokens 16 h + g (t[h][n][0], [1]) and 16 h + g + 8 ([2], [3]) for rows 8 n + 2 c, + 1
@@ -412,7 +416,6 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
                 }
             }
         }
-        const float lv = lg2_approx(top_d);
         if (tok + F::kTokens - 1 > seen_by_all || tok < window_end) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -457,15 +460,21 @@ __global__ void __launch_bounds__(kWarps * 32, (Few4<D, NT>::kBlocks)) kv4_attn_
                     for (int i = 0; i < D / 16; ++i) o[n][i][k] *= alpha, o[n][i][k + 2] *= alpha;
                 }
         }
+        float sum[NT][2], add[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) sum[n][k] = 0.f, add[n][k] = lv - less[n][k];
 #pragma unroll
         for (int h = 0; h < F::kSixteens; ++h) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    t[h][n][k] = ex2_approx(fmaf(t[h][n][k], row_c[n][k], -less[n][k]));
-                    t[h][n][k + 2] = ex2_approx(fmaf(t[h][n][k + 2], row_c[n][k], -less[n][k]));
-                    l[n][k] += t[h][n][k] + t[h][n][k + 2];
+                    t[h][n][k] = ex2_approx(fmaf(t[h][n][k], row_c[n][k], add[n][k]));
+                    t[h][n][k + 2] = ex2_approx(fmaf(t[h][n][k + 2], row_c[n][k], add[n][k]));
+                    sum[n][k] += t[h][n][k] + t[h][n][k + 2];
+                    if (h == F::kSixteens - 1) l[n][k] = fmaf(sum[n][k], down, l[n][k]);
                 }
             // values: of each group 4 dimensions (4 g ...) of tokens 2c, 2c + 1 and of 8 + 2c, 9 + 2c
             uint32_t w[2][kGroups];

@@ -610,6 +610,35 @@ def test_kv4_attention_extreme_values(b200, backend, attend, t, rows, size):
         check_attention(dev, attend, store(x * 1e-30, t), t, start, lens, 2, 1e30, **kw)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,rows", [(1, 1), (600, 1), (600, 5), (8, 70)])
+@pytest.mark.parametrize("power", [-90, 0, 100, 115, 120, 124])
+def test_kv4_light_tokens_count_at_every_size(b200, backend, attend, D, S, rows, power):
+    """16000 tokens whose value scales are all next to 2^power, read by one sequence and by so many that parts of it are
+    long: weights spread over many powers of two, and peaks with hundreds of light tokens around each, whose values differ in
+    their mean.  The sum of the weights must not lose what the results keep, nor the results what the sum keeps."""
+    rng = np.random.default_rng(rows)
+    N, P = 16000, 128
+    table, n = pages_for([N], P)
+    dev = Device(b200, backend, do.kv4_empty(n, 1, P, D), np.repeat(table, S, 0))
+    peaks = np.arange(77, N, 509)
+    for peaked in (False, True):
+        k = rng.normal(size=(N, 1, D)) * (0.05 if peaked else 1.0)
+        k[peaks] = 1.0
+        v = rng.uniform(-0.5, 0.5, (N, 1, D)) + 0.4
+        v[peaks] -= 0.8
+        v[..., ::32] = 1.0  # the largest of each group: -8 steps
+        do.kv4_write(dev.host, k, v * 2.0 ** (power + 3), table, [0, N], [N])
+        dev.put()
+        q = store(np.ones((S * rows, 1, D)) if peaked else rng.normal(size=(S * rows, 1, D)) * 2, "bf16")
+        scale = np.log(2.0 ** 14) / D if peaked else D ** -0.5  # a peak weighs as much as 2^14 light tokens
+        qb, y = backend.upload(q), backend.alloc(S * rows * D * 4)
+        attend.run(dev.cache, dev.batch(np.arange(S + 1) * rows, [N] * S), TYPES["bf16"], qb.ptr, 1, y.ptr, scale, causal=False, y_type=TYPES["f32"])
+        backend.synchronize()
+        got, want = y.get((S * rows, 1, D), np.float32), do.kv4_attention(dev.host, value(q, "bf16"), table, [0, S * rows], [N], scale, causal=False)
+        assert np.all(np.abs(got - want) <= 2.0 ** -10 * 2.0 ** (power + 3) + at_least_half_step(want, "f32"))
+
+
 @pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("rows", [4, 48])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
