@@ -1215,6 +1215,12 @@ class KV4Cache(ctypes.Structure):
     _fields_ = list(KVCache._fields_)
 
 
+def _not_a(op: str, cache, other: type) -> None:
+    """The two caches have the same fields, so the library cannot tell one from the other, and their memory has other sizes."""
+    if isinstance(cache, other):
+        raise B200Error(f"{op}: a {other.__name__} is another cache's memory")
+
+
 def _strides(nb):
     return None if nb is None else (ctypes.c_int64 * 2)(*[int(x) for x in nb])
 
@@ -1481,21 +1487,25 @@ class Backend:
 
     def kv_write(self, cache: KVCache, batch: KVBatch, ttype: int, k: int, v: int, k_nb=None, v_nb=None) -> None:
         """sam3b200_kv_write: rows of k and v (device addresses) quantised into the cache."""
+        _not_a("kv_write", cache, KV4Cache)
         _check(lib().sam3b200_kv_write(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
                                        v, _strides(v_nb)), "kv_write")
 
     def kv_read(self, cache: KVCache, batch: KVBatch, ttype: int, k: int, v: int, k_nb=None, v_nb=None) -> None:
         """sam3b200_kv_read: the last rows of each sequence back from the cache."""
+        _not_a("kv_read", cache, KV4Cache)
         _check(lib().sam3b200_kv_read(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
                                       v, _strides(v_nb)), "kv_read")
 
     def kv4_write(self, cache: KV4Cache, batch: KVBatch, ttype: int, k: int, v: int, k_nb=None, v_nb=None) -> None:
         """sam3b200_kv4_write: rows of k and v (device addresses) quantised into the 4-bit cache."""
+        _not_a("kv4_write", cache, KVCache)
         _check(lib().sam3b200_kv4_write(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
                                         v, _strides(v_nb)), "kv4_write")
 
     def kv4_read(self, cache: KV4Cache, batch: KVBatch, ttype: int, k: int, v: int, k_nb=None, v_nb=None) -> None:
         """sam3b200_kv4_read: the last rows of each sequence back from the 4-bit cache."""
+        _not_a("kv4_read", cache, KVCache)
         _check(lib().sam3b200_kv4_read(self.h, ctypes.addressof(cache), ctypes.addressof(batch), ttype, k, _strides(k_nb),
                                        v, _strides(v_nb)), "kv4_read")
 

@@ -46,6 +46,14 @@ def test_caches_and_batches_are_checked(b200, op):
     assert "null" in b200.last_error()
 
 
+def test_the_two_caches_are_told_apart(b200):
+    """KVCache and KV4Cache have the same fields: the bindings refuse one in place of the other before the library sees it."""
+    four, eight, batch = _cache(b200), b200.KVCache(A, A, A, A, 8, 2, 64, 128), _batch(b200)
+    for op, cache in (("kv_write", four), ("kv_read", four), ("kv4_write", eight), ("kv4_read", eight)):
+        with pytest.raises(b200.B200Error, match=f"{op}: a {type(cache).__name__} is another cache"):
+            getattr(b200.Backend, op)(None, cache, batch, b200.TYPE_F16, A, A)
+
+
 def test_rows_are_checked(b200):
     L, keep = b200.lib(), (_cache(b200), _batch(b200))
     c, b = ctypes.addressof(keep[0]), ctypes.addressof(keep[1])
