@@ -189,12 +189,13 @@ int sam3b200_mul_mat_dq16(sam3b200_backend *be, const sam3b200_weight *w, const 
  *   dst[m][n] = sum_k w[n][k] * x[m][k]  (+ bias[n]),  w[n][k] the block's value.
  * x: device rows of K elements of x_type (F32, F16, BF16), row stride ldx
  * elements; bias: device f32 [N] or NULL; dst: device rows of y_type (F32, or
- * x_type), row stride ldd.  Products are exact in codes and activations (F16
+ * x_type), row stride ldd, that share no element's memory with x or bias (one
+ * buffer's rows may hold both side by side).  Products are exact in codes and activations (F16
  * as they are; BF16, and F32 as a sum of two, in f16 after a power of two a row:
  * 2^-23 of an F32 element, and 2^-26 of the row's largest one where that is at
  * least 2^-112, may be lost), a block's sum is scaled and added in f32, in an
  * order that the shapes fix, and rounded once to y_type.  Infinities and NaN
- * give what the sum of their products with w[n][k] is.  The
+ * in x give what the sum of their products with w[n][k] is.  The
  * weights are the handle's own codes, with their scales a second time in 2
  * (Q4_1: 4) bytes a block, made by sam3b200_weight_upload.  Other weight types
  * and more rows are refused with an error: sam3b200_mul_mat takes them.

@@ -579,6 +579,24 @@ cudaError_t launch(Backend *be, VecArgs &a) {
 
 }  // namespace
 
+namespace {
+
+// `rows` runs of `bytes`, `step` bytes from one to the next.
+struct Runs {
+    uintptr_t at;
+    int64_t rows, step, bytes;
+};
+bool overlap(const Runs &a, const Runs &b) {
+    auto apart = [](uintptr_t x, int64_t nx, uintptr_t y, int64_t ny) { return x + nx <= y || y + ny <= x; };
+    if (apart(a.at, (a.rows - 1) * a.step + a.bytes, b.at, (b.rows - 1) * b.step + b.bytes)) return false;
+    for (int64_t i = 0; i < a.rows; ++i)
+        for (int64_t j = 0; j < b.rows; ++j)
+            if (!apart(a.at + i * a.step, a.bytes, b.at + j * b.step, b.bytes)) return true;
+    return false;
+}
+
+}  // namespace
+
 size_t vec_scale_bytes(int type, int N, int K) {
     return static_cast<size_t>((N + 15) / 16) * ((K + 127) / 128) * (type == SAM3B200_TYPE_Q4_1 ? 256 : 128);
 }
@@ -619,6 +637,13 @@ extern "C" int sam3b200_mul_mat_vec(sam3b200_backend *h, const sam3b200_weight *
         return SAM3B200_STATUS_FAILED;
     }
     if (M == 0) return SAM3B200_STATUS_SUCCESS;
+    // every block reads all of x, at times when others store
+    const Runs out{reinterpret_cast<uintptr_t>(dst), M, ldd * yb, static_cast<int64_t>(w->N) * yb};
+    if (overlap(out, {reinterpret_cast<uintptr_t>(x), M, ldx * xb, static_cast<int64_t>(w->K) * xb}) ||
+        (bias && overlap(out, {reinterpret_cast<uintptr_t>(bias), 1, 0, static_cast<int64_t>(w->N) * 4}))) {
+        set_error("mul_mat_vec: dst overlaps x or bias");
+        return SAM3B200_STATUS_FAILED;
+    }
     VecArgs a;
     a.codes = static_cast<const uint8_t *>(w->codes), a.scales = static_cast<const uint8_t *>(w->vec_scales);
     a.x = x, a.ldx = ldx, a.ldy = ldd, a.bias = bias, a.y = dst;

@@ -978,6 +978,31 @@ def test_vec_refusals(b200, backend):
         x.free()
 
 
+def test_vec_results_beside_and_over_x(b200, backend):
+    """x and dst in the same rows side by side, and in turn, are fine; dst over x or the bias is refused."""
+    rng = np.random.default_rng(7)
+    N, K, M, F16, F32 = 96, 64, 5, b200.TYPE_F16, b200.TYPE_F32
+    raw = do.blocks(rng, "q4_1", N, K)
+    w, x = backend.weight(b200.TYPE_Q4_1, raw, K, N), rng.normal(size=(M, K)).astype(np.float16)
+    want = check_vec(b200, backend, raw, "q4_1", N, K, x, "f16", "f16", handle=w)
+    for first in (True, False):  # x in front of dst, and behind
+        rows = np.zeros((M, K + N), np.float16)
+        at_x, at_y = (0, K) if first else (N, 0)
+        rows[:, at_x:at_x + K] = x
+        buf = backend.upload(rows)
+        backend.mul_mat_vec(w, buf.ptr + 2 * at_x, F16, M, buf.ptr + 2 * at_y, F16, ldx=K + N, ldy=K + N)
+        backend.synchronize()
+        got = buf.get(rows.shape, np.float16)
+        assert np.array_equal(got[:, at_x:at_x + K], x) and np.array_equal(got[:, at_y:at_y + N], want)
+    buf, b = backend.alloc(1 << 16), 1 << 12
+    for kw in (dict(y=buf.ptr), dict(y=buf.ptr + 2 * K - 2), dict(y=buf.ptr + 2 * K, ldx=K + N - 1, ldy=K + N - 1), dict(y=buf.ptr, y_type=F32),
+               dict(x=buf.ptr + 2 * N - 2, y=buf.ptr, M=1), dict(x=buf.ptr + 20 * N, y=buf.ptr, ldy=5 * N),
+               dict(y=buf.ptr + b, bias=buf.ptr + b + 2 * N * M - 4), dict(y=buf.ptr + b, bias=buf.ptr + b - 4 * N + 4)):
+        with pytest.raises(b200.B200Error, match="dst overlaps"):
+            backend.mul_mat_vec(w, **{**dict(x=buf.ptr, x_type=F16, M=M, y_type=F16), **kw})
+    w.free()
+
+
 # ---- together --------------------------------------------------------------------------------------------------
 
 
