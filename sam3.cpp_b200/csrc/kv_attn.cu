@@ -347,9 +347,11 @@ __global__ void __launch_bounds__(kWarps * 32, (Few<D, NT>::kBlocks)) kv_attn_fe
 
 constexpr int kMaxSplits = 256;  // most parts of a key range
 
-// The parts of a key range and the launch; `bit`: the kernel's of a.ready.
-template <typename F, int NT>
-cudaError_t few_launch(void (*kernel)(KvAttnArgs), KvAttnArgs &a, unsigned bit, int num_sms, cudaStream_t st) {
+// The parts of a key range and the launch.
+template <int D, int NT>
+cudaError_t launch(KvAttnArgs &a, int num_sms, cudaStream_t st) {
+    using F = Few<D, NT>;
+    constexpr unsigned kBit = 1u << (kReadyFew + 2 * (NT - 1) + (D == 64));
     const int64_t units = ((static_cast<int64_t>(a.b.n_rows) * a.group) >> (NT == 1 ? 3 : 4)) + a.b.n_seqs;
     // parts for two waves where there are few sequences and heads, for four where the lengths of many have to even out
     const int64_t wave = F::kBlocks * static_cast<int64_t>(num_sms), groups = units * a.c.heads;
@@ -367,18 +369,13 @@ cudaError_t few_launch(void (*kernel)(KvAttnArgs), KvAttnArgs &a, unsigned bit, 
     // With few sequences one that is far shorter than max_len (a captured step's bound) is cut finer, into all parts.
     a.chunk_short = static_cast<int>(2 * groups < wave ? std::min<int64_t>(least, a.chunk) : a.chunk);
     a.short_range = static_cast<int>(span / 2);
-    if (!(*a.ready & (1u << bit))) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+    if (!(*a.ready & kBit)) {
+        const cudaError_t e = cudaFuncSetAttribute(kv_attn_few_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
         if (e != cudaSuccess) return e;
-        *a.ready |= 1u << bit;
+        *a.ready |= kBit;
     }
     const dim3 grid(static_cast<unsigned>(units * a.splits), a.c.heads);
-    return launch_after(kernel, grid, kWarps * 32, F::kSmem, st, a);
-}
-
-template <int D, int NT>
-cudaError_t launch(KvAttnArgs &a, int num_sms, cudaStream_t st) {
-    return few_launch<Few<D, NT>, NT>(kv_attn_few_kernel<D, NT>, a, kReadyFew + 2 * (NT - 1) + (D == 64), num_sms, st);
+    return launch_after(kv_attn_few_kernel<D, NT>, grid, kWarps * 32, F::kSmem, st, a);
 }
 
 }  // namespace

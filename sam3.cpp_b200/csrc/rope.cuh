@@ -42,10 +42,6 @@ struct Stream8 {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
     }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
     __device__ __forceinline__ float operator[](int i) const { return to_f32(reinterpret_cast<const T *>(raw)[i]); }
 };
 
