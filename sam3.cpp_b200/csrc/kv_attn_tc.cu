@@ -147,7 +147,7 @@ __device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, f
 }
 
 // The largest of three numbers, NaN if one of them is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
@@ -600,8 +600,8 @@ __global__ void __launch_bounds__(Tc<D>::kThreads, 1) kv_attn_tc_kernel(const __
                     const uint32_t *y = &x[g >> 1][16 * (g & 1)];
                     float mx = __uint_as_float(y[0]);
 #pragma unroll
-                    for (int e = 1; e < 15; e += 2) mx = max3(mx, __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
-                    top = max3(top, fmaf(mx, fk[g], lv[g]), fmaf(__uint_as_float(y[15]), fk[g], lv[g]));
+                    for (int e = 1; e < 15; e += 2) mx = max3_nan(mx, __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
+                    top = max3_nan(top, fmaf(mx, fk[g], lv[g]), fmaf(__uint_as_float(y[15]), fk[g], lv[g]));
                 }
                 float alpha = 1.f;
                 if (!(top <= m + kLazy)) {  // a score that is NaN or +inf makes l NaN, and the row

@@ -650,7 +650,6 @@ extern "C" int sam3b200_mul_mat_vec(sam3b200_backend *h, const sam3b200_weight *
     a.M = static_cast<int>(M), a.N = w->N, a.K = w->K;
     a.cols = a.M * (x_type == SAM3B200_TYPE_F32 ? 2 : 1);
     a.sixteens = (a.N + 15) / 16, a.chunks = (a.K + 127) / 128;
-    a.w_log2 = 0, a.phase = a.chunks;
     a.y_type = y_type;
     a.aligned = reinterpret_cast<uintptr_t>(x) % (4 * xb) == 0 && ldx % 4 == 0;
     DeviceScope dev(be->device);
