@@ -413,7 +413,8 @@ int sam3b200_kv_attention_run(sam3b200_kv_attention *h, const sam3b200_kv_cache 
  * token, so a token's codes never change once they are written, and a page may
  * be shared before it is full.  Batches, pages, strides and errors are those
  * of the 8-bit cache; codes and scales are the caller's memory, 16-byte
- * aligned, and nothing has to be initialised. */
+ * aligned, and nothing has to be initialised.  n_pages * n_kv_heads *
+ * page_tokens is at most 2^31. */
 typedef struct sam3b200_kv4_cache {
     void *k_codes, *v_codes; /* device uint8 [n_pages][n_kv_heads][page_tokens][head_dim / 2]: dimension 2i in the low half of byte i, 2i + 1 in the high one */
     void *k_scale, *v_scale; /* device bf16 [n_pages][n_kv_heads][page_tokens][head_dim / 32] */
@@ -436,10 +437,12 @@ int sam3b200_kv4_read(sam3b200_backend *be, const sam3b200_kv4_cache *cache, con
 
 /* Attention over it, with sam3b200_kv_attention_run's handle, arguments, masks
  * and results.  Values reach the products exactly (11 bits), except that a
- * value below 2^-10 of the largest scale of the tokens near it may lose bits, at most 2^-24
- * of that scale; scales and softmax statistics are f32, softmax weights are
- * rounded to f16, BF16 queries to f16 as there: within 2^-10 of the largest
- * cached magnitude, plus the rounding to y's type.  That holds where the value
+ * value below 2^-10 of the largest scale of the tokens near it (those that its
+ * row does not see among them) may lose bits, at most 2^-24 of that scale;
+ * scales and softmax statistics are f32, softmax weights are rounded to f16, a
+ * quarter of them, by many rows, from exponentials good to 2^-13, BF16 queries to f16 as
+ * there: within 2^-10 of the largest magnitude cached for the sequence and kv head,
+ * plus the rounding to y's type.  That holds where the value
  * scales of the tokens that a row sees are 0 or at least 2^-90 and lie within
  * 2^100 of one another (2^20 beside a token of zeros), and where scale times a
  * key scale, and scale times a BF16 row's largest element, are ordinary f32

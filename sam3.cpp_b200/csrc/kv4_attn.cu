@@ -27,12 +27,16 @@
 // lane then has those of its tokens by one 16-byte load for two groups, ready
 // for arithmetic on pairs, in place of two conversions a token and group.
 //
-// What bounds it: instructions, some 650 a warp for 32 tokens of heads of 128
-// (4.6 KB; the issue slots are taken in two cycles of three), not the bytes.
+// What bounds it: a warp's chain for each block of tokens (copies, scales, scores,
+// maximum, exponentials, second product; some 680 instructions for 32 tokens of heads of 128, 4.6
+// KB) with four warps a scheduler.  The issue slots are taken in two cycles of
+// three (heads of 64: 58 %), no pipe is full (ALU 52 %, LSU 27 %, FMA and tensor
+// cores 24 %), memory runs at 60 % of the copy.
 // Measured: 64 sequences of 1000 ... 16100 tokens, 8 kv heads of 128, 4 query
-// heads each, 157 us (666 MB, 4.2 TB/s; the 8-bit cache takes 213); one sequence
+// heads each, 157 to 173 us (666 MB, 4.2 to 3.9 TB/s; the 8-bit cache takes 216);
+// a window of 1000 over them 38 (floor 11); one sequence
 // of 900 7.9 us; 3 ... 5 tokens of each of 4 sequences of 30000 ... 70000, 8
-// heads of 64, 36 us.  Scales taken from the stage by each lane: 169 for 161 of
+// heads of 64, 37 us.  Scales taken from the stage by each lane: 169 for 161 of
 // the first.  Copies by the bulk engine in place of 16-byte ones: 177, since the
 // waits take more instructions than the copies; 5 blocks an SM: 195, for lack of
 // registers; two stages, since 4 blocks with the widened scales have room for no
@@ -40,7 +44,11 @@
 // The parts are cut on the device, from all lengths (few_part): cut by the host
 // from the largest length, the last took 45 us, 24 sequences of 3000 ... 30000
 // 131 in place of 109, the first 161; the look at all lengths costs one sequence
-// of 900 0.7 us, and 64 of one length 157 in place of 149.  One wave of blocks
+// of 900 0.7 us, and 64 of one length 157 in place of 149.  Every block reads all
+// lengths, 128 sequences in one pass: 64, 128, 256, 512 and 1024 sequences of 500 ...
+// 1500 tokens, 8 kv heads of 128, take 35, 53, 85, 165 and 335 us (floors 11, 22, 47, 92, 183).  A
+// max_len 300 times the lengths: the first of these 38, 256 of them 87, the 4
+// sequences with heads of 64 49 in place of 37, since most blocks then find nothing.  One wave of blocks
 // with equal stretches of all the work, a block taking the end of one part and
 // the start of the next: 182 us, and 115 in place of 82 for 200 sequences of 100
 // ... 2500, whose starts and joins then follow one another.

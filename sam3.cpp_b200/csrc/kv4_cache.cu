@@ -11,9 +11,11 @@
 // A block takes up to 16 rows of a sequence for some of its slabs (a slab: one
 // head's keys, or its values), 8 values a thread and step, four threads a
 // group, the tokens of a slab side by side so that their codes leave as one
-// run; where the rows lie in the cache is looked up once for all slabs.  Bound by
-// memory, 2 (f16) bytes in and 0.56 out per value, and the other way round on
-// reading, with instructions close behind, so both work on packed 16-bit
+// run; where the rows lie in the cache is looked up once for all slabs.  2 (f16)
+// bytes in and 0.56 out per value, and the other way round on
+// reading; neither the memory (a third of the copy's rate) nor the issue slots (62 %)
+// are full: 983 and 1200 blocks of the ragged prompts below, at 4 and 5 an SM, are 1.66 and 1.62
+// waves, the last one two thirds full.  Fewer instructions shortened it most, so both work on packed 16-bit
 // numbers where the type has them:
 // - the largest magnitude and its sign by the bits (as whole numbers, the largest
 //   magnitude m is a maximum without sign, and the positive one exists if the
@@ -24,7 +26,7 @@
 //   residual is looked at, see round_quotients);
 // - code times d in the row's own type is the value rounded once.
 // Measured: ragged prompts of 15643 tokens in all, 8 heads of 128 in f16,
-// written and the 19116 then cached read back, 47.6 us (floor 27.9); one token each of 80 sequences and
+// written and the 19116 then cached read back, 47.6 to 48 us (floor 27.9; f32 rows 82, floor 49.7); one token each of 80 sequences and
 // its page back 9.8 us, the host's two calls.  With f32 arithmetic and a look up
 // of each slab's pages the prompts took 89 us.
 #include <algorithm>

@@ -46,10 +46,10 @@
 // us for the prompt then at 193), one lane polling for a warp (277), the
 // results by whole rows through shared memory (185 to 188: the loop's
 // registers).
-// Over the 4-bit cache the same prompt takes 165 us (832 TFLOP/s), since half
+// Over the 4-bit cache the same prompt takes 165 to 167 us (832 to 824 TFLOP/s), since half
 // the bytes come in and a page has no scale of its own to wait for, the 5184 rows
 // 448, and 4 parts of prompts of 400 to 800 tokens behind 2500 to 6700 (32 heads
-// on 4 of 128) 290 to 303, in place of 304.
+// on 4 of 128) 290 to 309, in place of 305.
 #include <algorithm>
 #include <type_traits>
 

@@ -4,18 +4,21 @@
 //   y[m][n] = sum over blocks b of d[n][b] (sum_k (code - 8) x[m][k])  + bias[n]         Q4_0
 //   y[m][n] = sum over b of d[n][b] (sum_k code x[m][k]) + mn[n][b] (sum_k x[m][k])  + bias[n]  Q4_1
 //
-// Bound by memory: 18 bytes a block of 32 weights, read once.  A block of 16
+// 18 bytes a block of 32 weights (Q4_1: 20) are read once.  A block of 16
 // warps an SM keeps x in shared memory; W of its warps share a tile of 16 or 32
 // rows of the weights, each with every W-th chunk of 128 k, which it copies by
 // cp.async into its own ring of shared memory.  The products run on mma.m16n8k16
 // f16 with f32 sums: the codes are its 16-row operand (exact in f16), the rows of
 // x its 8 columns, so up to 8 rows cost what one does, and the legacy matrix
 // instruction is wide enough for what memory delivers; widening the codes and
-// scaling the sums, 162 instructions a warp for 1 KB of codes (62 % of the issue
-// slots), is what comes next.  Measured: 49408 x 4096 Q4_0 by one row of f16 25.1
-// us (114 MB, 4.5 TB/s; 25.8 with blocks cut at whole tiles), 14339 x 4096 Q4_1 by
+// scaling the sums take 162 instructions a warp for 1 KB of codes (64 % of the issue
+// slots).  Measured: 49408 x 4096 Q4_0 by one row of f16 25.1 to 27.6
+// us (114 MB, 4.5 to 4.1 TB/s, 70 to 63 % of the copy; 25.8 with blocks cut at whole
+// tiles; Q4_1 29.8), 14339 x 4096 Q4_1 by
 // 6 rows of bf16 15.8 us, of which the launch, the staging of x and the end are
-// some 6.  Chunks dealt to the warps of a tile in turn, joined tile by tile, took
+// some 6; by 8, 9 and 16 rows of bf16 13.8 (Q4_0), 19.8 and 33 (Q4_0 27), by 4, 8 and 16 of f32 15.2, 26 and 55.
+// ptxas spills 12 to 40 bytes of the kernels for 9 and more columns with 32 weight
+// rows a warp, and of those for 17 and more.  Chunks dealt to the warps of a tile in turn, joined tile by tile, took
 // 28.7 us in place of 25.8; scales widened once
 // a warp through shared memory, for arithmetic on pairs, 26.6 (Q4_1 17 for 15.2).
 // Word t of each weight row's block (elements 4t ... and 16 + 4t ...) comes to a

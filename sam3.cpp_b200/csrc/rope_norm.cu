@@ -14,7 +14,13 @@
 // Measured: 21037 rows of 32 + 8 heads of 128 in bf16 87.8 us, 4.9 TB/s (the
 // rotation alone 77), with 70 % of the issue slots taken: a head costs the sums,
 // the shuffles and two conversions an element on top of the turn.  5184 rows of
-// 32 heads of 64, f32 to f16, 16.8 us (64 MB; floor 9.8): one wave of blocks.
+// 32 heads of 64, f32 to f16, 16.8 us (64 MB; floor 9.8), in 1296 blocks at 5 an
+// SM, 1.75 waves: no unit is busy (issue 42 %, DRAM 27 % of its nominal rate),
+// so it is the time from a block's first loads to its last stores, with a last
+// wave that leaves a quarter of the places empty.  rope_norm_any_kernel, for pairs
+// that do not come in eights and unaligned rows: the first with 61 pairs 421 us, the
+// second with 31 pairs 93.  (ptxas spills 8 to 20 bytes of the kernels from 16 bits
+// to f32, at 7 blocks an SM.)
 // Weights kept in registers for arithmetic on pairs: 124 us, for lack of them;
 // several row turns a block in place of one: 105.
 #include <algorithm>
@@ -59,6 +65,8 @@ __device__ __forceinline__ float weight_at(const void *w, int type, int i, float
     return to_f32(static_cast<const __nv_bfloat16 *>(w)[i]);
 }
 
+// Off by 2^-22 at most, beside the 14 roundings of 2^-24 that a head's sum and its use take: far below half a step of 16-bit
+// results (2^-11), and one instruction a head.
 __device__ __forceinline__ float rsqrt_approx(float x) {
     float y;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
