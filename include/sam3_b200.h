@@ -190,13 +190,13 @@ int sam3b200_mul_mat_dq16(sam3b200_backend *be, const sam3b200_weight *w, const 
  * x: device rows of K elements of x_type (F32, F16, BF16), row stride ldx
  * elements; bias: device f32 [N] or NULL; dst: device rows of y_type (F32, or
  * x_type), row stride ldd, that share no element's memory with x or bias (one
- * buffer's rows may hold both side by side).  Products are exact in codes and activations (F16
- * as they are; BF16, and F32 as a sum of two, in f16 after a power of two a row:
- * 2^-23 of an F32 element, and 2^-26 of the row's largest one where that is at
- * least 2^-112, may be lost), a block's sum is scaled and added in f32, in an
- * order that the shapes fix, and rounded once to y_type.  Infinities and NaN
- * in x give what the sum of their products with w[n][k] is.  The
- * weights are the handle's own codes, with their scales a second time in 2
+ * buffer's rows may hold both side by side).  Products are exact in codes and
+ * activations (F16 as they are; BF16, and F32 as a sum of two, in f16 after a
+ * power of two a row: 2^-23 of an F32 element, and 2^-26 of the row's largest
+ * one where that is at least 2^-112, may be lost), a block's sum is scaled and
+ * added in f32, in an order that the shapes fix, and rounded once to y_type.
+ * Infinities and NaN in x give what the sum of their products with w[n][k] is.
+ * The weights are the handle's own codes, with their scales a second time in 2
  * (Q4_1: 4) bytes a block, made by sam3b200_weight_upload.  Other weight types
  * and more rows are refused with an error: sam3b200_mul_mat takes them.
  * Allocates nothing.  Asynchronous on the backend stream. */
@@ -439,10 +439,10 @@ int sam3b200_kv4_read(sam3b200_backend *be, const sam3b200_kv4_cache *cache, con
  * and results.  Values reach the products exactly (11 bits), except that a
  * value below 2^-10 of the largest scale of the tokens near it (those that its
  * row does not see among them) may lose bits, at most 2^-24 of that scale;
- * scales and softmax statistics are f32, softmax weights are rounded to f16, a
- * quarter of them, by many rows, from exponentials good to 2^-13, BF16 queries to f16 as
- * there: within 2^-10 of the largest magnitude cached for the sequence and kv head,
- * plus the rounding to y's type.  That holds where the value
+ * scales and softmax statistics are f32, softmax weights are rounded to f16 (by
+ * many rows a quarter of them from exponentials good to 2^-13), BF16 queries to
+ * f16 as there: within 2^-10 of the largest magnitude cached for the sequence
+ * and kv head, plus the rounding to y's type.  That holds where the value
  * scales of the tokens that a row sees are 0 or at least 2^-90 and lie within
  * 2^100 of one another (2^20 beside a token of zeros), and where scale times a
  * key scale, and scale times a BF16 row's largest element, are ordinary f32

@@ -580,10 +580,6 @@ cudaError_t launch(Backend *be, VecArgs &a) {
     return launch<NT, 1, MINS, TX>(be, a);
 }
 
-}  // namespace
-
-namespace {
-
 // `rows` runs of `bytes`, `step` bytes from one to the next.
 struct Runs {
     uintptr_t at;
